@@ -191,7 +191,7 @@ def run(state):
     kind = case["kind"]
     with torch.no_grad():
         if own:
-            from nanoquant_amd.paged import paged_attention, paged_rope_write, verify_drafts
+            from nanoquant_amd.serve import paged_attention, paged_rope_write, verify_drafts
             s = state
             if kind == "write":
                 q = paged_rope_write(s["q"], s["k"], s["v"], s["cos"], s["sin"], s["positions"], s["k_pages"], s["v_pages"],
