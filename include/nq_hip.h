@@ -42,7 +42,8 @@ typedef enum {
     NQ_ERR_UNSUPPORTED = 7       /* valid request this build does not handle */
 } nq_status;
 
-typedef enum { NQ_F16 = 0, NQ_BF16 = 1 } nq_dtype;
+/* NQ_F32 is taken where an entry point says so. */
+typedef enum { NQ_F16 = 0, NQ_BF16 = 1, NQ_F32 = 2 } nq_dtype;
 
 typedef enum { NQ_PACK_LSB_FIRST = 0, NQ_PACK_HALF2 = 1 } nq_pack_method;
 
@@ -356,6 +357,77 @@ int nq_rope_kv_write(int dtype, const void* qkv, int64_t qkv_stride, void* k_cac
                      const void* rope_cos, const void* rope_sin, const int64_t* position, void* q_out,
                      int64_t q_stride, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                      int64_t max_len, nq_stream_t stream);
+
+/* ---------------------------------------------------------------- paged KV cache */
+
+/* A cache of many sequences with lengths of their own. The pool holds `pages` pages of page_size positions each,
+ *   k_pages, v_pages  dtype [pages, kv_heads, page_size, head_dim], 16-byte aligned
+ * and each sequence a row of the table,
+ *   table     device int32, `batch` rows of table_pages entries, table_stride >= table_pages entries apart: position p of
+ *             sequence b lies in page table[b][p / page_size] at row p % page_size. An entry outside [0, pages) is a page that
+ *             is not there (not yet, or no longer). Sequences may share pages that they only read.
+ *   positions device int64 [batch, tokens]: the position of each of the call's tokens, in any order. One outside
+ *             [0, table_pages * page_size) marks padding: nothing is written for it and its output row is zero.
+ * dtype NQ_F16 or NQ_BF16; heads a multiple of kv_heads, query head h uses kv head h / (heads / kv_heads).
+ * The reference has no counterpart: its harness keeps Hugging Face's static cache (kernel/test_decode.py:420-422). */
+
+/* Rotary embedding of new tokens and their write into the pages, one launch:
+ *   q, k, v   [batch, tokens] rows of q_stride / k_stride / v_stride elements (multiples of 8) holding heads, kv_heads and
+ *             kv_heads heads
+ *   rope_cos, rope_sin  [batch, tokens, head_dim], float32 with rope_float32, else dtype (the rotate-half convention)
+ *   q_out     [batch, tokens, heads * head_dim] = q cos + rotate_half(q) sin, the pages' key rows likewise; products and sum in
+ *             fp32, rounded once. Values are copied. Nothing is written to a page that is not there.
+ * Two tokens of the call must not name one row of one page (which of the two is left there would be open). head_dim a
+ * multiple of 16; q, k, v, cos, sin, q_out and the pages 16-byte aligned; q_out must not overlap the inputs. */
+int nq_paged_rope_write(int dtype, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, const void* rope_cos, const void* rope_sin, int rope_float32,
+                        const int64_t* positions, const int32_t* table, int64_t table_stride, int64_t table_pages,
+                        void* k_pages, void* v_pages, int64_t pages, int64_t page_size, void* q_out, int64_t batch,
+                        int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, nq_stream_t stream);
+
+/* Attention of one or several new tokens per sequence over its pages, which hold the tokens' own keys and values already:
+ *   q         [batch, tokens] rows of q_stride elements (a multiple of 8): rotated queries of heads heads
+ *   out       [batch, tokens, heads * head_dim] = sum_j p_j v_j, p = softmax(q . k_j * scaling) over the visible keys
+ * A token at position p sees key j iff j <= p, its page is there and, with window > 0, j > p - window or j < sinks (the last
+ * `window` positions and the first `sinks`). A token that sees no key gets zeros. Keys that a token does not see do not reach
+ * its result, whatever they hold; pages that no token sees are not read.
+ * Scores, softmax and sums in fp32; probabilities are rounded to dtype for the value product and summed as rounded.
+ *   workspace nq_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
+ *             not overlap.
+ * head_dim 64 or 128, page_size a multiple of 16, table_pages * page_size <= 2^30, else NQ_ERR_UNSUPPORTED. q, out and the
+ * pages 16-byte aligned. Results do not depend on what else runs or on the workspace's contents. */
+size_t nq_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t table_pages, int64_t page_size);
+int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t pages,
+                       int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_pages,
+                       const int64_t* positions, void* out, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t window, int64_t sinks, float scaling, void* workspace,
+                       size_t workspace_bytes, nq_stream_t stream);
+
+/* ---------------------------------------------------------------- drafted tokens */
+
+/* Verification of drafted tokens against the model's distributions, from given random numbers, so that the tokens that come
+ * out are distributed as the model's own (the next tokens of `batch` sequences):
+ *   logits      dtype (NQ_F16, NQ_BF16 or NQ_F32) rows of `vocab`, row_stride elements apart: row b * (drafts + 1) + i is the
+ *               model's distribution p_i after sequence b's first i drafts, p = softmax(logits / temperature)
+ *   draft       device int64 [batch, drafts]; the first entry outside [0, vocab) ends a sequence's drafts
+ *   draft_probs float32 [batch, drafts, vocab]: the distributions q_i that the drafts were drawn from, or NULL where they were
+ *               chosen without chance (q_i is then 1 at the draft)
+ *   uniforms    float32 [batch, drafts + 1] in [0, 1)
+ * Draft i is kept iff all before it are and uniforms[b][i] * q_i(x_i) < p_i(x_i). accepted[b] = their number n, and
+ * tokens[b] (int64 [batch, drafts + 1]) the n drafts, one token more, and -1 behind. That token is the first index at which
+ * the running sum of w passes uniforms[b][drafts] times its total: w = p_n where no draft was turned down, else
+ * max(p_n - q_n, 0) (p_n where that is zero everywhere). temperature 0 takes p as 1 at the first largest logit.
+ * A row with a NaN or an infinite largest logit has no distribution: its draft is turned down and the token is its argmax
+ * (the first NaN if there is one). Probabilities and sums in fp64. Three launches.
+ *   workspace   nq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
+ *               not overlap.
+ * Logits aligned to their size, draft_probs and uniforms to 4 bytes, whole numbers to 8. The reference has no counterpart: its
+ * harness samples one token a step with torch ops (src/nanoquant/kernel/test_decode.py:350-353). */
+size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
+int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
+                     const float* uniforms, float temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
+                     int64_t drafts, int64_t vocab, void* workspace, size_t workspace_bytes, nq_stream_t stream);
 
 /* ---------------------------------------------------------------- norm and activation of many tokens */
 

@@ -28,6 +28,7 @@ NQ_ERR_UNSUPPORTED = 7
 
 NQ_F16 = 0
 NQ_BF16 = 1
+NQ_F32 = 2
 NQ_PACK_LSB_FIRST = 0
 NQ_PACK_HALF2 = 1
 
@@ -88,6 +89,13 @@ SIGNATURES = {
                                        _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
     "nq_rope_kv_write": (_int, [_int, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                                  _vp]),
+    "nq_paged_rope_write": (_int, [_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _int, _vp, _vp, _i64, _i64, _vp, _vp, _i64,
+                                   _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "nq_paged_attention_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "nq_paged_attention": (_int, [_int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
+    "nq_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "nq_verify_drafts": (_int, [_int, _vp, _i64, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
     "nq_rms_norm": (_int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp]),
     "nq_silu_mul": (_int, [_int, _vp, _vp, _vp, _i64, _vp]),
     "nq_dense_gemv": (_int, [_int, _vp, _vp, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _i64, _i64, _vp]),

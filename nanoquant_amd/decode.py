@@ -30,7 +30,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from ._dispatch import launch as _launch, only_eager as _only_eager
 from .modules.linear import NanoQuantLinear
+from .serve import PagedKVCache, paged_rotary_attention
 
 LINEAR_NAMES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
@@ -103,36 +105,11 @@ def random_nanoquant_linear(in_features: int, out_features: int, rank: int, gene
     return lin
 
 
-def _only_eager(*tensors) -> bool:
-    """Whether a kernel may take the tensors' memory: nothing traces, transforms or differentiates them."""
-    for t in tensors:
-        if type(t) is not torch.Tensor and type(t) is not nn.Parameter:
-            return False
-    if torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() > 0:
-        return False
-    if torch._C._functorch.peek_interpreter_stack() is not None or torch.autograd.forward_ad._current_level >= 0:
-        return False
-    return not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
-
-
 def _pointwise_kernel_takes(x, other) -> bool:
     """Whether a row-wise HIP kernel may run on x and a second operand of its last dimension or shape."""
     return (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and other.dtype == x.dtype
             and other.device == x.device and x.numel() > 0 and x.shape[-1] % 8 == 0 and x.is_contiguous()
             and other.is_contiguous() and _only_eager(x, other) and x.data_ptr() % 16 == 0 and other.data_ptr() % 16 == 0)
-
-
-def _launch(what, fn, x, *args) -> None:
-    """``fn(*args, stream)`` on the device of x and its current stream. A small call is bound by this path: torch's device
-    guard and stream object took three of eleven microseconds."""
-    index = x.get_device()
-    if index == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _lib.check(status, what)
 
 
 def _plain(module, cls) -> bool:
@@ -385,8 +362,11 @@ class LlamaAttention(nn.Module):
         super().__init__()
         self.shape, self.layer = shape, layer
 
-    def forward(self, x, cos, sin, positions, cache: StaticKVCache, step_tables=None):
-        if step_tables is not None:  # one token per sequence
+    def forward(self, x, cos, sin, positions, cache: StaticKVCache | PagedKVCache, step_tables=None):
+        if isinstance(cache, PagedKVCache):
+            out = paged_rotary_attention(self.shape, self.layer, self.q_proj(x), self.k_proj(x), self.v_proj(x), cos, sin,
+                                         positions, cache)
+        elif step_tables is not None:  # one token per sequence
             B = x.shape[0]
             qk = torch.cat((self.q_proj(x), self.k_proj(x)), dim=-1).view(B, -1)
             out = rotary_attention_step(self.shape, self.layer, qk, self.v_proj(x).view(B, -1), step_tables,
@@ -429,6 +409,8 @@ class NanoQuantLlama(nn.Module):
     ``forward(ids [B, T], positions [T], cache)`` returns fp32 logits [B, T, vocab];
     ``positions`` is a device tensor of absolute positions, so the same call serves
     prefill (0..T-1) and a graph-captured one-token step (a position held on the device).
+    With a ``PagedKVCache`` the positions are [B, T], each sequence's own (or [T], the same for all),
+    -1 for padding, whose logits mean nothing.
     """
 
     def __init__(self, shape: LlamaShape, device=None, dtype=torch.float32):
@@ -456,13 +438,18 @@ class NanoQuantLlama(nn.Module):
         emb = torch.cat((freqs, freqs), dim=-1)
         return emb.cos().to(dtype), emb.sin().to(dtype)
 
-    def forward(self, ids, positions, cache: StaticKVCache, head=None):
+    def forward(self, ids, positions, cache: StaticKVCache | PagedKVCache, head=None):
         """fp32 logits of every position, or ``head(x)`` of the last layer's hidden states x [B, T, hidden] (a
         caller that needs the logits of a few positions only)."""
         x = self.model.embed_tokens(ids)
-        cos, sin = self.rope(positions, x.dtype)
-        consts = (self.step_eye, self.step_rot, self.step_mask_values)
-        tables = rotary_step_tables(cos, sin, positions, cache, x.dtype, consts=consts) if ids.shape[1] == 1 else None
+        if isinstance(cache, PagedKVCache):
+            positions = positions.expand(ids.shape).contiguous()
+            cos, sin = self.rope(positions, torch.float32)
+            tables = None
+        else:
+            cos, sin = self.rope(positions, x.dtype)
+            consts = (self.step_eye, self.step_rot, self.step_mask_values)
+            tables = rotary_step_tables(cos, sin, positions, cache, x.dtype, consts=consts) if ids.shape[1] == 1 else None
         for layer in self.model.layers:
             x = layer(x, cos, sin, positions, cache, tables)
         if head is not None:
