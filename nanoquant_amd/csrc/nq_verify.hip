@@ -307,7 +307,7 @@ extern "C" {
 size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
     if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > INT32_MAX || batch > INT32_MAX || drafts > INT32_MAX / 2) return 0;
     const int64_t chunks = ceil_div(vocab, kChunk);
-    if (batch * (drafts + 1) > INT32_MAX / chunks) return 0;
+    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks) return 0;  // blocks of 256 threads
     return static_cast<size_t>(batch) * (drafts + 2) * chunks * 16;
 }
 
