@@ -123,6 +123,7 @@ constexpr int kWaves = 4;          // of a block
 constexpr int kBlocks = 256;       // one a CU: its rings take most of the LDS
 constexpr int kEntries = 2048;     // (sequence, row group) pairs of a launch, whose key counts every block adds up
 constexpr int kLeastShare = 4;     // tiles a block takes at least: one a wave
+constexpr int kLeastTiles = 8;     // the same of rows_kernel's
 constexpr float kSlack = 8.0f;
 constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
 
@@ -138,6 +139,7 @@ struct PagedArgs {
     int window, sinks;  // window 0: none
     float scale;        // times log2(e)
     int row_groups, rows_kept;  // row groups a (sequence, kv head), rows of one that there are
+    int4* spans;        // [batch * row_groups]: Tiles, for rows_kernel's shares
     int2* desc;         // [batch * row_groups * kv_heads]: {first block * 2 + its slot, last block}
     float* part_o;      // [kBlocks][2][rows_kept][D]
     float2* part_ml;    // the same rows' {maximum, sum}
@@ -149,36 +151,140 @@ __device__ inline int real_position(const PagedArgs& a, int64_t row) {
     return p >= 0 && p < a.pages.capacity() ? static_cast<int>(p) : -1;
 }
 
-// The key tiles that the rows of an entry see: `sink_tiles` from the front, then those from window_tile on.
+// The key tiles that a group of rows sees: `sink_tiles` from the front, then those from window_tile on.
 struct Tiles {
     int sink_tiles, window_tile, count;
     __device__ int at(int i) const { return i < sink_tiles ? i : window_tile + i - sink_tiles; }
 };
 
-template <int RT>
-__device__ inline Tiles tiles_of(const PagedArgs& a, int entry) {
+// of rows whose real positions go from lo to hi (hi -1: none, which is one masked tile)
+template <int kKeys>
+__device__ inline Tiles tiles_between(const PagedArgs& a, int lo, int hi) {
+    Tiles r{0, 0, 1};
+    if (hi >= 0) {
+        const int start = a.window > 0 ? max(0, lo - a.window + 1) : 0;
+        r.window_tile = start / kKeys;
+        r.sink_tiles = min(r.window_tile, (min(a.sinks, start) + kKeys - 1) / kKeys);
+        r.count = r.sink_tiles + hi / kKeys - r.window_tile + 1;
+    }
+    return r;
+}
+
+// Row groups of `group` rows (token t, query head g of a kv head's G: row t G + g); entry = (sequence, row group).
+__device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
     const int b = entry / a.row_groups;
-    const int first = (entry - b * a.row_groups) * (16 * RT);  // row of the sequence
-    const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + 16 * RT - 1) / a.groups);
+    const int first = (entry - b * a.row_groups) * group;
+    const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + group - 1) / a.groups);
     int lo = INT32_MAX, hi = -1;
     for (int t = t0; t <= t1; ++t) {
         const int p = real_position(a, static_cast<int64_t>(b) * a.tokens + t);
         if (p >= 0) lo = min(lo, p);
         hi = max(hi, p);
     }
-    Tiles r{0, 0, 1};  // nothing to see: one masked tile
-    if (hi >= 0) {
-        const int start = a.window > 0 ? max(0, lo - a.window + 1) : 0;
-        r.window_tile = start / kTile;
-        r.sink_tiles = min(r.window_tile, (min(a.sinks, start) + kTile - 1) / kTile);
-        r.count = r.sink_tiles + hi / kTile - r.window_tile + 1;
+    return tiles_between<kTile>(a, lo, hi);
+}
+
+// A value that some rows of a product see and others do not reaches the others too where it is not finite (0 * inf). In tiles
+// that some rows see in part, such values are taken as 0, and these marks then make inf or NaN of the sums of the rows that do
+// see one: kind 0 marks +inf, 1 -inf, 2 NaN, each as 1 among zeros.
+template <typename T>
+__device__ inline uint32_t mark2(uint32_t v, int kind) {
+    constexpr uint32_t inf = T::ONE_PAIR == 0x3C003C00u ? 0x7C00u : 0x7F80u, one = T::ONE_PAIR & 0xFFFFu;
+    uint32_t r = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t x = (v >> (16 * h)) & 0xFFFFu;
+        const bool is = kind == 2 ? (x & 0x7FFFu) > inf : x == (kind ? inf | 0x8000u : inf);
+        r |= is ? one << (16 * h) : 0u;
     }
     return r;
 }
+// the finite ones of a pair, 0 for the others
+template <typename T>
+__device__ inline uint32_t finite2(uint32_t v) {
+    constexpr uint32_t inf = T::ONE_PAIR == 0x3C003C00u ? 0x7C00u : 0x7F80u;
+    return ((v & inf) != inf ? v & 0xFFFFu : 0u) | (((v >> 16) & inf) != inf ? v & 0xFFFF0000u : 0u);
+}
+__device__ inline float mark_value(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf(""); }
+
+// Which keys of a tile a row sees, a bit a key: arithmetic on words, since compares of every key with every row would each
+// hold a pair of scalar registers.
+__device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : 0xFFFFFFFFu >> (32 - n); }
+__device__ inline uint32_t seen_bits(int key0, int last, int start, int sinks) {  // of keys key0 .. key0 + 31
+    return low_bits(last - key0 + 1) & (~low_bits(start - key0) | low_bits(sinks - key0));
+}
+__device__ inline uint32_t bit_mask(uint32_t bits, int i) { return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), i, 1)); }
+__device__ inline float or_minus_inf(float x, uint32_t bits, int i) {  // x where bit i is set
+    return __builtin_bit_cast(float, bit_select(bit_mask(bits, i), __builtin_bit_cast(uint32_t, x), 0xFF800000u));
+}
+// both halves of a pair under bits i and i + 1
+__device__ inline uint32_t pair_mask(uint32_t bits, int i) { return bit_select(0xFFFFu, bit_mask(bits, i), bit_mask(bits, i + 1)); }
 
 template <typename T>
-__device__ inline uint32_t pack2(float a, float b) {
-    return static_cast<uint32_t>(T::from_float(a)) | (static_cast<uint32_t>(T::from_float(b)) << 16);
+__device__ inline uint32_t pack2(float a, float b);
+template <>
+__device__ inline uint32_t pack2<F16>(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+template <>
+__device__ inline uint32_t pack2<BF16>(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// All work of a launch is one line of units (entry, kv head, tile of keys), cut into equal shares for the blocks, so lengths
+// need neither be known on the host nor be alike. `count(e)`: the tiles of an entry; pre[e]: those of the entries before it.
+struct Shares {
+    int64_t share, first, end;  // units a block, and this block's
+    int entry;                  // of the first; -1: nothing to do
+};
+template <int kThreads, typename Count>
+__device__ inline Shares make_shares(const PagedArgs& a, int entries, int blocks, int least, int64_t* pre, int64_t* wave_total,
+                                     int* s_entry, Count count) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int per = (entries + kThreads - 1) / kThreads;
+    int64_t sum = 0;
+    for (int i = 0; i < per; ++i) {
+        const int e = t * per + i;
+        if (e < entries) {
+            pre[e] = sum;
+            sum += count(e);
+        }
+    }
+    int64_t incl = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t up = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += up;
+    }
+    if (lane == 63) wave_total[wave] = incl;
+    __syncthreads();
+    int64_t before = incl - sum;
+    for (int w = 0; w < wave; ++w) before += wave_total[w];
+    for (int i = 0; i < per; ++i) {
+        const int e = t * per + i;
+        if (e < entries) pre[e] += before;
+    }
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) all += wave_total[w];
+    if (t == 0) pre[entries] = all;
+    __syncthreads();
+    Shares r;
+    const int64_t total = all * a.kv_heads;
+    r.share = max<int64_t>((total + blocks - 1) / blocks, least);
+    r.first = blockIdx.x * r.share;
+    r.end = min(r.first + r.share, total);
+    if (r.first >= r.end) {
+        r.entry = -1;
+        return r;
+    }
+    for (int e = t; e < entries; e += kThreads)
+        if (pre[e] * a.kv_heads <= r.first && r.first < pre[e + 1] * a.kv_heads) *s_entry = e;
+    __syncthreads();
+    r.entry = __builtin_amdgcn_readfirstlane(*s_entry);
+    return r;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -192,10 +298,9 @@ __device__ inline float wave_cols_max(float v) {  // over the four lane groups t
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
-// Attention of a few rows (query head of a kv head's group, token) per sequence over its pages. All work is one line of
-// units (entry = (sequence, row group), kv head, tile of 32 keys), cut into equal shares for the blocks, so the lengths need
-// not be known on the host nor be alike; a (entry, kv head) that lies in one block is finished there, of the others the blocks
-// leave sums in the workspace that few_join_kernel adds. A wave takes every fourth tile of a share and keeps two in flight
+// Attention of a few rows (query head of a kv head's group, token) per sequence over its pages. An (entry, kv
+// head) that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that
+// join_kernel adds. A wave takes every fourth tile of a share and keeps two in flight
 // (DMA into its own ring: no barriers), and computes
 //   S^T = K Q^T      v_mfma_f32_16x16x32, A = 16 keys x 32 dimensions, B = 16 rows of queries
 //   O^T += V^T P^T   A = 16 dimensions x 32 keys, read transposed from the row-major tile, B = P^T: S^T's accumulator layout
@@ -217,47 +322,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int entries = a.batch * a.row_groups;
-
-    // the shares
-    {
-        const int per = (entries + 64 * kWaves - 1) / (64 * kWaves);
-        int64_t sum = 0;
-        for (int i = 0; i < per; ++i) {
-            const int e = t * per + i;
-            if (e < entries) {
-                pre[e] = sum;
-                sum += tiles_of<RT>(a, e).count;
-            }
-        }
-        int64_t incl = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t up = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += up;
-        }
-        if (lane == 63) wave_total[wave] = incl;
-        if (t == 0) s_entry = 0;
-        __syncthreads();
-        int64_t before = incl - sum;
-        for (int w = 0; w < wave; ++w) before += wave_total[w];
-        for (int i = 0; i < per; ++i) {
-            const int e = t * per + i;
-            if (e < entries) pre[e] += before;
-        }
-        if (t == 0) pre[entries] = wave_total[0] + wave_total[1] + wave_total[2] + wave_total[3];
-        __syncthreads();
-    }
-    const int64_t total = pre[entries] * a.kv_heads;
-    int64_t share = (total + kBlocks - 1) / kBlocks;
-    share = share < kLeastShare ? kLeastShare : share;
-    int64_t u = blockIdx.x * share;
-    const int64_t end = min(u + share, total);
-    if (u >= end) return;
-    for (int e = t; e < entries; e += 64 * kWaves)
-        if (pre[e] * a.kv_heads <= u && u < pre[e + 1] * a.kv_heads) s_entry = e;
-    __syncthreads();
-    int entry = __builtin_amdgcn_readfirstlane(s_entry);
+    const Shares shares = make_shares<64 * kWaves>(a, a.batch * a.row_groups, kBlocks, kLeastShare, pre, wave_total, &s_entry,
+                                                   [&](int e) { return tiles_of_few(a, e, 16 * RT).count; });
+    if (shares.entry < 0) return;
+    int entry = shares.entry;
+    int64_t u = shares.first;
 
     uint32_t voff[Instr];
 #pragma unroll
@@ -274,11 +343,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
         const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / count));
         const int64_t seg = seg0 + static_cast<int64_t>(kvh) * count;
         const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg));
-        const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(min<int64_t>(end - u, count - first)));
+        const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(min<int64_t>(shares.end - u, count - first)));
         const int b = entry / a.row_groups;
         const int row0 = (entry - b * a.row_groups) * (16 * RT);
         const int rows = min(16 * RT, a.tokens * a.groups - row0);
-        Tiles tiles = tiles_of<RT>(a, entry);
+        Tiles tiles = tiles_of_few(a, entry, 16 * RT);
         tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
         tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
 
@@ -360,13 +429,13 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                     const int swz = D == 128 ? c : c >> 1;
                     kf[h][kt] = *vec(kb + (16 * h + c) * D + 8 * ((4 * kt + g) ^ (swz & (C - 1))));
                 }
-            // which of the lane's keys (16 h + 4 g + i in bit 4 h + i) are there
             const bool there0 = page_of(key0) >= 0, there1 = page_of(key0 + 16) >= 0;
             const bool whole = there0 && there1 && key0 + kTile - 1 <= all_last &&
                                (key0 >= all_start || key0 + kTile <= a.sinks);
+            const uint32_t pages_there = (there0 ? 0xFFFFu : 0u) | (there1 ? 0xFFFF0000u : 0u);
             uint32_t some = 0;  // seen by some row of the wave's
             u32x4 pf[RT];
-            uint32_t seen[RT];
+            uint32_t seen[RT];  // the lane's key 16 h + 4 g + e in bit 16 h + e
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
@@ -374,27 +443,21 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                 for (int kt = 0; kt < D / 32; ++kt)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) s[h] = mfma16x16x32<T>(kf[h][kt], qf[rt][kt], s[h]);
-                seen[rt] = 0xFF;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[h] *= a.scale;
                 if (!whole) {
-                    seen[rt] = 0;
+                    seen[rt] = (seen_bits(key0, last[rt], start[rt], a.sinks) & pages_there) >> (4 * g);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + 16 * h + 4 * g + e;
-                            const bool see = (h ? there1 : there0) && key <= last[rt] && (key >= start[rt] || key < a.sinks);
-                            seen[rt] |= see ? 1u << (4 * h + e) : 0u;
-                        }
+                        for (int e = 0; e < 4; ++e) s[h][e] = or_minus_inf(s[h][e], seen[rt], 16 * h + e);
                     some |= seen[rt];
                 }
                 float top = -INFINITY;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[h][e] = (seen[rt] >> (4 * h + e)) & 1 ? s[h][e] * a.scale : -INFINITY;
-                        top = fmaxf(top, s[h][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, s[h][e]);
                 top = wave_cols_max(top);
                 if (__any(top > m[rt] + kSlack)) {
                     const float mn = fmaxf(m[rt], top);
@@ -414,58 +477,61 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                 }
                 lsum[rt] = mfma16x16x32<T>(u32x4{T::ONE_PAIR, T::ONE_PAIR, T::ONE_PAIR, T::ONE_PAIR}, pf[rt], lsum[rt]);
             }
-            u32x4 vf[D / 16];
             const int vr = 4 * g + (c >> 2);  // of 16: the row whose address the lane gives
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) {
+            auto read_v = [&](int dt) {
                 const int swz = D == 128 ? vr : vr >> 1;
                 const int at = 8 * ((2 * dt + ((c >> 1) & 1)) ^ (swz & (C - 1))) + 4 * (c & 1);
                 const uint2 lo = read_transposed(vb + vr * D + at), hi = read_transposed(vb + (16 + vr) * D + at);
-                vf[dt] = u32x4{lo.x, lo.y, hi.x, hi.y};
-            }
-            bool tainted = false;
+                return u32x4{lo.x, lo.y, hi.x, hi.y};
+            };
+            u32x4 keep;
             if (!whole) {
-                // values that no row sees are cleared (0 * NaN would reach every row); where a value that some rows see is
-                // not finite, the rows' sums are made one by one
 #pragma unroll
                 for (int off = 1; off < 16; off <<= 1) some |= __shfl_xor(some, off, 64);
-                float zero = 0.0f;
-                u32x4 keep;
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    keep[w] = ((some >> (2 * w)) & 1 ? 0xFFFFu : 0u) | ((some >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) {
-                    vf[dt] &= keep;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) zero = T::dot2(vf[dt][w], 0u, zero);
-                }
-                tainted = __any(zero != zero);
+                for (int w = 0; w < 4; ++w) keep[w] = pair_mask(some, 16 * (w >> 1) + 2 * (w & 1));
             }
-            if (!tainted) {
+            float zero = 0.0f;
+            constexpr int kAhead = 4;  // dimension tiles read together
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt)
+            for (int d0 = 0; d0 < D / 16; d0 += kAhead) {
+                u32x4 vf[kAhead];
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16x16x32<T>(vf[dt], pf[rt], o[rt][dt]);
-            } else {
+                for (int e = 0; e < kAhead; ++e) vf[e] = read_v(d0 + e);
+                if (!whole) {  // values that no row sees are cleared (rows behind a sequence's last, pages that are not
+                               // there), and those that are not finite
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    for (int k = 0; k < kTile; ++k) {
-                        const int from = 16 * ((k & 15) >> 2) + c;  // the lane that has the key's probability
-                        const int at = 4 * (k >> 4) + (k & 3);
-                        const uint32_t mine2 = at & 4 ? (at & 2 ? pf[rt][3] : pf[rt][2]) : (at & 2 ? pf[rt][1] : pf[rt][0]);
-                        const uint32_t pair = __shfl(mine2, from, 64);
-                        const bool see = (__shfl(seen[rt], from, 64) >> at) & 1;
-                        const float p = T::to_float(static_cast<uint16_t>(pair >> (16 * (at & 1))));
-                        const int swz = D == 128 ? k : k >> 1;
+                    for (int e = 0; e < kAhead; ++e)
 #pragma unroll
-                        for (int dt = 0; dt < D / 16; ++dt)
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t x = vf[e][w] & keep[w];
+                            zero = T::dot2(x, 0u, zero);
+                            vf[e][w] = finite2<T>(x);
+                        }
+                }
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int d = 16 * dt + 4 * g + e;
-                                const float v = T::to_float(vb[k * D + 8 * ((d >> 3) ^ (swz & (C - 1))) + (d & 7)]);
-                                o[rt][dt][e] = see ? fmaf(p, v, o[rt][dt][e]) : o[rt][dt][e];
-                            }
+                for (int e = 0; e < kAhead; ++e)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][d0 + e] = mfma16x16x32<T>(vf[e], pf[rt], o[rt][d0 + e]);
+            }
+            if (!whole && __any(zero != zero)) {
+#pragma unroll 1
+                for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt) {
+                        u32x4 vf = read_v(dt) & keep;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) vf[w] = mark2<T>(vf[w], kind);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            u32x4 sees;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) sees[w] = pair_mask(seen[rt], 16 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
+                            const f32x4 marks = mfma16x16x32<T>(vf, sees, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[rt][dt][e] += marks[e] > 0.0f ? mark_value(kind) : 0.0f;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
             }
             if (i + 2 < mine) {
@@ -525,9 +591,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
         }
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count - 1) / share)};
+                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count - 1) / shares.share)};
         u += n;
-        if (u >= end) return;
+        if (u >= shares.end) return;
         slot = 1;  // a share's first and last (entry, kv head) are the ones that it may not finish
         if (kvh + 1 == a.kv_heads) ++entry;
         __syncthreads();
@@ -535,8 +601,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
 }
 
 // Adds what the blocks left of one row of an (entry, kv head): the threads in groups of D / 4, a group a partial result.
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a) {
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_kernel(const PagedArgs a, int group) {
     constexpr int L4 = D / 4, Groups = 256 / L4;
     __shared__ float red[Groups][D];
     __shared__ float tops[4], sums[4];
@@ -548,20 +614,24 @@ __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a) {
     if (n == 1) return;
     const int entry = seg / a.kv_heads, kvh = seg - entry * a.kv_heads;
     const int b = entry / a.row_groups;
-    const int r = (entry - b * a.row_groups) * (16 * RT) + row;
+    const int r = (entry - b * a.row_groups) * group + row;
     if (r >= a.tokens * a.groups) return;
     // partial i: the first block's slot, then slot 0 of those behind it
     auto place = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : (first + i) * 2) * a.rows_kept + row; };
-    static_assert(kBlocks == 256, "a thread a block's statistics");
-    const float2 ml = t < n ? a.part_ml[place(t)] : float2{-INFINITY, 0.0f};
-    float top = ml.x;
+    float top = -INFINITY;
+    for (int i = t; i < n; i += 256) top = fmaxf(top, a.part_ml[place(i)].x);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
     if ((t & 63) == 0) tops[t >> 6] = top;
     __syncthreads();
     const float M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float mu = M == -INFINITY ? 0.0f : M;
-    const float l = wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - mu));
+    float l = 0.0f;
+    for (int i = t; i < n; i += 256) {
+        const float2 ml = a.part_ml[place(i)];
+        l += ml.y * __builtin_amdgcn_exp2f(ml.x - mu);
+    }
+    l = wave_sum(l);
     if ((t & 63) == 0) sums[t >> 6] = l;
     const int grp = t / L4, at = 4 * (t % L4);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -586,52 +656,511 @@ __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a) {
     }
 }
 
-int row_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
-// Sequences of a launch, and what it needs of the workspace.
-struct FewPlan {
-    int64_t rt, row_groups, rows_kept, batch;
-    size_t part_o, part_ml, desc, bytes;
+// ---------------------------------------------------------------- many rows
+
+constexpr int kKeys = 64;   // keys of a tile
+constexpr int kRowWaves = 4;
+constexpr int kRowEntries = 1024;  // as kEntries: two blocks of rows_kernel's smaller form fit a CU
+
+// An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes.
+__global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group, int entries) {
+    const int entry = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (entry >= entries) return;
+    const int b = entry / a.row_groups;
+    const int first = (entry - b * a.row_groups) * group;
+    const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + group - 1) / a.groups);
+    int lo = INT32_MAX, hi = -1;
+    for (int t = t0 + (threadIdx.x & 63); t <= t1; t += 64) {
+        const int p = real_position(a, static_cast<int64_t>(b) * a.tokens + t);
+        if (p >= 0) lo = min(lo, p);
+        hi = max(hi, p);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        lo = min(lo, __shfl_xor(lo, off, 64));
+        hi = max(hi, __shfl_xor(hi, off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        const Tiles r = tiles_between<kKeys>(a, lo, hi);
+        a.spans[entry] = int4{r.sink_tiles, r.window_tile, r.count, 0};
+    }
+}
+
+// Attention of many rows per sequence over its pages: blocks of 4 waves, 32 RW rows each (RW row tiles that share every key
+// and value read from LDS), over tiles of 64 keys, K and V row-major in LDS by DMA, two tiles in flight.
+//   S^T = K Q^T      v_mfma_f32_32x32x16, A = 32 keys x 16 dimensions, B = 32 rows of queries
+//   O^T += V^T P^T   A = 32 dimensions x 16 keys, read transposed, B = P^T: S^T's accumulator layout already, with keys
+//                    4 kg .. +3 and 8 + 4 kg .. +3 of each 16 in lane group kg
+// kShared: the work of all row groups in equal shares over the grid, as in few_kernel; otherwise a block takes a row group,
+// the last ones (the longest of a prompt) first.
+template <typename T, int D, int RW, bool kShared>
+__global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(const PagedArgs a) {
+    constexpr int C = D / 8;             // 16-byte chunks of a row
+    constexpr int RowsPer = 64 / C;      // rows of one DMA instruction
+    constexpr int Instr = 16 / RowsPer;  // instructions for 16 rows
+    constexpr int Group = 32 * RW * kRowWaves;
+    constexpr int KT = D / 16, DT = D / 32;
+    __shared__ __attribute__((aligned(16))) uint16_t kv[2][2][kKeys * D];  // [buffer][K, V]
+    __shared__ int there[2][4];                                           // the page of a tile's 16 keys
+    __shared__ int spans[2][kRowWaves];
+    __shared__ int64_t pre[kShared ? kRowEntries + 1 : 1];
+    __shared__ int64_t wave_total[kRowWaves];
+    __shared__ int s_entry;
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int c = lane & 31, kg = lane >> 5;
+    const int entries = a.batch * a.row_groups;
+
+    Shares shares{};
+    int entry, slot = 0;
+    int64_t u = 0;
+    if constexpr (kShared) {
+        shares = make_shares<64 * kRowWaves>(a, entries, static_cast<int>(gridDim.x), kLeastTiles, pre, wave_total, &s_entry,
+                                             [&](int e) { return a.spans[e].z; });
+        if (shares.entry < 0) return;
+        entry = shares.entry;
+        u = shares.first;
+    } else {
+        const int order = static_cast<int>(blockIdx.x) / (a.batch * a.kv_heads);
+        const int rest = static_cast<int>(blockIdx.x) - order * a.batch * a.kv_heads;
+        entry = rest / a.kv_heads * a.row_groups + a.row_groups - 1 - order;
+    }
+
+    uint32_t koff[Instr], voff[Instr];
+#pragma unroll
+    for (int j = 0; j < Instr; ++j) {
+        const int row = j * RowsPer + lane / C, pos = lane % C;
+        const int kswz = D == 128 ? row : row >> 1;
+        const int vswz = D == 128 ? ((row & 3) << 2) | (row >> 2) : (((row >> 1) & 1) << 2) | (row >> 2);
+        koff[j] = static_cast<uint32_t>(row * D * 2 + 16 * (pos ^ (kswz & (C - 1))));
+        voff[j] = static_cast<uint32_t>(row * D * 2 + 16 * (pos ^ vswz));
+    }
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(&kv[0][0][0])) + static_cast<uint32_t>(wave) * (16 * D * 2);
+    // positive, so that the largest product is the largest score: the queries take a negative factor's sign, and are zero for
+    // a factor of zero
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+
+    while (true) {
+        const int b = entry / a.row_groups;
+        const int row0 = (entry - b * a.row_groups) * Group + wave * (32 * RW);
+        const int rows = a.tokens * a.groups;
+        int kvh, first = 0, n, count;
+        int64_t seg = 0;
+        Tiles tiles;
+        if constexpr (kShared) {
+            const int64_t seg0 = pre[entry] * a.kv_heads;
+            count = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
+            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / count));
+            seg = seg0 + static_cast<int64_t>(kvh) * count;
+            first = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg));
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(min<int64_t>(shares.end - u, count - first)));
+            const int4 sp = a.spans[entry];
+            tiles = Tiles{sp.x, sp.y, sp.z};
+        } else {
+            kvh = static_cast<int>(blockIdx.x) % a.kv_heads;
+        }
+
+        u32x4 qf[RW][KT];
+        int last[RW], start[RW];
+        int lo = INT32_MAX, hi = -1, all_start = 0;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep_q = a.scale == 0.0f ? 0u : 0xFFFFFFFFu;
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw) {
+            const int r = min(row0 + 32 * rw + c, rows - 1);
+            const int tok = r / a.groups;
+            const int64_t q_row = static_cast<int64_t>(b) * a.tokens + tok;
+            last[rw] = row0 + 32 * rw + c < rows ? real_position(a, q_row) : -1;
+            start[rw] = a.window > 0 ? max(0, last[rw] - a.window + 1) : 0;
+            if (last[rw] >= 0) {
+                lo = min(lo, last[rw]);
+                all_start = max(all_start, start[rw]);
+            }
+            hi = max(hi, last[rw]);
+            const uint16_t* src = a.q + q_row * a.q_stride + static_cast<int64_t>(kvh * a.groups + r - tok * a.groups) * D + 8 * kg;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) qf[rw][kt] = *vec(src + 16 * kt);
+        }
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) qf[rw][kt][w] = (qf[rw][kt][w] ^ flip) & keep_q;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            lo = min(lo, __shfl_xor(lo, off, 64));
+            hi = max(hi, __shfl_xor(hi, off, 64));
+            all_start = max(all_start, __shfl_xor(all_start, off, 64));
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        all_start = __builtin_amdgcn_readfirstlane(all_start);
+        const int any_start = a.window > 0 ? max(0, lo == INT32_MAX ? 0 : lo - a.window + 1) : 0;  // the first key of some row
+        if constexpr (!kShared) {
+            if (lane == 0) {
+                spans[0][wave] = lo;
+                spans[1][wave] = hi;
+            }
+            __syncthreads();
+            int blo = INT32_MAX, bhi = -1;
+#pragma unroll
+            for (int w = 0; w < kRowWaves; ++w) {
+                blo = min(blo, spans[0][w]);
+                bhi = max(bhi, spans[1][w]);
+            }
+            tiles = tiles_between<kKeys>(a, blo, bhi);
+            count = n = __builtin_amdgcn_readfirstlane(tiles.count);
+        }
+        tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
+        tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
+
+        f32x16 o[RW][DT];
+        float m[RW], l[RW];
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw) {
+            m[rw] = -INFINITY;
+            l[rw] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[rw][dt][i] = 0.0f;
+        }
+        const __attribute__((address_space(4))) int32_t* table =
+            (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
+        // a wave brings a quarter of a tile: 16 keys, which lie in one page
+        auto issue = [&](int it, int buf) {
+            const int key = tiles.at(first + it) * kKeys + 16 * wave;
+            const int at = key / a.pages.page_size;
+            int page = at < a.pages.table_pages ? table[at] : -1;
+            page = page < a.pages.pages ? page : -1;
+            if (lane == 0) there[buf][wave] = page;
+            const int64_t from = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
+            const uint32_t lds = lds0 + static_cast<uint32_t>(buf) * (2 * kKeys * D * 2);
+#pragma unroll
+            for (int j = 0; j < Instr; ++j) dma16_lds(a.k_pages + from, koff[j], lds + 1024u * j);
+#pragma unroll
+            for (int j = 0; j < Instr; ++j) dma16_lds(a.v_pages + from, voff[j], lds + kKeys * D * 2u + 1024u * j);
+        };
+        issue(0, 0);
+        wait_vmcnt<0>();
+        barrier_keep_dma();
+        for (int it = 0; it < n; ++it) {
+            const int buf = it & 1;
+            if (it + 1 < n) issue(it + 1, buf ^ 1);
+            const int key0 = tiles.at(first + it) * kKeys;
+            if (key0 <= hi && (key0 + kKeys > any_start || key0 < a.sinks)) {  // some row of the wave sees some key
+                const uint16_t* kb = kv[buf][0];
+                const uint16_t* vb = kv[buf][1];
+                const int4 pg = *reinterpret_cast<const int4*>(&there[buf][0]);
+                const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0 && pg.z >= 0 && pg.w >= 0) &&
+                                   key0 + kKeys - 1 <= lo && (key0 >= all_start || key0 + kKeys <= a.sinks);
+                // operands are read a group of four ahead of the products that run; left to itself the compiler reads all
+                // of them first, or two and waits
+                f32x16 s[RW][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[rw][h][i] = 0.0f;
+                u32x4 kf[2][4];
+                auto read_k = [&](int q) {  // steps 2 q and 2 q + 1 of both halves
+                    const int kswz = D == 128 ? c : c >> 1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        kf[q & 1][e] = *vec(kb + (32 * (e & 1) + c) * D + 8 * ((2 * (2 * q + (e >> 1)) + kg) ^ (kswz & (C - 1))));
+                };
+                read_k(0);
+#pragma unroll
+                for (int q = 0; q < KT / 2; ++q) {
+                    if (q + 1 < KT / 2) read_k(q + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int rw = 0; rw < RW; ++rw)
+                            s[rw][e & 1] = mfma32x32x16<T>(kf[q & 1][e], qf[rw][2 * q + (e >> 1)], s[rw][e & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                uint32_t seen[RW][2], some[2] = {0u, 0u};  // key 32 h + 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4 of h
+                if (!whole) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t pages_there = ((h ? pg.z : pg.x) >= 0 ? 0xFFFFu : 0u) | ((h ? pg.w : pg.y) >= 0 ? 0xFFFF0000u : 0u);
+#pragma unroll
+                        for (int rw = 0; rw < RW; ++rw) {
+                            seen[rw][h] = (seen_bits(key0 + 32 * h, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
+                            some[h] |= seen[rw][h];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) s[rw][h][i] = or_minus_inf(s[rw][h][i], seen[rw][h], 8 * (i >> 2) + (i & 3));
+                        }
+                    }
+                }
+                u32x4 pf[RW][4];
+#pragma unroll
+                for (int rw = 0; rw < RW; ++rw) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rw][h][i]);
+                    top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
+                    if (__any(top > m[rw] + kSlack)) {
+                        const float mn = fmaxf(m[rw], top);
+                        const float keep = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
+                        m[rw] = mn;
+                        l[rw] *= keep;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep;
+                    }
+                    const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int i = 8 * (kt & 1) + 2 * w;
+                            pf[rw][kt][w] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][kt >> 1][i], scale, -mu)),
+                                                     __builtin_amdgcn_exp2f(fmaf(s[rw][kt >> 1][i + 1], scale, -mu)));
+                            l[rw] = T::dot2(pf[rw][kt][w], T::ONE_PAIR, l[rw]);
+                        }
+                    }
+                }
+                // the row of 16 keys that this lane names in a transposed read, and the place of its four dimensions
+                const int vr = 4 * kg + ((lane & 15) >> 2);
+                const int dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                auto read_v = [&](int kt, int dt) {
+                    uint2 part[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = vr + 8 * e;
+                        const int vswz = D == 128 ? ((row & 3) << 2) | (row >> 2) : (((row >> 1) & 1) << 2) | (row >> 2);
+                        const int d = 32 * dt + dim;
+                        part[e] = read_transposed(vb + (16 * kt + row) * D + 8 * ((d >> 3) ^ vswz) + (d & 7));
+                    }
+                    return u32x4{part[0].x, part[0].y, part[1].x, part[1].y};
+                };
+                u32x4 vf[2][DT];
+                auto read_vs = [&](int kt) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) vf[kt & 1][dt] = read_v(kt, dt);
+                };
+                read_vs(0);
+                if (!whole) {
+#pragma unroll
+                    for (int off = 1; off < 32; off <<= 1) {
+                        some[0] |= __shfl_xor(some[0], off, 64);
+                        some[1] |= __shfl_xor(some[1], off, 64);
+                    }
+                }
+                float zero = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) {
+                    if (kt < 3) read_vs(kt + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (!whole) {  // values that no row sees are cleared, and those that are not finite
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t keep = pair_mask(some[kt >> 1], 16 * (kt & 1) + 8 * (w >> 1) + 2 * (w & 1));
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt) {
+                                const uint32_t x = vf[kt & 1][dt][w] & keep;
+                                zero = T::dot2(x, 0u, zero);
+                                vf[kt & 1][dt][w] = finite2<T>(x);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[kt & 1][dt], pf[rw][kt], o[rw][dt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!whole && __any(zero != zero)) {
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int rw = 0; rw < RW; ++rw) {
+                                f32x16 marks;
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) marks[i] = 0.0f;
+#pragma unroll 1
+                                for (int kt = 0; kt < 4; ++kt) {
+                                    u32x4 x = read_v(kt, dt), sees;
+                                    const uint32_t any = (kt & 2 ? some[1] : some[0]) >> (16 * (kt & 1));
+                                    const uint32_t own = (kt & 2 ? seen[rw][1] : seen[rw][0]) >> (16 * (kt & 1));
+#pragma unroll
+                                    for (int w = 0; w < 4; ++w) {
+                                        x[w] = mark2<T>(x[w] & pair_mask(any, 8 * (w >> 1) + 2 * (w & 1)), kind);
+                                        sees[w] = pair_mask(own, 8 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
+                                    }
+                                    marks = mfma32x32x16<T>(x, sees, marks);
+                                }
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[rw][dt][i] += marks[i] > 0.0f ? mark_value(kind) : 0.0f;
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                }
+            }
+            wait_vmcnt<0>();
+            barrier_keep_dma();
+        }
+
+        const bool done = first == 0 && n == count;
+        uint16_t* ob = &kv[0][0][0] + wave * (32 * D);  // the wave's rows through LDS, a tile at a time, then whole rows to memory
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw) {
+            float L = l[rw] + __shfl_xor(l[rw], 32, 64);
+            float M = m[rw];
+            if (last[rw] < 0) {  // padding took part where the tile was whole
+                L = 0.0f;
+                M = -INFINITY;
+            }
+            const float inv = 1.0f / L;
+            if (kShared && !done) {
+                const int at = wave * (32 * RW) + 32 * rw + c;
+                if (row0 + 32 * rw + c < rows) {
+                    const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept + at;
+                    if (kg == 0) a.part_ml[part] = float2{M, L};
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            f32x4 x;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e];
+                            *reinterpret_cast<f32x4*>(a.part_o + part * D + 32 * dt + 8 * g4 + 4 * kg) = x;
+                        }
+                }
+                continue;
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e] * inv;
+                    *reinterpret_cast<uint2*>(ob + c * D + 8 * ((4 * dt + g4) ^ (c & (C - 1))) + 4 * kg) =
+                        uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+                }
+#pragma unroll
+            for (int j = 0; j < 32 / RowsPer; ++j) {
+                const int r = RowsPer * j + lane / C, ch = lane % C;
+                const u32x4 v = *vec(ob + r * D + 8 * (ch ^ (r & (C - 1))));
+                const int at_row = row0 + 32 * rw + r;
+                if (at_row < rows) {
+                    const int tok = at_row / a.groups;
+                    const int64_t to = ((static_cast<int64_t>(b) * a.tokens + tok) * a.heads + kvh * a.groups + at_row - tok * a.groups) * D;
+                    *reinterpret_cast<u32x4*>(a.out + to + 8 * ch) = v;
+                }
+            }
+        }
+        if constexpr (!kShared) return;
+        if (first == 0 && t == 0)
+            a.desc[entry * a.kv_heads + kvh] =
+                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count - 1) / shares.share)};
+        u += n;
+        if (u >= shares.end) return;
+        slot = 1;
+        if (kvh + 1 == a.kv_heads) ++entry;
+        __syncthreads();
+    }
+}
+
+// Which kernel a call runs, how many sequences a launch takes, and what it needs of the workspace.
+struct Plan {
+    bool few;            // few_kernel, else rows_kernel
+    bool shared;
+    int tiles;           // row tiles: of 16 rows a wave (few), of 32
+    int64_t group;       // rows of a row group
+    int64_t row_groups, rows_kept, batch, blocks;
+    size_t part_o, part_ml, desc, spans, bytes;
 };
 
-FewPlan few_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim) {
-    FewPlan p{};
-    p.rt = row_tiles(tokens * groups);
-    p.row_groups = ceil_div(tokens * groups, 16 * p.rt);
-    p.rows_kept = std::min(tokens * groups, 16 * p.rt);
-    p.batch = std::min({batch, std::max<int64_t>(1, kEntries / p.row_groups),
-                        std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads * p.rows_kept))});
-    p.part_o = static_cast<size_t>(kBlocks) * 2 * p.rows_kept * head_dim * sizeof(float);
-    p.part_ml = static_cast<size_t>(kBlocks) * 2 * p.rows_kept * sizeof(float2);
+Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t max_keys) {
+    Plan p{};
+    const int64_t rows = tokens * groups;
+    p.few = rows <= 64;
+    if (p.few) {
+        p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+        p.group = 16 * p.tiles;
+        p.shared = true;
+        p.blocks = kBlocks;
+    } else {
+        const int64_t large = ceil_div(rows, 256) * batch * kv_heads;
+        p.tiles = large >= 2 * kBlocks ? 2 : 1;
+        p.shared = false;
+        if (p.tiles == 1 && max_keys >= 4096) {
+            p.shared = true;
+            p.tiles = large >= kBlocks / 2 ? 2 : 1;
+        }
+        p.group = 128 * p.tiles;
+        p.blocks = p.tiles == 2 ? kBlocks : 2 * kBlocks;
+    }
+    p.row_groups = ceil_div(rows, p.group);
+    p.rows_kept = std::min(rows, p.group);
+    p.batch = batch;
+    if (p.shared) {
+        const int64_t entries = p.few ? kEntries : kRowEntries;
+        if (p.row_groups > entries) p.shared = false;  // a prompt this long fills the card
+        p.batch = std::min({batch, std::max<int64_t>(1, entries / p.row_groups),
+                            std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads * p.rows_kept))});
+    }
+    if (!p.shared) {
+        p.batch = std::min(batch, std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads)));
+        return p;
+    }
+    p.part_o = static_cast<size_t>(p.blocks) * 2 * p.rows_kept * head_dim * sizeof(float);
+    p.part_ml = static_cast<size_t>(p.blocks) * 2 * p.rows_kept * sizeof(float2);
+    p.spans = static_cast<size_t>(p.batch) * p.row_groups * sizeof(int4);
     p.desc = static_cast<size_t>(p.batch) * p.row_groups * kv_heads * sizeof(int2);
-    p.bytes = p.part_o + p.part_ml + p.desc;
+    p.part_ml = static_cast<size_t>(ceil_div(p.part_ml, 16) * 16);
+    p.bytes = p.part_o + p.part_ml + p.spans + p.desc;
     return p;
 }
 
-template <typename T, int D, int RT>
-void launch_few(const PagedArgs& a, hipStream_t st) {
-    few_kernel<T, D, RT><<<dim3(kBlocks), 64 * kWaves, 0, st>>>(a);
-    few_join_kernel<T, D, RT><<<dim3(static_cast<unsigned>(a.batch * a.row_groups * a.kv_heads * a.rows_kept)), 256, 0, st>>>(a);
+template <typename T, int D>
+void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
+    const unsigned segs = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.row_groups * a.kv_heads);
+    const dim3 grid(static_cast<unsigned>(plan.blocks));
+    if (plan.few) {
+        if (plan.tiles == 1) few_kernel<T, D, 1><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (plan.tiles == 2) few_kernel<T, D, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+        else few_kernel<T, D, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+    } else if (plan.shared) {
+        const int entries = a.batch * a.row_groups;
+        spans_kernel<<<dim3(static_cast<unsigned>(ceil_div(entries, 4))), 256, 0, st>>>(a, static_cast<int>(plan.group), entries);
+        if (plan.tiles == 1) rows_kernel<T, D, 1, true><<<grid, 64 * kRowWaves, 0, st>>>(a);
+        else rows_kernel<T, D, 2, true><<<grid, 64 * kRowWaves, 0, st>>>(a);
+    } else {
+        if (plan.tiles == 1) rows_kernel<T, D, 1, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
+        else rows_kernel<T, D, 2, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
+    }
+    if (plan.shared) join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(a.rows_kept)), 256, 0, st>>>(a, static_cast<int>(plan.group));
 }
 
 template <typename T, int D>
-void launch_paged(PagedArgs a, const FewPlan& plan, char* ws, hipStream_t st) {
+void launch_paged(PagedArgs a, const Plan& plan, char* ws, hipStream_t st) {
     a.row_groups = static_cast<int>(plan.row_groups);
     a.rows_kept = static_cast<int>(plan.rows_kept);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + plan.part_o);
-    a.desc = reinterpret_cast<int2*>(ws + plan.part_o + plan.part_ml);
-    const int batch = a.batch;
-    for (int b = 0; b < batch; b += static_cast<int>(plan.batch)) {
+    a.spans = reinterpret_cast<int4*>(ws + plan.part_o + plan.part_ml);
+    a.desc = reinterpret_cast<int2*>(ws + plan.part_o + plan.part_ml + plan.spans);
+    const int64_t batch = a.batch;
+    for (int64_t b = 0; b < batch; b += plan.batch) {
         PagedArgs s = a;
-        s.batch = std::min(static_cast<int>(plan.batch), batch - b);
-        s.q += static_cast<int64_t>(b) * a.tokens * a.q_stride;
-        s.positions += static_cast<int64_t>(b) * a.tokens;
+        s.batch = static_cast<int>(std::min(plan.batch, batch - b));
+        s.q += b * a.tokens * a.q_stride;
+        s.positions += b * a.tokens;
         s.pages.table += b * a.pages.table_stride;
-        s.out += static_cast<int64_t>(b) * a.tokens * a.heads * D;
-        if (plan.rt == 1) launch_few<T, D, 1>(s, st);
-        else if (plan.rt == 2) launch_few<T, D, 2>(s, st);
-        else launch_few<T, D, 4>(s, st);
+        s.out += b * a.tokens * a.heads * D;
+        launch_slice<T, D>(s, plan, st);
     }
 }
 
@@ -722,9 +1251,10 @@ int nq_paged_rope_write(int dtype, const void* q, int64_t q_stride, const void* 
 size_t nq_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                           int64_t table_pages, int64_t page_size) {
     if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65536 || batch > INT32_MAX ||
-        tokens > INT32_MAX || batch * tokens > INT32_MAX / heads)
+        tokens > INT32_MAX || batch * tokens > INT32_MAX / heads || table_pages <= 0 || page_size <= 0 ||
+        table_pages > kMaxKeys || page_size > kMaxKeys)
         return 0;
-    return few_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim).bytes;
+    return make_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size).bytes;
 }
 
 int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t pages,
@@ -747,7 +1277,7 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
         return fail(NQ_ERR_ALIGNMENT, "%s: q, out and the workspace must be 16-byte aligned", name);
     const size_t need = nq_paged_attention_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, table_pages, page_size);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
         return fail(NQ_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", name, workspace ? workspace_bytes : size_t{0}, need);
     PagedArgs a{};
     a.q = static_cast<const uint16_t*>(q);
@@ -765,7 +1295,7 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
     a.window = static_cast<int>(std::min(window, kMaxKeys));
     a.sinks = static_cast<int>(std::min(sinks, kMaxKeys));
     a.scale = scaling * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
-    const FewPlan plan = few_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim);
+    const Plan plan = make_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size);
     char* ws = static_cast<char*>(workspace);
     hipStream_t st = as_stream(stream);
     if (dtype == NQ_F16) {
