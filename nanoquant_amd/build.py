@@ -40,6 +40,8 @@ COMMON_FLAGS = [
 # accumulators between AGPRs and VGPRs on every loop trip (more such moves than MFMAs).
 FILE_FLAGS = {
     "nq_gemv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    # the same in the paged attention: its outputs are rescaled now and then, and went through both files for it
+    "nq_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

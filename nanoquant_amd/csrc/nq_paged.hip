@@ -852,82 +852,6 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
             if (key0 <= hi && (key0 + kKeys > any_start || key0 < a.sinks)) {  // some row of the wave sees some key
                 const uint16_t* kb = kv[buf][0];
                 const uint16_t* vb = kv[buf][1];
-                const int4 pg = *reinterpret_cast<const int4*>(&there[buf][0]);
-                const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0 && pg.z >= 0 && pg.w >= 0) &&
-                                   key0 + kKeys - 1 <= lo && (key0 >= all_start || key0 + kKeys <= a.sinks);
-                // operands are read a group of four ahead of the products that run; left to itself the compiler reads all
-                // of them first, or two and waits
-                f32x16 s[RW][2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int rw = 0; rw < RW; ++rw)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[rw][h][i] = 0.0f;
-                u32x4 kf[2][4];
-                auto read_k = [&](int q) {  // steps 2 q and 2 q + 1 of both halves
-                    const int kswz = D == 128 ? c : c >> 1;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        kf[q & 1][e] = *vec(kb + (32 * (e & 1) + c) * D + 8 * ((2 * (2 * q + (e >> 1)) + kg) ^ (kswz & (C - 1))));
-                };
-                read_k(0);
-#pragma unroll
-                for (int q = 0; q < KT / 2; ++q) {
-                    if (q + 1 < KT / 2) read_k(q + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int rw = 0; rw < RW; ++rw)
-                            s[rw][e & 1] = mfma32x32x16<T>(kf[q & 1][e], qf[rw][2 * q + (e >> 1)], s[rw][e & 1]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                uint32_t seen[RW][2], some[2] = {0u, 0u};  // key 32 h + 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4 of h
-                if (!whole) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t pages_there = ((h ? pg.z : pg.x) >= 0 ? 0xFFFFu : 0u) | ((h ? pg.w : pg.y) >= 0 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                        for (int rw = 0; rw < RW; ++rw) {
-                            seen[rw][h] = (seen_bits(key0 + 32 * h, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
-                            some[h] |= seen[rw][h];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) s[rw][h][i] = or_minus_inf(s[rw][h][i], seen[rw][h], 8 * (i >> 2) + (i & 3));
-                        }
-                    }
-                }
-                u32x4 pf[RW][4];
-#pragma unroll
-                for (int rw = 0; rw < RW; ++rw) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rw][h][i]);
-                    top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
-                    if (__any(top > m[rw] + kSlack)) {
-                        const float mn = fmaxf(m[rw], top);
-                        const float keep = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
-                        m[rw] = mn;
-                        l[rw] *= keep;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep;
-                    }
-                    const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const int i = 8 * (kt & 1) + 2 * w;
-                            pf[rw][kt][w] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][kt >> 1][i], scale, -mu)),
-                                                     __builtin_amdgcn_exp2f(fmaf(s[rw][kt >> 1][i + 1], scale, -mu)));
-                            l[rw] = T::dot2(pf[rw][kt][w], T::ONE_PAIR, l[rw]);
-                        }
-                    }
-                }
                 // the row of 16 keys that this lane names in a transposed read, and the place of its four dimensions
                 const int vr = 4 * kg + ((lane & 15) >> 2);
                 const int dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -942,68 +866,130 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                     }
                     return u32x4{part[0].x, part[0].y, part[1].x, part[1].y};
                 };
-                u32x4 vf[2][DT];
+                // operands are read a group of four ahead of the products that run; left to itself the compiler reads all of
+                // them first, or two and waits
+                u32x4 kf[2][4], vf[2][DT];
+                auto read_ks = [&](int h, int q) {
+                    const int kswz = D == 128 ? c : c >> 1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        kf[q & 1][e] = *vec(kb + (32 * h + c) * D + 8 * ((2 * (4 * q + e) + kg) ^ (kswz & (C - 1))));
+                };
                 auto read_vs = [&](int kt) {
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) vf[kt & 1][dt] = read_v(kt, dt);
                 };
-                read_vs(0);
-                if (!whole) {
 #pragma unroll
-                    for (int off = 1; off < 32; off <<= 1) {
-                        some[0] |= __shfl_xor(some[0], off, 64);
-                        some[1] |= __shfl_xor(some[1], off, 64);
+                for (int h = 0; h < 2; ++h) {  // 32 keys at a time
+                    const int half0 = key0 + 32 * h;
+                    const int2 pg = *reinterpret_cast<const int2*>(&there[buf][2 * h]);
+                    const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0) && half0 + 31 <= lo &&
+                                       (half0 >= all_start || half0 + 32 <= a.sinks);
+                    f32x16 s[RW];
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[rw][i] = 0.0f;
+                    read_ks(h, 0);
+#pragma unroll
+                    for (int q = 0; q < KT / 4; ++q) {
+                        if (q + 1 < KT / 4) read_ks(h, q + 1);
+                        else read_vs(2 * h);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int rw = 0; rw < RW; ++rw) s[rw] = mfma32x32x16<T>(kf[q & 1][e], qf[rw][4 * q + e], s[rw]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                }
-                float zero = 0.0f;
+                    uint32_t seen[RW], some = 0u;  // the lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
+                    if (!whole) {
+                        const uint32_t pages_there = (pg.x >= 0 ? 0xFFFFu : 0u) | (pg.y >= 0 ? 0xFFFF0000u : 0u);
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) {
-                    if (kt < 3) read_vs(kt + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (!whole) {  // values that no row sees are cleared, and those that are not finite
+                        for (int rw = 0; rw < RW; ++rw) {
+                            seen[rw] = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
+                            some |= seen[rw];
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t keep = pair_mask(some[kt >> 1], 16 * (kt & 1) + 8 * (w >> 1) + 2 * (w & 1));
+                            for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen[rw], 8 * (i >> 2) + (i & 3));
+                        }
 #pragma unroll
-                            for (int dt = 0; dt < DT; ++dt) {
-                                const uint32_t x = vf[kt & 1][dt][w] & keep;
-                                zero = T::dot2(x, 0u, zero);
-                                vf[kt & 1][dt][w] = finite2<T>(x);
-                            }
+                        for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
+                    }
+                    u32x4 pf[RW][2];
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw) {
+                        float top = s[rw][0];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rw][i]);
+                        top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
+                        // the reference point of the exponentials follows the running maximum only once that is 8 above it:
+                        // exponentials up to 2^8 round the same, and most steps rescale nothing
+                        if (__any(top > m[rw] + kSlack)) {
+                            const float mn = fmaxf(m[rw], top);
+                            const float keep = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
+                            m[rw] = mn;
+                            l[rw] *= keep;
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep;
+                        }
+                        const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) {
+                            pf[rw][w >> 2][w & 3] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][2 * w], scale, -mu)),
+                                                             __builtin_amdgcn_exp2f(fmaf(s[rw][2 * w + 1], scale, -mu)));
+                            l[rw] = T::dot2(pf[rw][w >> 2][w & 3], T::ONE_PAIR, l[rw]);
                         }
                     }
+                    float zero = 0.0f;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        if (k2 == 0) read_vs(2 * h + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (!whole) {  // values that no row sees are cleared, and those that are not finite
 #pragma unroll
-                        for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[kt & 1][dt], pf[rw][kt], o[rw][dt]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (!whole && __any(zero != zero)) {
-#pragma unroll 1
-                    for (int kind = 0; kind < 3; ++kind)
+                            for (int w = 0; w < 4; ++w) {
+                                const uint32_t keep = pair_mask(some, 16 * k2 + 8 * (w >> 1) + 2 * (w & 1));
+#pragma unroll
+                                for (int dt = 0; dt < DT; ++dt) {
+                                    const uint32_t x = vf[k2][dt][w] & keep;
+                                    zero = T::dot2(x, 0u, zero);
+                                    vf[k2][dt][w] = finite2<T>(x);
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                            for (int rw = 0; rw < RW; ++rw) {
-                                f32x16 marks;
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) marks[i] = 0.0f;
+                            for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[k2][dt], pf[rw][k2], o[rw][dt]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (!whole && __any(zero != zero)) {
 #pragma unroll 1
-                                for (int kt = 0; kt < 4; ++kt) {
-                                    u32x4 x = read_v(kt, dt), sees;
-                                    const uint32_t any = (kt & 2 ? some[1] : some[0]) >> (16 * (kt & 1));
-                                    const uint32_t own = (kt & 2 ? seen[rw][1] : seen[rw][0]) >> (16 * (kt & 1));
+                        for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
-                                    for (int w = 0; w < 4; ++w) {
-                                        x[w] = mark2<T>(x[w] & pair_mask(any, 8 * (w >> 1) + 2 * (w & 1)), kind);
-                                        sees[w] = pair_mask(own, 8 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
+                            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                                for (int rw = 0; rw < RW; ++rw) {
+                                    f32x16 marks;
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) marks[i] = 0.0f;
+#pragma unroll 1
+                                    for (int k2 = 0; k2 < 2; ++k2) {
+                                        u32x4 x = read_v(2 * h + k2, dt), sees;
+#pragma unroll
+                                        for (int w = 0; w < 4; ++w) {
+                                            x[w] = mark2<T>(x[w] & pair_mask(some >> (16 * k2), 8 * (w >> 1) + 2 * (w & 1)), kind);
+                                            sees[w] = pair_mask(seen[rw] >> (16 * k2), 8 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
+                                        }
+                                        marks = mfma32x32x16<T>(x, sees, marks);
                                     }
-                                    marks = mfma32x32x16<T>(x, sees, marks);
-                                }
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[rw][dt][i] += marks[i] > 0.0f ? mark_value(kind) : 0.0f;
-                                __builtin_amdgcn_sched_barrier(0);
-                            }
+                                    for (int i = 0; i < 16; ++i) o[rw][dt][i] += marks[i] > 0.0f ? mark_value(kind) : 0.0f;
+                                    __builtin_amdgcn_sched_barrier(0);
+                                }
+                    }
                 }
             }
             wait_vmcnt<0>();
