@@ -151,6 +151,11 @@ __device__ inline int real_position(const PagedArgs& a, int64_t row) {
     return p >= 0 && p < a.pages.capacity() ? static_cast<int>(p) : -1;
 }
 
+__device__ inline int64_t out_row(const PagedArgs& a, int b, int kvh, int r) {  // row r of a sequence and kv head
+    const int tok = r / a.groups;
+    return (static_cast<int64_t>(b) * a.tokens + tok) * a.heads + kvh * a.groups + r - tok * a.groups;
+}
+
 // The key tiles that a group of rows sees: `sink_tiles` from the front, then those from window_tile on.
 struct Tiles {
     int sink_tiles, window_tile, count;
@@ -576,9 +581,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                 const int r = row0 + 16 * rt + row;
                 if (done) {
                     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                    const int tok = r / a.groups;
-                    const int64_t at = ((static_cast<int64_t>(b) * a.tokens + tok) * a.heads + kvh * a.groups + r - tok * a.groups) * D;
-                    *reinterpret_cast<u32x4*>(a.out + at + 8 * ch) =
+                    *reinterpret_cast<u32x4*>(a.out + out_row(a, b, kvh, r) * D + 8 * ch) =
                         u32x4{pack2<T>(lo[0] * inv, lo[1] * inv), pack2<T>(lo[2] * inv, lo[3] * inv),
                               pack2<T>(hi[0] * inv, hi[1] * inv), pack2<T>(hi[2] * inv, hi[3] * inv)};
                 } else {
@@ -600,43 +603,50 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
     }
 }
 
-// Adds what the blocks left of one row of an (entry, kv head): the threads in groups of D / 4, a group a partial result.
+// Where the partial results of an (entry, kv head) lie: n blocks from `first` on took part, the first with its slot, the others
+// with their slot 0.
+struct Parts {
+    int place0, first, n;
+    __device__ int64_t row(const PagedArgs& a, int i, int row) const {
+        return static_cast<int64_t>(i == 0 ? place0 : (first + i) * 2) * a.rows_kept + row;
+    }
+};
+__device__ inline Parts parts_of(const PagedArgs& a, int seg) {
+    const int2 d = a.desc[seg];
+    return Parts{d.x, d.x >> 1, d.y - (d.x >> 1) + 1};
+}
+
+// Adds what the blocks left of one row of an (entry, kv head), for few rows of which many blocks may hold a part: the threads
+// in groups of D / 4, a group a partial result.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(const PagedArgs a, int group) {
+__global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int group) {
     constexpr int L4 = D / 4, Groups = 256 / L4;
     __shared__ float red[Groups][D];
     __shared__ float tops[4], sums[4];
     const int t = threadIdx.x;
     const int seg = static_cast<int>(blockIdx.x) / a.rows_kept;
     const int row = static_cast<int>(blockIdx.x) - seg * a.rows_kept;
-    const int2 d = a.desc[seg];
-    const int first = d.x >> 1, n = d.y - first + 1;
-    if (n == 1) return;
+    const Parts parts = parts_of(a, seg);
+    if (parts.n == 1) return;
     const int entry = seg / a.kv_heads, kvh = seg - entry * a.kv_heads;
     const int b = entry / a.row_groups;
     const int r = (entry - b * a.row_groups) * group + row;
     if (r >= a.tokens * a.groups) return;
-    // partial i: the first block's slot, then slot 0 of those behind it
-    auto place = [&](int i) { return static_cast<int64_t>(i == 0 ? d.x : (first + i) * 2) * a.rows_kept + row; };
-    float top = -INFINITY;
-    for (int i = t; i < n; i += 256) top = fmaxf(top, a.part_ml[place(i)].x);
+    static_assert(kBlocks <= 256, "a thread a block's statistics");
+    const float2 ml = t < parts.n ? a.part_ml[parts.row(a, t, row)] : float2{-INFINITY, 0.0f};
+    float top = ml.x;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
     if ((t & 63) == 0) tops[t >> 6] = top;
     __syncthreads();
     const float M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float mu = M == -INFINITY ? 0.0f : M;
-    float l = 0.0f;
-    for (int i = t; i < n; i += 256) {
-        const float2 ml = a.part_ml[place(i)];
-        l += ml.y * __builtin_amdgcn_exp2f(ml.x - mu);
-    }
-    l = wave_sum(l);
+    const float l = wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - mu));
     if ((t & 63) == 0) sums[t >> 6] = l;
     const int grp = t / L4, at = 4 * (t % L4);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = grp; i < n; i += Groups) {
-        const int64_t p = place(i);
+    for (int i = grp; i < parts.n; i += Groups) {
+        const int64_t p = parts.row(a, i, row);
         const float f = __builtin_amdgcn_exp2f(a.part_ml[p].x - mu);
         o += f * *reinterpret_cast<const f32x4*>(a.part_o + p * D + at);
     }
@@ -650,12 +660,61 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedArgs a, int group)
             x += red[i][2 * t];
             y += red[i][2 * t + 1];
         }
-        const int tok = r / a.groups;
-        const int64_t to = ((static_cast<int64_t>(b) * a.tokens + tok) * a.heads + kvh * a.groups + r - tok * a.groups) * D;
-        *reinterpret_cast<uint32_t*>(a.out + to + 2 * t) = pack2<T>(x * inv, y * inv);
+        *reinterpret_cast<uint32_t*>(a.out + out_row(a, b, kvh, r) * D + 2 * t) = pack2<T>(x * inv, y * inv);
     }
 }
 
+// The same for many rows, of which a few blocks hold a part: D / 8 threads a row, eight dimensions each, the parts one after
+// the other.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void rows_join_kernel(const PagedArgs a, int group) {
+    constexpr int C = D / 8, Rows = 256 / C;
+    const int t = threadIdx.x;
+    const int blocks = (a.rows_kept + Rows - 1) / Rows;
+    const int seg = static_cast<int>(blockIdx.x) / blocks;
+    const Parts parts = parts_of(a, seg);
+    if (parts.n == 1) return;
+    const int row = (static_cast<int>(blockIdx.x) - seg * blocks) * Rows + t / C;
+    const int entry = seg / a.kv_heads, kvh = seg - entry * a.kv_heads;
+    const int b = entry / a.row_groups;
+    const int r = (entry - b * a.row_groups) * group + row;
+    if (row >= a.rows_kept || r >= a.tokens * a.groups) return;
+    const int at = 8 * (t % C);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    for (int i0 = 0; i0 < parts.n; i0 += 4) {
+        float2 ml[4];
+        f32x4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // those past the last read it again, with a weight of zero
+            const int64_t p = parts.row(a, min(i0 + i, parts.n - 1), row);
+            ml[i] = a.part_ml[p];
+            x[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + at);
+            y[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + at + 4);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(M - mu);
+        M = top;
+        L *= keep;
+        lo *= keep;
+        hi *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i0 + i >= parts.n) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mu);
+            L += f * ml[i].y;
+            lo += f * x[i];
+            hi += f * y[i];
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<u32x4*>(a.out + out_row(a, b, kvh, r) * D + at) =
+        u32x4{pack2<T>(lo[0] * inv, lo[1] * inv), pack2<T>(lo[2] * inv, lo[3] * inv), pack2<T>(hi[0] * inv, hi[1] * inv),
+              pack2<T>(hi[2] * inv, hi[3] * inv)};
+}
 
 // ---------------------------------------------------------------- many rows
 
@@ -1039,11 +1098,7 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                 const int r = RowsPer * j + lane / C, ch = lane % C;
                 const u32x4 v = *vec(ob + r * D + 8 * (ch ^ (r & (C - 1))));
                 const int at_row = row0 + 32 * rw + r;
-                if (at_row < rows) {
-                    const int tok = at_row / a.groups;
-                    const int64_t to = ((static_cast<int64_t>(b) * a.tokens + tok) * a.heads + kvh * a.groups + at_row - tok * a.groups) * D;
-                    *reinterpret_cast<u32x4*>(a.out + to + 8 * ch) = v;
-                }
+                if (at_row < rows) *reinterpret_cast<u32x4*>(a.out + out_row(a, b, kvh, at_row) * D + 8 * ch) = v;
             }
         }
         if constexpr (!kShared) return;
@@ -1127,7 +1182,9 @@ void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
         if (plan.tiles == 1) rows_kernel<T, D, 1, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
         else rows_kernel<T, D, 2, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
     }
-    if (plan.shared) join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(a.rows_kept)), 256, 0, st>>>(a, static_cast<int>(plan.group));
+    const int group = static_cast<int>(plan.group);
+    if (plan.few) few_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(a.rows_kept)), 256, 0, st>>>(a, group);
+    else if (plan.shared) rows_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(ceil_div(a.rows_kept, 256 / (D / 8)))), 256, 0, st>>>(a, group);
 }
 
 template <typename T, int D>
