@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "nq_common.h"
+#include "nq_wave.h"
 
 namespace nq {
 namespace {
@@ -298,11 +299,6 @@ __device__ inline uint2 read_transposed(const uint16_t* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
-__device__ inline float wave_cols_max(float v) {  // over the four lane groups that hold a column
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-
 // Attention of a few rows (query head of a kv head's group, token) per sequence over its pages. An (entry, kv
 // head) that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that
 // join_kernel adds. A wave takes every fourth tile of a share and keeps two in flight
@@ -463,7 +459,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top = fmaxf(top, s[h][e]);
-                top = wave_cols_max(top);
+                top = max_xor32(max_xor16(top));  // the lane groups that hold a column
                 if (__any(top > m[rt] + kSlack)) {
                     const float mn = fmaxf(m[rt], top);
                     const float keep = __builtin_amdgcn_exp2f(m[rt] - (mn == -INFINITY ? 0.0f : mn));
@@ -980,7 +976,7 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                         float top = s[rw][0];
 #pragma unroll
                         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rw][i]);
-                        top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
+                        top = max_xor32(top) * scale;
                         // the reference point of the exponentials follows the running maximum only once that is 8 above it:
                         // exponentials up to 2^8 round the same, and most steps rescale nothing
                         if (__any(top > m[rw] + kSlack)) {

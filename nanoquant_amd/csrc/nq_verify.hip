@@ -1,35 +1,140 @@
 // Verification of drafted tokens: softmax statistics of every row of logits, the accept tests, and one token by inverse CDF
-// from the row where the drafts end. Three launches:
-//   1. row_stats_kernel, a block per (row, chunk of 4096 logits): the chunk's largest logit m_c (with its index) and
+// from the row where the drafts end. Four launches:
+//   1. row_stats_kernel, a block per (row, chunk of 4096 or 16384 logits): the chunk's largest logit m_c (with its index) and
 //      z_c = sum exp((x - m_c) / T);
-//   2. chunk_sums_kernel, a block per (sequence, chunk): joins the rows' statistics, walks the accept tests
-//      u q(x) < p(x) and adds up its chunk of w = max(p - q, 0) and of p for the row that the walk ends at;
-//   3. pick_token_kernel, a block per sequence: the chunk in which the running sum of w passes u times its total, then the
+//   2. walk_kernel, a block per sequence: joins its rows' statistics and makes the accept tests u q(x) < p(x);
+//   3. batch_sums_kernel, a block per (sequence, 4096 logits): the sums of w = max(p - q, 0) and of p over its part of the row
+//      that the tests ended at;
+//   4. pick_token_kernel, a block per sequence: the part in which the running sum of w passes u times its total, then the
 //      index within it.
-// Probabilities and their sums are fp64: the token is where a running sum over up to 10^5 terms passes a number, and its
-// fp32 rounding would move a visible share of the borders between tokens.
+// Probabilities and their sums are fp64: the token is where a running sum over up to 10^5 terms passes a number, and fp32
+// rounding would move a visible share of the borders between tokens.
 #include <algorithm>
 
 #include "nq_common.h"
+#include "nq_wave.h"
 
 namespace nq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                   // logits a thread
-constexpr int kChunk = kThreads * kPer;    // logits a block
-
 struct F32 {};
 
+// Logits come in aligned pieces of 16 bytes, whatever the row's alignment: piece k of a row holds its elements
+// k * N - lead .. + N - 1, of which those outside the row (of its first and last piece) are not used.
 template <typename T>
 struct Elem {
-    typedef uint16_t type;
+    static constexpr int N = 8;
     __device__ static float get(const void* p, int64_t i) { return T::to_float(static_cast<const uint16_t*>(p)[i]); }
+    __device__ static void unpack(const u32x4& v, float* x) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = T::to_float(static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1))));
+    }
 };
 template <>
 struct Elem<F32> {
+    static constexpr int N = 4;
     __device__ static float get(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+    __device__ static void unpack(const u32x4& v, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = v[i];  // of the vector's element itself, bit_cast takes the first
+            x[i] = __builtin_bit_cast(float, w);
+        }
+    }
 };
+
+constexpr int kBatch = 16;  // logits a thread takes at a time
+
+template <typename T>
+struct Row {
+    static constexpr int N = Elem<T>::N, kPieces = kBatch / N;
+    const u32x4* pieces;
+    int lead, vocab, last;  // piece
+    __device__ Row(const void* logits, int64_t first, int64_t vocab_) {
+        constexpr int size = 16 / N;
+        const char* at = static_cast<const char*>(logits) + first * size;
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+        pieces = reinterpret_cast<const u32x4*>(at - off);
+        lead = off / size;
+        vocab = static_cast<int>(vocab_);
+        last = (vocab + lead - 1) / N;
+    }
+    // Batch k of a row is its elements k kThreads kBatch - lead on; element i of this thread's is element(k, i).
+    __device__ int element(int k, int i) const {
+        return (k * (kPieces * kThreads) + (i / N) * kThreads + static_cast<int>(threadIdx.x)) * N - lead + i % N;
+    }
+    __device__ void load(int k, u32x4* v) const {  // past the last piece, which is not used, the last
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) v[i] = pieces[min((k * kPieces + i) * kThreads + static_cast<int>(threadIdx.x), last)];
+    }
+    // -inf for what lies outside the row
+    __device__ void unpack(int k, const u32x4* v, float* x) const {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) Elem<T>::unpack(v[i], x + N * i);
+        if (k == 0 || (k + 1) * (kBatch * kThreads) - lead > vocab) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) x[i] = static_cast<unsigned>(element(k, i)) < static_cast<unsigned>(vocab) ? x[i] : -INFINITY;
+        }
+    }
+};
+
+// exp(d) for d <= 0 as p t: n = round(128 d / ln2), t = 2^(n / 128) from a table, with n / 128's whole part added to its
+// exponent, and a polynomial p of |r| <= ln2 / 256 (table-driven exp, Tang 1989), whose first term left out is below 2^-49. n
+// comes as the low bits of a sum with 1.5 * 2^52. Below -700 exp(d) counts as exp(-700), which is nothing beside 1. A table of
+// 32 entries, a copy in every pair of LDS banks, and one term more cost 10%: the arithmetic bounds this, not the table's reads.
+constexpr int kTable = 128;
+__device__ const double kPowers[kTable] = {  // 2^(i / 128)
+    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0, 0x1.059b0d3158574p+0,
+    0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0, 0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0,
+    0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0, 0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0,
+    0x1.15a98c8a58e51p+0, 0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
+    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0, 0x1.2387a6e756238p+0,
+    0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0, 0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0,
+    0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0, 0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0,
+    0x1.356c55f929ff1p+0, 0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
+    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0, 0x1.44e086061892dp+0,
+    0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0, 0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0,
+    0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0, 0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0,
+    0x1.58d12d497c7fdp+0, 0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
+    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0, 0x1.6a09e667f3bcdp+0,
+    0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0, 0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0,
+    0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0, 0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0,
+    0x1.80427543e1a12p+0, 0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0, 0x1.93737b0cdc5e5p+0,
+    0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0, 0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0,
+    0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0, 0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ac36bbfd3f37ap+0, 0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0, 0x1.c199bdd85529cp+0,
+    0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0, 0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0,
+    0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0, 0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0,
+    0x1.dd321f301b460p+0, 0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
+    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0, 0x1.f50765b6e4540p+0,
+    0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0,
+};
+__device__ inline void fill_table(double* table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = kPowers[threadIdx.x];
+}
+__device__ inline void exp_parts(double d, const double* table, double& p, double& t) {
+    constexpr double kMagic = 6755399441055744.0;
+    d = fmax(d, -700.0);
+    const double sum = fma(d, kTable * 1.4426950408889634, kMagic);
+    const double r = fma(sum - kMagic, -0.6931471805599453 / kTable, d);
+    p = fma(r, 1.0 / 24, 1.0 / 6);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0);
+    const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 bits = __builtin_bit_cast(u32x2, table[n & (kTable - 1)]);
+    bits.y += (n & ~(kTable - 1u)) << 13;
+    t = __builtin_bit_cast(double, bits);
+}
+__device__ inline double exp_of(double d, const double* table) {
+    double p, t;
+    exp_parts(d, table, p, t);
+    return p * t;
+}
 
 // (order of x, index) as one number whose maximum is torch.argmax's choice: the first largest, the first NaN if there is one.
 __device__ inline uint64_t rank_of(float x, uint32_t index) {
@@ -50,16 +155,19 @@ __device__ inline uint64_t wave_max64(uint64_t v) {
     for (int off = 32; off > 0; off >>= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), off, 64)));
     return v;
 }
-__device__ inline double wave_sum64(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-}
-
 struct Stat {
     uint64_t rank;  // of the largest logit
     double z;       // sum exp((x - largest) / T); 0 where the largest is no finite number
 };
+
+// Where a sequence's drafts end.
+struct Walk {
+    int kept;    // accepted drafts: the row that the next token comes from
+    int draft;   // that row's draft where it was turned down (w = max(p - q, 0)), else -1
+    Stat stat;   // of that row
+    double inv_z;
+};
+static_assert(sizeof(Stat) == 16 && sizeof(Walk) == 32, "as the workspace's size counts them");
 
 struct VerifyArgs {
     const void* logits;
@@ -71,229 +179,331 @@ struct VerifyArgs {
     int64_t* accepted;
     int64_t* tokens;
     int64_t vocab;
-    int drafts, chunks;
-    Stat* stats;   // [batch * (drafts + 1)][chunks]
-    double2* sums; // [batch][chunks]: of w and of p
+    int drafts, chunks, batches, row_batches;  // chunks a row, batches a chunk and a row
+    Stat* stats;    // [batch * (drafts + 1)][chunks]
+    double2* sums;  // [batch][row_batches]: of w and of p
+    Walk* walks;    // [batch]
 };
 
+// A chunk is a.batches batches. A thread goes through its own with its own running maximum, so that the block meets once, at
+// the end. Bound by fp64 arithmetic: about 20 instructions an element, 12 of them fp64.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a) {
+    __shared__ double table[kTable];
     __shared__ uint64_t ranks[kThreads / 64];
     __shared__ double zs[kThreads / 64];
+    __shared__ uint32_t index;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t row = blockIdx.x / a.chunks;
-    const int64_t base = static_cast<int64_t>(blockIdx.x - row * a.chunks) * kChunk;
-    float x[kPer];
-    uint64_t best = 0;
+    const int k0 = static_cast<int>(blockIdx.x - row * a.chunks) * a.batches;
+    const Row<T> src(a.logits, row * a.row_stride, a.vocab);
+    const int n = min(a.batches, a.row_batches - k0);
+    u32x4 v[Row<T>::kPieces];
+    src.load(k0, v);
+    fill_table(table);
+    if (t == 0) index = 0xFFFFFFFFu;
+    __syncthreads();
+    float m = -INFINITY, odd = 0.0f;  // odd: NaN where an element is no finite number
+    int found = k0;                   // the batch that m is of
+    double z = 0.0;
+    for (int k = 0; k < n; ++k) {
+        float x[kBatch];
+        src.unpack(k0 + k, v, x);
+        if (k + 1 < n) src.load(k0 + k + 1, v);
+        float top = x[0];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int64_t j = base + t + i * kThreads;
-        x[i] = j < a.vocab ? Elem<T>::get(a.logits, row * a.row_stride + j) : -INFINITY;
-        if (j < a.vocab) best = max(best, rank_of(x[i], static_cast<uint32_t>(j)));
+        for (int i = 0; i < kBatch; ++i) {
+            top = fmaxf(top, x[i]);
+            odd = fmaf(x[i], 0.0f, odd);
+        }
+        if (top > m) {
+            z *= exp_of((static_cast<double>(m) - top) * a.inv_t, table);
+            m = top;
+            found = k0 + k;
+        }
+        const double base = -static_cast<double>(m == -INFINITY ? 0.0f : m) * a.inv_t;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            double p, power;
+            exp_parts(fma(static_cast<double>(x[i]), a.inv_t, base), table, p, power);
+            z = fma(p, power, z);
+        }
     }
-    best = wave_max64(best);
+    // the largest of the block, and its first index: only threads that hold it look for it again, those with a NaN in all of
+    // their batches
+    float nan = m;
+    int nan_at = found;
+    if (odd != odd) {
+        for (int k = n - 1; k >= 0; --k) {
+            float x[kBatch];
+            src.load(k0 + k, v);
+            src.unpack(k0 + k, v, x);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (x[i] != x[i]) {
+                    nan = x[i];
+                    nan_at = k0 + k;
+                }
+        }
+    }
+    const uint64_t own = rank_of(nan, 0xFFFFFFFFu);
+    uint64_t best = wave_max64(own);
     if (lane == 0) ranks[wave] = best;
     __syncthreads();
     best = max(max(ranks[0], ranks[1]), max(ranks[2], ranks[3]));
-    const float m = rank_value(best);
-    double z = 0.0;
-    if (finite(m) && a.inv_t != 0.0) {
+    if (own == best) {
+        float x[kBatch];
+        src.load(nan_at, v);
+        src.unpack(nan_at, v, x);
+        uint32_t at = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) z += exp((static_cast<double>(x[i]) - m) * a.inv_t);
+        for (int i = kBatch - 1; i >= 0; --i) {
+            const int j = src.element(nan_at, i);
+            if (j >= 0 && j < src.vocab && rank_of(x[i], 0xFFFFFFFFu) == best) at = static_cast<uint32_t>(j);
+        }
+        if (at != 0xFFFFFFFFu) atomicMin(&index, at);
     }
-    z = wave_sum64(z);
+    const float top = rank_value(best);
+    z = finite(top) && m != -INFINITY ? z * exp_of((static_cast<double>(m) - top) * a.inv_t, table) : 0.0;
+    z = wave_total(z);
     if (lane == 0) zs[wave] = z;
     __syncthreads();
-    if (t == 0) a.stats[blockIdx.x] = Stat{best, (zs[0] + zs[1]) + (zs[2] + zs[3])};
+    if (t == 0) a.stats[blockIdx.x] = Stat{(best & ~uint64_t{0xFFFFFFFFu}) | static_cast<uint32_t>(~index), (zs[0] + zs[1]) + (zs[2] + zs[3])};
 }
 
-// A row's statistics from its chunks', in every lane of the wave that calls it.
-__device__ inline Stat join_row(const VerifyArgs& a, int64_t row, int lane) {
+// A row's statistics from its chunks', in the 16 lanes that call it together.
+__device__ inline Stat join_row(const VerifyArgs& a, int64_t row, const double* table) {
+    const int l = threadIdx.x & 15;
+    const Stat* stats = a.stats + row * a.chunks;
     uint64_t best = 0;
-    for (int c = lane; c < a.chunks; c += 64) best = max(best, a.stats[row * a.chunks + c].rank);
-    best = wave_max64(best);
+    for (int c = l; c < a.chunks; c += 16) best = max(best, stats[c].rank);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) best = max(best, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(best), off, 64)));
     const float m = rank_value(best);
     double z = 0.0;
     if (finite(m))
-        for (int c = lane; c < a.chunks; c += 64) {
-            const Stat s = a.stats[row * a.chunks + c];
+        for (int c = l; c < a.chunks; c += 16) {
+            const Stat s = stats[c];
             const float mc = rank_value(s.rank);
-            if (finite(mc)) z += s.z * exp((static_cast<double>(mc) - m) * a.inv_t);  // a chunk of -inf adds nothing
+            if (finite(mc)) z += s.z * exp_of((static_cast<double>(mc) - m) * a.inv_t, table);  // -inf adds nothing
         }
-    return Stat{best, wave_sum64(z)};
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) z += __shfl_xor(z, off, 64);
+    return Stat{best, z};
 }
 
-// Where a sequence's drafts end.
-struct Walk {
-    int kept;       // accepted drafts: the row that the next token comes from
-    bool less_q;    // that row's draft was turned down: w = max(p - q, 0)
-    Stat stat;      // of that row
-};
-
+// The whole block, 16 lanes a row, 16 rows at a time: the rows' tests do not wait for each other.
 template <typename T>
-__device__ Walk walk(const VerifyArgs& a, int64_t b) {
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    __shared__ int ends;  // 2 * row + (1: turned down)
-    if (t == 0) ends = 2 * a.drafts;
+__global__ __launch_bounds__(kThreads) void walk_kernel(const VerifyArgs a) {
+    __shared__ double table[kTable];
+    __shared__ int end;  // 2 * row + (1: turned down) of the first row that ends the drafts
+    __shared__ Stat stats[kThreads / 16];
+    const int t = threadIdx.x, group = t >> 4;
+    const int64_t b = blockIdx.x;
+    if (t == 0) end = INT32_MAX;
+    fill_table(table);
     __syncthreads();
-    for (int i = wave; i <= a.drafts; i += kThreads / 64) {
-        const int64_t row = b * (a.drafts + 1) + i;
-        if (i == a.drafts) break;
-        const int64_t x = a.draft[b * a.drafts + i];
-        if (x < 0 || x >= a.vocab) {
-            if (lane == 0) atomicMin(&ends, 2 * i);
-            break;
+    for (int i0 = 0;; i0 += kThreads / 16) {
+        const int i = i0 + group;
+        if (i <= a.drafts) {
+            const int64_t row = b * (a.drafts + 1) + i;
+            const int64_t x = i < a.drafts ? a.draft[b * a.drafts + i] : -1;
+            const bool real = x >= 0 && x < a.vocab;
+            const double u = a.uniforms[row];
+            const float logit = real ? Elem<T>::get(a.logits, row * a.row_stride + x) : 0.0f;
+            const float qx = real && a.draft_probs ? a.draft_probs[(b * a.drafts + i) * a.vocab + x] : 1.0f;
+            const Stat st = join_row(a, row, table);
+            const float m = rank_value(st.rank);
+            double p = 0.0;
+            if (a.inv_t == 0.0 || !finite(m)) p = finite(m) && rank_index(st.rank) == x ? 1.0 : 0.0;
+            else if (logit != -INFINITY) p = exp_of((static_cast<double>(logit) - m) * a.inv_t, table) / st.z;
+            const double q = a.inv_t != 0.0 ? qx : 1.0;
+            if ((t & 15) == 0) {
+                stats[group] = st;
+                if (!real) atomicMin(&end, 2 * i);
+                else if (!(u * q < p)) atomicMin(&end, 2 * i + 1);
+            }
         }
-        const Stat s = join_row(a, row, lane);
-        const float m = rank_value(s.rank);
-        double p = 0.0;
-        if (a.inv_t == 0.0 || !finite(m)) p = finite(m) && rank_index(s.rank) == x ? 1.0 : 0.0;
-        else p = exp((static_cast<double>(Elem<T>::get(a.logits, row * a.row_stride + x)) - m) * a.inv_t) / s.z;
-        const double q = a.draft_probs && a.inv_t != 0.0 ? a.draft_probs[(b * a.drafts + i) * a.vocab + x] : 1.0;
-        const double u = a.uniforms[b * (a.drafts + 1) + i];
-        if (!(u * q < p)) {
-            if (lane == 0) atomicMin(&ends, 2 * i + 1);
-            break;
-        }
+        __syncthreads();
+        if (end != INT32_MAX) break;  // the last row ends them at the latest
+        __syncthreads();
     }
-    __syncthreads();
-    Walk w;
-    w.kept = ends >> 1;
-    w.less_q = ends & 1;
-    w.stat = join_row(a, b * (a.drafts + 1) + w.kept, lane);
-    return w;
+    if (t == 0) {
+        const Stat st = stats[(end >> 1) % (kThreads / 16)];
+        const int64_t draft = end & 1 ? a.draft[b * a.drafts + (end >> 1)] : -1;
+        a.walks[b] = Walk{end >> 1, static_cast<int>(draft), st, 1.0 / st.z};
+    }
 }
 
-// p and w of token j.
+// w and p of an element x of the row where the drafts ended, q there.
+__device__ inline double2 weights(const VerifyArgs& a, const Walk& w, float x, double q, const double* table) {
+    const double p = x == -INFINITY ? 0.0 : exp_of((static_cast<double>(x) - rank_value(w.stat.rank)) * a.inv_t, table) * w.inv_z;
+    return double2{w.draft >= 0 ? (p > q ? p - q : 0.0) : p, p};
+}
+
+// q of a thread's batch: that of the drafter, or 1 at the draft x.
 template <typename T>
-__device__ inline double2 weights(const VerifyArgs& a, int64_t b, const Walk& w, int64_t j, int64_t x) {
-    const int64_t row = b * (a.drafts + 1) + w.kept;
-    const double p =
-        exp((static_cast<double>(Elem<T>::get(a.logits, row * a.row_stride + j)) - rank_value(w.stat.rank)) * a.inv_t) / w.stat.z;
-    if (!w.less_q) return double2{p, p};
-    const double q = a.draft_probs ? a.draft_probs[(b * a.drafts + w.kept) * a.vocab + j] : (j == x ? 1.0 : 0.0);
-    return double2{p > q ? p - q : 0.0, p};
+__device__ inline void batch_q(const Row<T>& src, const float* q, int x, int k, float* qv) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int j = src.element(k, i);
+        qv[i] = q ? q[min(max(j, 0), src.vocab - 1)] : j == x ? 1.0f : 0.0f;
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void chunk_sums_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(kThreads) void batch_sums_kernel(const VerifyArgs a) {
+    __shared__ double table[kTable];
     __shared__ double2 part[kThreads / 64];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int64_t b = blockIdx.x / a.chunks;
-    const int64_t base = static_cast<int64_t>(blockIdx.x - b * a.chunks) * kChunk;
-    const Walk w = walk<T>(a, b);
+    const int64_t b = blockIdx.x / a.row_batches;
+    const int k = static_cast<int>(blockIdx.x - b * a.row_batches);
+    const Walk w = a.walks[b];
+    fill_table(table);
+    __syncthreads();
     if (a.inv_t == 0.0 || !finite(rank_value(w.stat.rank))) return;  // the token is the argmax
-    const int64_t x = w.less_q ? a.draft[b * a.drafts + w.kept] : -1;
+    const Row<T> src(a.logits, (b * (a.drafts + 1) + w.kept) * a.row_stride, a.vocab);
+    const float* q = w.draft >= 0 && a.draft_probs ? a.draft_probs + (b * a.drafts + w.kept) * a.vocab : nullptr;
+    u32x4 v[Row<T>::kPieces];
+    float x16[kBatch], q16[kBatch];
+    src.load(k, v);
+    batch_q(src, q, w.draft, k, q16);
+    src.unpack(k, v, x16);
     double2 s = {0.0, 0.0};
-    for (int i = 0; i < kPer; ++i) {
-        const int64_t j = base + t + i * kThreads;
-        if (j >= a.vocab) break;
-        const double2 e = weights<T>(a, b, w, j, x);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const double2 e = weights(a, w, x16[i], q16[i], table);
         s.x += e.x;
         s.y += e.y;
     }
-    s.x = wave_sum64(s.x);
-    s.y = wave_sum64(s.y);
+    s.x = wave_total(s.x);
+    s.y = wave_total(s.y);
     if (lane == 0) part[wave] = s;
     __syncthreads();
     if (t == 0)
         a.sums[blockIdx.x] = double2{(part[0].x + part[1].x) + (part[2].x + part[3].x), (part[0].y + part[1].y) + (part[2].y + part[3].y)};
 }
 
+// The elements of a batch lie over the threads in runs of N, piece by piece: a running sum goes over the threads of a piece,
+// then on to the next.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pick_token_kernel(const VerifyArgs a) {
-    __shared__ int s_chunk, s_last;
-    __shared__ double s_left;
-    __shared__ int64_t s_index[2];
-    __shared__ double part[kThreads];
+    constexpr int N = Elem<T>::N, kPieces = Row<T>::kPieces, kWaves = kThreads / 64;
+    __shared__ double table[kTable];
+    __shared__ int s_batch, s_plain;
+    __shared__ double s_target, s_before;
+    __shared__ int s_first, s_last;
+    __shared__ double part[kPieces][kWaves];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t b = blockIdx.x;
-    const Walk w = walk<T>(a, b);
+    const Walk w = a.walks[b];
+    fill_table(table);
     int64_t token = rank_index(w.stat.rank);
     if (a.inv_t != 0.0 && finite(rank_value(w.stat.rank))) {
-        const double2* sums = a.sums + b * a.chunks;
+        const double2* sums = a.sums + b * a.row_batches;
         if (wave == 0) {
             double total = 0.0, total_p = 0.0;
-            for (int c = lane; c < a.chunks; c += 64) {
+            for (int c = lane; c < a.row_batches; c += 64) {
                 total += sums[c].x;
                 total_p += sums[c].y;
             }
-            total = wave_sum64(total);
-            total_p = wave_sum64(total_p);
-            const bool plain = !(total > 0.0);
+            total = wave_total(total);
+            total_p = wave_total(total_p);
+            const bool plain = !(total > 0.0);  // nothing left: the row itself
             const double target = a.uniforms[b * (a.drafts + 1) + a.drafts] * (plain ? total_p : total);
-            // the first chunk whose running sum passes the target; the last one with a positive sum where rounding hides it
-            double run = 0.0, left = 0.0;
-            int chunk = -1, last = 0;
-            for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
+            // the first part whose running sum passes the target; the last one with a positive sum where rounding hides it
+            double run = 0.0, before = 0.0;
+            int found = -1, last = 0;
+            for (int c0 = 0; c0 < a.row_batches && found < 0; c0 += 64) {
                 const int c = c0 + lane;
-                const double v = c < a.chunks ? (plain ? sums[c].y : sums[c].x) : 0.0;
-                double incl = v;
-#pragma unroll
-                for (int off = 1; off < 64; off <<= 1) {
-                    const double up = __shfl_up(incl, off, 64);
-                    if (lane >= off) incl += up;
-                }
+                const double v = c < a.row_batches ? (plain ? sums[c].y : sums[c].x) : 0.0;
+                const double incl = wave_scan(v);
                 const uint64_t pass = __ballot(v > 0.0 && run + incl > target);
                 const uint64_t some = __ballot(v > 0.0);
                 if (some) last = c0 + 63 - __builtin_clzll(some);
                 if (pass) {
                     const int at = __builtin_ctzll(pass);
-                    chunk = c0 + at;
-                    left = target - (run + __shfl(incl - v, at, 64));
+                    found = c0 + at;
+                    before = run + read_lane(incl - v, __builtin_amdgcn_readfirstlane(at));
                 }
-                run += __shfl(incl, 63, 64);
+                run += read_lane(incl, 63);
             }
             if (lane == 0) {
-                s_chunk = chunk < 0 ? last : chunk;
-                s_left = chunk < 0 ? INFINITY : left;
-                s_last = plain;
+                s_batch = found < 0 ? last : found;
+                s_target = found < 0 ? INFINITY : target;
+                s_before = before;
+                s_plain = plain;
+                s_first = INT32_MAX;  // the first index that passes
+                s_last = -1;          // the last one with a positive weight
             }
         }
-        if (t == 0) {
-            s_index[0] = INT64_MAX;  // the first index that passes
-            s_index[1] = -1;         // the last one with a positive weight
-        }
         __syncthreads();
-        const bool plain = s_last;
-        const int64_t x = w.less_q ? a.draft[b * a.drafts + w.kept] : -1;
-        const int64_t base = static_cast<int64_t>(s_chunk) * kChunk + t * kPer;
-        double v[kPer], sum = 0.0;
-        for (int i = 0; i < kPer; ++i) {
-            v[i] = 0.0;
-            if (base + i < a.vocab) {
-                const double2 e = weights<T>(a, b, w, base + i, x);
-                v[i] = plain ? e.y : e.x;
+        const bool plain = s_plain;
+        const double target = s_target;
+        const int k = s_batch;
+        const Row<T> src(a.logits, (b * (a.drafts + 1) + w.kept) * a.row_stride, a.vocab);
+        const float* q = w.draft >= 0 && a.draft_probs ? a.draft_probs + (b * a.drafts + w.kept) * a.vocab : nullptr;
+        u32x4 v[kPieces];
+        float x16[kBatch], q16[kBatch];
+        src.load(k, v);
+        batch_q(src, q, w.draft, k, q16);
+        src.unpack(k, v, x16);
+        double weight[kBatch], sum[kPieces], incl[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            sum[i] = 0.0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double2 both = weights(a, w, x16[N * i + e], q16[N * i + e], table);
+                weight[N * i + e] = plain ? both.y : both.x;
+                sum[i] += weight[N * i + e];
             }
-            sum += v[i];
+            incl[i] = wave_scan(sum[i]);
+            if (lane == 63) part[i][wave] = incl[i];
         }
-        part[t] = sum;
         __syncthreads();
-        double run = 0.0;
-        for (int i = 0; i < t; ++i) run += part[i];
-        int64_t first = INT64_MAX, last = -1;
-        for (int i = 0; i < kPer; ++i) {
-            run += v[i];
-            if (v[i] > 0.0) {
-                last = base + i;
-                if (run > s_left && first == INT64_MAX) first = base + i;
+        double before = s_before;
+        int first = INT32_MAX, last = -1;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            double run = before + (incl[i] - sum[i]);
+#pragma unroll
+            for (int o = 0; o < kWaves; ++o) {
+                const double whole = part[i][o];
+                run += o < wave ? whole : 0.0;
+                before += whole;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                run += weight[N * i + e];
+                if (weight[N * i + e] > 0.0) {
+                    last = src.element(k, N * i + e);
+                    if (run > target) first = min(first, last);
+                }
             }
         }
-        atomicMin(reinterpret_cast<unsigned long long*>(&s_index[0]), static_cast<unsigned long long>(first));
-        if (last >= 0) atomicMax(reinterpret_cast<long long*>(&s_index[1]), static_cast<long long>(last));
+        if (first != INT32_MAX) atomicMin(&s_first, first);
+        if (last >= 0) atomicMax(&s_last, last);
         __syncthreads();
-        token = s_index[0] != INT64_MAX ? s_index[0] : s_index[1];
+        token = s_first != INT32_MAX ? s_first : s_last;
     }
     if (t == 0) a.accepted[b] = w.kept;
     for (int i = t; i <= a.drafts; i += kThreads)
         a.tokens[b * (a.drafts + 1) + i] = i < w.kept ? a.draft[b * a.drafts + i] : (i == w.kept ? token : -1);
 }
 
+// Batches of a row, which may begin up to 7 elements into its first piece, and of a chunk: one, or four where there are chunks
+// enough to fill the card, for a block's fixed part (its table, reductions of 64-bit numbers) costs as much as half a batch.
+int64_t row_batches_of(int64_t vocab) { return ceil_div(vocab + 7, kBatch * kThreads); }
+int64_t batches_of(int64_t rows, int64_t vocab) { return rows * row_batches_of(vocab) >= 4096 ? 4 : 1; }
+int64_t chunks_of(int64_t rows, int64_t vocab) { return ceil_div(row_batches_of(vocab), batches_of(rows, vocab)); }
+
 template <typename T>
 void launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t st) {
     const int64_t rows = batch * (a.drafts + 1);
     row_stats_kernel<T><<<dim3(static_cast<unsigned>(rows * a.chunks)), kThreads, 0, st>>>(a);
-    chunk_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.chunks)), kThreads, 0, st>>>(a);
+    walk_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
+    batch_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.row_batches)), kThreads, 0, st>>>(a);
     pick_token_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
 }
 
@@ -305,10 +515,11 @@ using namespace nq;
 extern "C" {
 
 size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab) {
-    if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > INT32_MAX || batch > INT32_MAX || drafts > INT32_MAX / 2) return 0;
-    const int64_t chunks = ceil_div(vocab, kChunk);
-    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks) return 0;  // blocks of 256 threads
-    return static_cast<size_t>(batch) * (drafts + 2) * chunks * 16;
+    if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > (1 << 30) || batch > INT32_MAX || drafts > INT32_MAX / 2) return 0;
+    if (batch > (int64_t{1} << 23) / (drafts + 1)) return 0;
+    const int64_t chunks = chunks_of(batch * (drafts + 1), vocab);
+    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks || batch > (int64_t{1} << 23) / row_batches_of(vocab)) return 0;  // blocks of 256 threads
+    return static_cast<size_t>(batch) * (((drafts + 1) * chunks + row_batches_of(vocab)) * 16 + 32);
 }
 
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
@@ -341,9 +552,12 @@ int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const in
     a.tokens = tokens;
     a.vocab = vocab;
     a.drafts = static_cast<int>(drafts);
-    a.chunks = static_cast<int>(ceil_div(vocab, kChunk));
+    a.chunks = static_cast<int>(chunks_of(batch * (drafts + 1), vocab));
+    a.batches = static_cast<int>(batches_of(batch * (drafts + 1), vocab));
+    a.row_batches = static_cast<int>(row_batches_of(vocab));
     a.stats = static_cast<Stat*>(workspace);
     a.sums = reinterpret_cast<double2*>(a.stats + batch * (drafts + 1) * a.chunks);
+    a.walks = reinterpret_cast<Walk*>(a.sums + batch * a.row_batches);
     if (dtype == NQ_F16) launch_verify<F16>(a, batch, as_stream(stream));
     else if (dtype == NQ_BF16) launch_verify<BF16>(a, batch, as_stream(stream));
     else launch_verify<F32>(a, batch, as_stream(stream));

@@ -1,0 +1,48 @@
+// Reductions and scans over a wave without LDS: a ds_bpermute (what __shfl compiles to) takes over a hundred cycles on a
+// chain of dependent steps, these a few each.
+#pragma once
+
+#include "nq_common.h"
+
+namespace nq {
+
+// Largest over lanes l, l ^ 16, l ^ 32 and l ^ 48; over l and l ^ 32.
+__device__ inline float max_xor32(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // {low half twice, high half twice}
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ inline float max_xor16(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);  // the even rows of 16 lanes twice, the odd ones twice
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+
+// v of the lane that a DPP control names, 0 where there is none or the row is masked out.
+template <int kControl, int kRows>
+__device__ inline double dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u), kControl, kRows, 0xF, false));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kControl, kRows, 0xF, false));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Inclusive running sum over the lanes: shifts within rows of 16, then each row's last lane to the rows behind it.
+__device__ inline double wave_scan(double v) {
+    v += dpp<0x111, 0xF>(v);  // row_shr:1
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    v += dpp<0x118, 0xF>(v);
+    v += dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ inline double read_lane(double v, int lane) {  // the same lane for the whole wave
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), lane));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ inline double wave_total(double v) { return read_lane(wave_scan(v), 63); }
+
+}  // namespace nq
