@@ -3,7 +3,7 @@
 //   1. row_stats_kernel, a block per (row, chunk of 4096 or 16384 logits): the chunk's largest logit m_c (with its index) and
 //      z_c = sum exp((x - m_c) / T);
 //   2. walk_kernel, a block per sequence: joins its rows' statistics and makes the accept tests u q(x) < p(x);
-//   3. batch_sums_kernel, a block per (sequence, 4096 logits): the sums of w = max(p - q, 0) and of p over its part of the row
+//   3. part_sums_kernel, a block per (sequence, 4096 logits): the sums of w = max(p - q, 0) and of p over its part of the row
 //      that the tests ended at;
 //   4. pick_token_kernel, a block per sequence: the part in which the running sum of w passes u times its total, then the
 //      index within it.
@@ -44,7 +44,8 @@ struct Elem<F32> {
     }
 };
 
-constexpr int kBatch = 16;  // logits a thread takes at a time
+constexpr int kPart = 4096;             // logits a block takes at a time
+constexpr int kBatch = kPart / kThreads;  // and a thread of row_stats_kernel's
 
 template <typename T>
 struct Row {
@@ -60,7 +61,7 @@ struct Row {
         vocab = static_cast<int>(vocab_);
         last = (vocab + lead - 1) / N;
     }
-    // Batch k of a row is its elements k kThreads kBatch - lead on; element i of this thread's is element(k, i).
+    // Part k of a row is its elements k kPart - lead on; element i of this thread's is element(k, i).
     __device__ int element(int k, int i) const {
         return (k * (kPieces * kThreads) + (i / N) * kThreads + static_cast<int>(threadIdx.x)) * N - lead + i % N;
     }
@@ -150,11 +151,6 @@ __device__ inline float rank_value(uint64_t r) {
 }
 __device__ inline bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-__device__ inline uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), off, 64)));
-    return v;
-}
 struct Stat {
     uint64_t rank;  // of the largest logit
     double z;       // sum exp((x - largest) / T); 0 where the largest is no finite number
@@ -179,13 +175,13 @@ struct VerifyArgs {
     int64_t* accepted;
     int64_t* tokens;
     int64_t vocab;
-    int drafts, chunks, batches, row_batches;  // chunks a row, batches a chunk and a row
+    int drafts, chunks, parts, row_parts;  // chunks a row, parts a chunk and a row
     Stat* stats;    // [batch * (drafts + 1)][chunks]
-    double2* sums;  // [batch][row_batches]: of w and of p
+    double2* sums;  // [batch][row_parts]: of w and of p
     Walk* walks;    // [batch]
 };
 
-// A chunk is a.batches batches. A thread goes through its own with its own running maximum, so that the block meets once, at
+// A chunk is a.parts parts. A thread goes through its own with its own running maximum, so that the block meets once, at
 // the end. Bound by fp64 arithmetic: about 20 instructions an element, 12 of them fp64.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a) {
@@ -195,16 +191,16 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
     __shared__ uint32_t index;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t row = blockIdx.x / a.chunks;
-    const int k0 = static_cast<int>(blockIdx.x - row * a.chunks) * a.batches;
+    const int k0 = static_cast<int>(blockIdx.x - row * a.chunks) * a.parts;
     const Row<T> src(a.logits, row * a.row_stride, a.vocab);
-    const int n = min(a.batches, a.row_batches - k0);
+    const int n = min(a.parts, a.row_parts - k0);
     u32x4 v[Row<T>::kPieces];
     src.load(k0, v);
     fill_table(table);
     if (t == 0) index = 0xFFFFFFFFu;
     __syncthreads();
     float m = -INFINITY, odd = 0.0f;  // odd: NaN where an element is no finite number
-    int found = k0;                   // the batch that m is of
+    int found = k0;                   // the part that m is of
     double z = 0.0;
     for (int k = 0; k < n; ++k) {
         float x[kBatch];
@@ -230,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
         }
     }
     // the largest of the block, and its first index: only threads that hold it look for it again, those with a NaN in all of
-    // their batches
+    // their parts
     float nan = m;
     int nan_at = found;
     if (odd != odd) {
@@ -247,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
         }
     }
     const uint64_t own = rank_of(nan, 0xFFFFFFFFu);
-    uint64_t best = wave_max64(own);
+    uint64_t best = wave_largest(own);
     if (lane == 0) ranks[wave] = best;
     __syncthreads();
     best = max(max(ranks[0], ranks[1]), max(ranks[2], ranks[3]));
@@ -335,101 +331,127 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(const VerifyArgs a) {
     }
 }
 
-// w and p of an element x of the row where the drafts ended, q there.
-__device__ inline double2 weights(const VerifyArgs& a, const Walk& w, float x, double q, const double* table) {
-    const double p = x == -INFINITY ? 0.0 : exp_of((static_cast<double>(x) - rank_value(w.stat.rank)) * a.inv_t, table) * w.inv_z;
-    return double2{w.draft >= 0 ? (p > q ? p - q : 0.0) : p, p};
-}
-
-// q of a thread's batch: that of the drafter, or 1 at the draft x.
+// A part of a row, a piece a thread of 4096 / N: its p and w.
 template <typename T>
-__device__ inline void batch_q(const Row<T>& src, const float* q, int x, int k, float* qv) {
+struct Part {
+    static constexpr int N = Elem<T>::N, kThreads = kPart / N;
+    int first;  // the piece's first element
+    double p[N], w[N];
+    __device__ Part(const VerifyArgs& a, int64_t b, int part, const Walk& walk, const double* table) {
+        const Row<T> src(a.logits, (b * (a.drafts + 1) + walk.kept) * a.row_stride, a.vocab);
+        const int piece = part * kThreads + static_cast<int>(threadIdx.x);
+        first = piece * N - src.lead;
+        const u32x4 v = src.pieces[min(piece, src.last)];
+        float x[N], q[N];
+        const bool inside = first >= 0 && first + N <= src.vocab;
+        if (walk.draft >= 0 && a.draft_probs) {
+            const float* row = a.draft_probs + (b * a.drafts + walk.kept) * a.vocab;
+            typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));  // any row begins at a multiple of 4 bytes
+            if (inside) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        const int j = src.element(k, i);
-        qv[i] = q ? q[min(max(j, 0), src.vocab - 1)] : j == x ? 1.0f : 0.0f;
+                for (int i = 0; i < N; i += 4) {
+                    const f32x4a four = *reinterpret_cast<const f32x4a*>(row + first + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[i + e] = four[e];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) q[i] = row[min(max(first + i, 0), src.vocab - 1)];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) q[i] = first + i == walk.draft ? 1.0f : 0.0f;
+        }
+        Elem<T>::unpack(v, x);
+        const double top = rank_value(walk.stat.rank);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool none = x[i] == -INFINITY || !(inside || static_cast<unsigned>(first + i) < static_cast<unsigned>(src.vocab));
+            p[i] = none ? 0.0 : exp_of((static_cast<double>(x[i]) - top) * a.inv_t, table) * walk.inv_z;
+            w[i] = walk.draft >= 0 ? (p[i] > q[i] ? p[i] - q[i] : 0.0) : p[i];
+        }
     }
-}
+};
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void batch_sums_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(Part<T>::kThreads) void part_sums_kernel(const VerifyArgs a) {
+    constexpr int kWaves = Part<T>::kThreads / 64;
     __shared__ double table[kTable];
-    __shared__ double2 part[kThreads / 64];
+    __shared__ double2 sums[kWaves];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int64_t b = blockIdx.x / a.row_batches;
-    const int k = static_cast<int>(blockIdx.x - b * a.row_batches);
-    const Walk w = a.walks[b];
+    const int64_t b = blockIdx.x / a.row_parts;
+    const Walk walk = a.walks[b];
     fill_table(table);
     __syncthreads();
-    if (a.inv_t == 0.0 || !finite(rank_value(w.stat.rank))) return;  // the token is the argmax
-    const Row<T> src(a.logits, (b * (a.drafts + 1) + w.kept) * a.row_stride, a.vocab);
-    const float* q = w.draft >= 0 && a.draft_probs ? a.draft_probs + (b * a.drafts + w.kept) * a.vocab : nullptr;
-    u32x4 v[Row<T>::kPieces];
-    float x16[kBatch], q16[kBatch];
-    src.load(k, v);
-    batch_q(src, q, w.draft, k, q16);
-    src.unpack(k, v, x16);
+    if (a.inv_t == 0.0 || !finite(rank_value(walk.stat.rank))) return;  // the token is the argmax
+    const Part<T> part(a, b, static_cast<int>(blockIdx.x - b * a.row_parts), walk, table);
     double2 s = {0.0, 0.0};
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        const double2 e = weights(a, w, x16[i], q16[i], table);
-        s.x += e.x;
-        s.y += e.y;
+    for (int i = 0; i < Part<T>::N; ++i) {
+        s.x += part.w[i];
+        s.y += part.p[i];
     }
     s.x = wave_total(s.x);
     s.y = wave_total(s.y);
-    if (lane == 0) part[wave] = s;
+    if (lane == 0) sums[wave] = s;
     __syncthreads();
-    if (t == 0)
-        a.sums[blockIdx.x] = double2{(part[0].x + part[1].x) + (part[2].x + part[3].x), (part[0].y + part[1].y) + (part[2].y + part[3].y)};
+    if (t == 0) {
+        for (int i = 1; i < kWaves; ++i) {
+            s.x += sums[i].x;
+            s.y += sums[i].y;
+        }
+        a.sums[blockIdx.x] = s;
+    }
 }
 
-// The elements of a batch lie over the threads in runs of N, piece by piece: a running sum goes over the threads of a piece,
-// then on to the next.
+// Bound by latency: what does not depend on the walk is loaded with it.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void pick_token_kernel(const VerifyArgs a) {
-    constexpr int N = Elem<T>::N, kPieces = Row<T>::kPieces, kWaves = kThreads / 64;
+__global__ __launch_bounds__(Part<T>::kThreads) void pick_token_kernel(const VerifyArgs a) {
+    constexpr int N = Elem<T>::N, kThreads = Part<T>::kThreads, kWaves = kThreads / 64;
     __shared__ double table[kTable];
-    __shared__ int s_batch, s_plain;
+    __shared__ int s_part, s_plain;
     __shared__ double s_target, s_before;
     __shared__ int s_first, s_last;
-    __shared__ double part[kPieces][kWaves];
+    __shared__ double sums_of[kWaves];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t b = blockIdx.x;
-    const Walk w = a.walks[b];
+    const double2* sums = a.sums + b * a.row_parts;
+    const double2 own = wave == 0 && lane < a.row_parts ? sums[lane] : double2{0.0, 0.0};
+    const double u = a.uniforms[b * (a.drafts + 1) + a.drafts];
+    const int64_t draft = t < a.drafts ? a.draft[b * a.drafts + t] : -1;
+    const Walk walk = a.walks[b];
     fill_table(table);
-    int64_t token = rank_index(w.stat.rank);
-    if (a.inv_t != 0.0 && finite(rank_value(w.stat.rank))) {
-        const double2* sums = a.sums + b * a.row_batches;
+    int64_t token = rank_index(walk.stat.rank);
+    if (a.inv_t != 0.0 && finite(rank_value(walk.stat.rank))) {
         if (wave == 0) {
-            double total = 0.0, total_p = 0.0;
-            for (int c = lane; c < a.row_batches; c += 64) {
+            double total = own.x, total_p = own.y;
+            for (int c = lane + 64; c < a.row_parts; c += 64) {
                 total += sums[c].x;
                 total_p += sums[c].y;
             }
             total = wave_total(total);
             total_p = wave_total(total_p);
             const bool plain = !(total > 0.0);  // nothing left: the row itself
-            const double target = a.uniforms[b * (a.drafts + 1) + a.drafts] * (plain ? total_p : total);
+            const double target = u * (plain ? total_p : total);
             // the first part whose running sum passes the target; the last one with a positive sum where rounding hides it
             double run = 0.0, before = 0.0;
             int found = -1, last = 0;
-            for (int c0 = 0; c0 < a.row_batches && found < 0; c0 += 64) {
-                const int c = c0 + lane;
-                const double v = c < a.row_batches ? (plain ? sums[c].y : sums[c].x) : 0.0;
+            for (int c0 = 0; c0 < a.row_parts && found < 0; c0 += 64) {
+                const double2 both = c0 == 0 ? own : c0 + lane < a.row_parts ? sums[c0 + lane] : double2{0.0, 0.0};
+                const double v = plain ? both.y : both.x;
                 const double incl = wave_scan(v);
                 const uint64_t pass = __ballot(v > 0.0 && run + incl > target);
                 const uint64_t some = __ballot(v > 0.0);
                 if (some) last = c0 + 63 - __builtin_clzll(some);
                 if (pass) {
-                    const int at = __builtin_ctzll(pass);
+                    const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(pass));
                     found = c0 + at;
-                    before = run + read_lane(incl - v, __builtin_amdgcn_readfirstlane(at));
+                    before = run + read_lane(incl - v, at);
                 }
                 run += read_lane(incl, 63);
             }
             if (lane == 0) {
-                s_batch = found < 0 ? last : found;
+                s_part = found < 0 ? last : found;
                 s_target = found < 0 ? INFINITY : target;
                 s_before = before;
                 s_plain = plain;
@@ -440,71 +462,51 @@ __global__ __launch_bounds__(kThreads) void pick_token_kernel(const VerifyArgs a
         __syncthreads();
         const bool plain = s_plain;
         const double target = s_target;
-        const int k = s_batch;
-        const Row<T> src(a.logits, (b * (a.drafts + 1) + w.kept) * a.row_stride, a.vocab);
-        const float* q = w.draft >= 0 && a.draft_probs ? a.draft_probs + (b * a.drafts + w.kept) * a.vocab : nullptr;
-        u32x4 v[kPieces];
-        float x16[kBatch], q16[kBatch];
-        src.load(k, v);
-        batch_q(src, q, w.draft, k, q16);
-        src.unpack(k, v, x16);
-        double weight[kBatch], sum[kPieces], incl[kPieces];
+        const Part<T> part(a, b, s_part, walk, table);
+        double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            sum[i] = 0.0;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const double2 both = weights(a, w, x16[N * i + e], q16[N * i + e], table);
-                weight[N * i + e] = plain ? both.y : both.x;
-                sum[i] += weight[N * i + e];
-            }
-            incl[i] = wave_scan(sum[i]);
-            if (lane == 63) part[i][wave] = incl[i];
-        }
+        for (int i = 0; i < N; ++i) sum += plain ? part.p[i] : part.w[i];
+        const double incl = wave_scan(sum);
+        if (lane == 63) sums_of[wave] = incl;
         __syncthreads();
-        double before = s_before;
+        double run = s_before + wave_total(lane < wave ? sums_of[lane % kWaves] : 0.0) + (incl - sum);
         int first = INT32_MAX, last = -1;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            double run = before + (incl[i] - sum[i]);
-#pragma unroll
-            for (int o = 0; o < kWaves; ++o) {
-                const double whole = part[i][o];
-                run += o < wave ? whole : 0.0;
-                before += whole;
-            }
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                run += weight[N * i + e];
-                if (weight[N * i + e] > 0.0) {
-                    last = src.element(k, N * i + e);
-                    if (run > target) first = min(first, last);
-                }
+        for (int i = 0; i < N; ++i) {
+            const double weight = plain ? part.p[i] : part.w[i];
+            run += weight;
+            if (weight > 0.0) {
+                last = part.first + i;
+                if (run > target) first = min(first, last);
             }
         }
-        if (first != INT32_MAX) atomicMin(&s_first, first);
-        if (last >= 0) atomicMax(&s_last, last);
+        // of a wave its first lane that passes and its last one with a weight
+        const uint64_t passes = __ballot(first != INT32_MAX), some = __ballot(last >= 0);
+        if (passes && lane == __builtin_ctzll(passes)) atomicMin(&s_first, first);
+        if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&s_last, last);
         __syncthreads();
         token = s_first != INT32_MAX ? s_first : s_last;
     }
-    if (t == 0) a.accepted[b] = w.kept;
-    for (int i = t; i <= a.drafts; i += kThreads)
-        a.tokens[b * (a.drafts + 1) + i] = i < w.kept ? a.draft[b * a.drafts + i] : (i == w.kept ? token : -1);
+    if (t == 0) a.accepted[b] = walk.kept;
+    for (int i = t; i <= a.drafts; i += kThreads) {
+        const int64_t kept = i == t ? draft : a.draft[b * a.drafts + min(i, a.drafts - 1)];
+        a.tokens[b * (a.drafts + 1) + i] = i < walk.kept ? kept : (i == walk.kept ? token : -1);
+    }
 }
 
-// Batches of a row, which may begin up to 7 elements into its first piece, and of a chunk: one, or four where there are chunks
-// enough to fill the card, for a block's fixed part (its table, reductions of 64-bit numbers) costs as much as half a batch.
-int64_t row_batches_of(int64_t vocab) { return ceil_div(vocab + 7, kBatch * kThreads); }
-int64_t batches_of(int64_t rows, int64_t vocab) { return rows * row_batches_of(vocab) >= 4096 ? 4 : 1; }
-int64_t chunks_of(int64_t rows, int64_t vocab) { return ceil_div(row_batches_of(vocab), batches_of(rows, vocab)); }
+// Parts of a row, which may begin up to 7 elements into its first piece, and of a chunk: one, or four where there are chunks
+// enough to fill the card, for a block's fixed part (its table, reductions of 64-bit numbers) costs as much as half a part.
+int64_t row_parts_of(int64_t vocab) { return ceil_div(vocab + 7, kBatch * kThreads); }
+int64_t parts_of(int64_t rows, int64_t vocab) { return rows * row_parts_of(vocab) >= 4096 ? 4 : 1; }
+int64_t chunks_of(int64_t rows, int64_t vocab) { return ceil_div(row_parts_of(vocab), parts_of(rows, vocab)); }
 
 template <typename T>
 void launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t st) {
     const int64_t rows = batch * (a.drafts + 1);
     row_stats_kernel<T><<<dim3(static_cast<unsigned>(rows * a.chunks)), kThreads, 0, st>>>(a);
     walk_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
-    batch_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.row_batches)), kThreads, 0, st>>>(a);
-    pick_token_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
+    part_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.row_parts)), Part<T>::kThreads, 0, st>>>(a);
+    pick_token_kernel<T><<<dim3(static_cast<unsigned>(batch)), Part<T>::kThreads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -518,8 +520,8 @@ size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
     if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > (1 << 30) || batch > INT32_MAX || drafts > INT32_MAX / 2) return 0;
     if (batch > (int64_t{1} << 23) / (drafts + 1)) return 0;
     const int64_t chunks = chunks_of(batch * (drafts + 1), vocab);
-    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks || batch > (int64_t{1} << 23) / row_batches_of(vocab)) return 0;  // blocks of 256 threads
-    return static_cast<size_t>(batch) * (((drafts + 1) * chunks + row_batches_of(vocab)) * 16 + 32);
+    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks || batch > (int64_t{1} << 23) / row_parts_of(vocab)) return 0;  // blocks of 256 threads
+    return static_cast<size_t>(batch) * (((drafts + 1) * chunks + row_parts_of(vocab)) * 16 + 32);
 }
 
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
@@ -553,11 +555,11 @@ int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const in
     a.vocab = vocab;
     a.drafts = static_cast<int>(drafts);
     a.chunks = static_cast<int>(chunks_of(batch * (drafts + 1), vocab));
-    a.batches = static_cast<int>(batches_of(batch * (drafts + 1), vocab));
-    a.row_batches = static_cast<int>(row_batches_of(vocab));
+    a.parts = static_cast<int>(parts_of(batch * (drafts + 1), vocab));
+    a.row_parts = static_cast<int>(row_parts_of(vocab));
     a.stats = static_cast<Stat*>(workspace);
     a.sums = reinterpret_cast<double2*>(a.stats + batch * (drafts + 1) * a.chunks);
-    a.walks = reinterpret_cast<Walk*>(a.sums + batch * a.row_batches);
+    a.walks = reinterpret_cast<Walk*>(a.sums + batch * a.row_parts);
     if (dtype == NQ_F16) launch_verify<F16>(a, batch, as_stream(stream));
     else if (dtype == NQ_BF16) launch_verify<BF16>(a, batch, as_stream(stream));
     else launch_verify<F32>(a, batch, as_stream(stream));

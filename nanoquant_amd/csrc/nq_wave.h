@@ -18,13 +18,16 @@ __device__ inline float max_xor16(float v) {
     return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 
-// v of the lane that a DPP control names, 0 where there is none or the row is masked out.
+// u of the lane that a DPP control names, 0 where there is none or the row is masked out.
 template <int kControl, int kRows>
-__device__ inline double dpp(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+__device__ inline uint64_t dpp(uint64_t u) {
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u), kControl, kRows, 0xF, false));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kControl, kRows, 0xF, false));
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+template <int kControl, int kRows>
+__device__ inline double dpp(double v) {
+    return __builtin_bit_cast(double, dpp<kControl, kRows>(__builtin_bit_cast(uint64_t, v)));
 }
 
 // Inclusive running sum over the lanes: shifts within rows of 16, then each row's last lane to the rows behind it.
@@ -37,11 +40,23 @@ __device__ inline double wave_scan(double v) {
     v += dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
-__device__ inline double read_lane(double v, int lane) {  // the same lane for the whole wave
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+__device__ inline uint64_t read_lane(uint64_t u, int lane) {  // the same lane for the whole wave
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), lane));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ inline double read_lane(double v, int lane) {
+    return __builtin_bit_cast(double, read_lane(__builtin_bit_cast(uint64_t, v), lane));
+}
+__device__ inline uint64_t wave_largest(uint64_t v) {
+    auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+    v = larger(v, dpp<0x111, 0xF>(v));
+    v = larger(v, dpp<0x112, 0xF>(v));
+    v = larger(v, dpp<0x114, 0xF>(v));
+    v = larger(v, dpp<0x118, 0xF>(v));
+    v = larger(v, dpp<0x142, 0xA>(v));
+    v = larger(v, dpp<0x143, 0xC>(v));
+    return read_lane(v, 63);
 }
 __device__ inline double wave_total(double v) { return read_lane(wave_scan(v), 63); }
 
