@@ -118,7 +118,9 @@ SIGNATURES = {
 
 # The functions that libnq_ops.so (the torch operators) calls, in the order of its nq_ops_bind.
 OPS_FUNCTIONS = ("nq_gemv_workspace_bytes", "nq_gemv", "nq_gemm_onebit_workspace_bytes", "nq_gemm_onebit",
-                 "nq_gemm_nanoquant_workspace_bytes", "nq_gemm_nanoquant")
+                 "nq_gemm_nanoquant_workspace_bytes", "nq_gemm_nanoquant", "nq_paged_rope_write",
+                 "nq_paged_attention_workspace_bytes", "nq_paged_attention", "nq_verify_drafts_workspace_bytes",
+                 "nq_verify_drafts")
 
 _lock = threading.Lock()
 _lib = None

@@ -15,6 +15,7 @@
 #include <torch/library.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "../../../include/nq_hip.h"
 
@@ -31,8 +32,13 @@ struct Library {
     decltype(&nq_gemm_onebit) onebit;
     decltype(&nq_gemm_nanoquant_workspace_bytes) nanoquant_bytes;
     decltype(&nq_gemm_nanoquant) nanoquant;
+    decltype(&nq_paged_rope_write) paged_write;
+    decltype(&nq_paged_attention_workspace_bytes) paged_attention_bytes;
+    decltype(&nq_paged_attention) paged_attention;
+    decltype(&nq_verify_drafts_workspace_bytes) verify_bytes;
+    decltype(&nq_verify_drafts) verify;
 };
-constexpr int kFunctions = 6;
+constexpr int kFunctions = 11;
 std::atomic<const Library*> g_library{nullptr};
 
 int dtype_code(at::ScalarType t) { return t == at::kHalf ? NQ_F16 : NQ_BF16; }
@@ -152,6 +158,114 @@ Tensor nanoquant(const Tensor& x, const Tensor& v_words, const Tensor& u_words, 
     return op.call(x, v_words, u_words, s_g, s_l, s_h, workspace);
 }
 
+// The paged cache's operators (nanoquant_amd/serve.py): the well-formed calls on memory that the kernels read where it lies.
+// For any other call they give nothing, and the function in Python goes on to check it, to lay tensors out or to run torch ops.
+
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+// Elements between the rows of x [batch, tokens, width], 0 where a kernel cannot read them.
+int64_t row_stride(const Tensor& x, int64_t batch, int64_t tokens) {
+    const int64_t width = x.size(2), stride = tokens > 1 ? x.stride(1) : batch > 1 ? x.stride(0) : width;
+    const bool fits = x.stride(2) == 1 && stride % 8 == 0 && stride >= width && aligned16(x) &&
+                      (tokens == 1 || batch == 1 || x.stride(0) == tokens * stride);
+    return fits ? stride : 0;
+}
+
+// The pool [pages, kv_heads, page_size, head_dim], the table and the positions of a call whose tokens are like q.
+bool pages_ok(const Library* lib, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+              const Tensor& positions) {
+    if (!lib || !q.is_cuda() || (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) || q.dim() != 3 ||
+        q.numel() == 0 || k_pages.dim() != 4 || k_pages.numel() == 0 || table.dim() != 2 || positions.dim() != 2)
+        return false;
+    const int64_t width = k_pages.size(1) * k_pages.size(3);
+    return plain(k_pages, q, q.scalar_type()) && plain(v_pages, q, q.scalar_type()) && k_pages.sizes() == v_pages.sizes() &&
+           aligned16(k_pages) && aligned16(v_pages) && plain(positions, q, at::kLong) && positions.size(0) == q.size(0) &&
+           positions.size(1) == q.size(1) && q.size(2) % width == 0 && table.device() == q.device() &&
+           table.scalar_type() == at::kInt && table.size(0) == q.size(0) && table.size(1) > 0 && table.stride(1) == 1 &&
+           table.stride(0) >= table.size(1) && table.size(1) <= (int64_t{1} << 30) / k_pages.size(2);
+}
+
+OptTensor paged_write(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos, const Tensor& sin,
+                      const Tensor& positions, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    if (!pages_ok(lib, q, k_pages, v_pages, table, positions)) return std::nullopt;
+    const int64_t B = q.size(0), T = q.size(1), KV = k_pages.size(1), S = k_pages.size(2), D = k_pages.size(3);
+    const auto type = q.scalar_type(), rope = cos.scalar_type();
+    auto tokens_ok = [&](const Tensor& t) {
+        return t.device() == q.device() && t.scalar_type() == type && t.dim() == 3 && t.size(0) == B && t.size(1) == T &&
+               t.size(2) == KV * D;
+    };
+    auto table_ok = [&](const Tensor& t) {
+        return plain(t, q, rope) && t.numel() == B * T * D && t.size(-1) == D && aligned16(t);
+    };
+    if (D % 16 || !tokens_ok(k) || !tokens_ok(v) || (rope != type && rope != at::kFloat) || cos.dim() == 0 ||
+        cos.sizes() != sin.sizes() || !table_ok(cos) || !table_ok(sin))
+        return std::nullopt;
+    const int64_t qs = row_stride(q, B, T), ks = row_stride(k, B, T), vs = row_stride(v, B, T);
+    if (qs == 0 || ks == 0 || vs == 0) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty(q.sizes(), q.options());
+    if (lib->paged_write(dtype_code(type), q.const_data_ptr(), qs, k.const_data_ptr(), ks, v.const_data_ptr(), vs,
+                         cos.const_data_ptr(), sin.const_data_ptr(), rope == at::kFloat,
+                         static_cast<const int64_t*>(positions.const_data_ptr()), static_cast<const int32_t*>(table.const_data_ptr()),
+                         table.stride(0), table.size(1), k_pages.mutable_data_ptr(), v_pages.mutable_data_ptr(), k_pages.size(0), S,
+                         out.mutable_data_ptr(), B, T, q.size(2) / D, KV, D, stream_of(q)) != NQ_OK)
+        return std::nullopt;
+    return out;
+}
+
+OptTensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                          const Tensor& positions, int64_t window, int64_t sinks, std::optional<double> scale) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    if (!pages_ok(lib, q, k_pages, v_pages, table, positions)) return std::nullopt;
+    const int64_t B = q.size(0), T = q.size(1), KV = k_pages.size(1), S = k_pages.size(2), D = k_pages.size(3), H = q.size(2) / D;
+    const int64_t qs = row_stride(q, B, T);
+    if ((D != 64 && D != 128) || S % 16 || qs == 0 || window < 0 || sinks < 0) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty(q.sizes(), q.options());
+    const size_t bytes = lib->paged_attention_bytes(B, T, H, KV, D, table.size(1), S);
+    const Tensor ws = bytes ? scratch(bytes, q) : Tensor();
+    const float factor = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D)));
+    if (lib->paged_attention(dtype_code(q.scalar_type()), q.const_data_ptr(), qs, k_pages.const_data_ptr(),
+                             v_pages.const_data_ptr(), k_pages.size(0), S, static_cast<const int32_t*>(table.const_data_ptr()),
+                             table.stride(0), table.size(1), static_cast<const int64_t*>(positions.const_data_ptr()),
+                             out.mutable_data_ptr(), B, T, H, KV, D, window, sinks, factor,
+                             bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(q)) != NQ_OK)
+        return std::nullopt;
+    return out;
+}
+
+// {accepted, tokens}, or an empty list.
+std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Tensor& uniforms, const OptTensor& draft_probs,
+                           double temperature) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    const auto type = logits.scalar_type();
+    if (!lib || !logits.is_cuda() || logits.dim() != 3 || drafts.dim() != 2 || uniforms.dim() != 2 || logits.numel() == 0 ||
+        (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat))
+        return {};
+    const int64_t B = logits.size(0), n = logits.size(1) - 1, V = logits.size(2);
+    if (logits.stride(2) != 1 || logits.stride(1) < V || (B > 1 && logits.stride(0) != (n + 1) * logits.stride(1)) ||
+        !plain(drafts, logits, at::kLong) || drafts.size(0) != B || drafts.size(1) != n || !plain(uniforms, logits, at::kFloat) ||
+        uniforms.size(0) != B || uniforms.size(1) != n + 1 || !(temperature >= 0.0) ||
+        static_cast<float>(temperature) > 3.402823466e38f || (temperature > 0.0 && static_cast<float>(temperature) == 0.0f))
+        return {};
+    if (draft_probs.has_value() && (!plain(*draft_probs, logits, at::kFloat) || draft_probs->dim() != 3 ||
+                                    draft_probs->size(0) != B || draft_probs->size(1) != n || draft_probs->size(2) != V))
+        return {};
+    const size_t bytes = lib->verify_bytes(B, n, V);
+    if (bytes == 0) return {};
+    const c10::DeviceGuard guard(logits.device());
+    Tensor accepted = at::empty({B}, drafts.options()), tokens = at::empty({B, n + 1}, drafts.options());
+    const Tensor ws = scratch(bytes, logits);
+    if (lib->verify(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), logits.stride(1),
+                    static_cast<const int64_t*>(drafts.const_data_ptr()), static_cast<const float*>(data_of(draft_probs)),
+                    static_cast<const float*>(uniforms.const_data_ptr()), static_cast<float>(temperature),
+                    static_cast<int64_t*>(accepted.mutable_data_ptr()), static_cast<int64_t*>(tokens.mutable_data_ptr()), B, n, V,
+                    ws.mutable_data_ptr(), bytes, stream_of(logits)) != NQ_OK)
+        return {};
+    return {accepted, tokens};
+}
+
 }  // namespace
 
 // The addresses of the C ABI's functions, in Library's order, once the HIP library is loaded (the table lives as long
@@ -165,6 +279,11 @@ extern "C" int nq_ops_bind(void* const* functions, int count) {
     library.onebit = reinterpret_cast<decltype(library.onebit)>(functions[3]);
     library.nanoquant_bytes = reinterpret_cast<decltype(library.nanoquant_bytes)>(functions[4]);
     library.nanoquant = reinterpret_cast<decltype(library.nanoquant)>(functions[5]);
+    library.paged_write = reinterpret_cast<decltype(library.paged_write)>(functions[6]);
+    library.paged_attention_bytes = reinterpret_cast<decltype(library.paged_attention_bytes)>(functions[7]);
+    library.paged_attention = reinterpret_cast<decltype(library.paged_attention)>(functions[8]);
+    library.verify_bytes = reinterpret_cast<decltype(library.verify_bytes)>(functions[9]);
+    library.verify = reinterpret_cast<decltype(library.verify)>(functions[10]);
     g_library.store(&library, std::memory_order_release);
     return 0;
 }
@@ -176,4 +295,10 @@ TORCH_LIBRARY_IMPL(binary_kernels, CUDA, m) {
     m.impl("nanoquant_dyn_forward", &gemv);
     m.impl("marlin_onebit_forward", &onebit);
     m.impl("marlin_nanoquant_forward", &nanoquant);
+}
+
+TORCH_LIBRARY_IMPL(nanoquant_amd, CUDA, m) {
+    m.impl("paged_rope_write", &paged_write);
+    m.impl("paged_attention", &paged_attention);
+    m.impl("verify_drafts", &verify);
 }

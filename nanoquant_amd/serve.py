@@ -8,6 +8,9 @@ own, and the check of drafted tokens.
   chunks of prompts, optionally under a sliding window with a few first tokens that stay visible.
 * :func:`verify_drafts` keeps or turns down drafted tokens by the model's logits and given random numbers.
 
+Calls of well-laid-out tensors on the GPU go through the C++ of ``libnq_ops.so`` (``csrc/torch_ops/nq_ops.cpp``): a small call
+is bound by its host path. What that does not take is checked, copied into place or refused here.
+
 float16 and bfloat16 tensors on the GPU run the HIP library (``nq_paged_rope_write``, ``nq_paged_attention``,
 ``nq_verify_drafts``); CPU tensors, float32 models, head sizes other than 64 and 128 and page sizes that are no multiple of 16
 run torch ops with the same results but for rounding. The reference has no counterpart: its harness decodes one batch on
@@ -23,6 +26,25 @@ from . import _lib
 from ._dispatch import launch as _launch, only_eager as _only_eager
 
 _HALF = (torch.float16, torch.bfloat16)
+
+_OPS = torch.library.Library("nanoquant_amd", "FRAGMENT")
+for _schema in (
+        "paged_rope_write(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor positions, Tensor(a!) k_pages, "
+        "Tensor(b!) v_pages, Tensor table) -> Tensor?",
+        "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor positions, int window, int sinks, "
+        "float? scale) -> Tensor?",
+        "verify_drafts(Tensor logits, Tensor drafts, Tensor uniforms, Tensor? draft_probs, float temperature) -> Tensor[]"):
+    _OPS.define(_schema)
+
+
+def _native(name):
+    """The operator in C++, or None where ``libnq_ops.so`` is missing or older."""
+    if _lib.ops is None or not torch._C._dispatch_has_kernel_for_dispatch_key(f"nanoquant_amd::{name}", "CUDA"):
+        return None
+    return getattr(torch.ops.nanoquant_amd, name).default
+
+
+_native_write, _native_attention, _native_verify = (_native(n) for n in ("paged_rope_write", "paged_attention", "verify_drafts"))
 
 
 class PagedKVCache:
@@ -153,6 +175,10 @@ def paged_rope_write(q, k, v, cos, sin, positions, k_pages, v_pages, table):
     outside the table (-1 for padding) writes nothing and gives zero queries; a page that is not there is not written. Two
     tokens of a call must not name the same row of a page."""
     what = "paged_rope_write"
+    if _native_write is not None and q.is_cuda and _only_eager(q, k, v, cos, sin, positions, k_pages, v_pages, table):
+        out = _native_write(q, k, v, cos, sin, positions, k_pages, v_pages, table)
+        if out is not None:
+            return out
     B, T, N, KV, S, D = _check_pages(what, k_pages, v_pages, table, positions, q.dtype, q.device)
     if (q.dim() != 3 or q.shape[:2] != positions.shape or q.shape[2] % (KV * D) or q.shape[2] == 0
             or tuple(k.shape) != (B, T, KV * D) or v.shape != k.shape):
@@ -208,6 +234,10 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     j < sinks. A token that sees none, or whose position is outside the table (-1 for padding), gets zeros. ``scale`` is
     D ** -0.5 unless given."""
     what = "paged_attention"
+    if _native_attention is not None and q.is_cuda and _only_eager(q, k_pages, v_pages, table, positions):
+        out = _native_attention(q, k_pages, v_pages, table, positions, window, sinks, scale)
+        if out is not None:
+            return out
     B, T, N, KV, S, D = _check_pages(what, k_pages, v_pages, table, positions, q.dtype, q.device)
     if q.dim() != 3 or q.shape[:2] != positions.shape or q.shape[2] % (KV * D) or q.shape[2] == 0:
         raise ValueError(f"{what}: q {tuple(q.shape)} does not fit {B} x {T} tokens and pages of {KV} heads of {D}")
@@ -283,6 +313,11 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
     uniforms[n] times its total: w = max(p - q, 0) where a draft was turned down (p where that is zero), else p. A row with a
     NaN or an infinite largest logit turns its draft down and gives its argmax. Probabilities and sums are float64."""
     what = "verify_drafts"
+    given = (logits, drafts, uniforms) if draft_probs is None else (logits, drafts, uniforms, draft_probs)
+    if _native_verify is not None and logits.is_cuda and _only_eager(*given):
+        out = _native_verify(logits, drafts, uniforms, draft_probs, temperature)
+        if out:
+            return tuple(out)
     if logits.dim() != 3 or drafts.dim() != 2 or logits.shape[0] != drafts.shape[0] or logits.shape[1] != drafts.shape[1] + 1:
         raise ValueError(f"{what}: logits must be [batch, drafts + 1, vocab] and drafts [batch, drafts], got "
                          f"{tuple(logits.shape)} and {tuple(drafts.shape)}")
@@ -296,11 +331,10 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
         raise TypeError(f"{what}: logits float32, float16 or bfloat16, drafts int64, uniforms and draft_probs float32")
     if not 0.0 <= temperature < math.inf:
         raise ValueError(f"{what}: the temperature must be a finite number from 0, got {temperature}")
-    given = (logits, drafts, uniforms) if draft_probs is None else (logits, drafts, uniforms, draft_probs)
     for t in given:
         if t.device != logits.device:
             raise ValueError(f"{what}: tensors on {t.device} and {logits.device}")
-    if logits.is_cuda and V <= 0x7fffffff and _only_eager(*given):
+    if logits.is_cuda and V <= 1 << 30 and _only_eager(*given):
         accepted = torch.empty(B, dtype=torch.int64, device=logits.device)
         tokens = torch.empty(B, n + 1, dtype=torch.int64, device=logits.device)
         if B == 0:
