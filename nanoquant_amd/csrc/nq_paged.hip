@@ -7,6 +7,13 @@
 namespace nq {
 namespace {
 
+// A pointer that is the same for the whole wave, in scalar registers.
+__device__ inline const uint16_t* uniform(const uint16_t* p) {
+    const uint64_t u = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+    return reinterpret_cast<const uint16_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 __device__ inline const u32x4* vec(const uint16_t* p) { return reinterpret_cast<const u32x4*>(p); }
 
 // The page of position p of a sequence, -1 where there is none.
@@ -119,11 +126,11 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteArgs a) {
     *reinterpret_cast<u32x4*>(dst + half) = hi;
 }
 
-constexpr int kTile = 32;          // keys a wave takes at a time
+constexpr int kTile = 32;          // keys a wave of few_kernel takes at a time
 constexpr int kWaves = 4;          // of a block
-constexpr int kBlocks = 256;       // one a CU: its rings take most of the LDS
-constexpr int kEntries = 2048;     // (sequence, row group) pairs of a launch, whose key counts every block adds up
-constexpr int kLeastShare = 4;     // tiles a block takes at least: one a wave
+constexpr int kCUs = 256;
+constexpr int kEntries = 1024;     // (sequence, row group) pairs of a launch, whose key counts every block adds up
+constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
 constexpr float kSlack = 8.0f;
 constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
@@ -142,7 +149,7 @@ struct PagedArgs {
     int row_groups, rows_kept;  // row groups a (sequence, kv head), rows of one that there are
     int4* spans;        // [batch * row_groups]: Tiles, for rows_kernel's shares
     int2* desc;         // [batch * row_groups * kv_heads]: {first block * 2 + its slot, last block}
-    float* part_o;      // [kBlocks][2][rows_kept][D]
+    float* part_o;      // [blocks][2][rows_kept][D]
     float2* part_ml;    // the same rows' {maximum, sum}
 };
 
@@ -245,8 +252,8 @@ struct Shares {
     int64_t share, first, end;  // units a block, and this block's
     int entry;                  // of the first; -1: nothing to do
 };
-template <int kThreads, typename Count>
-__device__ inline Shares make_shares(const PagedArgs& a, int entries, int blocks, int least, int64_t* pre, int64_t* wave_total,
+template <int kThreads, int kBlocks, typename Count>
+__device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
                                      int* s_entry, Count count) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int per = (entries + kThreads - 1) / kThreads;
@@ -279,7 +286,7 @@ __device__ inline Shares make_shares(const PagedArgs& a, int entries, int blocks
     __syncthreads();
     Shares r;
     const int64_t total = all * a.kv_heads;
-    r.share = max<int64_t>((total + blocks - 1) / blocks, least);
+    r.share = max<int64_t>((total + kBlocks - 1) / kBlocks, least);
     r.first = blockIdx.x * r.share;
     r.end = min(r.first + r.share, total);
     if (r.first >= r.end) {
@@ -307,24 +314,32 @@ __device__ inline uint2 read_transposed(const uint16_t* p) {
 //   O^T += V^T P^T   A = 16 dimensions x 32 keys, read transposed from the row-major tile, B = P^T: S^T's accumulator layout
 //                    already, with keys 4 g .. +3 and 16 + 4 g .. +3 in lane group g
 // and the probabilities' sums as one more product with ones, from the rounded values that the value product takes.
+template <int D, int RT>
+struct FewShape {
+    static constexpr bool kWide = RT == 4 && D == 128;  // too many registers for two blocks on a CU
+    static constexpr int kPerCU = kWide ? 1 : 2, kBlocks = kPerCU * kCUs;
+    static constexpr int kStages = kWide || D == 64 ? 2 : 1;  // tiles in a wave's ring: 16 KB, 32 where a block has the CU
+};
+
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_kernel(const PagedArgs a) {
+    using Shape = FewShape<D, RT>;
     constexpr int C = D / 8;                  // 16-byte chunks of a row
     constexpr int RowsPer = 64 / C;           // rows of one DMA instruction
     constexpr int Instr = 16 / RowsPer;       // instructions for 16 rows
-    constexpr int PerTile = 4 * Instr;        // K and V, two 16-row halves
-    constexpr int TileElems = kTile * D;
-    __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][2][2][TileElems];
+    constexpr int Half = 2 * Instr;           // for a tile's keys, or its values
+    constexpr int S = Shape::kStages, TileElems = kTile * D;
+    __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][S][2][TileElems];
     __shared__ int64_t pre[kEntries + 1];
     __shared__ int64_t wave_total[kWaves];
-    __shared__ float stat_m[kWaves][16 * RT], stat_l[kWaves][16 * RT];
+    __shared__ float stat_m[kWaves][16], stat_l[kWaves][16];
     __shared__ int s_entry;
     static_assert(sizeof(ring) >= sizeof(float) * kWaves * 16 * D, "the rings hold the waves' sums of 16 rows");
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const Shares shares = make_shares<64 * kWaves>(a, a.batch * a.row_groups, kBlocks, kLeastShare, pre, wave_total, &s_entry,
-                                                   [&](int e) { return tiles_of_few(a, e, 16 * RT).count; });
+    const Shares shares = make_shares<64 * kWaves, Shape::kBlocks>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
+                                                                   [&](int e) { return tiles_of_few(a, e, 16 * RT).count; });
     if (shares.entry < 0) return;
     int entry = shares.entry;
     int64_t u = shares.first;
@@ -340,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
     int slot = 0;
     while (true) {
         const int64_t seg0 = pre[entry] * a.kv_heads;
-        const int count = static_cast<int>(pre[entry + 1] - pre[entry]);
+        const int count = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
         const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / count));
         const int64_t seg = seg0 + static_cast<int64_t>(kvh) * count;
         const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg));
@@ -351,6 +366,52 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
         Tiles tiles = tiles_of_few(a, entry, 16 * RT);
         tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
         tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
+
+        const __attribute__((address_space(4))) int32_t* table =
+            (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
+        // the pages of a tile's halves, -1 where there is none (past the table's end too)
+        auto page_of = [&](int key) {
+            const int at = key / a.pages.page_size;
+            if (at >= a.pages.table_pages) return -1;
+            const int page = table[at];
+            return page >= 0 && page < a.pages.pages ? page : -1;
+        };
+        // a tile's keys and values go out on their own, the next ones as soon as these have been read
+        struct Places {
+            int64_t at[2];  // of the halves, in elements
+            int there;      // bit h: half h's page is there
+        };
+        auto places_of = [&](int i) {
+            const int key0 = tiles.at(first + wave + kWaves * i) * kTile;
+            Places p;
+            p.there = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = key0 + 16 * h, page = __builtin_amdgcn_readfirstlane(page_of(key));
+                p.there |= page >= 0 ? 1 << h : 0;
+                p.at[h] = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
+            }
+            return p;
+        };
+        auto issue = [&](const uint16_t* pool, const Places& p, int stage, int which) {
+            const uint32_t lds = ring_lds + static_cast<uint32_t>((stage * 2 + which) * TileElems) * 2u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint16_t* from = uniform(pool + p.at[h]);
+#pragma unroll
+                for (int j = 0; j < Instr; ++j) dma16_lds(from, voff[j], lds + static_cast<uint32_t>(h * 16 * D) * 2u + 1024u * j);
+            }
+        };
+        const int mine = n > wave ? (n - wave + kWaves - 1) / kWaves : 0;
+        int there[S] = {};  // of the tiles that are out, the oldest first
+#pragma unroll
+        for (int st = 0; st < S; ++st)
+            if (st < mine) {
+                const Places p = places_of(st);
+                there[st] = p.there;
+                issue(a.k_pages, p, st, 0);
+                issue(a.v_pages, p, st, 1);
+            }
 
         u32x4 qf[RT][D / 32];
         int last[RT], start[RT];
@@ -388,40 +449,24 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
             for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 
-        const __attribute__((address_space(4))) int32_t* table =
-            (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
-        // the pages of a tile's halves, -1 where there is none (past the table's end too)
-        auto page_of = [&](int key) {
-            const int at = key / a.pages.page_size;
-            if (at >= a.pages.table_pages) return -1;
-            const int page = table[at];
-            return page >= 0 && page < a.pages.pages ? page : -1;
-        };
-        auto issue = [&](int i, int buf) {
-            const int key0 = tiles.at(first + wave + kWaves * i) * kTile;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * h;
-                const int page = __builtin_amdgcn_readfirstlane(max(0, page_of(key)));
-                const int64_t at = ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
-                const uint32_t lds = ring_lds + static_cast<uint32_t>(buf * 2 * TileElems + h * 16 * D) * 2u;
-#pragma unroll
-                for (int j = 0; j < Instr; ++j) dma16_lds(a.k_pages + at, voff[j], lds + 1024u * j);
-#pragma unroll
-                for (int j = 0; j < Instr; ++j) dma16_lds(a.v_pages + at, voff[j], lds + 2u * TileElems + 1024u * j);
-            }
-        };
-        const int mine = n > wave ? (n - wave + kWaves - 1) / kWaves : 0;
-        if (mine > 0) issue(0, 0);
-        if (mine > 1) issue(1, 1);
-        for (int i = 0; i < mine; ++i) {
-            const int buf = i & 1;
-            if (i + 1 < mine) wait_vmcnt<PerTile>();
+        // waits until the oldest outstanding part (a tile's keys, or values) has come, `behind` parts having gone out since
+        auto wait_part = [&](int behind) {
+            if (behind >= 3) wait_vmcnt<(S == 2 ? 3 : 1) * Half>();
+            else if (behind == 2) wait_vmcnt<(S == 2 ? 2 : 1) * Half>();
+            else if (behind == 1) wait_vmcnt<Half>();
             else wait_vmcnt<0>();
             asm volatile("" ::: "memory");
-            const uint16_t* kb = ring[wave][buf][0];
-            const uint16_t* vb = ring[wave][buf][1];
+        };
+        auto reads_ended = [] { __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4)); };  // lgkmcnt 0
+        for (int i = 0; i < mine; ++i) {
+            const int stage = S == 1 ? 0 : i & 1, ahead = min(mine - 1 - i, S - 1);  // tiles out behind this one
+            const uint16_t* kb = ring[wave][stage][0];
+            const uint16_t* vb = ring[wave][stage][1];
             const int key0 = tiles.at(first + wave + kWaves * i) * kTile;
+            const bool more = i + S < mine;
+            Places next{};
+            if (more) next = places_of(i + S);
+            wait_part(1 + 2 * ahead);
             u32x4 kf[2][D / 32];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -430,51 +475,73 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                     const int swz = D == 128 ? c : c >> 1;
                     kf[h][kt] = *vec(kb + (16 * h + c) * D + 8 * ((4 * kt + g) ^ (swz & (C - 1))));
                 }
-            const bool there0 = page_of(key0) >= 0, there1 = page_of(key0 + 16) >= 0;
-            const bool whole = there0 && there1 && key0 + kTile - 1 <= all_last &&
+            if (more) {
+                reads_ended();
+                issue(a.k_pages, next, stage, 0);
+            }
+            const bool whole = there[0] == 3 && key0 + kTile - 1 <= all_last &&
                                (key0 >= all_start || key0 + kTile <= a.sinks);
-            const uint32_t pages_there = (there0 ? 0xFFFFu : 0u) | (there1 ? 0xFFFF0000u : 0u);
+            const uint32_t pages_there = (there[0] & 1 ? 0xFFFFu : 0u) | (there[0] & 2 ? 0xFFFF0000u : 0u);
             uint32_t some = 0;  // seen by some row of the wave's
             u32x4 pf[RT];
             uint32_t seen[RT];  // the lane's key 16 h + 4 g + e in bit 16 h + e
+            f32x4 s[RT][2];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int kt = 0; kt < D / 32; ++kt)
+                for (int h = 0; h < 2; ++h) s[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) s[h] = mfma16x16x32<T>(kf[h][kt], qf[rt][kt], s[h]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) s[h] *= a.scale;
-                if (!whole) {
-                    seen[rt] = (seen_bits(key0, last[rt], start[rt], a.sinks) & pages_there) >> (4 * g);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[h][e] = or_minus_inf(s[h][e], seen[rt], 16 * h + e);
-                    some |= seen[rt];
-                }
-                float top = -INFINITY;
+            for (int kt = 0; kt < D / 32; ++kt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, s[h][e]);
-                top = max_xor32(max_xor16(top));  // the lane groups that hold a column
-                if (__any(top > m[rt] + kSlack)) {
-                    const float mn = fmaxf(m[rt], top);
+                    for (int rt = 0; rt < RT; ++rt) s[rt][h] = mfma16x16x32<T>(kf[h][kt], qf[rt][kt], s[rt][h]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[rt][h] *= a.scale;
+            if (!whole) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    seen[rt] = (seen_bits(key0, last[rt], start[rt], a.sinks) & pages_there) >> (4 * g);
+                    some |= seen[rt];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[rt][h][e] = or_minus_inf(s[rt][h][e], seen[rt], 16 * h + e);
+                }
+            }
+            // the reference point of the exponentials follows the running maximum only once that is 8 above it: exponentials
+            // up to 2^8 round the same, and most tiles rescale nothing
+            float top[RT];
+            bool grows = false;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                top[rt] = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
+                                fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+                top[rt] = max_xor32(max_xor16(top[rt]));  // the lane groups that hold a column
+                grows |= top[rt] > m[rt] + kSlack;
+            }
+            if (__any(grows)) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float mn = fmaxf(m[rt], top[rt]);
                     const float keep = __builtin_amdgcn_exp2f(m[rt] - (mn == -INFINITY ? 0.0f : mn));
                     m[rt] = mn;
                     lsum[rt] *= keep;
 #pragma unroll
                     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= keep;
                 }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
                 const float mu = m[rt] == -INFINITY ? 0.0f : m[rt];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][e] = __builtin_amdgcn_exp2f(s[h][e] - mu);
-                    pf[rt][2 * h] = pack2<T>(s[h][0], s[h][1]);
-                    pf[rt][2 * h + 1] = pack2<T>(s[h][2], s[h][3]);
+                    for (int e = 0; e < 4; ++e) s[rt][h][e] = __builtin_amdgcn_exp2f(s[rt][h][e] - mu);
+                    pf[rt][2 * h] = pack2<T>(s[rt][h][0], s[rt][h][1]);
+                    pf[rt][2 * h + 1] = pack2<T>(s[rt][h][2], s[rt][h][3]);
                 }
                 lsum[rt] = mfma16x16x32<T>(u32x4{T::ONE_PAIR, T::ONE_PAIR, T::ONE_PAIR, T::ONE_PAIR}, pf[rt], lsum[rt]);
             }
@@ -494,6 +561,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
             }
             float zero = 0.0f;
             constexpr int kAhead = 4;  // dimension tiles read together
+            wait_part(2 * ahead + more);
 #pragma unroll
             for (int d0 = 0; d0 < D / 16; d0 += kAhead) {
                 u32x4 vf[kAhead];
@@ -535,10 +603,13 @@ __global__ __launch_bounds__(64 * kWaves, 1) void few_kernel(const PagedArgs a) 
                         __builtin_amdgcn_sched_barrier(0);
                     }
             }
-            if (i + 2 < mine) {
-                __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4));  // the buffer's reads have ended (lgkmcnt 0)
-                issue(i + 2, buf);
+            if (more) {
+                reads_ended();
+                issue(a.v_pages, next, stage, 1);
             }
+#pragma unroll
+            for (int st = 0; st + 1 < S; ++st) there[st] = there[st + 1];
+            there[S - 1] = next.there;
         }
 
         // the waves' sums, joined through the rings a row group at a time
@@ -613,12 +684,12 @@ __device__ inline Parts parts_of(const PagedArgs& a, int seg) {
 }
 
 // Adds what the blocks left of one row of an (entry, kv head), for few rows of which many blocks may hold a part: the threads
-// in groups of D / 4, a group a partial result.
+// in groups of D / 4, a group every Groups-th part. Bound by latency: where the parts lie, then the parts, then their sums.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int group) {
-    constexpr int L4 = D / 4, Groups = 256 / L4;
+    constexpr int L4 = D / 4, Groups = 256 / L4, kAhead = 4;
     __shared__ float red[Groups][D];
-    __shared__ float tops[4], sums[4];
+    __shared__ float2 stat[Groups];
     const int t = threadIdx.x;
     const int seg = static_cast<int>(blockIdx.x) / a.rows_kept;
     const int row = static_cast<int>(blockIdx.x) - seg * a.rows_kept;
@@ -628,34 +699,52 @@ __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int gr
     const int b = entry / a.row_groups;
     const int r = (entry - b * a.row_groups) * group + row;
     if (r >= a.tokens * a.groups) return;
-    static_assert(kBlocks <= 256, "a thread a block's statistics");
-    const float2 ml = t < parts.n ? a.part_ml[parts.row(a, t, row)] : float2{-INFINITY, 0.0f};
-    float top = ml.x;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    if ((t & 63) == 0) tops[t >> 6] = top;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float mu = M == -INFINITY ? 0.0f : M;
-    const float l = wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - mu));
-    if ((t & 63) == 0) sums[t >> 6] = l;
     const int grp = t / L4, at = 4 * (t % L4);
+    float M = -INFINITY, L = 0.0f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = grp; i < parts.n; i += Groups) {
-        const int64_t p = parts.row(a, i, row);
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[p].x - mu);
-        o += f * *reinterpret_cast<const f32x4*>(a.part_o + p * D + at);
+    for (int i0 = grp; i0 < parts.n; i0 += kAhead * Groups) {
+        float2 ml[kAhead];
+        f32x4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {  // those past the last read it again
+            const int64_t p = parts.row(a, min(i0 + i * Groups, parts.n - 1), row);
+            ml[i] = a.part_ml[p];
+            x[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + at);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(M - mu);
+        M = top;
+        L *= keep;
+        o *= keep;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mu);
+            const bool in = i0 + i * Groups < parts.n;
+            L = in ? fmaf(f, ml[i].y, L) : L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = in ? fmaf(f, x[i][e], o[e]) : o[e];
+        }
     }
     *reinterpret_cast<f32x4*>(&red[grp][at]) = o;
+    if (at == 0) stat[grp] = float2{M, L};
     __syncthreads();
     if (t < D / 2) {
-        const float L = sums[0] + sums[1] + sums[2] + sums[3];
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        float x = 0.0f, y = 0.0f;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < Groups; ++i) top = fmaxf(top, stat[i].x);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
         for (int i = 0; i < Groups; ++i) {
-            x += red[i][2 * t];
-            y += red[i][2 * t + 1];
+            const float f = __builtin_amdgcn_exp2f(stat[i].x - mu);
+            sum = fmaf(f, stat[i].y, sum);
+            x = fmaf(f, red[i][2 * t], x);
+            y = fmaf(f, red[i][2 * t + 1], y);
         }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         *reinterpret_cast<uint32_t*>(a.out + out_row(a, b, kvh, r) * D + 2 * t) = pack2<T>(x * inv, y * inv);
     }
 }
@@ -716,7 +805,6 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const PagedArgs a, int g
 
 constexpr int kKeys = 64;   // keys of a tile
 constexpr int kRowWaves = 4;
-constexpr int kRowEntries = 1024;  // as kEntries: two blocks of rows_kernel's smaller form fit a CU
 
 // An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes.
 __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group, int entries) {
@@ -759,7 +847,7 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
     __shared__ __attribute__((aligned(16))) uint16_t kv[2][2][kKeys * D];  // [buffer][K, V]
     __shared__ int there[2][4];                                           // the page of a tile's 16 keys
     __shared__ int spans[2][kRowWaves];
-    __shared__ int64_t pre[kShared ? kRowEntries + 1 : 1];
+    __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
     __shared__ int64_t wave_total[kRowWaves];
     __shared__ int s_entry;
     const int t = threadIdx.x, lane = t & 63;
@@ -771,8 +859,8 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
     int entry, slot = 0;
     int64_t u = 0;
     if constexpr (kShared) {
-        shares = make_shares<64 * kRowWaves>(a, entries, static_cast<int>(gridDim.x), kLeastTiles, pre, wave_total, &s_entry,
-                                             [&](int e) { return a.spans[e].z; });
+        shares = make_shares<64 * kRowWaves, (RW == 1 ? 2 : 1) * kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry,
+                                                                      [&](int e) { return a.spans[e].z; });
         if (shares.entry < 0) return;
         entry = shares.entry;
         u = shares.first;
@@ -891,11 +979,12 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
             page = page < a.pages.pages ? page : -1;
             if (lane == 0) there[buf][wave] = page;
             const int64_t from = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
+            const uint16_t *k_from = uniform(a.k_pages + from), *v_from = uniform(a.v_pages + from);
             const uint32_t lds = lds0 + static_cast<uint32_t>(buf) * (2 * kKeys * D * 2);
 #pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(a.k_pages + from, koff[j], lds + 1024u * j);
+            for (int j = 0; j < Instr; ++j) dma16_lds(k_from, koff[j], lds + 1024u * j);
 #pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(a.v_pages + from, voff[j], lds + kKeys * D * 2u + 1024u * j);
+            for (int j = 0; j < Instr; ++j) dma16_lds(v_from, voff[j], lds + kKeys * D * 2u + 1024u * j);
         };
         issue(0, 0);
         wait_vmcnt<0>();
@@ -970,17 +1059,22 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
 #pragma unroll
                         for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
                     }
+                    // the reference point of the exponentials follows the running maximum only once that is 8 above it
                     u32x4 pf[RW][2];
+                    float top[RW];
+                    bool grows = false;
 #pragma unroll
                     for (int rw = 0; rw < RW; ++rw) {
-                        float top = s[rw][0];
+                        top[rw] = s[rw][0];
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rw][i]);
-                        top = max_xor32(top) * scale;
-                        // the reference point of the exponentials follows the running maximum only once that is 8 above it:
-                        // exponentials up to 2^8 round the same, and most steps rescale nothing
-                        if (__any(top > m[rw] + kSlack)) {
-                            const float mn = fmaxf(m[rw], top);
+                        for (int i = 1; i < 16; ++i) top[rw] = fmaxf(top[rw], s[rw][i]);
+                        top[rw] = max_xor32(top[rw]) * scale;
+                        grows |= top[rw] > m[rw] + kSlack;
+                    }
+                    if (__any(grows)) {
+#pragma unroll
+                        for (int rw = 0; rw < RW; ++rw) {
+                            const float mn = fmaxf(m[rw], top[rw]);
                             const float keep = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
                             m[rw] = mn;
                             l[rw] *= keep;
@@ -989,6 +1083,9 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep;
                         }
+                    }
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw) {
                         const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
 #pragma unroll
                         for (int w = 0; w < 8; ++w) {
@@ -1127,23 +1224,23 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
         p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
         p.group = 16 * p.tiles;
         p.shared = true;
-        p.blocks = kBlocks;
+        p.blocks = p.tiles < 4 || head_dim == 64 ? 2 * kCUs : kCUs;  // FewShape's
     } else {
         const int64_t large = ceil_div(rows, 256) * batch * kv_heads;
-        p.tiles = large >= 2 * kBlocks ? 2 : 1;
+        p.tiles = large >= 2 * kCUs ? 2 : 1;
         p.shared = false;
         if (p.tiles == 1 && max_keys >= 4096) {
             p.shared = true;
-            p.tiles = large >= kBlocks / 2 ? 2 : 1;
+            p.tiles = large >= kCUs / 2 ? 2 : 1;
         }
         p.group = 128 * p.tiles;
-        p.blocks = p.tiles == 2 ? kBlocks : 2 * kBlocks;
+        p.blocks = p.tiles == 2 ? kCUs : 2 * kCUs;
     }
     p.row_groups = ceil_div(rows, p.group);
     p.rows_kept = std::min(rows, p.group);
     p.batch = batch;
     if (p.shared) {
-        const int64_t entries = p.few ? kEntries : kRowEntries;
+        const int64_t entries = kEntries;
         if (p.row_groups > entries) p.shared = false;  // a prompt this long fills the card
         p.batch = std::min({batch, std::max<int64_t>(1, entries / p.row_groups),
                             std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads * p.rows_kept))});
