@@ -129,7 +129,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteArgs a) {
 constexpr int kTile = 32;          // keys a wave of few_kernel takes at a time
 constexpr int kWaves = 4;          // of a block
 constexpr int kCUs = 256;
-constexpr int kEntries = 1024;     // (sequence, row group) pairs of a launch, whose key counts every block adds up
+// (sequence, row group) pairs of a launch, whose key counts every block adds up: two blocks of either kernel fit a CU's LDS
+constexpr int kFewEntries = 512, kEntries = 1024;
 constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
 constexpr float kSlack = 8.0f;
@@ -189,10 +190,15 @@ __device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
     const int first = (entry - b * a.row_groups) * group;
     const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + group - 1) / a.groups);
     int lo = INT32_MAX, hi = -1;
-    for (int t = t0; t <= t1; ++t) {
-        const int p = real_position(a, static_cast<int64_t>(b) * a.tokens + t);
-        if (p >= 0) lo = min(lo, p);
-        hi = max(hi, p);
+    for (int t = t0; t <= t1; t += 8) {
+        int p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = real_position(a, static_cast<int64_t>(b) * a.tokens + min(t + i, t1));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lo = p[i] >= 0 ? min(lo, p[i]) : lo;
+            hi = max(hi, p[i]);
+        }
     }
     return tiles_between<kTile>(a, lo, hi);
 }
@@ -316,7 +322,7 @@ __device__ inline uint2 read_transposed(const uint16_t* p) {
 // and the probabilities' sums as one more product with ones, from the rounded values that the value product takes.
 template <int D, int RT>
 struct FewShape {
-    static constexpr bool kWide = RT == 4 && D == 128;  // too many registers for two blocks on a CU
+    static constexpr bool kWide = RT >= 3 && D == 128;  // too many registers for two blocks on a CU
     static constexpr int kPerCU = kWide ? 1 : 2, kBlocks = kPerCU * kCUs;
     static constexpr int kStages = kWide || D == 64 ? 2 : 1;  // tiles in a wave's ring: 16 KB, 32 where a block has the CU
 };
@@ -330,7 +336,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     constexpr int Half = 2 * Instr;           // for a tile's keys, or its values
     constexpr int S = Shape::kStages, TileElems = kTile * D;
     __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][S][2][TileElems];
-    __shared__ int64_t pre[kEntries + 1];
+    __shared__ int64_t pre[kFewEntries + 1];
+    __shared__ int2 spans[kFewEntries];  // {sink_tiles, window_tile}
     __shared__ int64_t wave_total[kWaves];
     __shared__ float stat_m[kWaves][16], stat_l[kWaves][16];
     __shared__ int s_entry;
@@ -339,7 +346,11 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
     const Shares shares = make_shares<64 * kWaves, Shape::kBlocks>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
-                                                                   [&](int e) { return tiles_of_few(a, e, 16 * RT).count; });
+                                                                   [&](int e) {
+                                                                       const Tiles r = tiles_of_few(a, e, 16 * RT);
+                                                                       spans[e] = int2{r.sink_tiles, r.window_tile};
+                                                                       return r.count;
+                                                                   });
     if (shares.entry < 0) return;
     int entry = shares.entry;
     int64_t u = shares.first;
@@ -363,9 +374,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         const int b = entry / a.row_groups;
         const int row0 = (entry - b * a.row_groups) * (16 * RT);
         const int rows = min(16 * RT, a.tokens * a.groups - row0);
-        Tiles tiles = tiles_of_few(a, entry, 16 * RT);
-        tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
-        tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
+        const Tiles tiles{__builtin_amdgcn_readfirstlane(spans[entry].x), __builtin_amdgcn_readfirstlane(spans[entry].y), count};
 
         const __attribute__((address_space(4))) int32_t* table =
             (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
@@ -1221,10 +1230,10 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     const int64_t rows = tokens * groups;
     p.few = rows <= 64;
     if (p.few) {
-        p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+        p.tiles = static_cast<int>(ceil_div(rows, 16));
         p.group = 16 * p.tiles;
         p.shared = true;
-        p.blocks = p.tiles < 4 || head_dim == 64 ? 2 * kCUs : kCUs;  // FewShape's
+        p.blocks = p.tiles < 3 || head_dim == 64 ? 2 * kCUs : kCUs;  // FewShape's
     } else {
         const int64_t large = ceil_div(rows, 256) * batch * kv_heads;
         p.tiles = large >= 2 * kCUs ? 2 : 1;
@@ -1240,7 +1249,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     p.rows_kept = std::min(rows, p.group);
     p.batch = batch;
     if (p.shared) {
-        const int64_t entries = kEntries;
+        const int64_t entries = p.few ? kFewEntries : kEntries;
         if (p.row_groups > entries) p.shared = false;  // a prompt this long fills the card
         p.batch = std::min({batch, std::max<int64_t>(1, entries / p.row_groups),
                             std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads * p.rows_kept))});
@@ -1265,6 +1274,7 @@ void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
     if (plan.few) {
         if (plan.tiles == 1) few_kernel<T, D, 1><<<grid, 64 * kWaves, 0, st>>>(a);
         else if (plan.tiles == 2) few_kernel<T, D, 2><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (plan.tiles == 3) few_kernel<T, D, 3><<<grid, 64 * kWaves, 0, st>>>(a);
         else few_kernel<T, D, 4><<<grid, 64 * kWaves, 0, st>>>(a);
     } else if (plan.shared) {
         const int entries = a.batch * a.row_groups;
