@@ -203,29 +203,6 @@ __device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
     return tiles_between<kTile>(a, lo, hi);
 }
 
-// A value that some rows of a product see and others do not reaches the others too where it is not finite (0 * inf). In tiles
-// that some rows see in part, such values are taken as 0, and these marks then make inf or NaN of the sums of the rows that do
-// see one: kind 0 marks +inf, 1 -inf, 2 NaN, each as 1 among zeros.
-template <typename T>
-__device__ inline uint32_t mark2(uint32_t v, int kind) {
-    constexpr uint32_t inf = T::ONE_PAIR == 0x3C003C00u ? 0x7C00u : 0x7F80u, one = T::ONE_PAIR & 0xFFFFu;
-    uint32_t r = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t x = (v >> (16 * h)) & 0xFFFFu;
-        const bool is = kind == 2 ? (x & 0x7FFFu) > inf : x == (kind ? inf | 0x8000u : inf);
-        r |= is ? one << (16 * h) : 0u;
-    }
-    return r;
-}
-// the finite ones of a pair, 0 for the others
-template <typename T>
-__device__ inline uint32_t finite2(uint32_t v) {
-    constexpr uint32_t inf = T::ONE_PAIR == 0x3C003C00u ? 0x7C00u : 0x7F80u;
-    return ((v & inf) != inf ? v & 0xFFFFu : 0u) | (((v >> 16) & inf) != inf ? v & 0xFFFF0000u : 0u);
-}
-__device__ inline float mark_value(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf(""); }
-
 // Which keys of a tile a row sees, a bit a key: arithmetic on words, since compares of every key with every row would each
 // hold a pair of scalar registers.
 __device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : 0xFFFFFFFFu >> (32 - n); }
@@ -312,6 +289,45 @@ __device__ inline uint2 read_transposed(const uint16_t* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
+// A value that some rows of a product see and others do not reaches the others too where it is not finite (0 * inf, 0 * NaN).
+// A block that finds one in a tile that its rows see in part makes its result here instead: a wave a row, a key at a time,
+// with lane l at dimensions l and, of 128, l + 64. For data of which no speed is asked.
+template <typename T, int D>
+__device__ inline void slow_rows(const PagedArgs& a, int b, int kvh, int row0, int rows, const Tiles& tiles, int keys,
+                                                    int first, int n, bool done, int64_t part) {
+    constexpr int N = D / 64;
+    const int lane = threadIdx.x & 63;
+    for (int row = threadIdx.x >> 6; row < rows; row += static_cast<int>(blockDim.x) >> 6) {
+        const int tok = (row0 + row) / a.groups;
+        const int64_t q_row = static_cast<int64_t>(b) * a.tokens + tok;
+        const int last = real_position(a, q_row), start = a.window > 0 ? max(0, last - a.window + 1) : 0;
+        const uint16_t* q = a.q + q_row * a.q_stride + static_cast<int64_t>(kvh * a.groups + row0 + row - tok * a.groups) * D + lane;
+        float o[N], m = -INFINITY, l = 0.0f;
+        for (int i = 0; i < N; ++i) o[i] = 0.0f;
+        for (int tile = first; tile < first + n; ++tile)
+            for (int key = tiles.at(tile) * keys; key < (tiles.at(tile) + 1) * keys; ++key) {
+                const int slot = key / a.pages.page_size;
+                const int page = slot < a.pages.table_pages ? a.pages.page(b, slot) : -1;
+                if (key > last || !(key >= start || key < a.sinks) || page < 0) continue;
+                const int64_t at = ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D + lane;
+                float s = 0.0f;
+                for (int i = 0; i < N; ++i) s = fmaf(T::to_float(q[64 * i]), T::to_float(a.k_pages[at + 64 * i]), s);
+                s = wave_sum(s) * a.scale;
+                const float top = fmaxf(m, s);
+                const float keep = __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(s - top);
+                const bool none = top == -INFINITY && s == s;  // scores of -inf so far
+                m = top;
+                l = none ? 0.0f : fmaf(l, keep, e);
+                for (int i = 0; i < N; ++i) o[i] = none ? 0.0f : fmaf(e, T::to_float(a.v_pages[at + 64 * i]), o[i] * keep);
+            }
+        for (int i = 0; i < N; ++i) {
+            if (done) a.out[out_row(a, b, kvh, row0 + row) * D + lane + 64 * i] = T::from_float(l == 0.0f ? 0.0f : o[i] / l);
+            else a.part_o[(part + row) * D + lane + 64 * i] = o[i];
+        }
+        if (!done && lane == 0) a.part_ml[part + row] = float2{m, l};
+    }
+}
+
 // Attention of a few rows (query head of a kv head's group, token) per sequence over its pages. An (entry, kv
 // head) that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that
 // join_kernel adds. A wave takes every fourth tile of a share and keeps two in flight
@@ -341,10 +357,12 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     __shared__ int64_t wave_total[kWaves];
     __shared__ float stat_m[kWaves][16], stat_l[kWaves][16];
     __shared__ int s_entry;
+    __shared__ int s_tainted[2];  // a value that is not finite in a tile that the rows see in part: this (entry, kv head)'s, the next's
     static_assert(sizeof(ring) >= sizeof(float) * kWaves * 16 * D, "the rings hold the waves' sums of 16 rows");
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
+    if (t < 2) s_tainted[t] = 0;
     const Shares shares = make_shares<64 * kWaves, Shape::kBlocks>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
                                                                    [&](int e) {
                                                                        const Tiles r = tiles_of_few(a, e, 16 * RT);
@@ -363,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         voff[j] = static_cast<uint32_t>(row * D * 2 + 16 * ((lane % C) ^ (swz & (C - 1))));
     }
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(&ring[wave][0][0][0]));
-    int slot = 0;
+    int slot = 0, turn = 0;
     while (true) {
         const int64_t seg0 = pre[entry] * a.kv_heads;
         const int count = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
@@ -493,7 +511,6 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             const uint32_t pages_there = (there[0] & 1 ? 0xFFFFu : 0u) | (there[0] & 2 ? 0xFFFF0000u : 0u);
             uint32_t some = 0;  // seen by some row of the wave's
             u32x4 pf[RT];
-            uint32_t seen[RT];  // the lane's key 16 h + 4 g + e in bit 16 h + e
             f32x4 s[RT][2];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -512,12 +529,13 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             if (!whole) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    seen[rt] = (seen_bits(key0, last[rt], start[rt], a.sinks) & pages_there) >> (4 * g);
-                    some |= seen[rt];
+                    // the lane's key 16 h + 4 g + e in bit 16 h + e
+                    const uint32_t seen = (seen_bits(key0, last[rt], start[rt], a.sinks) & pages_there) >> (4 * g);
+                    some |= seen;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[rt][h][e] = or_minus_inf(s[rt][h][e], seen[rt], 16 * h + e);
+                        for (int e = 0; e < 4; ++e) s[rt][h][e] = or_minus_inf(s[rt][h][e], seen, 16 * h + e);
                 }
             }
             // the reference point of the exponentials follows the running maximum only once that is 8 above it: exponentials
@@ -576,15 +594,13 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
                 u32x4 vf[kAhead];
 #pragma unroll
                 for (int e = 0; e < kAhead; ++e) vf[e] = read_v(d0 + e);
-                if (!whole) {  // values that no row sees are cleared (rows behind a sequence's last, pages that are not
-                               // there), and those that are not finite
+                if (!whole) {  // values that no row sees are cleared: rows behind a sequence's last, pages that are not there
 #pragma unroll
                     for (int e = 0; e < kAhead; ++e)
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            const uint32_t x = vf[e][w] & keep[w];
-                            zero = T::dot2(x, 0u, zero);
-                            vf[e][w] = finite2<T>(x);
+                            vf[e][w] &= keep[w];
+                            zero = T::dot2(vf[e][w], 0u, zero);  // NaN where one is not finite
                         }
                 }
 #pragma unroll
@@ -592,26 +608,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) o[rt][d0 + e] = mfma16x16x32<T>(vf[e], pf[rt], o[rt][d0 + e]);
             }
-            if (!whole && __any(zero != zero)) {
-#pragma unroll 1
-                for (int kind = 0; kind < 3; ++kind)
-#pragma unroll
-                    for (int dt = 0; dt < D / 16; ++dt) {
-                        u32x4 vf = read_v(dt) & keep;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) vf[w] = mark2<T>(vf[w], kind);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            u32x4 sees;
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) sees[w] = pair_mask(seen[rt], 16 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
-                            const f32x4 marks = mfma16x16x32<T>(vf, sees, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[rt][dt][e] += marks[e] > 0.0f ? mark_value(kind) : 0.0f;
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
+            if (zero != zero) s_tainted[turn] = 1;
             if (more) {
                 reads_ended();
                 issue(a.v_pages, next, stage, 1);
@@ -626,15 +623,18 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept;
         float* red = reinterpret_cast<float*>(&ring[0][0][0][0]);
         __syncthreads();
+        const bool tainted = s_tainted[turn] != 0;
+        if (tainted) slow_rows<T, D>(a, b, kvh, row0, rows, tiles, kTile, first, n, done, part);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            if (tainted) break;
             if (rt > 0) __syncthreads();
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt)
                 *reinterpret_cast<f32x4*>(red + (wave * 16 + c) * D + 4 * ((4 * dt + g) ^ c)) = o[rt][dt];
-            if (g == 0) {  // a row of padding took part where the tile was whole: -inf says that its sums are none
+            if (g == 0) {  // a row of padding took part where the tile was whole: its sums are none
                 stat_m[wave][c] = last[rt] < 0 ? -INFINITY : m[rt];
-                stat_l[wave][c] = lsum[rt][0];
+                stat_l[wave][c] = last[rt] < 0 ? 0.0f : lsum[rt][0];
             }
             __syncthreads();
             for (int id = t; id < 16 * C; id += 64 * kWaves) {
@@ -648,7 +648,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
                 f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) {
-                    if (stat_m[w][row] == -INFINITY) continue;
+                    if (stat_l[w][row] == 0.0f) continue;
                     const float f = __builtin_amdgcn_exp2f(stat_m[w][row] - mu);
                     L += f * stat_l[w][row];
                     lo += f * *reinterpret_cast<const f32x4*>(red + (w * 16 + row) * D + 4 * ((2 * ch) ^ row));
@@ -675,6 +675,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         if (u >= shares.end) return;
         slot = 1;  // a share's first and last (entry, kv head) are the ones that it may not finish
         if (kvh + 1 == a.kv_heads) ++entry;
+        if (t == 0) s_tainted[turn ^ 1] = 0;
+        turn ^= 1;
         __syncthreads();
     }
 }
@@ -859,13 +861,15 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
     __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
     __shared__ int64_t wave_total[kRowWaves];
     __shared__ int s_entry;
+    __shared__ int s_tainted[2];  // as few_kernel's
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 31, kg = lane >> 5;
     const int entries = a.batch * a.row_groups;
 
+    if (t < 2) s_tainted[t] = 0;
     Shares shares{};
-    int entry, slot = 0;
+    int entry, slot = 0, turn = 0;
     int64_t u = 0;
     if constexpr (kShared) {
         shares = make_shares<64 * kRowWaves, (RW == 1 ? 2 : 1) * kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry,
@@ -1055,15 +1059,15 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                             for (int rw = 0; rw < RW; ++rw) s[rw] = mfma32x32x16<T>(kf[q & 1][e], qf[rw][4 * q + e], s[rw]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    uint32_t seen[RW], some = 0u;  // the lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
+                    uint32_t some = 0u;  // seen by some row, the lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
                     if (!whole) {
                         const uint32_t pages_there = (pg.x >= 0 ? 0xFFFFu : 0u) | (pg.y >= 0 ? 0xFFFF0000u : 0u);
 #pragma unroll
                         for (int rw = 0; rw < RW; ++rw) {
-                            seen[rw] = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
-                            some |= seen[rw];
+                            const uint32_t seen = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
+                            some |= seen;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen[rw], 8 * (i >> 2) + (i & 3));
+                            for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen, 8 * (i >> 2) + (i & 3));
                         }
 #pragma unroll
                         for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
@@ -1108,15 +1112,14 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                     for (int k2 = 0; k2 < 2; ++k2) {
                         if (k2 == 0) read_vs(2 * h + 1);
                         __builtin_amdgcn_sched_barrier(0);
-                        if (!whole) {  // values that no row sees are cleared, and those that are not finite
+                        if (!whole) {  // values that no row sees are cleared
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
                                 const uint32_t keep = pair_mask(some, 16 * k2 + 8 * (w >> 1) + 2 * (w & 1));
 #pragma unroll
                                 for (int dt = 0; dt < DT; ++dt) {
-                                    const uint32_t x = vf[k2][dt][w] & keep;
-                                    zero = T::dot2(x, 0u, zero);
-                                    vf[k2][dt][w] = finite2<T>(x);
+                                    vf[k2][dt][w] &= keep;
+                                    zero = T::dot2(vf[k2][dt][w], 0u, zero);  // NaN where one is not finite
                                 }
                             }
                         }
@@ -1126,31 +1129,7 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
                             for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[k2][dt], pf[rw][k2], o[rw][dt]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    if (!whole && __any(zero != zero)) {
-#pragma unroll 1
-                        for (int kind = 0; kind < 3; ++kind)
-#pragma unroll
-                            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                                for (int rw = 0; rw < RW; ++rw) {
-                                    f32x16 marks;
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) marks[i] = 0.0f;
-#pragma unroll 1
-                                    for (int k2 = 0; k2 < 2; ++k2) {
-                                        u32x4 x = read_v(2 * h + k2, dt), sees;
-#pragma unroll
-                                        for (int w = 0; w < 4; ++w) {
-                                            x[w] = mark2<T>(x[w] & pair_mask(some >> (16 * k2), 8 * (w >> 1) + 2 * (w & 1)), kind);
-                                            sees[w] = pair_mask(seen[rw] >> (16 * k2), 8 * (w >> 1) + 2 * (w & 1)) & T::ONE_PAIR;
-                                        }
-                                        marks = mfma32x32x16<T>(x, sees, marks);
-                                    }
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) o[rw][dt][i] += marks[i] > 0.0f ? mark_value(kind) : 0.0f;
-                                    __builtin_amdgcn_sched_barrier(0);
-                                }
-                    }
+                    if (zero != zero) s_tainted[turn] = 1;
                 }
             }
             wait_vmcnt<0>();
@@ -1158,9 +1137,16 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
         }
 
         const bool done = first == 0 && n == count;
+        const bool tainted = s_tainted[turn] != 0;
+        if (tainted) {
+            const int group0 = (entry - b * a.row_groups) * Group;
+            slow_rows<T, D>(a, b, kvh, group0, min(Group, rows - group0), tiles, kKeys, first, n, done,
+                            (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept);
+        }
         uint16_t* ob = &kv[0][0][0] + wave * (32 * D);  // the wave's rows through LDS, a tile at a time, then whole rows to memory
 #pragma unroll
         for (int rw = 0; rw < RW; ++rw) {
+            if (tainted) break;
             float L = l[rw] + __shfl_xor(l[rw], 32, 64);
             float M = m[rw];
             if (last[rw] < 0) {  // padding took part where the tile was whole
@@ -1211,6 +1197,8 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
         if (u >= shares.end) return;
         slot = 1;
         if (kvh + 1 == a.kv_heads) ++entry;
+        if (t == 0) s_tainted[turn ^ 1] = 0;
+        turn ^= 1;
         __syncthreads();
     }
 }
