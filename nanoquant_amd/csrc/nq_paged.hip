@@ -1,5 +1,6 @@
 // A KV cache in pages: the rotary write of new tokens and the attention that reads it.
 #include <algorithm>
+#include <type_traits>
 
 #include "nq_common.h"
 #include "nq_wave.h"
@@ -815,7 +816,6 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const PagedArgs a, int g
 // ---------------------------------------------------------------- many rows
 
 constexpr int kKeys = 64;   // keys of a tile
-constexpr int kRowWaves = 4;
 
 // An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes.
 __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group, int entries) {
@@ -841,29 +841,38 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
     }
 }
 
-// Attention of many rows per sequence over its pages: blocks of 4 waves, 32 RW rows each (RW row tiles that share every key
-// and value read from LDS), over tiles of 64 keys, K and V row-major in LDS by DMA, two tiles in flight.
+// Attention of many rows per sequence over its pages, tiles of 64 keys that a block's waves share, K and V row-major in rings of
+// four tiles by DMA:
 //   S^T = K Q^T      v_mfma_f32_32x32x16, A = 32 keys x 16 dimensions, B = 32 rows of queries
 //   O^T += V^T P^T   A = 32 dimensions x 16 keys, read transposed, B = P^T: S^T's accumulator layout already, with keys
 //                    4 kg .. +3 and 8 + 4 kg .. +3 of each 16 in lane group kg
+// RW 2: 4 waves of 64 rows, which read every operand for two row tiles. One wave a SIMD, so its own instructions have to keep
+// both units busy: a step (32 keys) makes its exponentials among the products of the next step's scores and of the values of
+// the one before.
+// RW 1: 8 waves, 32 rows each, of which waves w and w + 4 have the same rows and a half each of every tile's keys: for grids
+// that leave a CU one block. Their sums are joined through LDS.
 // kShared: the work of all row groups in equal shares over the grid, as in few_kernel; otherwise a block takes a row group,
 // the last ones (the longest of a prompt) first.
 template <typename T, int D, int RW, bool kShared>
-__global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_kernel(const PagedArgs a) {
+    constexpr int NW = RW == 1 ? 8 : 4;  // waves
     constexpr int C = D / 8;             // 16-byte chunks of a row
     constexpr int RowsPer = 64 / C;      // rows of one DMA instruction
     constexpr int Instr = 16 / RowsPer;  // instructions for 16 rows
-    constexpr int Group = 32 * RW * kRowWaves;
-    constexpr int KT = D / 16, DT = D / 32;
-    __shared__ __attribute__((aligned(16))) uint16_t kv[2][2][kKeys * D];  // [buffer][K, V]
-    __shared__ int there[2][4];                                           // the page of a tile's 16 keys
-    __shared__ int spans[2][kRowWaves];
+    constexpr int Group = 128 * RW;
+    constexpr int KT = D / 16, DT = D / 32, KG = KT / 2;
+    constexpr int TileElems = kKeys * D;
+    constexpr bool kSkew = RW == 2 && D == 64;
+    __shared__ __attribute__((aligned(16))) uint16_t kring[4][TileElems], vring[4][TileElems];
+    __shared__ int there[4][4];  // the page of a tile's 16 keys
+    __shared__ int spans[2][4];
     __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
-    __shared__ int64_t wave_total[kRowWaves];
+    __shared__ int64_t wave_total[NW];
     __shared__ int s_entry;
     __shared__ int s_tainted[2];  // as few_kernel's
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int rwave = wave & 3, grp = wave >> 2;  // its rows, and of the two halves of RW 1
     const int c = lane & 31, kg = lane >> 5;
     const int entries = a.batch * a.row_groups;
 
@@ -872,8 +881,7 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
     int entry, slot = 0, turn = 0;
     int64_t u = 0;
     if constexpr (kShared) {
-        shares = make_shares<64 * kRowWaves, (RW == 1 ? 2 : 1) * kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry,
-                                                                      [&](int e) { return a.spans[e].z; });
+        shares = make_shares<64 * NW, kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry, [&](int e) { return a.spans[e].z; });
         if (shares.entry < 0) return;
         entry = shares.entry;
         u = shares.first;
@@ -892,14 +900,33 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
         koff[j] = static_cast<uint32_t>(row * D * 2 + 16 * (pos ^ (kswz & (C - 1))));
         voff[j] = static_cast<uint32_t>(row * D * 2 + 16 * (pos ^ vswz));
     }
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(&kv[0][0][0])) + static_cast<uint32_t>(wave) * (16 * D * 2);
+    const uint32_t klds = __builtin_amdgcn_readfirstlane(lds_addr(&kring[0][0])) + static_cast<uint32_t>(rwave) * (16 * D * 2);
+    const uint32_t vlds = __builtin_amdgcn_readfirstlane(lds_addr(&vring[0][0])) + static_cast<uint32_t>(rwave) * (16 * D * 2);
     // positive, so that the largest product is the largest score: the queries take a negative factor's sign, and are zero for
     // a factor of zero
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+    // the row of 16 keys that this lane names in a transposed read, and the place of its four dimensions
+    const int vr = 4 * kg + ((lane & 15) >> 2);
+    const int dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    auto read_k = [&](const uint16_t* half, int kt) {
+        const int kswz = D == 128 ? c : c >> 1;
+        return *vec(half + c * D + 8 * ((2 * kt + kg) ^ (kswz & (C - 1))));
+    };
+    auto read_v = [&](const uint16_t* half, int k2, int dt) {
+        uint2 part[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = vr + 8 * e;
+            const int vswz = D == 128 ? ((row & 3) << 2) | (row >> 2) : (((row >> 1) & 1) << 2) | (row >> 2);
+            const int d = 32 * dt + dim;
+            part[e] = read_transposed(half + (16 * k2 + row) * D + 8 * ((d >> 3) ^ vswz) + (d & 7));
+        }
+        return u32x4{part[0].x, part[0].y, part[1].x, part[1].y};
+    };
 
     while (true) {
         const int b = entry / a.row_groups;
-        const int row0 = (entry - b * a.row_groups) * Group + wave * (32 * RW);
+        const int row0 = (entry - b * a.row_groups) * Group + rwave * (32 * RW);
         const int rows = a.tokens * a.groups;
         int kvh, first = 0, n, count;
         int64_t seg = 0;
@@ -940,9 +967,12 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
 #pragma unroll
         for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) qf[rw][kt][w] = (qf[rw][kt][w] ^ flip) & keep_q;
+                // in accumulation registers, from which the products take them as they are: the vector registers hold the rest
+                if constexpr (RW == 2) asm volatile("" : "+a"(qf[rw][kt]));
+            }
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             lo = min(lo, __shfl_xor(lo, off, 64));
@@ -955,13 +985,13 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
         const int any_start = a.window > 0 ? max(0, lo == INT32_MAX ? 0 : lo - a.window + 1) : 0;  // the first key of some row
         if constexpr (!kShared) {
             if (lane == 0) {
-                spans[0][wave] = lo;
-                spans[1][wave] = hi;
+                spans[0][rwave] = lo;
+                spans[1][rwave] = hi;
             }
             __syncthreads();
             int blo = INT32_MAX, bhi = -1;
 #pragma unroll
-            for (int w = 0; w < kRowWaves; ++w) {
+            for (int w = 0; w < 4; ++w) {
                 blo = min(blo, spans[0][w]);
                 bhi = max(bhi, spans[1][w]);
             }
@@ -985,208 +1015,360 @@ __global__ __launch_bounds__(64 * kRowWaves, RW == 1 ? 2 : 1) void rows_kernel(c
         const __attribute__((address_space(4))) int32_t* table =
             (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
         // a wave brings a quarter of a tile: 16 keys, which lie in one page
-        auto issue = [&](int it, int buf) {
-            const int key = tiles.at(first + it) * kKeys + 16 * wave;
+        auto place = [&](int it, bool note) {
+            const int key = tiles.at(first + it) * kKeys + 16 * rwave;
             const int at = key / a.pages.page_size;
             int page = at < a.pages.table_pages ? table[at] : -1;
             page = page < a.pages.pages ? page : -1;
-            if (lane == 0) there[buf][wave] = page;
-            const int64_t from = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
-            const uint16_t *k_from = uniform(a.k_pages + from), *v_from = uniform(a.v_pages + from);
-            const uint32_t lds = lds0 + static_cast<uint32_t>(buf) * (2 * kKeys * D * 2);
-#pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(k_from, koff[j], lds + 1024u * j);
-#pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(v_from, voff[j], lds + kKeys * D * 2u + 1024u * j);
+            if (note && lane == 0) there[it & 3][rwave] = page;
+            return ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
         };
-        issue(0, 0);
-        wait_vmcnt<0>();
-        barrier_keep_dma();
-        for (int it = 0; it < n; ++it) {
-            const int buf = it & 1;
-            if (it + 1 < n) issue(it + 1, buf ^ 1);
-            const int key0 = tiles.at(first + it) * kKeys;
-            if (key0 <= hi && (key0 + kKeys > any_start || key0 < a.sinks)) {  // some row of the wave sees some key
-                const uint16_t* kb = kv[buf][0];
-                const uint16_t* vb = kv[buf][1];
-                // the row of 16 keys that this lane names in a transposed read, and the place of its four dimensions
-                const int vr = 4 * kg + ((lane & 15) >> 2);
-                const int dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                auto read_v = [&](int kt, int dt) {
-                    uint2 part[2];
+        auto issue_k = [&](int it, int64_t from) {
+            const uint16_t* p = uniform(a.k_pages + from);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int row = vr + 8 * e;
-                        const int vswz = D == 128 ? ((row & 3) << 2) | (row >> 2) : (((row >> 1) & 1) << 2) | (row >> 2);
-                        const int d = 32 * dt + dim;
-                        part[e] = read_transposed(vb + (16 * kt + row) * D + 8 * ((d >> 3) ^ vswz) + (d & 7));
+            for (int j = 0; j < Instr; ++j) dma16_lds(p, koff[j], klds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
+        };
+        auto issue_v = [&](int it, int64_t from) {
+            const uint16_t* p = uniform(a.v_pages + from);
+#pragma unroll
+            for (int j = 0; j < Instr; ++j) dma16_lds(p, voff[j], vlds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
+        };
+        auto live = [&](int key0) {  // some row of the wave sees some key of 32
+            return key0 <= hi && (key0 + 32 > any_start || key0 < a.sinks);
+        };
+        // scores that a row does not see become -inf; returns whether every row sees every key, and what some row sees: the
+        // lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
+        auto mask = [&](f32x16 (&s)[RW], int it, int h, uint32_t& some) {
+            const int half0 = tiles.at(first + it) * kKeys + 32 * h;
+            const int2 pg = *reinterpret_cast<const int2*>(&there[it & 3][2 * h]);
+            const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0) && half0 + 31 <= lo &&
+                               (half0 >= all_start || half0 + 32 <= a.sinks);
+            some = 0xFFFFFFFFu;
+            if (!whole) {
+                some = 0u;
+                const uint32_t pages_there = (pg.x >= 0 ? 0xFFFFu : 0u) | (pg.y >= 0 ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (int rw = 0; rw < RW; ++rw) {
+                    const uint32_t seen = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
+                    some |= seen;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen, 8 * (i >> 2) + (i & 3));
+                }
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
+            }
+            return whole;
+        };
+        // The reference point of the exponentials follows the running maximum only once that is 8 above it: exponentials up to
+        // 2^8 round the same, and most steps rescale nothing. What the sums so far have to be multiplied by, if so.
+        auto follow = [&](const f32x16 (&s)[RW], float (&keep)[RW]) {
+            float top[RW];
+            bool grows = false;
+#pragma unroll
+            for (int rw = 0; rw < RW; ++rw) {
+                top[rw] = s[rw][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top[rw] = fmaxf(top[rw], s[rw][i]);
+                top[rw] = max_xor32(top[rw]) * scale;
+                grows |= top[rw] > m[rw] + kSlack;
+            }
+            const bool any = __any(grows);
+            if (any) {
+#pragma unroll
+                for (int rw = 0; rw < RW; ++rw) {
+                    const float mn = fmaxf(m[rw], top[rw]);
+                    keep[rw] = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
+                    m[rw] = mn;
+                    l[rw] *= keep[rw];
+                }
+            }
+            return any;
+        };
+        auto rescale = [&](const float (&keep)[RW]) {
+#pragma unroll
+            for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep[rw];
+        };
+        // two probabilities of a row tile, rounded, and into its sum as rounded
+        auto prob2 = [&](const f32x16 (&s)[RW], u32x4 (&p)[RW][2], int rw, int w) {
+            const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
+            p[rw][w >> 2][w & 3] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][2 * w], scale, -mu)),
+                                            __builtin_amdgcn_exp2f(fmaf(s[rw][2 * w + 1], scale, -mu)));
+            l[rw] = T::dot2(p[rw][w >> 2][w & 3], T::ONE_PAIR, l[rw]);
+        };
+        // O^T += V^T P^T of 32 keys; values that no row sees are cleared
+        auto values = [&](const uint16_t* half, const u32x4 (&p)[RW][2], bool whole, uint32_t some) {
+            float zero = 0.0f;
+            u32x4 vf[2][DT];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = read_v(half, 0, dt);
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+                if (k2 == 0) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) vf[1][dt] = read_v(half, 1, dt);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (!whole) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t keep = pair_mask(some, 16 * k2 + 8 * (w >> 1) + 2 * (w & 1));
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            vf[k2][dt][w] &= keep;
+                            zero = T::dot2(vf[k2][dt][w], 0u, zero);  // NaN where one is not finite
+                        }
                     }
-                    return u32x4{part[0].x, part[0].y, part[1].x, part[1].y};
-                };
-                // operands are read a group of four ahead of the products that run; left to itself the compiler reads all of
-                // them first, or two and waits
-                u32x4 kf[2][4], vf[2][DT];
-                auto read_ks = [&](int h, int q) {
-                    const int kswz = D == 128 ? c : c >> 1;
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        kf[q & 1][e] = *vec(kb + (32 * h + c) * D + 8 * ((2 * (4 * q + e) + kg) ^ (kswz & (C - 1))));
-                };
-                auto read_vs = [&](int kt) {
+                for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) vf[kt & 1][dt] = read_v(kt, dt);
-                };
+                    for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[k2][dt], p[rw][k2], o[rw][dt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (zero != zero) s_tainted[turn] = 1;
+        };
+        // S^T = K Q^T of 32 keys, operands read ahead of the products that run
+        auto scores = [&](const uint16_t* half, f32x16 (&s)[RW]) {
+            u32x4 kf[2][KG];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {  // 32 keys at a time
-                    const int half0 = key0 + 32 * h;
-                    const int2 pg = *reinterpret_cast<const int2*>(&there[buf][2 * h]);
-                    const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0) && half0 + 31 <= lo &&
-                                       (half0 >= all_start || half0 + 32 <= a.sinks);
+            for (int e = 0; e < KG; ++e) kf[0][e] = read_k(half, e);
+#pragma unroll
+            for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[rw][i] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (q == 0) {
+#pragma unroll
+                    for (int e = 0; e < KG; ++e) kf[1][e] = read_k(half, KG + e);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < KG; ++e)
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw) s[rw] = mfma32x32x16<T>(kf[q][e], qf[rw][KG * q + e], s[rw]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+
+        if constexpr (!kSkew) {
+            // with two groups of waves, the first brings keys, the other values, three tiles ahead
+            constexpr int kOut = RW == 1 ? Instr : 2 * Instr;  // of a wave, a tile
+            auto issue = [&](int it) {
+                const int64_t from = place(it, grp == 0);
+                if (grp == 0) issue_k(it, from);
+                if (RW == 2 || grp == 1) issue_v(it, from);
+            };
+            for (int it = 0; it < 3 && it < n; ++it) issue(it);
+            for (int it = 0; it < n; ++it) {
+                const int behind = min(n - 1 - it, 2);  // tiles out behind this one
+                if (behind == 2) wait_vmcnt<2 * kOut>();
+                else if (behind == 1) wait_vmcnt<kOut>();
+                else wait_vmcnt<0>();
+                barrier_keep_dma();
+                if (it + 3 < n) issue(it + 3);  // where the tile before this one was
+#pragma unroll
+                for (int hh = 0; hh < RW; ++hh) {
+                    const int h = RW == 1 ? grp : hh;
+                    if (!live(tiles.at(first + it) * kKeys + 32 * h)) continue;
                     f32x16 s[RW];
+                    scores(kring[it & 3] + 32 * h * D, s);
+                    uint32_t some;
+                    const bool whole = mask(s, it, h, some);
+                    float keep[RW];
+                    if (follow(s, keep)) rescale(keep);
+                    u32x4 p[RW][2];
 #pragma unroll
                     for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) s[rw][i] = 0.0f;
-                    read_ks(h, 0);
-#pragma unroll
-                    for (int q = 0; q < KT / 4; ++q) {
-                        if (q + 1 < KT / 4) read_ks(h, q + 1);
-                        else read_vs(2 * h);
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int rw = 0; rw < RW; ++rw) s[rw] = mfma32x32x16<T>(kf[q & 1][e], qf[rw][4 * q + e], s[rw]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    uint32_t some = 0u;  // seen by some row, the lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
-                    if (!whole) {
-                        const uint32_t pages_there = (pg.x >= 0 ? 0xFFFFu : 0u) | (pg.y >= 0 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                        for (int rw = 0; rw < RW; ++rw) {
-                            const uint32_t seen = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
-                            some |= seen;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen, 8 * (i >> 2) + (i & 3));
-                        }
-#pragma unroll
-                        for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
-                    }
-                    // the reference point of the exponentials follows the running maximum only once that is 8 above it
-                    u32x4 pf[RW][2];
-                    float top[RW];
-                    bool grows = false;
-#pragma unroll
-                    for (int rw = 0; rw < RW; ++rw) {
-                        top[rw] = s[rw][0];
-#pragma unroll
-                        for (int i = 1; i < 16; ++i) top[rw] = fmaxf(top[rw], s[rw][i]);
-                        top[rw] = max_xor32(top[rw]) * scale;
-                        grows |= top[rw] > m[rw] + kSlack;
-                    }
-                    if (__any(grows)) {
-#pragma unroll
-                        for (int rw = 0; rw < RW; ++rw) {
-                            const float mn = fmaxf(m[rw], top[rw]);
-                            const float keep = __builtin_amdgcn_exp2f(m[rw] - (mn == -INFINITY ? 0.0f : mn));
-                            m[rw] = mn;
-                            l[rw] *= keep;
-#pragma unroll
-                            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep;
-                        }
-                    }
-#pragma unroll
-                    for (int rw = 0; rw < RW; ++rw) {
-                        const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
-#pragma unroll
-                        for (int w = 0; w < 8; ++w) {
-                            pf[rw][w >> 2][w & 3] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][2 * w], scale, -mu)),
-                                                             __builtin_amdgcn_exp2f(fmaf(s[rw][2 * w + 1], scale, -mu)));
-                            l[rw] = T::dot2(pf[rw][w >> 2][w & 3], T::ONE_PAIR, l[rw]);
-                        }
-                    }
-                    float zero = 0.0f;
-#pragma unroll
-                    for (int k2 = 0; k2 < 2; ++k2) {
-                        if (k2 == 0) read_vs(2 * h + 1);
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (!whole) {  // values that no row sees are cleared
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const uint32_t keep = pair_mask(some, 16 * k2 + 8 * (w >> 1) + 2 * (w & 1));
-#pragma unroll
-                                for (int dt = 0; dt < DT; ++dt) {
-                                    vf[k2][dt][w] &= keep;
-                                    zero = T::dot2(vf[k2][dt][w], 0u, zero);  // NaN where one is not finite
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[k2][dt], pf[rw][k2], o[rw][dt]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    if (zero != zero) s_tainted[turn] = 1;
+                        for (int w = 0; w < 8; ++w) prob2(s, p, rw, w);
+                    values(vring[it & 3] + 32 * h * D, p, whole, some);
                 }
             }
-            wait_vmcnt<0>();
-            barrier_keep_dma();
+        } else {
+            // At the start of iteration it: the keys of the next tile too and the values of this one have come (they went out two
+            // iterations ago); those of tiles it + 3 and it + 2 go out, where tiles it - 1 and it - 2 were.
+            int64_t from = 0;  // of the last tile whose keys went out
+            auto issue = [&](int it) {
+                if (it + 2 >= 0 && it + 2 < n) issue_v(it + 2, from);
+                if (it + 3 < n) {
+                    from = place(it + 3, true);
+                    issue_k(it + 3, from);
+                }
+            };
+            for (int it = -3; it < 0; ++it) issue(it);
+            f32x16 s[2][RW];     // of the tile's halves
+            u32x4 p[2][RW][2];
+            int pending = 0;     // whether the last step's values are still to be added: 1, or 2 where they need a mask
+            uint32_t pending_some = 0;
+            for (int it = 0; it < n; ++it) {
+                const int behind = (it + 2 < n ? 1 : 0) + (it + 1 < n ? 1 : 0);  // parts that went out in the last iteration
+                if (behind == 2) wait_vmcnt<2 * Instr>();
+                else if (behind == 1) wait_vmcnt<Instr>();
+                else wait_vmcnt<0>();
+                barrier_keep_dma();
+                issue(it);
+                if (it == 0) scores(kring[0], s[0]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint16_t* next_k = h == 0 ? kring[it & 3] + 32 * D : kring[(it + 1) & 3];
+                    const uint16_t* last_v = h == 0 ? vring[(it + 3) & 3] + 32 * D : vring[it & 3];
+                    if (!live(tiles.at(first + it) * kKeys + 32 * h)) {
+                        if (pending) values(last_v, p[h ^ 1], pending == 1, pending_some);
+                        pending = 0;
+                        scores(next_k, s[h ^ 1]);
+                        continue;
+                    }
+                    uint32_t some;
+                    const bool whole = mask(s[h], it, h, some);
+                    float keep[RW];
+                    const bool grew = follow(s[h], keep);
+                    if (pending == 2) values(last_v, p[h ^ 1], false, pending_some);
+                    auto step = [&](auto with) {
+                        constexpr bool kValues = decltype(with)::value;
+                        u32x4 kf[2][KG], vf[2][DT];
+#pragma unroll
+                        for (int e = 0; e < KG; ++e) kf[0][e] = read_k(next_k, e);
+                        if constexpr (kValues) {
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = read_v(last_v, 0, dt);
+                        }
+#pragma unroll
+                        for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) s[h ^ 1][rw][i] = 0.0f;
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {  // a quarter of the exponentials with a group of products each
+                            if (q == 0) {
+#pragma unroll
+                                for (int e = 0; e < KG; ++e) kf[1][e] = read_k(next_k, KG + e);
+                            }
+                            if constexpr (kValues) {
+                                if (q == 1) {
+#pragma unroll
+                                    for (int dt = 0; dt < DT; ++dt) vf[1][dt] = read_v(last_v, 1, dt);
+                                }
+                            }
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) prob2(s[h], p[h], q >> 1, 4 * (q & 1) + w);
+                            if (q % 2 == 0) {
+#pragma unroll
+                                for (int e = 0; e < KG; ++e)
+#pragma unroll
+                                    for (int rw = 0; rw < RW; ++rw)
+                                        s[h ^ 1][rw] = mfma32x32x16<T>(kf[q >> 1][e], qf[rw][KG * (q >> 1) + e], s[h ^ 1][rw]);
+                            } else if constexpr (kValues) {
+#pragma unroll
+                                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                                    for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q >> 1][dt], p[h ^ 1][rw][q >> 1], o[rw][dt]);
+                            }
+                            if (q % 2 == 0 || kValues) {
+#pragma unroll
+                                for (int x = 0; x < KG * RW; ++x) {
+                                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a product,
+                                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // an LDS read,
+                                    __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 3 : 6, 0);  // and vector instructions
+                                }
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    };
+                    if (pending == 1) step(std::true_type{});
+                    else step(std::false_type{});
+                    if (grew) rescale(keep);
+                    pending = whole ? 1 : 2;
+                    pending_some = some;
+                }
+            }
+            if (pending) values(vring[(n - 1) & 3] + 32 * D, p[1], pending == 1, pending_some);
         }
 
         const bool done = first == 0 && n == count;
+        __syncthreads();
         const bool tainted = s_tainted[turn] != 0;
         if (tainted) {
             const int group0 = (entry - b * a.row_groups) * Group;
             slow_rows<T, D>(a, b, kvh, group0, min(Group, rows - group0), tiles, kKeys, first, n, done,
                             (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept);
         }
-        uint16_t* ob = &kv[0][0][0] + wave * (32 * D);  // the wave's rows through LDS, a tile at a time, then whole rows to memory
+        // the halves' sums: the second group's through the key ring, its statistics through the value ring's first 2 KB
+        if (RW == 1 && !tainted) {
+            float* red = reinterpret_cast<float*>(&kring[0][0]);
+            float* stat = reinterpret_cast<float*>(&vring[0][0]);
+            static_assert(RW == 2 || sizeof(kring) >= DT * 16 * 256 * sizeof(float), "the key ring holds a group's sums");
+            if (grp == 1) {
 #pragma unroll
-        for (int rw = 0; rw < RW; ++rw) {
-            if (tainted) break;
-            float L = l[rw] + __shfl_xor(l[rw], 32, 64);
-            float M = m[rw];
-            if (last[rw] < 0) {  // padding took part where the tile was whole
-                L = 0.0f;
-                M = -INFINITY;
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) red[(16 * dt + i) * 256 + (t & 255)] = o[0][dt][i];
+                stat[t & 255] = m[0];
+                stat[256 + (t & 255)] = l[0];
             }
-            const float inv = 1.0f / L;
-            if (kShared && !done) {
-                const int at = wave * (32 * RW) + 32 * rw + c;
-                if (row0 + 32 * rw + c < rows) {
-                    const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept + at;
-                    if (kg == 0) a.part_ml[part] = float2{M, L};
+            __syncthreads();
+            if (grp == 0) {
+                const float m1 = stat[t], mn = fmaxf(m[0], m1);
+                const float mu = mn == -INFINITY ? 0.0f : mn;
+                const float f0 = __builtin_amdgcn_exp2f(m[0] - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+                m[0] = mn;
+                l[0] = l[0] * f0 + stat[256 + t] * f1;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
+                for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                        for (int g4 = 0; g4 < 4; ++g4) {
-                            f32x4 x;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e];
-                            *reinterpret_cast<f32x4*>(a.part_o + part * D + 32 * dt + 8 * g4 + 4 * kg) = x;
-                        }
-                }
-                continue;
+                    for (int i = 0; i < 16; ++i) o[0][dt][i] = o[0][dt][i] * f0 + red[(16 * dt + i) * 256 + t] * f1;
             }
+        }
+        // a wave's rows through LDS, a row tile at a time, then whole rows to memory
+        uint16_t* ob = (RW == 1 ? &vring[0][0] + 1024 : &kring[0][0]) + rwave * (32 * D);
+        if (grp == 0 && !tainted) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+            for (int rw = 0; rw < RW; ++rw) {
+                float L = l[rw] + __shfl_xor(l[rw], 32, 64);
+                float M = m[rw];
+                if (last[rw] < 0) {  // padding took part where the tile was whole
+                    L = 0.0f;
+                    M = -INFINITY;
+                }
+                const float inv = 1.0f / L;
+                if (kShared && !done) {
+                    const int at = rwave * (32 * RW) + 32 * rw + c;
+                    if (row0 + 32 * rw + c < rows) {
+                        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept + at;
+                        if (kg == 0) a.part_ml[part] = float2{M, L};
 #pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    float x[4];
+                        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e] * inv;
-                    *reinterpret_cast<uint2*>(ob + c * D + 8 * ((4 * dt + g4) ^ (c & (C - 1))) + 4 * kg) =
-                        uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+                            for (int g4 = 0; g4 < 4; ++g4) {
+                                f32x4 x;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e];
+                                *reinterpret_cast<f32x4*>(a.part_o + part * D + 32 * dt + 8 * g4 + 4 * kg) = x;
+                            }
+                    }
+                    continue;
                 }
 #pragma unroll
-            for (int j = 0; j < 32 / RowsPer; ++j) {
-                const int r = RowsPer * j + lane / C, ch = lane % C;
-                const u32x4 v = *vec(ob + r * D + 8 * (ch ^ (r & (C - 1))));
-                const int at_row = row0 + 32 * rw + r;
-                if (at_row < rows) *reinterpret_cast<u32x4*>(a.out + out_row(a, b, kvh, at_row) * D + 8 * ch) = v;
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e] * inv;
+                        *reinterpret_cast<uint2*>(ob + c * D + 8 * ((4 * dt + g4) ^ (c & (C - 1))) + 4 * kg) =
+                            uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+                    }
+#pragma unroll
+                for (int j = 0; j < 32 / RowsPer; ++j) {
+                    const int r = RowsPer * j + lane / C, ch = lane % C;
+                    const u32x4 v = *vec(ob + r * D + 8 * (ch ^ (r & (C - 1))));
+                    const int at_row = row0 + 32 * rw + r;
+                    if (at_row < rows) *reinterpret_cast<u32x4*>(a.out + out_row(a, b, kvh, at_row) * D + 8 * ch) = v;
+                }
             }
         }
         if constexpr (!kShared) return;
@@ -1231,7 +1413,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
             p.tiles = large >= kCUs / 2 ? 2 : 1;
         }
         p.group = 128 * p.tiles;
-        p.blocks = p.tiles == 2 ? kCUs : 2 * kCUs;
+        p.blocks = kCUs;
     }
     p.row_groups = ceil_div(rows, p.group);
     p.rows_kept = std::min(rows, p.group);
@@ -1267,11 +1449,11 @@ void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
     } else if (plan.shared) {
         const int entries = a.batch * a.row_groups;
         spans_kernel<<<dim3(static_cast<unsigned>(ceil_div(entries, 4))), 256, 0, st>>>(a, static_cast<int>(plan.group), entries);
-        if (plan.tiles == 1) rows_kernel<T, D, 1, true><<<grid, 64 * kRowWaves, 0, st>>>(a);
-        else rows_kernel<T, D, 2, true><<<grid, 64 * kRowWaves, 0, st>>>(a);
+        if (plan.tiles == 1) rows_kernel<T, D, 1, true><<<grid, 512, 0, st>>>(a);
+        else rows_kernel<T, D, 2, true><<<grid, 256, 0, st>>>(a);
     } else {
-        if (plan.tiles == 1) rows_kernel<T, D, 1, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
-        else rows_kernel<T, D, 2, false><<<dim3(segs), 64 * kRowWaves, 0, st>>>(a);
+        if (plan.tiles == 1) rows_kernel<T, D, 1, false><<<dim3(segs), 512, 0, st>>>(a);
+        else rows_kernel<T, D, 2, false><<<dim3(segs), 256, 0, st>>>(a);
     }
     const int group = static_cast<int>(plan.group);
     if (plan.few) few_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(a.rows_kept)), 256, 0, st>>>(a, group);
