@@ -841,6 +841,17 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
     }
 }
 
+// Asks the scheduler for products one by one, each followed by an LDS read where there is one and kOther vector instructions.
+template <int kProducts, int kOther>
+__device__ inline void interleave() {
+#pragma unroll
+    for (int x = 0; x < kProducts; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kOther, 0);
+    }
+}
+
 // Attention of many rows per sequence over its pages, tiles of 64 keys that a block's waves share, K and V row-major in rings of
 // four tiles by DMA:
 //   S^T = K Q^T      v_mfma_f32_32x32x16, A = 32 keys x 16 dimensions, B = 32 rows of queries
@@ -862,7 +873,6 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
     constexpr int Group = 128 * RW;
     constexpr int KT = D / 16, DT = D / 32, KG = KT / 2;
     constexpr int TileElems = kKeys * D;
-    constexpr bool kSkew = RW == 2 && D == 64;
     __shared__ __attribute__((aligned(16))) uint16_t kring[4][TileElems], vring[4][TileElems];
     __shared__ int there[4][4];  // the page of a tile's 16 keys
     __shared__ int spans[2][4];
@@ -1038,15 +1048,13 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         };
         // scores that a row does not see become -inf; returns whether every row sees every key, and what some row sees: the
         // lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
-        auto mask = [&](f32x16 (&s)[RW], int it, int h, uint32_t& some) {
-            const int half0 = tiles.at(first + it) * kKeys + 32 * h;
-            const int2 pg = *reinterpret_cast<const int2*>(&there[it & 3][2 * h]);
-            const bool whole = __builtin_amdgcn_readfirstlane(pg.x >= 0 && pg.y >= 0) && half0 + 31 <= lo &&
+        auto mask = [&](f32x16 (&s)[RW], int half0, int page0, int page1, uint32_t& some) {
+            const bool whole = __builtin_amdgcn_readfirstlane((page0 | page1) >= 0) && half0 + 31 <= lo &&
                                (half0 >= all_start || half0 + 32 <= a.sinks);
             some = 0xFFFFFFFFu;
             if (!whole) {
                 some = 0u;
-                const uint32_t pages_there = (pg.x >= 0 ? 0xFFFFu : 0u) | (pg.y >= 0 ? 0xFFFF0000u : 0u);
+                const uint32_t pages_there = (page0 >= 0 ? 0xFFFFu : 0u) | (page1 >= 0 ? 0xFFFF0000u : 0u);
 #pragma unroll
                 for (int rw = 0; rw < RW; ++rw) {
                     const uint32_t seen = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
@@ -1155,138 +1163,121 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             }
         };
 
-        if constexpr (!kSkew) {
-            // with two groups of waves, the first brings keys, the other values, three tiles ahead
-            constexpr int kOut = RW == 1 ? Instr : 2 * Instr;  // of a wave, a tile
-            auto issue = [&](int it) {
-                const int64_t from = place(it, grp == 0);
-                if (grp == 0) issue_k(it, from);
-                if (RW == 2 || grp == 1) issue_v(it, from);
-            };
-            for (int it = 0; it < 3 && it < n; ++it) issue(it);
-            for (int it = 0; it < n; ++it) {
-                const int behind = min(n - 1 - it, 2);  // tiles out behind this one
-                if (behind == 2) wait_vmcnt<2 * kOut>();
-                else if (behind == 1) wait_vmcnt<kOut>();
-                else wait_vmcnt<0>();
-                barrier_keep_dma();
-                if (it + 3 < n) issue(it + 3);  // where the tile before this one was
-#pragma unroll
-                for (int hh = 0; hh < RW; ++hh) {
-                    const int h = RW == 1 ? grp : hh;
-                    if (!live(tiles.at(first + it) * kKeys + 32 * h)) continue;
-                    f32x16 s[RW];
-                    scores(kring[it & 3] + 32 * h * D, s);
-                    uint32_t some;
-                    const bool whole = mask(s, it, h, some);
+        // with two groups of waves, the first brings keys, the other values, three tiles ahead
+        constexpr int kOut = RW == 1 ? Instr : 2 * Instr;  // of a wave, a tile
+        auto issue = [&](int it) {
+            const int64_t from = place(it, grp == 0);
+            if (grp == 0) issue_k(it, from);
+            if (RW == 2 || grp == 1) issue_v(it, from);
+        };
+        for (int it = 0; it < 3 && it < n; ++it) issue(it);
+        int4 pages4;
+        int key0;
+        auto come = [&](int it) {  // waits for a tile, and sends for one where the tile before it was
+            const int behind = min(n - 1 - it, 2);  // tiles out behind this one
+            if (behind == 2) wait_vmcnt<2 * kOut>();
+            else if (behind == 1) wait_vmcnt<kOut>();
+            else wait_vmcnt<0>();
+            barrier_keep_dma();
+            pages4 = *reinterpret_cast<const int4*>(&there[it & 3][0]);
+            if (it + 3 < n) issue(it + 3);
+            key0 = tiles.at(first + it) * kKeys;
+        };
+        auto all_whole = [&] {  // every row sees all of the tile
+            return __builtin_amdgcn_readfirstlane((pages4.x | pages4.y | pages4.z | pages4.w) >= 0) && key0 + kKeys - 1 <= lo &&
+                   (key0 >= all_start || key0 + kKeys <= a.sinks);
+        };
+        int it = 0;
+        come(0);
+        while (it < n) {
+            if constexpr (RW == 2) {
+                // tiles that every row sees whole, in a loop of their own (with the others in one, its registers did not
+                // suffice): the exponentials of a half among the products of the other
+                while (all_whole()) {
+                    const uint16_t* kt0 = kring[it & 3];
+                    const uint16_t* vt0 = vring[it & 3];
+                    f32x16 s[2][RW];
+                    u32x4 p[2][RW][2], kf[2][KG], vf[2][DT];
                     float keep[RW];
-                    if (follow(s, keep)) rescale(keep);
-                    u32x4 p[RW][2];
+                    scores(kt0, s[0]);
+#pragma unroll
+                    for (int e = 0; e < KG; ++e) kf[0][e] = read_k(kt0 + 32 * D, e);
+                    if (follow(s[0], keep)) rescale(keep);
 #pragma unroll
                     for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
-                        for (int w = 0; w < 8; ++w) prob2(s, p, rw, w);
-                    values(vring[it & 3] + 32 * h * D, p, whole, some);
-                }
-            }
-        } else {
-            // At the start of iteration it: the keys of the next tile too and the values of this one have come (they went out two
-            // iterations ago); those of tiles it + 3 and it + 2 go out, where tiles it - 1 and it - 2 were.
-            int64_t from = 0;  // of the last tile whose keys went out
-            auto issue = [&](int it) {
-                if (it + 2 >= 0 && it + 2 < n) issue_v(it + 2, from);
-                if (it + 3 < n) {
-                    from = place(it + 3, true);
-                    issue_k(it + 3, from);
-                }
-            };
-            for (int it = -3; it < 0; ++it) issue(it);
-            f32x16 s[2][RW];     // of the tile's halves
-            u32x4 p[2][RW][2];
-            int pending = 0;     // whether the last step's values are still to be added: 1, or 2 where they need a mask
-            uint32_t pending_some = 0;
-            for (int it = 0; it < n; ++it) {
-                const int behind = (it + 2 < n ? 1 : 0) + (it + 1 < n ? 1 : 0);  // parts that went out in the last iteration
-                if (behind == 2) wait_vmcnt<2 * Instr>();
-                else if (behind == 1) wait_vmcnt<Instr>();
-                else wait_vmcnt<0>();
-                barrier_keep_dma();
-                issue(it);
-                if (it == 0) scores(kring[0], s[0]);
+                        for (int i = 0; i < 16; ++i) s[1][rw][i] = 0.0f;
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint16_t* next_k = h == 0 ? kring[it & 3] + 32 * D : kring[(it + 1) & 3];
-                    const uint16_t* last_v = h == 0 ? vring[(it + 3) & 3] + 32 * D : vring[it & 3];
-                    if (!live(tiles.at(first + it) * kKeys + 32 * h)) {
-                        if (pending) values(last_v, p[h ^ 1], pending == 1, pending_some);
-                        pending = 0;
-                        scores(next_k, s[h ^ 1]);
-                        continue;
-                    }
-                    uint32_t some;
-                    const bool whole = mask(s[h], it, h, some);
-                    float keep[RW];
-                    const bool grew = follow(s[h], keep);
-                    if (pending == 2) values(last_v, p[h ^ 1], false, pending_some);
-                    auto step = [&](auto with) {
-                        constexpr bool kValues = decltype(with)::value;
-                        u32x4 kf[2][KG], vf[2][DT];
+                    for (int q = 0; q < 2; ++q) {
 #pragma unroll
-                        for (int e = 0; e < KG; ++e) kf[0][e] = read_k(next_k, e);
-                        if constexpr (kValues) {
-#pragma unroll
-                            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = read_v(last_v, 0, dt);
+                        for (int e = 0; e < KG; ++e) {
+                            if (q == 0) kf[1][e] = read_k(kt0 + 32 * D, KG + e);
+                            else if (e < DT) vf[0][e] = read_v(vt0, 0, e);
                         }
 #pragma unroll
-                        for (int rw = 0; rw < RW; ++rw)
+                        for (int w = 0; w < 8; ++w) prob2(s[0], p[0], q, w);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) s[h ^ 1][rw][i] = 0.0f;
+                        for (int e = 0; e < KG; ++e)
+#pragma unroll
+                            for (int rw = 0; rw < RW; ++rw) s[1][rw] = mfma32x32x16<T>(kf[q][e], qf[rw][KG * q + e], s[1][rw]);
+                        interleave<KG * RW, 52 / (KG * RW)>();
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const bool grew = follow(s[1], keep);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) vf[1 - q][dt] = q == 0 ? read_v(vt0, 1, dt) : read_v(vt0 + 32 * D, 0, dt);
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) prob2(s[1], p[1], q, w);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q][dt], p[0][rw][q], o[rw][dt]);
+                        interleave<DT * RW, 52 / (DT * RW)>();
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (grew) rescale(keep);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        if (q == 0) {
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt) vf[1][dt] = read_v(vt0 + 32 * D, 1, dt);
+                        }
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {  // a quarter of the exponentials with a group of products each
-                            if (q == 0) {
+                        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                                for (int e = 0; e < KG; ++e) kf[1][e] = read_k(next_k, KG + e);
-                            }
-                            if constexpr (kValues) {
-                                if (q == 1) {
-#pragma unroll
-                                    for (int dt = 0; dt < DT; ++dt) vf[1][dt] = read_v(last_v, 1, dt);
-                                }
-                            }
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) prob2(s[h], p[h], q >> 1, 4 * (q & 1) + w);
-                            if (q % 2 == 0) {
-#pragma unroll
-                                for (int e = 0; e < KG; ++e)
-#pragma unroll
-                                    for (int rw = 0; rw < RW; ++rw)
-                                        s[h ^ 1][rw] = mfma32x32x16<T>(kf[q >> 1][e], qf[rw][KG * (q >> 1) + e], s[h ^ 1][rw]);
-                            } else if constexpr (kValues) {
-#pragma unroll
-                                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                                    for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q >> 1][dt], p[h ^ 1][rw][q >> 1], o[rw][dt]);
-                            }
-                            if (q % 2 == 0 || kValues) {
-#pragma unroll
-                                for (int x = 0; x < KG * RW; ++x) {
-                                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a product,
-                                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // an LDS read,
-                                    __builtin_amdgcn_sched_group_barrier(0x002, D == 128 ? 3 : 6, 0);  // and vector instructions
-                                }
-                            }
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    };
-                    if (pending == 1) step(std::true_type{});
-                    else step(std::false_type{});
-                    if (grew) rescale(keep);
-                    pending = whole ? 1 : 2;
-                    pending_some = some;
+                            for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q][dt], p[1][rw][q], o[rw][dt]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (++it == n) break;
+                    come(it);
                 }
+                if (it == n) break;
             }
-            if (pending) values(vring[(n - 1) & 3] + 32 * D, p[1], pending == 1, pending_some);
+            const uint16_t* kt0 = kring[it & 3];
+            const uint16_t* vt0 = vring[it & 3];
+#pragma unroll
+            for (int hh = 0; hh < RW; ++hh) {
+                const int h = RW == 1 ? grp : hh;
+                if (!live(key0 + 32 * h)) continue;
+                f32x16 s[RW];
+                scores(kt0 + 32 * h * D, s);
+                uint32_t some;
+                const bool whole = mask(s, key0 + 32 * h, h ? pages4.z : pages4.x, h ? pages4.w : pages4.y, some);
+                float keep[RW];
+                if (follow(s, keep)) rescale(keep);
+                u32x4 p[RW][2];
+#pragma unroll
+                for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) prob2(s, p, rw, w);
+                values(vt0 + 32 * h * D, p, whole, some);
+            }
+            if (++it < n) come(it);
         }
 
         const bool done = first == 0 && n == count;
