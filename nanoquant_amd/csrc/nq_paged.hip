@@ -1239,6 +1239,9 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                         interleave<DT * RW, 52 / (DT * RW)>();
                         __builtin_amdgcn_sched_barrier(0);
                     }
+                    // or they are made behind the branch, where they are used
+#pragma unroll
+                    for (int rw = 0; rw < RW; ++rw) asm volatile("" : "+v"(p[1][rw][0]), "+v"(p[1][rw][1]));
                     if (grew) rescale(keep);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
