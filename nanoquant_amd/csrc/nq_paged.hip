@@ -841,17 +841,6 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
     }
 }
 
-// Asks the scheduler for products one by one, each followed by an LDS read where there is one and kOther vector instructions.
-template <int kProducts, int kOther>
-__device__ inline void interleave() {
-#pragma unroll
-    for (int x = 0; x < kProducts; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, kOther, 0);
-    }
-}
-
 // Attention of many rows per sequence over its pages, tiles of 64 keys that a block's waves share, K and V row-major in rings of
 // four tiles by DMA:
 //   S^T = K Q^T      v_mfma_f32_32x32x16, A = 32 keys x 16 dimensions, B = 32 rows of queries
@@ -874,7 +863,6 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
     constexpr int KT = D / 16, DT = D / 32, KG = KT / 2;
     constexpr int TileElems = kKeys * D;
     __shared__ __attribute__((aligned(16))) uint16_t kring[4][TileElems], vring[4][TileElems];
-    __shared__ int there[4][4];  // the page of a tile's 16 keys
     __shared__ int spans[2][4];
     __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
     __shared__ int64_t wave_total[NW];
@@ -1022,16 +1010,30 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[rw][dt][i] = 0.0f;
         }
-        const __attribute__((address_space(4))) int32_t* table =
-            (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
-        // a wave brings a quarter of a tile: 16 keys, which lie in one page
-        auto place = [&](int it, bool note) {
-            const int key = tiles.at(first + it) * kKeys + 16 * rwave;
-            const int at = key / a.pages.page_size;
-            int page = at < a.pages.table_pages ? table[at] : -1;
-            page = page < a.pages.pages ? page : -1;
-            if (note && lane == 0) there[it & 3][rwave] = page;
-            return ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
+        // a wave brings a quarter of a tile: 16 keys, which lie in one page. Where they are, for 64 tiles at a time, a lane each:
+        // a scalar load and a division for every tile stood in its way
+        int my_page = 0, my_rest = 0, my_there = 0;
+        uint32_t there = 0u;  // bit 4 (it % 4) + i: the page of keys 16 i .. +15 of tile `it` is there
+        auto look_up = [&](int it) {
+            const int key = tiles.at(first + min(it + lane, n - 1)) * kKeys;
+            my_there = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (key + 16 * i) / a.pages.page_size;
+                const int page = at < a.pages.table_pages ? a.pages.page(b, at) : -1;
+                my_there |= page >= 0 ? 1 << i : 0;
+                if (i == rwave) {
+                    my_page = max(page, 0);
+                    my_rest = key + 16 * i - at * a.pages.page_size;
+                }
+            }
+        };
+        auto place = [&](int it) {
+            if ((it & 63) == 0) look_up(it);
+            const int at = it & 63, by = 4 * (it & 3);
+            there = (there & ~(15u << by)) | static_cast<uint32_t>(__builtin_amdgcn_readlane(my_there, at)) << by;
+            const int page = __builtin_amdgcn_readlane(my_page, at), rest = __builtin_amdgcn_readlane(my_rest, at);
+            return ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + rest) * D;
         };
         auto issue_k = [&](int it, int64_t from) {
             const uint16_t* p = uniform(a.k_pages + from);
@@ -1048,13 +1050,12 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         };
         // scores that a row does not see become -inf; returns whether every row sees every key, and what some row sees: the
         // lane's key 8 (i / 4) + 4 kg + i % 4 in bit 8 (i / 4) + i % 4
-        auto mask = [&](f32x16 (&s)[RW], int half0, int page0, int page1, uint32_t& some) {
-            const bool whole = __builtin_amdgcn_readfirstlane((page0 | page1) >= 0) && half0 + 31 <= lo &&
-                               (half0 >= all_start || half0 + 32 <= a.sinks);
+        auto mask = [&](f32x16 (&s)[RW], int half0, uint32_t pages, uint32_t& some) {  // pages: 2 bits
+            const bool whole = pages == 3u && half0 + 31 <= lo && (half0 >= all_start || half0 + 32 <= a.sinks);
             some = 0xFFFFFFFFu;
             if (!whole) {
                 some = 0u;
-                const uint32_t pages_there = (page0 >= 0 ? 0xFFFFu : 0u) | (page1 >= 0 ? 0xFFFF0000u : 0u);
+                const uint32_t pages_there = (pages & 1u ? 0xFFFFu : 0u) | (pages & 2u ? 0xFFFF0000u : 0u);
 #pragma unroll
                 for (int rw = 0; rw < RW; ++rw) {
                     const uint32_t seen = (seen_bits(half0, last[rw], start[rw], a.sinks) & pages_there) >> (4 * kg);
@@ -1100,12 +1101,33 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[rw][dt][i] *= keep[rw];
         };
-        // two probabilities of a row tile, rounded, and into its sum as rounded
-        auto prob2 = [&](const f32x16 (&s)[RW], u32x4 (&p)[RW][2], int rw, int w) {
+        // two probabilities of a row tile; rounded, and into its sum as rounded
+        auto exp2x2 = [&](const f32x16 (&s)[RW], int rw, int w) {
             const float mu = m[rw] == -INFINITY ? 0.0f : m[rw];
-            p[rw][w >> 2][w & 3] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[rw][2 * w], scale, -mu)),
-                                            __builtin_amdgcn_exp2f(fmaf(s[rw][2 * w + 1], scale, -mu)));
+            return float2{__builtin_amdgcn_exp2f(fmaf(s[rw][2 * w], scale, -mu)),
+                          __builtin_amdgcn_exp2f(fmaf(s[rw][2 * w + 1], scale, -mu))};
+        };
+        auto keep2 = [&](float2 e, u32x4 (&p)[RW][2], int rw, int w) {
+            p[rw][w >> 2][w & 3] = pack2<T>(e.x, e.y);
             l[rw] = T::dot2(p[rw][w >> 2][w & 3], T::ONE_PAIR, l[rw]);
+        };
+        // `kProducts` products, and a row tile's probabilities spread among them in this order: the exponentials of one step are
+        // rounded in the next
+        auto among = [&](const f32x16 (&s)[RW], u32x4 (&p)[RW][2], int rw, auto products, auto&& product) {
+            constexpr int kProducts = decltype(products)::value, kEach = 8 / kProducts;
+            float2 e[kEach];
+#pragma unroll
+            for (int x = 0; x <= kProducts; ++x) {
+                if (x < kProducts) product(x);
+                float2 next[kEach];
+#pragma unroll
+                for (int y = 0; y < kEach; ++y) {
+                    if (x < kProducts) next[y] = exp2x2(s, rw, kEach * x + y);
+                    if (x > 0) keep2(e[y], p, rw, kEach * (x - 1) + y);
+                    e[y] = next[y];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         // O^T += V^T P^T of 32 keys; values that no row sees are cleared
         auto values = [&](const uint16_t* half, const u32x4 (&p)[RW][2], bool whole, uint32_t some) {
@@ -1139,11 +1161,13 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             }
             if (zero != zero) s_tainted[turn] = 1;
         };
-        // S^T = K Q^T of 32 keys, operands read ahead of the products that run
-        auto scores = [&](const uint16_t* half, f32x16 (&s)[RW]) {
-            u32x4 kf[2][KG];
+        u32x4 kf[2][KG];
+        // S^T = K Q^T of 32 keys, operands read ahead of the products that run, the first half of them by `come` if `begun`
+        auto scores = [&](const uint16_t* half, f32x16 (&s)[RW], bool begun) {
+            if (!begun) {
 #pragma unroll
-            for (int e = 0; e < KG; ++e) kf[0][e] = read_k(half, e);
+                for (int e = 0; e < KG; ++e) kf[0][e] = read_k(half, e);
+            }
 #pragma unroll
             for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
@@ -1166,12 +1190,11 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         // with two groups of waves, the first brings keys, the other values, three tiles ahead
         constexpr int kOut = RW == 1 ? Instr : 2 * Instr;  // of a wave, a tile
         auto issue = [&](int it) {
-            const int64_t from = place(it, grp == 0);
+            const int64_t from = place(it);
             if (grp == 0) issue_k(it, from);
             if (RW == 2 || grp == 1) issue_v(it, from);
         };
         for (int it = 0; it < 3 && it < n; ++it) issue(it);
-        int4 pages4;
         int key0;
         auto come = [&](int it) {  // waits for a tile, and sends for one where the tile before it was
             const int behind = min(n - 1 - it, 2);  // tiles out behind this one
@@ -1179,13 +1202,15 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             else if (behind == 1) wait_vmcnt<kOut>();
             else wait_vmcnt<0>();
             barrier_keep_dma();
-            pages4 = *reinterpret_cast<const int4*>(&there[it & 3][0]);
+            if constexpr (RW == 2) {
+#pragma unroll
+                for (int e = 0; e < KG; ++e) kf[0][e] = read_k(kring[it & 3], e);
+            }
             if (it + 3 < n) issue(it + 3);
             key0 = tiles.at(first + it) * kKeys;
         };
-        auto all_whole = [&] {  // every row sees all of the tile
-            return __builtin_amdgcn_readfirstlane((pages4.x | pages4.y | pages4.z | pages4.w) >= 0) && key0 + kKeys - 1 <= lo &&
-                   (key0 >= all_start || key0 + kKeys <= a.sinks);
+        auto all_whole = [&](int it) {  // every row sees all of the tile
+            return (there >> (4 * (it & 3)) & 15u) == 15u && key0 + kKeys - 1 <= lo && (key0 >= all_start || key0 + kKeys <= a.sinks);
         };
         int it = 0;
         come(0);
@@ -1193,13 +1218,13 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             if constexpr (RW == 2) {
                 // tiles that every row sees whole, in a loop of their own (with the others in one, its registers did not
                 // suffice): the exponentials of a half among the products of the other
-                while (all_whole()) {
+                while (all_whole(it)) {
                     const uint16_t* kt0 = kring[it & 3];
                     const uint16_t* vt0 = vring[it & 3];
                     f32x16 s[2][RW];
-                    u32x4 p[2][RW][2], kf[2][KG], vf[2][DT];
+                    u32x4 p[2][RW][2], vf[2][DT];
                     float keep[RW];
-                    scores(kt0, s[0]);
+                    scores(kt0, s[0], true);
 #pragma unroll
                     for (int e = 0; e < KG; ++e) kf[0][e] = read_k(kt0 + 32 * D, e);
                     if (follow(s[0], keep)) rescale(keep);
@@ -1215,14 +1240,11 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                             if (q == 0) kf[1][e] = read_k(kt0 + 32 * D, KG + e);
                             else if (e < DT) vf[0][e] = read_v(vt0, 0, e);
                         }
-#pragma unroll
-                        for (int w = 0; w < 8; ++w) prob2(s[0], p[0], q, w);
-#pragma unroll
-                        for (int e = 0; e < KG; ++e)
-#pragma unroll
-                            for (int rw = 0; rw < RW; ++rw) s[1][rw] = mfma32x32x16<T>(kf[q][e], qf[rw][KG * q + e], s[1][rw]);
-                        interleave<KG * RW, 52 / (KG * RW)>();
                         __builtin_amdgcn_sched_barrier(0);
+                        among(s[0], p[0], q, std::integral_constant<int, KG * RW>{}, [&](int x) {
+                            const int e = x / RW, rw = x % RW;
+                            s[1][rw] = mfma32x32x16<T>(kf[q][e], qf[rw][KG * q + e], s[1][rw]);
+                        });
                     }
                     const bool grew = follow(s[1], keep);
                     __builtin_amdgcn_sched_barrier(0);
@@ -1230,14 +1252,11 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                     for (int q = 0; q < 2; ++q) {
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt) vf[1 - q][dt] = q == 0 ? read_v(vt0, 1, dt) : read_v(vt0 + 32 * D, 0, dt);
-#pragma unroll
-                        for (int w = 0; w < 8; ++w) prob2(s[1], p[1], q, w);
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q][dt], p[0][rw][q], o[rw][dt]);
-                        interleave<DT * RW, 52 / (DT * RW)>();
                         __builtin_amdgcn_sched_barrier(0);
+                        among(s[1], p[1], q, std::integral_constant<int, DT * RW>{}, [&](int x) {
+                            const int dt = x / RW, rw = x % RW;
+                            o[rw][dt] = mfma32x32x16<T>(vf[q][dt], p[0][rw][q], o[rw][dt]);
+                        });
                     }
                     // or they are made behind the branch, where they are used
 #pragma unroll
@@ -1268,16 +1287,16 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                 const int h = RW == 1 ? grp : hh;
                 if (!live(key0 + 32 * h)) continue;
                 f32x16 s[RW];
-                scores(kt0 + 32 * h * D, s);
+                scores(kt0 + 32 * h * D, s, false);
                 uint32_t some;
-                const bool whole = mask(s, key0 + 32 * h, h ? pages4.z : pages4.x, h ? pages4.w : pages4.y, some);
+                const bool whole = mask(s, key0 + 32 * h, there >> (4 * (it & 3) + 2 * h) & 3u, some);
                 float keep[RW];
                 if (follow(s, keep)) rescale(keep);
                 u32x4 p[RW][2];
 #pragma unroll
                 for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
-                    for (int w = 0; w < 8; ++w) prob2(s, p, rw, w);
+                    for (int w = 0; w < 8; ++w) keep2(exp2x2(s, rw, w), p, rw, w);
                 values(vt0 + 32 * h * D, p, whole, some);
             }
             if (++it < n) come(it);
