@@ -134,6 +134,8 @@ constexpr int kCUs = 256;
 constexpr int kFewEntries = 512, kEntries = 1024;
 constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
+// what an (entry, kv head) costs on top of its tiles, in tiles: its queries, its first tiles' way from memory, its sums' join
+constexpr int kFewStart = 4, kStart = 1;
 constexpr float kSlack = 8.0f;
 constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
 
@@ -236,7 +238,7 @@ struct Shares {
     int64_t share, first, end;  // units a block, and this block's
     int entry;                  // of the first; -1: nothing to do
 };
-template <int kThreads, int kBlocks, typename Count>
+template <int kThreads, int kBlocks, int kCharge, typename Count>
 __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
                                      int* s_entry, Count count) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -246,7 +248,7 @@ __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least,
         const int e = t * per + i;
         if (e < entries) {
             pre[e] = sum;
-            sum += count(e);
+            sum += count(e) + kCharge;
         }
     }
     int64_t incl = sum;
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
     if (t < 2) s_tainted[t] = 0;
-    const Shares shares = make_shares<64 * kWaves, Shape::kBlocks>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
+    const Shares shares = make_shares<64 * kWaves, Shape::kBlocks, kFewStart>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
                                                                    [&](int e) {
                                                                        const Tiles r = tiles_of_few(a, e, 16 * RT);
                                                                        spans[e] = int2{r.sink_tiles, r.window_tile};
@@ -385,11 +387,13 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     int slot = 0, turn = 0;
     while (true) {
         const int64_t seg0 = pre[entry] * a.kv_heads;
-        const int count = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
-        const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / count));
-        const int64_t seg = seg0 + static_cast<int64_t>(kvh) * count;
-        const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg));
-        const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(min<int64_t>(shares.end - u, count - first)));
+        const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry])), count = units - kFewStart;
+        const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / units));
+        const int64_t seg = seg0 + static_cast<int64_t>(kvh) * units;
+        const int first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart);
+        u = min(shares.end, seg + units);
+        const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart - first;
+        if (n <= 0) return;  // the share ended before its first tile
         const int b = entry / a.row_groups;
         const int row0 = (entry - b * a.row_groups) * (16 * RT);
         const int rows = min(16 * RT, a.tokens * a.groups - row0);
@@ -671,8 +675,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         }
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count - 1) / shares.share)};
-        u += n;
+                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + units - 1) / shares.share)};
         if (u >= shares.end) return;
         slot = 1;  // a share's first and last (entry, kv head) are the ones that it may not finish
         if (kvh + 1 == a.kv_heads) ++entry;
@@ -879,7 +882,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
     int entry, slot = 0, turn = 0;
     int64_t u = 0;
     if constexpr (kShared) {
-        shares = make_shares<64 * NW, kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry, [&](int e) { return a.spans[e].z; });
+        shares = make_shares<64 * NW, kCUs, kStart>(a, entries, kLeastTiles, pre, wave_total, &s_entry, [&](int e) { return a.spans[e].z; });
         if (shares.entry < 0) return;
         entry = shares.entry;
         u = shares.first;
@@ -931,11 +934,14 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         Tiles tiles;
         if constexpr (kShared) {
             const int64_t seg0 = pre[entry] * a.kv_heads;
-            count = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
-            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / count));
-            seg = seg0 + static_cast<int64_t>(kvh) * count;
-            first = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg));
-            n = __builtin_amdgcn_readfirstlane(static_cast<int>(min<int64_t>(shares.end - u, count - first)));
+            const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
+            count = units - kStart;
+            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / units));
+            seg = seg0 + static_cast<int64_t>(kvh) * units;
+            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart);
+            u = min(shares.end, seg + units);
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart - first;
+            if (n <= 0) return;  // the share ended before its first tile
             const int4 sp = a.spans[entry];
             tiles = Tiles{sp.x, sp.y, sp.z};
         } else {
@@ -1387,8 +1393,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count - 1) / shares.share)};
-        u += n;
+                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count + kStart - 1) / shares.share)};
         if (u >= shares.end) return;
         slot = 1;
         if (kvh + 1 == a.kv_heads) ++entry;
