@@ -1,7 +1,7 @@
 // Verification of drafted tokens: softmax statistics of every row of logits, the accept tests, and one token by inverse CDF
 // from the row where the drafts end. Four launches:
-//   1. row_stats_kernel, a block per (row, chunk of 4096 or 16384 logits): the chunk's largest logit m_c (with its index) and
-//      z_c = sum exp((x - m_c) / T);
+//   1. row_stats_kernel, a block per (row, chunk of one or more parts of 4096 logits): the chunk's largest logit m_c (with its
+//      index) and z_c = sum exp((x - m_c) / T);
 //   2. walk_kernel, a block per sequence: joins its rows' statistics and makes the accept tests u q(x) < p(x);
 //   3. part_sums_kernel, a block per (sequence, 4096 logits): the sums of w = max(p - q, 0) and of p over its part of the row
 //      that the tests ended at;
@@ -82,7 +82,8 @@ struct Row {
 
 // exp(d) for d <= 0 as p t: n = round(128 d / ln2), t = 2^(n / 128) from a table, with n / 128's whole part added to its
 // exponent, and a polynomial p of |r| <= ln2 / 256 (table-driven exp, Tang 1989), whose first term left out is below 2^-49. n
-// comes as the low bits of a sum with 1.5 * 2^52. Below -700 exp(d) counts as exp(-700), which is nothing beside 1. A table of
+// comes as the low bits of a sum with 1.5 * 2^52. The copy in LDS has i << 13 taken from the upper word of entry i, so that
+// all of n << 13 is added to it (an exponent's one is 2^20). Below -700 exp(d) counts as exp(-700), which is nothing beside 1. A table of
 // 32 entries, a copy in every pair of LDS banks, and one term more cost 10%: the arithmetic bounds this, not the table's reads.
 constexpr int kTable = 128;
 __device__ const double kPowers[kTable] = {  // 2^(i / 128)
@@ -114,7 +115,8 @@ __device__ const double kPowers[kTable] = {  // 2^(i / 128)
     0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0,
 };
 __device__ inline void fill_table(double* table) {
-    if (threadIdx.x < kTable) table[threadIdx.x] = kPowers[threadIdx.x];
+    if (threadIdx.x < kTable)
+        table[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, kPowers[threadIdx.x]) - (static_cast<uint64_t>(threadIdx.x) << 45));
 }
 __device__ inline void exp_parts(double d, const double* table, double& p, double& t) {
     constexpr double kMagic = 6755399441055744.0;
@@ -128,7 +130,7 @@ __device__ inline void exp_parts(double d, const double* table, double& p, doubl
     const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     u32x2 bits = __builtin_bit_cast(u32x2, table[n & (kTable - 1)]);
-    bits.y += (n & ~(kTable - 1u)) << 13;
+    bits.y += n << 13;
     t = __builtin_bit_cast(double, bits);
 }
 __device__ inline double exp_of(double d, const double* table) {
@@ -199,7 +201,8 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
     fill_table(table);
     if (t == 0) index = 0xFFFFFFFFu;
     __syncthreads();
-    float m = -INFINITY, odd = 0.0f;  // odd: NaN where an element is no finite number
+    float m = -INFINITY;
+    bool odd = false;  // some element is a NaN
     int found = k0;                   // the part that m is of
     double z = 0.0;
     for (int k = 0; k < n; ++k) {
@@ -208,9 +211,9 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
         if (k + 1 < n) src.load(k0 + k + 1, v);
         float top = x[0];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            top = fmaxf(top, x[i]);
-            odd = fmaf(x[i], 0.0f, odd);
+        for (int i = 0; i < kBatch; i += 2) {
+            top = fmaxf(top, fmaxf(x[i], x[i + 1]));
+            odd |= __builtin_isunordered(x[i], x[i + 1]);
         }
         if (top > m) {
             z *= exp_of((static_cast<double>(m) - top) * a.inv_t, table);
@@ -229,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(const VerifyArgs a)
     // their parts
     float nan = m;
     int nan_at = found;
-    if (odd != odd) {
+    if (odd) {
         for (int k = n - 1; k >= 0; --k) {
             float x[kBatch];
             src.load(k0 + k, v);
@@ -494,10 +497,14 @@ __global__ __launch_bounds__(Part<T>::kThreads) void pick_token_kernel(const Ver
     }
 }
 
-// Parts of a row, which may begin up to 7 elements into its first piece, and of a chunk: one, or four where there are chunks
-// enough to fill the card, for a block's fixed part (its table, reductions of 64-bit numbers) costs as much as half a part.
+// Parts of a row, which may begin up to 7 elements into its first piece; chunks of a row, each of as many parts as make all
+// rows' chunks come into the card at once (8 blocks a CU), for a block's fixed part (its table, reductions of 64-bit numbers)
+// costs as much as half a part, and a second round of blocks as much as the first.
 int64_t row_parts_of(int64_t vocab) { return ceil_div(vocab + 7, kBatch * kThreads); }
-int64_t parts_of(int64_t rows, int64_t vocab) { return rows * row_parts_of(vocab) >= 4096 ? 4 : 1; }
+int64_t parts_of(int64_t rows, int64_t vocab) {
+    const int64_t most = std::max<int64_t>(1, 2048 / rows);
+    return ceil_div(row_parts_of(vocab), most);
+}
 int64_t chunks_of(int64_t rows, int64_t vocab) { return ceil_div(row_parts_of(vocab), parts_of(rows, vocab)); }
 
 template <typename T>
