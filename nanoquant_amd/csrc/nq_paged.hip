@@ -864,7 +864,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
     constexpr int Instr = 16 / RowsPer;  // instructions for 16 rows
     constexpr int Group = 128 * RW;
     constexpr int KT = D / 16, DT = D / 32, KG = KT / 2;
-    constexpr int TileElems = kKeys * D;
+    constexpr int TileElems = kKeys * D, kStep = RW == 1 ? 2 : 1;  // tiles from one of a wave's to its next
     __shared__ __attribute__((aligned(16))) uint16_t kring[4][TileElems], vring[4][TileElems];
     __shared__ int spans[2][4];
     __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
@@ -1035,7 +1035,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             }
         };
         auto place = [&](int it) {
-            if ((it & 63) == 0) look_up(it);
+            if ((it & 63) < kStep) look_up(it & ~63);
             const int at = it & 63, by = 4 * (it & 3);
             there = (there & ~(15u << by)) | static_cast<uint32_t>(__builtin_amdgcn_readlane(my_there, at)) << by;
             const int page = __builtin_amdgcn_readlane(my_page, at), rest = __builtin_amdgcn_readlane(my_rest, at);
@@ -1117,10 +1117,10 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             p[rw][w >> 2][w & 3] = pack2<T>(e.x, e.y);
             l[rw] = T::dot2(p[rw][w >> 2][w & 3], T::ONE_PAIR, l[rw]);
         };
-        // `kProducts` products, and a row tile's probabilities spread among them in this order: the exponentials of one step are
+        // `kProducts` products, and half q of the probabilities spread among them in this order: the exponentials of one step are
         // rounded in the next
-        auto among = [&](const f32x16 (&s)[RW], u32x4 (&p)[RW][2], int rw, auto products, auto&& product) {
-            constexpr int kProducts = decltype(products)::value, kEach = 8 / kProducts;
+        auto among = [&](const f32x16 (&s)[RW], u32x4 (&p)[RW][2], int q, auto products, auto&& product) {
+            constexpr int kProducts = decltype(products)::value, kEach = 4 * RW / kProducts;
             float2 e[kEach];
 #pragma unroll
             for (int x = 0; x <= kProducts; ++x) {
@@ -1128,8 +1128,9 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                 float2 next[kEach];
 #pragma unroll
                 for (int y = 0; y < kEach; ++y) {
-                    if (x < kProducts) next[y] = exp2x2(s, rw, kEach * x + y);
-                    if (x > 0) keep2(e[y], p, rw, kEach * (x - 1) + y);
+                    const int at = 4 * RW * q + kEach * x + y;
+                    if (x < kProducts) next[y] = exp2x2(s, at / 8, at % 8);
+                    if (x > 0) keep2(e[y], p, (at - kEach) / 8, (at - kEach) % 8);
                     e[y] = next[y];
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -1193,35 +1194,40 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             }
         };
 
-        // with two groups of waves, the first brings keys, the other values, three tiles ahead
-        constexpr int kOut = RW == 1 ? Instr : 2 * Instr;  // of a wave, a tile
+        // The waves of a group send for their tiles: all of them three ahead, every other one the next ahead.
+        constexpr int kOut = 2 * Instr;  // instructions of a wave, a tile
         auto issue = [&](int it) {
             const int64_t from = place(it);
-            if (grp == 0) issue_k(it, from);
-            if (RW == 2 || grp == 1) issue_v(it, from);
+            issue_k(it, from);
+            issue_v(it, from);
         };
-        for (int it = 0; it < 3 && it < n; ++it) issue(it);
+        for (int it = grp; it < (RW == 1 ? 4 : 3) && it < n; it += kStep) issue(it);
         int key0;
-        auto come = [&](int it) {  // waits for a tile, and sends for one where the tile before it was
-            const int behind = min(n - 1 - it, 2);  // tiles out behind this one
-            if (behind == 2) wait_vmcnt<2 * kOut>();
-            else if (behind == 1) wait_vmcnt<kOut>();
-            else wait_vmcnt<0>();
-            barrier_keep_dma();
+        auto come = [&](int it) {  // waits for a tile, and sends for one where the group's tile before it was
             if constexpr (RW == 2) {
-#pragma unroll
-                for (int e = 0; e < KG; ++e) kf[0][e] = read_k(kring[it & 3], e);
+                const int behind = min(n - 1 - it, 2);  // tiles out behind this one
+                if (behind == 2) wait_vmcnt<2 * kOut>();
+                else if (behind == 1) wait_vmcnt<kOut>();
+                else wait_vmcnt<0>();
+            } else {
+                if (it < 2 && it + 2 < n) wait_vmcnt<kOut>();
+                else wait_vmcnt<0>();
             }
-            if (it + 3 < n) issue(it + 3);
+            barrier_keep_dma();
+#pragma unroll
+            for (int e = 0; e < KG; ++e) kf[0][e] = read_k(kring[it & 3], e);
+            if ((RW == 2 || it >= 2) && it + 4 - kStep < n) issue(it + 4 - kStep);
             key0 = tiles.at(first + it) * kKeys;
         };
         auto all_whole = [&](int it) {  // every row sees all of the tile
-            return (there >> (4 * (it & 3)) & 15u) == 15u && key0 + kKeys - 1 <= lo && (key0 >= all_start || key0 + kKeys <= a.sinks);
+            return it < n && (there >> (4 * (it & 3)) & 15u) == 15u && key0 + kKeys - 1 <= lo && (key0 >= all_start || key0 + kKeys <= a.sinks);
         };
-        int it = 0;
-        come(0);
-        while (it < n) {
-            if constexpr (RW == 2) {
+        // the groups take the same number of steps, the last of which may be none of the second's
+        const int end = RW == 1 ? ((n + 1) & ~1) + grp : n;
+        int it = grp;
+        come(it);
+        while (it < end) {
+            {
                 // tiles that every row sees whole, in a loop of their own (with the others in one, its registers did not
                 // suffice): the exponentials of a half among the products of the other
                 while (all_whole(it)) {
@@ -1281,17 +1287,17 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                             for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[q][dt], p[1][rw][q], o[rw][dt]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    if (++it == n) break;
+                    it += kStep;
+                    if (it >= end) break;
                     come(it);
                 }
-                if (it == n) break;
+                if (it >= end) break;
             }
             const uint16_t* kt0 = kring[it & 3];
             const uint16_t* vt0 = vring[it & 3];
 #pragma unroll
-            for (int hh = 0; hh < RW; ++hh) {
-                const int h = RW == 1 ? grp : hh;
-                if (!live(key0 + 32 * h)) continue;
+            for (int h = 0; h < 2; ++h) {
+                if (it >= n || !live(key0 + 32 * h)) continue;
                 f32x16 s[RW];
                 scores(kt0 + 32 * h * D, s, false);
                 uint32_t some;
@@ -1305,7 +1311,8 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                     for (int w = 0; w < 8; ++w) keep2(exp2x2(s, rw, w), p, rw, w);
                 values(vt0 + 32 * h * D, p, whole, some);
             }
-            if (++it < n) come(it);
+            it += kStep;
+            if (it < end) come(it);
         }
 
         const bool done = first == 0 && n == count;
