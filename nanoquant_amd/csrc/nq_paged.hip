@@ -1,5 +1,6 @@
 // A KV cache in pages: the rotary write of new tokens and the attention that reads it.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "nq_common.h"
@@ -135,7 +136,7 @@ constexpr int kFewEntries = 512, kEntries = 1024;
 constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
 // what an (entry, kv head) costs on top of its tiles, in tiles: its queries, its first tiles' way from memory, its sums' join
-constexpr int kFewStart = 8, kStart = 1;
+constexpr int kFewStart = 8, kStart = 4;
 constexpr float kSlack = 8.0f;
 constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
 
@@ -238,6 +239,9 @@ struct Shares {
     int64_t share, first, end;  // units a block, and this block's
     int entry;                  // of the first; -1: nothing to do
 };
+// a / b for 0 <= a < 2^42 and b < 2^26: the quotient in fp64 is off by less than its distance from the next integer.
+__device__ inline int quotient(int64_t a, int b) { return static_cast<int>(static_cast<double>(a) / b); }
+
 template <int kThreads, int kBlocks, int kCharge, typename Count>
 __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
                                      int* s_entry, Count count) {
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     while (true) {
         const int64_t seg0 = pre[entry] * a.kv_heads;
         const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry])), count = units - kFewStart;
-        const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / units));
+        const int kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
         const int64_t seg = seg0 + static_cast<int64_t>(kvh) * units;
         const int first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart);
         u = min(shares.end, seg + units);
@@ -936,17 +940,64 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             const int64_t seg0 = pre[entry] * a.kv_heads;
             const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
             count = units - kStart;
-            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>((u - seg0) / units));
+            kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
             seg = seg0 + static_cast<int64_t>(kvh) * units;
             first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart);
             u = min(shares.end, seg + units);
             n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart - first;
             if (n <= 0) return;  // the share ended before its first tile
             const int4 sp = a.spans[entry];
-            tiles = Tiles{sp.x, sp.y, sp.z};
+            tiles = Tiles{__builtin_amdgcn_readfirstlane(sp.x), __builtin_amdgcn_readfirstlane(sp.y), sp.z};
         } else {
             kvh = static_cast<int>(blockIdx.x) % a.kv_heads;
         }
+
+        // a wave brings a quarter of a tile: 16 keys, which lie in one page. Where they are, for 64 tiles at a time, a lane each:
+        // a scalar load and a division for every tile stood in its way
+        int my_page = 0, my_rest = 0, my_there = 0;
+        uint32_t there = 0u;  // bit 4 (it % 4) + i: the page of keys 16 i .. +15 of tile `it` is there
+        auto look_up = [&](int it) {
+            const int key = tiles.at(first + min(it + lane, n - 1)) * kKeys;
+            my_there = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (key + 16 * i) / a.pages.page_size;
+                const int page = at < a.pages.table_pages ? a.pages.page(b, at) : -1;
+                my_there |= page >= 0 ? 1 << i : 0;
+                if (i == rwave) {
+                    my_page = max(page, 0);
+                    my_rest = key + 16 * i - at * a.pages.page_size;
+                }
+            }
+        };
+        auto place = [&](int it) {
+            if ((it & 63) < kStep) look_up(it & ~63);
+            const int at = it & 63, by = 4 * (it & 3);
+            there = (there & ~(15u << by)) | static_cast<uint32_t>(__builtin_amdgcn_readlane(my_there, at)) << by;
+            const int page = __builtin_amdgcn_readlane(my_page, at), rest = __builtin_amdgcn_readlane(my_rest, at);
+            return ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + rest) * D;
+        };
+        auto issue_k = [&](int it, int64_t from) {
+            const uint16_t* p = uniform(a.k_pages + from);
+#pragma unroll
+            for (int j = 0; j < Instr; ++j) dma16_lds(p, koff[j], klds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
+        };
+        auto issue_v = [&](int it, int64_t from) {
+            const uint16_t* p = uniform(a.v_pages + from);
+#pragma unroll
+            for (int j = 0; j < Instr; ++j) dma16_lds(p, voff[j], vlds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
+        };
+        // The waves of a group send for their tiles: all of them three ahead, every other one the next ahead.
+        constexpr int kOut = 2 * Instr;  // instructions of a wave, a tile
+        auto issue = [&](int it) {
+            const int64_t from = place(it);
+            issue_k(it, from);
+            issue_v(it, from);
+        };
+        auto begin = [&] {
+            for (int it = grp; it < (RW == 1 ? 4 : 3) && it < n; it += kStep) issue(it);
+        };
+        if constexpr (kShared) begin();  // while the queries come
 
         u32x4 qf[RW][KT];
         int last[RW], start[RW];
@@ -1000,10 +1051,11 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                 bhi = max(bhi, spans[1][w]);
             }
             tiles = tiles_between<kKeys>(a, blo, bhi);
+            tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
+            tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
             count = n = __builtin_amdgcn_readfirstlane(tiles.count);
+            begin();
         }
-        tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
-        tiles.window_tile = __builtin_amdgcn_readfirstlane(tiles.window_tile);
 
         f32x16 o[RW][DT];
         float m[RW], l[RW];
@@ -1016,41 +1068,6 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[rw][dt][i] = 0.0f;
         }
-        // a wave brings a quarter of a tile: 16 keys, which lie in one page. Where they are, for 64 tiles at a time, a lane each:
-        // a scalar load and a division for every tile stood in its way
-        int my_page = 0, my_rest = 0, my_there = 0;
-        uint32_t there = 0u;  // bit 4 (it % 4) + i: the page of keys 16 i .. +15 of tile `it` is there
-        auto look_up = [&](int it) {
-            const int key = tiles.at(first + min(it + lane, n - 1)) * kKeys;
-            my_there = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = (key + 16 * i) / a.pages.page_size;
-                const int page = at < a.pages.table_pages ? a.pages.page(b, at) : -1;
-                my_there |= page >= 0 ? 1 << i : 0;
-                if (i == rwave) {
-                    my_page = max(page, 0);
-                    my_rest = key + 16 * i - at * a.pages.page_size;
-                }
-            }
-        };
-        auto place = [&](int it) {
-            if ((it & 63) < kStep) look_up(it & ~63);
-            const int at = it & 63, by = 4 * (it & 3);
-            there = (there & ~(15u << by)) | static_cast<uint32_t>(__builtin_amdgcn_readlane(my_there, at)) << by;
-            const int page = __builtin_amdgcn_readlane(my_page, at), rest = __builtin_amdgcn_readlane(my_rest, at);
-            return ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + rest) * D;
-        };
-        auto issue_k = [&](int it, int64_t from) {
-            const uint16_t* p = uniform(a.k_pages + from);
-#pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(p, koff[j], klds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
-        };
-        auto issue_v = [&](int it, int64_t from) {
-            const uint16_t* p = uniform(a.v_pages + from);
-#pragma unroll
-            for (int j = 0; j < Instr; ++j) dma16_lds(p, voff[j], vlds + static_cast<uint32_t>(it & 3) * (TileElems * 2) + 1024u * j);
-        };
         auto live = [&](int key0) {  // some row of the wave sees some key of 32
             return key0 <= hi && (key0 + 32 > any_start || key0 < a.sinks);
         };
@@ -1194,14 +1211,6 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             }
         };
 
-        // The waves of a group send for their tiles: all of them three ahead, every other one the next ahead.
-        constexpr int kOut = 2 * Instr;  // instructions of a wave, a tile
-        auto issue = [&](int it) {
-            const int64_t from = place(it);
-            issue_k(it, from);
-            issue_v(it, from);
-        };
-        for (int it = grp; it < (RW == 1 ? 4 : 3) && it < n; it += kStep) issue(it);
         int key0;
         auto come = [&](int it) {  // waits for a tile, and sends for one where the group's tile before it was
             if constexpr (RW == 2) {
@@ -1423,20 +1432,32 @@ struct Plan {
 Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t max_keys) {
     Plan p{};
     const int64_t rows = tokens * groups;
-    p.few = rows <= 64;
+    // Times in tiles of 64 keys, as rows_kernel takes them with 128 rows a block (1 us), from measurements of 11 and 29 shapes;
+    // `fill` is how often its row groups fill the card, `longest` and `mean` are what a row group may see.
+    const double fill = static_cast<double>(ceil_div(rows, 128) * batch * kv_heads) / kCUs;
+    const double longest = max_keys / 64.0, mean = std::max<int64_t>(max_keys - tokens / 2, max_keys / 2) / 64.0;
+    // few_kernel reads at the card's rate whatever the grid, 1.9 for a card full, and joins for 7 more than rows_kernel takes.
+    // 64 rows a sequence and 8 kv heads: 9 sequences in 2900 keys 45 us against 56, 32 sequences 91 against 78; a sequence of
+    // 64 tokens and 32 kv heads in 8000 keys 48 us against 131, in 64 keys 18 against 11.
+    p.few = rows <= 16 || (rows <= 64 && longest * (1.0 - 1.9 * fill) > 7.0);
     if (p.few) {
         p.tiles = static_cast<int>(ceil_div(rows, 16));
         p.group = 16 * p.tiles;
         p.shared = true;
         p.blocks = p.tiles < 3 || head_dim == 64 ? 2 * kCUs : kCUs;  // FewShape's
     } else {
-        const int64_t large = ceil_div(rows, 256) * batch * kv_heads;
-        p.tiles = large >= 2 * kCUs ? 2 : 1;
-        p.shared = false;
-        if (p.tiles == 1 && max_keys >= 4096) {
-            p.shared = true;
-            p.tiles = large >= kCUs / 2 ? 2 : 1;
-        }
+        // Two row tiles a wave where the rows fill them, and a grid of them the card nearly twice: 64 heads of 8 kv heads, a
+        // prompt of 2000 tokens 93 us against 106, but 1500 tokens in 8000 keys 461 against 406, and 64 sequences of 64 rows in
+        // 1000 keys 93 against 60. With the work shared the card is always full: 700 tokens in 8000 keys 222 us against 233,
+        // but 800 tokens of 32 kv heads, which leave an eighth of the row tiles empty, 174 against 158.
+        const int64_t large = ceil_div(rows, 256);
+        const bool full = 2 * large * 15 <= ceil_div(rows, 128) * 16;
+        p.tiles = full && large * batch * kv_heads >= 7 * kCUs / 4 ? 2 : 1;
+        // Shares make up for a grid that leaves CUs without work, or runs a round more for a few blocks, and cost 25: 700 tokens
+        // of 64 heads of 8 kv heads in 2000 keys 81 us against 70, in 4000 128 against 132, in 8000 222 against 262; 200 tokens
+        // of 32 kv heads in 2000 keys 45 against 41, in 4000 53 against 74.
+        p.shared = p.tiles == 1 && std::max(longest, std::ceil(fill) * mean) > fill * mean + 25.0;
+        if (p.shared && full) p.tiles = 2;
         p.group = 128 * p.tiles;
         p.blocks = kCUs;
     }
