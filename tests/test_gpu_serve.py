@@ -71,6 +71,97 @@ def test_attention(case, dtype):
     assert (y[pos < 0] == 0).all()
 
 
+# (heads, kv_heads, head_dim, page_size, lengths, tokens, window, sinks, columns of the table), every kernel with every number
+# of row tiles, those that share the work of all sequences out over the card and those that do not
+KERNELS = {
+    "few": [
+        (4, 2, 64, 32, [650], 10, 0, 0, 0),
+        (8, 1, 128, 16, [700, 90], 3, 0, 0, 0),
+        (8, 1, 64, 16, [720], 5, 0, 0, 0),
+        (6, 2, 128, 48, [800, 333], 13, 0, 0, 0),
+        (16, 2, 128, 16, [700], 8, 0, 0, 0),
+        (4, 4, 64, 64, [900, 20], 50, 0, 0, 0),
+        (8, 1, 128, 16, [1500, 700], 7, 600, 20, 0),
+        (8, 1, 64, 16, [1100, 650, 9], 6, 100, 0, 0),
+        # more sequences than one launch takes, and a table much wider than the lengths
+        (2, 1, 64, 16, [n % 45 + 1 for n in range(600)], 1, 0, 0, 0),
+        (3, 3, 128, 16, [50, 7, 33], 15, 0, 0, 400),
+    ],
+    "shares": [
+        (4, 2, 128, 64, [4100, 700], 50, 0, 0, 0),
+        (8, 2, 64, 16, [3300], 30, 0, 0, 0),
+        (8, 1, 128, 32, [4000, 2900], 32, 0, 0, 0),
+        (4, 4, 64, 48, [3500], 250, 0, 0, 0),
+        (8, 1, 128, 16, [5000], 32, 4000, 70, 0),
+        (8, 2, 64, 16, [5000, 300], 100, 200, 1, 0),
+        (2, 2, 128, 16, [200, 150], 130, 0, 0, 200),
+        (8, 1, 64, 16, [n % 70 + 9 for n in range(1030)], 9, 0, 0, 125),
+    ],
+    "groups": [
+        (8, 2, 128, 16, [300, 90], 9, 0, 0, 0),
+        (3, 3, 64, 16, [20, 64], 20, 0, 0, 0),
+        (4, 2, 128, 64, [333], 200, 0, 0, 0),
+        (4, 2, 64, 64, [333], 200, 90, 3, 0),
+        (64, 8, 128, 16, [n * 37 % 270 + 1 for n in range(56)], 32, 0, 0, 0),
+        (64, 8, 64, 32, [n * 53 % 330 + 32 for n in range(56)], 32, 100, 5, 0),
+        (32, 32, 64, 16, [257, 300, 511, 256], 1000, 0, 0, 0),
+        (16, 16, 128, 48, [600, 250, 333, 577, 100, 512, 511], 1020, 0, 0, 0),
+    ],
+}
+
+
+@pytest.mark.parametrize("kernel,case", [(k, c) for k, cases in KERNELS.items() for c in cases],
+                         ids=lambda e: e if isinstance(e, str) else "x".join(str(len(x) if isinstance(x, list) else x) for x in e))
+def test_attention_kernels(kernel, case):
+    heads, kv, dim, page, lengths, tokens, window, sinks, columns = case
+    dtype = HALF[len(lengths) % 2]
+    print("\n[case] paged attention", kernel, heads, kv, dim, page, len(lengths), tokens, window, sinks, dtype, flush=True)
+    q, k, v, table, pos = oracle.paged_case(heads, kv, dim, page, lengths, tokens, dtype, "cuda", window=window, sinks=sinks)
+    if columns:
+        table = torch.nn.functional.pad(table, (0, columns - table.shape[1]), value=-1)
+    # only row groups that blocks have for themselves need no workspace
+    bytes_ = _lib.load().nq_paged_attention_workspace_bytes(len(lengths), tokens, heads, kv, dim, table.shape[1], page)
+    assert (bytes_ == 0) == (kernel == "groups")
+    y = paged_attention(q, k, v, table, pos, window, sinks)
+    ref, spread = oracle.attention(q, k, v, table, pos, window, sinks)
+    _check(y, ref, spread, dtype, max(lengths))
+    assert torch.equal(y, paged_attention(q, k, v, table, pos, window, sinks))
+    assert (y[pos < 0] == 0).all()
+
+
+@pytest.mark.parametrize("length,tokens", [(40, 1), (700, 1), (700, 9), (700, 40), (40, 40), (300, 150), (3000, 100)])
+def test_keys_that_are_not_finite_reach_the_tokens_that_see_them(length, tokens):
+    q, k, v, table, pos = oracle.paged_case(4, 2, 128, 16, [length], tokens, torch.bfloat16, "cuda")
+    want = paged_attention(q, k, v, table, pos).view(tokens, 2, 2, 128)
+    k[int(table[0, 0]), 1, 5, 3] = math.nan
+    y = paged_attention(q, k, v, table, pos).view(tokens, 2, 2, 128)
+    seen = (pos[0] >= 5).cpu()
+    assert y[seen, 1].isnan().all() and torch.equal(y[:, 0], want[:, 0])
+    assert torch.equal(y[~seen], want[~seen])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 100])
+def test_calls_through_python_equal_those_through_the_library_of_operators(tokens, monkeypatch):
+    from nanoquant_amd import serve
+    q, k, v, table, pos = oracle.paged_case(8, 2, 128, 16, [300, 120], tokens, torch.float16, "cuda")
+    cos, sin = torch.randn(2, 2, tokens, 128, device="cuda").unbind(0)
+    logits, drafts, u, probs = _drafts(3, tokens, 700, False, torch.float32, seed=tokens)
+
+    def all_calls():
+        pools = k.clone(), v.clone()
+        heads = q[..., :256].contiguous()
+        return (paged_attention(q, k, v, table, pos, 64, 2), paged_rope_write(q, heads, heads, cos, sin, pos, *pools, table),
+                *(p.nan_to_num(7.0) for p in pools), *verify_drafts(logits, drafts, u, probs, 0.7))
+
+    natives = (serve._native_attention, serve._native_write, serve._native_verify)
+    assert None not in natives
+    assert natives[0](q, k, v, table, pos, 64, 2, None) is not None  # it takes the call
+    want = all_calls()
+    for name in ("_native_attention", "_native_write", "_native_verify"):
+        monkeypatch.setattr(serve, name, None)
+    assert all(torch.equal(a, b) for a, b in zip(all_calls(), want))
+
+
 @pytest.mark.parametrize("case", ATTENTION, ids=ids)
 def test_attention_counts_its_keys(case):
     """Queries of zero make every probability 1, so with values of 0 and 1 the sums are whole numbers and the result their
@@ -250,6 +341,22 @@ def test_verify_rows_without_a_distribution():
             got = verify_drafts(logits, drafts, u, q, temperature)
             assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
     assert got[1][:3, 0].tolist() == [5000, 9000, 0]
+
+
+@pytest.mark.parametrize("case", [(300, 3, 16390), (90, 7, 12300), (2100, 0, 4100), (700, 2, 30)], ids=ids)
+def test_verify_of_many_rows(case):
+    """Chunks of several parts: rows alike in number to what the card holds, and more."""
+    print("\n[case] verify", case, flush=True)
+    B, n, V = case
+    logits, drafts, u, probs = _drafts(B, n, V, False, torch.bfloat16, seed=V)
+    logits[0, 0, V - 1] = logits[1, 0, V // 2] = math.nan
+    logits[2, 0, V - 2] = math.inf
+    logits[3, 0, 1:] = -math.inf
+    logits[4, 0, :V - 1] = -math.inf
+    logits[5, 0] = -math.inf
+    want = oracle.verify(logits, drafts, u, probs)
+    got = verify_drafts(logits, drafts, u, probs)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
 
 
 def test_verify_at_the_ends_of_the_random_numbers():
