@@ -1,11 +1,12 @@
 // Verification of drafted tokens: softmax statistics of every row of logits, the accept tests, and one token by inverse CDF
-// from the row where the drafts end. Four launches:
+// from the row where the drafts end. Three launches:
 //   1. row_stats_kernel, a block per (row, chunk of one or more parts of 4096 logits): the chunk's largest logit m_c (with its
 //      index) and z_c = sum exp((x - m_c) / T);
-//   2. walk_kernel, a block per sequence: joins its rows' statistics and makes the accept tests u q(x) < p(x);
-//   3. part_sums_kernel, a block per (sequence, 4096 logits): the sums of w = max(p - q, 0) and of p over its part of the row
-//      that the tests ended at;
-//   4. pick_token_kernel, a block per sequence: the part in which the running sum of w passes u times its total, then the
+//   2. part_sums_kernel, a block per (sequence, 4096 logits): joins the sequence's rows' statistics and makes the accept tests
+//      u q(x) < p(x), every block of a sequence for itself (four drafts of one sequence against 32000 logits: 15.7 us
+//      against 18.0 with a launch for the tests, seven of 64 against 100003: 63.3 against 62.3), then the sums of
+//      w = max(p - q, 0) and of p over its part of the row that the tests ended at;
+//   3. pick_token_kernel, a block per sequence: the part in which the running sum of w passes u times its total, then the
 //      index within it.
 // Probabilities and their sums are fp64: the token is where a running sum over up to 10^5 terms passes a number, and fp32
 // rounding would move a visible share of the borders between tokens.
@@ -291,16 +292,14 @@ __device__ inline Stat join_row(const VerifyArgs& a, int64_t row, const double* 
     return Stat{best, z};
 }
 
-// The whole block, 16 lanes a row, 16 rows at a time: the rows' tests do not wait for each other.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void walk_kernel(const VerifyArgs a) {
-    __shared__ double table[kTable];
+// Where the drafts of sequence b end, by the whole block: 16 lanes a row, blockDim / 16 rows at a time, whose tests do not wait
+// for each other.
+template <typename T, int kThreads>
+__device__ inline Walk walk_of(const VerifyArgs& a, int64_t b, const double* table) {
     __shared__ int end;  // 2 * row + (1: turned down) of the first row that ends the drafts
     __shared__ Stat stats[kThreads / 16];
     const int t = threadIdx.x, group = t >> 4;
-    const int64_t b = blockIdx.x;
     if (t == 0) end = INT32_MAX;
-    fill_table(table);
     __syncthreads();
     for (int i0 = 0;; i0 += kThreads / 16) {
         const int i = i0 + group;
@@ -327,11 +326,10 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(const VerifyArgs a) {
         if (end != INT32_MAX) break;  // the last row ends them at the latest
         __syncthreads();
     }
-    if (t == 0) {
-        const Stat st = stats[(end >> 1) % (kThreads / 16)];
-        const int64_t draft = end & 1 ? a.draft[b * a.drafts + (end >> 1)] : -1;
-        a.walks[b] = Walk{end >> 1, static_cast<int>(draft), st, 1.0 / st.z};
-    }
+    const int at = end;
+    const Stat st = stats[(at >> 1) % (kThreads / 16)];
+    const int64_t draft = at & 1 ? a.draft[b * a.drafts + (at >> 1)] : -1;
+    return Walk{at >> 1, static_cast<int>(draft), st, 1.0 / st.z};
 }
 
 // A part of a row, a piece a thread of 4096 / N: its p and w.
@@ -383,11 +381,12 @@ __global__ __launch_bounds__(Part<T>::kThreads) void part_sums_kernel(const Veri
     __shared__ double2 sums[kWaves];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t b = blockIdx.x / a.row_parts;
-    const Walk walk = a.walks[b];
     fill_table(table);
-    __syncthreads();
+    const Walk walk = walk_of<T, Part<T>::kThreads>(a, b, table);
+    const int at = static_cast<int>(blockIdx.x - b * a.row_parts);
+    if (at == 0 && t == 0) a.walks[b] = walk;
     if (a.inv_t == 0.0 || !finite(rank_value(walk.stat.rank))) return;  // the token is the argmax
-    const Part<T> part(a, b, static_cast<int>(blockIdx.x - b * a.row_parts), walk, table);
+    const Part<T> part(a, b, at, walk, table);
     double2 s = {0.0, 0.0};
 #pragma unroll
     for (int i = 0; i < Part<T>::N; ++i) {
@@ -511,7 +510,6 @@ template <typename T>
 void launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t st) {
     const int64_t rows = batch * (a.drafts + 1);
     row_stats_kernel<T><<<dim3(static_cast<unsigned>(rows * a.chunks)), kThreads, 0, st>>>(a);
-    walk_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
     part_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.row_parts)), Part<T>::kThreads, 0, st>>>(a);
     pick_token_kernel<T><<<dim3(static_cast<unsigned>(batch)), Part<T>::kThreads, 0, st>>>(a);
 }
