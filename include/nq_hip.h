@@ -390,12 +390,14 @@ int nq_paged_rope_write(int dtype, const void* q, int64_t q_stride, const void* 
  *   out       [batch, tokens, heads * head_dim] = sum_j p_j v_j, p = softmax(q . k_j * scaling) over the visible keys
  * A token at position p sees key j iff j <= p, its page is there and, with window > 0, j > p - window or j < sinks (the last
  * `window` positions and the first `sinks`). A token that sees no key gets zeros. Keys that a token does not see do not reach
- * its result, whatever they hold; pages that no token sees are not read.
+ * its result, whatever they hold.
  * Scores, softmax and sums in fp32; probabilities are rounded to dtype for the value product and summed as rounded.
  *   workspace nq_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
  *             not overlap.
- * head_dim 64 or 128, page_size a multiple of 16, table_pages * page_size <= 2^30, else NQ_ERR_UNSUPPORTED. q, out and the
- * pages 16-byte aligned. Results do not depend on what else runs or on the workspace's contents. */
+ * head_dim 64 or 128, page_size a multiple of 16, table_pages * page_size <= 2^30, heads <= 65536 and batch * tokens * heads
+ * < 2^31, else NQ_ERR_UNSUPPORTED. q, out and the pages 16-byte aligned. Results do not depend on what else runs or on the
+ * workspace's contents; another table_pages may choose other kernels, whose roundings differ. Those are chosen for sequences
+ * about as long as their rows of the table allow: the lengths are on the device. */
 size_t nq_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                           int64_t table_pages, int64_t page_size);
 int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t pages,
@@ -419,10 +421,11 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * the running sum of w passes uniforms[b][drafts] times its total: w = p_n where no draft was turned down, else
  * max(p_n - q_n, 0) (p_n where that is zero everywhere). temperature 0 takes p as 1 at the first largest logit.
  * A row with a NaN or an infinite largest logit has no distribution: its draft is turned down and the token is its argmax
- * (the first NaN if there is one). Probabilities and sums in fp64. Four launches.
+ * (the first NaN if there is one). Probabilities and sums in fp64. Three launches.
  *   workspace   nq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
  *               not overlap.
- * Logits aligned to their size, draft_probs and uniforms to 4 bytes, whole numbers to 8. The reference has no counterpart: its
+ * vocab <= 2^30, and at most 2^23 rows of logits and 2^23 pieces of 4096 of a row a sequence, else NQ_ERR_UNSUPPORTED (and a
+ * workspace of 0 bytes). Logits aligned to their size, draft_probs and uniforms to 4 bytes, whole numbers to 8. The reference has no counterpart: its
  * harness samples one token a step with torch ops (src/nanoquant/kernel/test_decode.py:350-353). */
 size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,

@@ -65,7 +65,8 @@ __device__ inline void table8(const void* base, int64_t at, float* f) {
 }
 
 // One thread per (token, head of q, k or v, eight dimensions d of the first half): it holds d and d + D / 2, the rotary pair,
-// so x0 cos0 - x1 sin0 and x1 cos1 + x0 sin1 take two 16-byte loads and two stores.
+// so x0 cos0 - x1 sin0 and x1 cos1 + x0 sin1 take two 16-byte loads and two stores. Bound by memory: 2158 tokens of 64 heads of
+// 8 kv heads, 105 MB in 22.6 us, launch and all (4.6 TB/s; a large copy runs at 5.1); one token by the launch, 8.4 us.
 template <typename T, typename R>
 __global__ __launch_bounds__(256) void paged_write_kernel(const WriteArgs a) {
     const int half = a.head_dim / 2;
@@ -135,7 +136,9 @@ constexpr int kCUs = 256;
 constexpr int kFewEntries = 512, kEntries = 1024;
 constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
-// what an (entry, kv head) costs on top of its tiles, in tiles: its queries, its first tiles' way from memory, its sums' join
+// what an (entry, kv head) costs on top of its tiles, in tiles: its queries, its first tiles' way from memory, its sums' join.
+// Uncounted, blocks that have many short ones end last: five tokens of nine sequences of 300 to 6000 keys 53 us against 46, 17
+// sequences' next tokens 66 against 63.5; two chunks of 700 tokens, heads of 64, 147 against 145.
 constexpr int kFewStart = 8, kStart = 4;
 constexpr float kSlack = 8.0f;
 constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
@@ -335,14 +338,20 @@ __device__ inline void slow_rows(const PagedArgs& a, int b, int kvh, int row0, i
     }
 }
 
-// Attention of a few rows (query head of a kv head's group, token) per sequence over its pages. An (entry, kv
-// head) that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that
-// join_kernel adds. A wave takes every fourth tile of a share and keeps two in flight
-// (DMA into its own ring: no barriers), and computes
+// Attention of a few rows (query head of a kv head's group, token) per sequence over its pages: p_j = 2^(s_j - m), out =
+// sum p_j v_j / sum p_j with m, once 8 below the running maximum of s = q k scale log2(e), moved up to it. An (entry, kv head)
+// that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that few_join_kernel
+// adds. A wave takes every fourth tile of a share, and its own ring (DMA, no barriers) takes the next tile's keys as soon as
+// these have been read, its values likewise, and computes
 //   S^T = K Q^T      v_mfma_f32_16x16x32, A = 16 keys x 32 dimensions, B = 16 rows of queries
 //   O^T += V^T P^T   A = 16 dimensions x 32 keys, read transposed from the row-major tile, B = P^T: S^T's accumulator layout
 //                    already, with keys 4 g .. +3 and 16 + 4 g .. +3 in lane group g
-// and the probabilities' sums as one more product with ones, from the rounded values that the value product takes.
+// and the probabilities' sums as one more product with ones, from the rounded values that the value product takes (rounded to
+// the type as that product's operand, so what is divided by is the sum of what was taken).
+// Bound by the read of keys and values: 64 sequences of 4000 to 16000 keys, 8 kv heads, 2.67 GB in 460 us, join and all (5.8
+// TB/s), 17 of 20 to 8000 63.5 us (4.7 TB/s). Small calls by latency: 1000 keys of 32 kv heads 8.4 us and 3.5 the join. Two
+// blocks on a CU hold as much in flight as one with rings twice as large and hide each other's waits (with keys and values sent
+// for on their own, 81 -> 66 us for the 17 sequences); three and four row tiles of 128 dimensions need the registers of both.
 template <int D, int RT>
 struct FewShape {
     static constexpr bool kWide = RT >= 3 && D == 128;  // too many registers for two blocks on a CU
@@ -703,7 +712,8 @@ __device__ inline Parts parts_of(const PagedArgs& a, int seg) {
 }
 
 // Adds what the blocks left of one row of an (entry, kv head), for few rows of which many blocks may hold a part: the threads
-// in groups of D / 4, a group every Groups-th part. Bound by latency: where the parts lie, then the parts, then their sums.
+// in groups of D / 4, a group every Groups-th part. Bound by latency: where the parts lie, then the parts, then their sums;
+// 3.5 us for one token of 32 kv heads in four parts each, 5.1 for 40 rows of 72 (sequence, kv head) pairs.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int group) {
     constexpr int L4 = D / 4, Groups = 256 / L4, kAhead = 4;
@@ -769,7 +779,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int gr
 }
 
 // The same for many rows, of which a few blocks hold a part: D / 8 threads a row, eight dimensions each, the parts one after
-// the other.
+// the other. 7 us for 5600 rows of 8 kv heads.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void rows_join_kernel(const PagedArgs a, int group) {
     constexpr int C = D / 8, Rows = 256 / C;
@@ -824,7 +834,8 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const PagedArgs a, int g
 
 constexpr int kKeys = 64;   // keys of a tile
 
-// An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes.
+// An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes. 4.7 us; in every
+// block of rows_kernel, whose entries have hundreds of tokens, it would cost more.
 __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group, int entries) {
     const int entry = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (entry >= entries) return;
@@ -853,11 +864,18 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
 //   S^T = K Q^T      v_mfma_f32_32x32x16, A = 32 keys x 16 dimensions, B = 32 rows of queries
 //   O^T += V^T P^T   A = 32 dimensions x 16 keys, read transposed, B = P^T: S^T's accumulator layout already, with keys
 //                    4 kg .. +3 and 8 + 4 kg .. +3 of each 16 in lane group kg
-// RW 2: 4 waves of 64 rows, which read every operand for two row tiles. One wave a SIMD, so its own instructions have to keep
-// both units busy: a step (32 keys) makes its exponentials among the products of the next step's scores and of the values of
-// the one before.
-// RW 1: 8 waves, 32 rows each, of which waves w and w + 4 have the same rows and a half each of every tile's keys: for grids
-// that leave a CU one block. Their sums are joined through LDS.
+// A tile that every row sees whole runs in a loop that orders products and exponentials by hand: scores of its first 32 keys;
+// scores of the others among the first ones' exponentials; values of the first among the others' exponentials; values of the
+// others. Left to the scheduler, half of the exponentials stood in front of the products (349 us against 338 for the chunk
+// below, page lookups for 64 tiles at a time included).
+// RW 2: 4 waves of 64 rows, which read every operand for two row tiles. One wave a SIMD: what it waits for, nobody fills.
+// RW 1: 8 waves, 32 rows each, of which waves w and w + 4 have the same rows and take the tiles in turn, so two waves a SIMD
+// fill each other's waits; they read each operand twice as often as RW 2's for the same rows. Their sums are joined through
+// LDS. (A half of each tile's keys to either, in step at every barrier: a prompt of 1000 tokens 28.5 us against 25.3.)
+// Bound by products and exponentials of a wave in turn: 4001 tokens of 64 heads of 8 kv heads under a window of 2047, RW 2,
+// 331 us (817 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
+// instructions, of which about half overlap, 1100 waits for LDS and barriers, 480 scalar instructions. A prompt of 1000 tokens,
+// 32 heads, RW 1: 25.3 us, of which the longest row group's 16 tiles take 16.
 // kShared: the work of all row groups in equal shares over the grid, as in few_kernel; otherwise a block takes a row group,
 // the last ones (the longest of a prompt) first.
 template <typename T, int D, int RW, bool kShared>
@@ -1438,8 +1456,9 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     const double longest = max_keys / 64.0, mean = std::max<int64_t>(max_keys - tokens / 2, max_keys / 2) / 64.0;
     // few_kernel reads at the card's rate whatever the grid, 1.9 for a card full, and joins for 7 more than rows_kernel takes.
     // 64 rows a sequence and 8 kv heads: 9 sequences in 2900 keys 45 us against 56, 32 sequences 91 against 78; a sequence of
-    // 64 tokens and 32 kv heads in 8000 keys 48 us against 131, in 64 keys 18 against 11.
-    p.few = rows <= 16 || (rows <= 64 && longest * (1.0 - 1.9 * fill) > 7.0);
+    // 64 tokens and 32 kv heads in 8000 keys 48 us against 131, in 64 keys 18 against 11. Past 3200 keys its shares are worth
+    // more than that whatever the grid: one long sequence among short ones would have a row group's block run on alone.
+    p.few = rows <= 16 || (rows <= 64 && (longest > 50.0 || longest * (1.0 - 1.9 * fill) > 7.0));
     if (p.few) {
         p.tiles = static_cast<int>(ceil_div(rows, 16));
         p.group = 16 * p.tiles;

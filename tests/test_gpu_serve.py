@@ -324,6 +324,17 @@ def test_verify(case, temperature, dtype):
         assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
 
 
+@pytest.mark.parametrize("temperature", [1e-37, 1e-20, 1e-9, 1e-3, 50.0, 1e30])
+def test_verify_at_extreme_temperatures(temperature):
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, drafts, u, probs = _drafts(7, 3, 5001, False, dtype, seed=12)
+        drafts[:3] = logits[:3, :3].argmax(-1)
+        for q in (probs, None):
+            want = oracle.verify(logits, drafts, u, q, torch.tensor(temperature, dtype=torch.float32).item())
+            got = verify_drafts(logits, drafts, u, q, temperature)
+            assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 def test_verify_rows_without_a_distribution():
     logits, drafts, u, probs = _drafts(8, 2, 9001, False, torch.float32, seed=3)
     drafts[:] = 4000
