@@ -421,7 +421,7 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * the running sum of w passes uniforms[b][drafts] times its total: w = p_n where no draft was turned down, else
  * max(p_n - q_n, 0) (p_n where that is zero everywhere). temperature 0 takes p as 1 at the first largest logit.
  * A row with a NaN or an infinite largest logit has no distribution: its draft is turned down and the token is its argmax
- * (the first NaN if there is one). Probabilities and sums in fp64. Three launches.
+ * (the first NaN if there is one). Probabilities and sums in fp64. Three or four launches.
  *   workspace   nq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
  *               not overlap.
  * vocab <= 2^30, and at most 2^23 rows of logits and 2^23 pieces of 4096 of a row a sequence, else NQ_ERR_UNSUPPORTED (and a

@@ -1,11 +1,12 @@
 // Verification of drafted tokens: softmax statistics of every row of logits, the accept tests, and one token by inverse CDF
-// from the row where the drafts end. Three launches:
+// from the row where the drafts end:
 //   1. row_stats_kernel, a block per (row, chunk of one or more parts of 4096 logits): the chunk's largest logit m_c (with its
 //      index) and z_c = sum exp((x - m_c) / T);
-//   2. part_sums_kernel, a block per (sequence, 4096 logits): joins the sequence's rows' statistics and makes the accept tests
-//      u q(x) < p(x), every block of a sequence for itself (four drafts of one sequence against 32000 logits: 15.7 us
-//      against 18.0 with a launch for the tests, seven of 64 against 100003: 63.3 against 62.3), then the sums of
-//      w = max(p - q, 0) and of p over its part of the row that the tests ended at;
+//   2. the accept tests u q(x) < p(x) with the rows' joined statistics, and part_sums_kernel, a block per (sequence, 4096
+//      logits): the sums of w = max(p - q, 0) and of p over its part of the row that the tests ended at. Up to three blocks a
+//      CU every block makes its sequence's tests itself, beyond that a launch of their own does, a block a sequence: seven
+//      drafts against 100000 bf16 logits 26.4 us against 28.2 for 16 sequences, 37.2 against 38.2 for 32, 61.2 against 59.4
+//      for 64 (42.3 against 41.4 and 70.0 against 65.5 for 32 and 64 in fp32);
 //   3. pick_token_kernel, a block per sequence: the part in which the running sum of w passes u times its total, then the
 //      index within it.
 // Probabilities and their sums are fp64: the token is where a running sum over up to 10^5 terms passes a number, and fp32
@@ -18,7 +19,7 @@
 namespace nq {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kCUs = 256;
 struct F32 {};
 
 // Logits come in aligned pieces of 16 bytes, whatever the row's alignment: piece k of a row holds its elements
@@ -334,6 +335,14 @@ __device__ inline Walk walk_of(const VerifyArgs& a, int64_t b, const double* tab
     return Walk{at >> 1, static_cast<int>(draft), st, 1.0 / st.z};
 }
 
+template <typename T>
+__global__ __launch_bounds__(kThreads) void walk_kernel(const VerifyArgs a) {
+    __shared__ double table[kTable];
+    fill_table(table);
+    const Walk walk = walk_of<T, kThreads>(a, blockIdx.x, table);
+    if (threadIdx.x == 0) a.walks[blockIdx.x] = walk;
+}
+
 // A part of a row, a piece a thread of 4096 / N: its p and w.
 template <typename T>
 struct Part {
@@ -377,7 +386,7 @@ struct Part {
 };
 
 // Bound by latency too, of the statistics, of the tests, then of the part: 10 us for 64 sequences of 25 parts.
-template <typename T>
+template <typename T, bool kTests>
 __global__ __launch_bounds__(Part<T>::kThreads) void part_sums_kernel(const VerifyArgs a) {
     constexpr int kWaves = Part<T>::kThreads / 64;
     __shared__ double table[kTable];
@@ -385,9 +394,15 @@ __global__ __launch_bounds__(Part<T>::kThreads) void part_sums_kernel(const Veri
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t b = blockIdx.x / a.row_parts;
     fill_table(table);
-    const Walk walk = walk_of<T, Part<T>::kThreads>(a, b, table);
+    Walk walk;
+    if constexpr (kTests) {
+        walk = walk_of<T, Part<T>::kThreads>(a, b, table);
+    } else {
+        walk = a.walks[b];
+        __syncthreads();
+    }
     const int at = static_cast<int>(blockIdx.x - b * a.row_parts);
-    if (at == 0 && t == 0) a.walks[b] = walk;
+    if (kTests && at == 0 && t == 0) a.walks[b] = walk;
     if (a.inv_t == 0.0 || !finite(rank_value(walk.stat.rank))) return;  // the token is the argmax
     const Part<T> part(a, b, at, walk, table);
     double2 s = {0.0, 0.0};
@@ -514,7 +529,13 @@ template <typename T>
 void launch_verify(const VerifyArgs& a, int64_t batch, hipStream_t st) {
     const int64_t rows = batch * (a.drafts + 1);
     row_stats_kernel<T><<<dim3(static_cast<unsigned>(rows * a.chunks)), kThreads, 0, st>>>(a);
-    part_sums_kernel<T><<<dim3(static_cast<unsigned>(batch * a.row_parts)), Part<T>::kThreads, 0, st>>>(a);
+    const dim3 grid(static_cast<unsigned>(batch * a.row_parts));
+    if (batch * a.row_parts <= 3 * kCUs) {
+        part_sums_kernel<T, true><<<grid, Part<T>::kThreads, 0, st>>>(a);
+    } else {
+        walk_kernel<T><<<dim3(static_cast<unsigned>(batch)), kThreads, 0, st>>>(a);
+        part_sums_kernel<T, false><<<grid, Part<T>::kThreads, 0, st>>>(a);
+    }
     pick_token_kernel<T><<<dim3(static_cast<unsigned>(batch)), Part<T>::kThreads, 0, st>>>(a);
 }
 
