@@ -341,7 +341,7 @@ __device__ inline void slow_rows(const PagedArgs& a, int b, int kvh, int row0, i
 // Attention of a few rows (query head of a kv head's group, token) per sequence over its pages: p_j = 2^(s_j - m), out =
 // sum p_j v_j / sum p_j with m, once 8 below the running maximum of s = q k scale log2(e), moved up to it. An (entry, kv head)
 // that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that few_join_kernel
-// adds. A wave takes every fourth tile of a share, and its own ring (DMA, no barriers) takes the next tile's keys as soon as
+// adds (kShared; otherwise a block has an (entry, kv head)). A wave takes every fourth tile of its block's, and its own ring (DMA, no barriers) takes the next tile's keys as soon as
 // these have been read, its values likewise, and computes
 //   S^T = K Q^T      v_mfma_f32_16x16x32, A = 16 keys x 32 dimensions, B = 16 rows of queries
 //   O^T += V^T P^T   A = 16 dimensions x 32 keys, read transposed from the row-major tile, B = P^T: S^T's accumulator layout
@@ -359,7 +359,7 @@ struct FewShape {
     static constexpr int kStages = kWide || D == 64 ? 2 : 1;  // tiles in a wave's ring: 16 KB, 32 where a block has the CU
 };
 
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool kShared>
 __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_kernel(const PagedArgs a) {
     using Shape = FewShape<D, RT>;
     constexpr int C = D / 8;                  // 16-byte chunks of a row
@@ -368,8 +368,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     constexpr int Half = 2 * Instr;           // for a tile's keys, or its values
     constexpr int S = Shape::kStages, TileElems = kTile * D;
     __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][S][2][TileElems];
-    __shared__ int64_t pre[kFewEntries + 1];
-    __shared__ int2 spans[kFewEntries];  // {sink_tiles, window_tile}
+    __shared__ int64_t pre[kShared ? kFewEntries + 1 : 1];
+    __shared__ int2 spans[kShared ? kFewEntries : 1];  // {sink_tiles, window_tile}
     __shared__ int64_t wave_total[kWaves];
     __shared__ float stat_m[kWaves][16], stat_l[kWaves][16];
     __shared__ int s_entry;
@@ -379,15 +379,22 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
     if (t < 2) s_tainted[t] = 0;
-    const Shares shares = make_shares<64 * kWaves, Shape::kBlocks, kFewStart>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
-                                                                   [&](int e) {
-                                                                       const Tiles r = tiles_of_few(a, e, 16 * RT);
-                                                                       spans[e] = int2{r.sink_tiles, r.window_tile};
-                                                                       return r.count;
-                                                                   });
-    if (shares.entry < 0) return;
-    int entry = shares.entry;
-    int64_t u = shares.first;
+    Shares shares{};
+    int entry;
+    int64_t u = 0;
+    if constexpr (kShared) {
+        shares = make_shares<64 * kWaves, Shape::kBlocks, kFewStart>(a, a.batch * a.row_groups, kLeastShare, pre, wave_total, &s_entry,
+                                                                     [&](int e) {
+                                                                         const Tiles r = tiles_of_few(a, e, 16 * RT);
+                                                                         spans[e] = int2{r.sink_tiles, r.window_tile};
+                                                                         return r.count;
+                                                                     });
+        if (shares.entry < 0) return;
+        entry = shares.entry;
+        u = shares.first;
+    } else {
+        entry = static_cast<int>(blockIdx.x) / a.kv_heads;
+    }
 
     uint32_t voff[Instr];
 #pragma unroll
@@ -399,18 +406,29 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(&ring[wave][0][0][0]));
     int slot = 0, turn = 0;
     while (true) {
-        const int64_t seg0 = pre[entry] * a.kv_heads;
-        const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry])), count = units - kFewStart;
-        const int kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
-        const int64_t seg = seg0 + static_cast<int64_t>(kvh) * units;
-        const int first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart);
-        u = min(shares.end, seg + units);
-        const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart - first;
-        if (n <= 0) return;  // the share ended before its first tile
+        int kvh, first = 0, n, units = 0;
+        int64_t seg = 0;
+        Tiles tiles;
+        if constexpr (kShared) {
+            const int64_t seg0 = pre[entry] * a.kv_heads;
+            units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
+            kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
+            seg = seg0 + static_cast<int64_t>(kvh) * units;
+            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart);
+            u = min(shares.end, seg + units);
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart - first;
+            if (n <= 0) return;  // the share ended before its first tile
+            tiles = Tiles{__builtin_amdgcn_readfirstlane(spans[entry].x), __builtin_amdgcn_readfirstlane(spans[entry].y), units - kFewStart};
+        } else {
+            kvh = static_cast<int>(blockIdx.x) - entry * a.kv_heads;
+            const Tiles r = tiles_of_few(a, entry, 16 * RT);
+            n = __builtin_amdgcn_readfirstlane(r.count);
+            tiles = Tiles{__builtin_amdgcn_readfirstlane(r.sink_tiles), __builtin_amdgcn_readfirstlane(r.window_tile), n};
+        }
+        const int count = tiles.count;
         const int b = entry / a.row_groups;
         const int row0 = (entry - b * a.row_groups) * (16 * RT);
         const int rows = min(16 * RT, a.tokens * a.groups - row0);
-        const Tiles tiles{__builtin_amdgcn_readfirstlane(spans[entry].x), __builtin_amdgcn_readfirstlane(spans[entry].y), count};
 
         const __attribute__((address_space(4))) int32_t* table =
             (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(b) * a.pages.table_stride);
@@ -686,6 +704,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
                 }
             }
         }
+        if constexpr (!kShared) return;
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
                 int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + units - 1) / shares.share)};
@@ -876,7 +895,7 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
 // 331 us (817 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
 // instructions, of which about half overlap, 1100 waits for LDS and barriers, 480 scalar instructions. A prompt of 1000 tokens,
 // 32 heads, RW 1: 25.3 us, of which the longest row group's 16 tiles take 16.
-// kShared: the work of all row groups in equal shares over the grid, as in few_kernel; otherwise a block takes a row group,
+// kShared: the work of all row groups in equal shares over the grid, as few_kernel's; otherwise a block takes a row group,
 // the last ones (the longest of a prompt) first.
 template <typename T, int D, int RW, bool kShared>
 __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_kernel(const PagedArgs a) {
@@ -1462,7 +1481,11 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     if (p.few) {
         p.tiles = static_cast<int>(ceil_div(rows, 16));
         p.group = 16 * p.tiles;
-        p.shared = true;
+        // One row tile also without shares, a block an (entry, kv head): no plan of shares and no join, 4 us, but a block is as
+        // long as its sequence. 32 kv heads of one sequence of 480 keys 8.8 us against 10.6, of 1000 13.2 against 11.7, of
+        // eight sequences of 2000 43.8 against 46.5, of 1 to 4000 57 against 51; 8 kv heads of 64 sequences of 1 to 4000 keys
+        // 108.7 against 109.9. Not past 4096 keys, where one long sequence would run on alone.
+        p.shared = rows > 16 || max_keys > std::max<int64_t>(640, std::min<int64_t>(4096, 8 * batch * kv_heads));
         p.blocks = p.tiles < 3 || head_dim == 64 ? 2 * kCUs : kCUs;  // FewShape's
     } else {
         // Two row tiles a wave where the rows fill them, and a grid of them the card nearly twice: 64 heads of 8 kv heads, a
@@ -1507,10 +1530,11 @@ void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
     const unsigned segs = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.row_groups * a.kv_heads);
     const dim3 grid(static_cast<unsigned>(plan.blocks));
     if (plan.few) {
-        if (plan.tiles == 1) few_kernel<T, D, 1><<<grid, 64 * kWaves, 0, st>>>(a);
-        else if (plan.tiles == 2) few_kernel<T, D, 2><<<grid, 64 * kWaves, 0, st>>>(a);
-        else if (plan.tiles == 3) few_kernel<T, D, 3><<<grid, 64 * kWaves, 0, st>>>(a);
-        else few_kernel<T, D, 4><<<grid, 64 * kWaves, 0, st>>>(a);
+        if (!plan.shared) few_kernel<T, D, 1, false><<<dim3(segs), 64 * kWaves, 0, st>>>(a);
+        else if (plan.tiles == 1) few_kernel<T, D, 1, true><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (plan.tiles == 2) few_kernel<T, D, 2, true><<<grid, 64 * kWaves, 0, st>>>(a);
+        else if (plan.tiles == 3) few_kernel<T, D, 3, true><<<grid, 64 * kWaves, 0, st>>>(a);
+        else few_kernel<T, D, 4, true><<<grid, 64 * kWaves, 0, st>>>(a);
     } else if (plan.shared) {
         const int entries = a.batch * a.row_groups;
         spans_kernel<<<dim3(static_cast<unsigned>(ceil_div(entries, 4))), 256, 0, st>>>(a, static_cast<int>(plan.group), entries);
@@ -1521,8 +1545,9 @@ void launch_slice(const PagedArgs& a, const Plan& plan, hipStream_t st) {
         else rows_kernel<T, D, 2, false><<<dim3(segs), 256, 0, st>>>(a);
     }
     const int group = static_cast<int>(plan.group);
+    if (!plan.shared) return;
     if (plan.few) few_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(a.rows_kept)), 256, 0, st>>>(a, group);
-    else if (plan.shared) rows_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(ceil_div(a.rows_kept, 256 / (D / 8)))), 256, 0, st>>>(a, group);
+    else rows_join_kernel<T, D><<<dim3(segs * static_cast<unsigned>(ceil_div(a.rows_kept, 256 / (D / 8)))), 256, 0, st>>>(a, group);
 }
 
 template <typename T, int D>

@@ -84,7 +84,7 @@ KERNELS = {
         (8, 1, 128, 16, [1500, 700], 7, 600, 20, 0),
         (8, 1, 64, 16, [1100, 650, 9], 6, 100, 0, 0),
         # more sequences than one launch takes, and a table much wider than the lengths
-        (2, 1, 64, 16, [n % 45 + 1 for n in range(600)], 1, 0, 0, 0),
+        (2, 1, 64, 16, [n % 45 + 1 for n in range(600)], 1, 0, 0, 300),
         (3, 3, 128, 16, [50, 7, 33], 15, 0, 0, 400),
     ],
     "shares": [
@@ -98,6 +98,12 @@ KERNELS = {
         (8, 1, 64, 16, [n % 70 + 9 for n in range(1030)], 9, 0, 0, 125),
     ],
     "groups": [
+        (4, 4, 128, 16, [1, 17, 300], 1, 0, 0, 0),
+        (8, 1, 64, 32, [600, 64], 2, 0, 0, 0),
+        (4, 2, 128, 16, [600, 31, 2], 3, 100, 5, 0),
+        (16, 1, 64, 16, [500, 33], 1, 33, 40, 0),
+        (8, 2, 128, 48, [n * 9 % 600 + 1 for n in range(70)], 1, 0, 0, 0),
+        (2, 2, 64, 16, [n * 61 % 1900 + 1 for n in range(130)], 1, 0, 0, 0),
         (8, 2, 128, 16, [300, 90], 9, 0, 0, 0),
         (3, 3, 64, 16, [20, 64], 20, 0, 0, 0),
         (4, 2, 128, 64, [333], 200, 0, 0, 0),
