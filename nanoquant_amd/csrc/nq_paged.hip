@@ -1466,13 +1466,14 @@ struct Plan {
     size_t part_o, part_ml, desc, spans, bytes;
 };
 
-Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t max_keys) {
+// `max_keys` that a row group may see, `mean_keys` one among the others
+Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t max_keys, int64_t mean_keys) {
     Plan p{};
     const int64_t rows = tokens * groups;
     // Times in tiles of 64 keys, as rows_kernel takes them with 128 rows a block (1 us), from measurements of 11 and 29 shapes;
     // `fill` is how often its row groups fill the card, `longest` and `mean` are what a row group may see.
     const double fill = static_cast<double>(ceil_div(rows, 128) * batch * kv_heads) / kCUs;
-    const double longest = max_keys / 64.0, mean = std::max<int64_t>(max_keys - tokens / 2, max_keys / 2) / 64.0;
+    const double longest = max_keys / 64.0, mean = mean_keys / 64.0;
     // few_kernel reads at the card's rate whatever the grid, 1.9 for a card full, and joins for 7 more than rows_kernel takes.
     // 64 rows a sequence and 8 kv heads: 9 sequences in 2900 keys 45 us against 56, 32 sequences 91 against 78; a sequence of
     // 64 tokens and 32 kv heads in 8000 keys 48 us against 131, in 64 keys 18 against 11. Past 3200 keys its shares are worth
@@ -1523,6 +1524,17 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     p.part_ml = static_cast<size_t>(ceil_div(p.part_ml, 16) * 16);
     p.bytes = p.part_o + p.part_ml + p.spans + p.desc;
     return p;
+}
+
+// The plan of a call. A window makes row groups shorter than the table; the workspace's size does not know it, so its plan has to
+// make do with that.
+Plan plan_of(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t max_keys, int64_t window,
+             int64_t sinks) {
+    const Plan p = make_plan(batch, tokens, groups, kv_heads, head_dim, max_keys, std::max(max_keys - tokens / 2, max_keys / 2));
+    if (window == 0) return p;
+    const int64_t visible = std::min(max_keys, window + sinks + std::min(tokens, ceil_div(256, groups)) + 64);
+    const Plan q = make_plan(batch, tokens, groups, kv_heads, head_dim, visible, visible);
+    return q.bytes <= p.bytes ? q : p;
 }
 
 template <typename T, int D>
@@ -1660,7 +1672,7 @@ size_t nq_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t
         tokens > INT32_MAX || batch * tokens > INT32_MAX / heads || table_pages <= 0 || page_size <= 0 ||
         table_pages > kMaxKeys || page_size > kMaxKeys)
         return 0;
-    return make_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size).bytes;
+    return plan_of(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size, 0, 0).bytes;
 }
 
 int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t pages,
@@ -1682,7 +1694,10 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
     if (!q || !out) return fail(NQ_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
         return fail(NQ_ERR_ALIGNMENT, "%s: q, out and the workspace must be 16-byte aligned", name);
-    const size_t need = nq_paged_attention_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, table_pages, page_size);
+    window = std::min(window, kMaxKeys);
+    sinks = std::min(sinks, kMaxKeys);
+    const Plan plan = plan_of(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size, window, sinks);
+    const size_t need = plan.bytes;
     if (need && (!workspace || workspace_bytes < need))
         return fail(NQ_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", name, workspace ? workspace_bytes : size_t{0}, need);
     PagedArgs a{};
@@ -1698,10 +1713,9 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
     a.groups = static_cast<int>(heads / kv_heads);
-    a.window = static_cast<int>(std::min(window, kMaxKeys));
-    a.sinks = static_cast<int>(std::min(sinks, kMaxKeys));
+    a.window = static_cast<int>(window);
+    a.sinks = static_cast<int>(sinks);
     a.scale = scaling * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
-    const Plan plan = make_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim, table_pages * page_size);
     char* ws = static_cast<char*>(workspace);
     hipStream_t st = as_stream(stream);
     if (dtype == NQ_F16) {

@@ -86,6 +86,10 @@ KERNELS = {
         # more sequences than one launch takes, and a table much wider than the lengths
         (2, 1, 64, 16, [n % 45 + 1 for n in range(600)], 1, 0, 0, 300),
         (3, 3, 128, 16, [50, 7, 33], 15, 0, 0, 400),
+        (4, 2, 128, 16, [3000, 2500], 1, 2000, 40, 0),
+        # under windows that leave a block little to read
+        (4, 2, 128, 16, [3000, 2500, 4], 1, 100, 4, 0),
+        (8, 2, 64, 32, [2000, 5], 2, 33, 0, 0),
     ],
     "shares": [
         (4, 2, 128, 64, [4100, 700], 50, 0, 0, 0),
