@@ -349,7 +349,7 @@ __device__ inline void slow_rows(const PagedArgs& a, int b, int kvh, int row0, i
 // and the probabilities' sums as one more product with ones, from the rounded values that the value product takes (rounded to
 // the type as that product's operand, so what is divided by is the sum of what was taken).
 // Bound by the read of keys and values: 64 sequences of 4000 to 16000 keys, 8 kv heads, 2.67 GB in 460 us, join and all (5.8
-// TB/s), 17 of 20 to 8000 63.5 us (4.7 TB/s). Small calls by latency: 1000 keys of 32 kv heads 8.4 us and 3.5 the join. Two
+// TB/s), 17 of 20 to 8000 63.5 us (4.7 TB/s). Small calls by latency: 1000 keys of 32 kv heads 8.9 us and 3.3 the join. Two
 // blocks on a CU hold as much in flight as one with rings twice as large and hide each other's waits (with keys and values sent
 // for on their own, 81 -> 66 us for the 17 sequences); three and four row tiles of 128 dimensions need the registers of both.
 template <int D, int RT>
@@ -732,7 +732,7 @@ __device__ inline Parts parts_of(const PagedArgs& a, int seg) {
 
 // Adds what the blocks left of one row of an (entry, kv head), for few rows of which many blocks may hold a part: the threads
 // in groups of D / 4, a group every Groups-th part. Bound by latency: where the parts lie, then the parts, then their sums;
-// 3.5 us for one token of 32 kv heads in four parts each, 5.1 for 40 rows of 72 (sequence, kv head) pairs.
+// 3.3 us for one token of 32 kv heads in eight parts each, 5.0 for 40 rows of 72 (sequence, kv head) pairs.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int group) {
     constexpr int L4 = D / 4, Groups = 256 / L4, kAhead = 4;
@@ -892,7 +892,7 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
 // fill each other's waits; they read each operand twice as often as RW 2's for the same rows. Their sums are joined through
 // LDS. (A half of each tile's keys to either, in step at every barrier: a prompt of 1000 tokens 28.5 us against 25.3.)
 // Bound by products and exponentials of a wave in turn: 4001 tokens of 64 heads of 8 kv heads under a window of 2047, RW 2,
-// 331 us (817 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
+// 329 us (822 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
 // instructions, of which about half overlap, 1100 waits for LDS and barriers, 480 scalar instructions. A prompt of 1000 tokens,
 // 32 heads, RW 1: 25.3 us, of which the longest row group's 16 tiles take 16.
 // kShared: the work of all row groups in equal shares over the grid, as few_kernel's; otherwise a block takes a row group,
