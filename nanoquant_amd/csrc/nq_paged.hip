@@ -339,10 +339,11 @@ __device__ inline void slow_rows(const PagedArgs& a, int b, int kvh, int row0, i
 }
 
 // Attention of a few rows (query head of a kv head's group, token) per sequence over its pages: p_j = 2^(s_j - m), out =
-// sum p_j v_j / sum p_j with m, once 8 below the running maximum of s = q k scale log2(e), moved up to it. An (entry, kv head)
-// that lies in one block's share is finished there, of the others the blocks leave sums in the workspace that few_join_kernel
-// adds (kShared; otherwise a block has an (entry, kv head)). A wave takes every fourth tile of its block's, and its own ring (DMA, no barriers) takes the next tile's keys as soon as
-// these have been read, its values likewise, and computes
+// sum p_j v_j / sum p_j of s = q k scale log2(e), with m moved up to the running maximum wherever that is more than 8 above it.
+// kShared: an (entry, kv head) that lies in one block's share is finished there, of the others the blocks leave sums in the
+// workspace that few_join_kernel adds; otherwise a block has an (entry, kv head) for itself. A wave takes every fourth tile of
+// its block's, and its own ring (DMA, no barriers) takes the next tile's keys as soon as these have been read, its values
+// likewise, and computes
 //   S^T = K Q^T      v_mfma_f32_16x16x32, A = 16 keys x 32 dimensions, B = 16 rows of queries
 //   O^T += V^T P^T   A = 16 dimensions x 32 keys, read transposed from the row-major tile, B = P^T: S^T's accumulator layout
 //                    already, with keys 4 g .. +3 and 16 + 4 g .. +3 in lane group g

@@ -444,6 +444,31 @@ def test_captured_steps_follow_the_table_and_the_positions():
         cache.reserve(1, 110 + 60 * step)
 
 
+def test_captured_steps_that_share_their_work():
+    """The same for calls with a workspace (one token, drafts, a chunk; long tables), each graph holding two calls in a row."""
+    k, v = (torch.randn(400, 2, 16, 128, device="cuda").bfloat16() for _ in range(2))
+    table = torch.randperm(400, device="cuda")[:390].view(2, 195).int()
+    stream, graphs = torch.cuda.Stream(), []
+    for tokens in (1, 9, 40):
+        assert _lib.load().nq_paged_attention_workspace_bytes(2, tokens, 8, 2, 128, 195, 16) > 0
+        q = torch.randn(2, 2, tokens, 1024, device="cuda").bfloat16()
+        pos = torch.zeros(2, tokens, dtype=torch.int64, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = [paged_attention(x, k, v, table, pos) for x in q]
+        graphs.append((graph, q, pos, out))
+    for step in range(4):
+        for graph, q, pos, out in graphs:
+            base = torch.tensor([[700 * step], [3000 - 900 * step]], device="cuda")
+            pos.copy_(base + torch.arange(pos.shape[1], device="cuda"))
+            graph.replay()
+            got = [o.clone() for o in out]
+            assert all(torch.equal(g, paged_attention(x, k, v, table, pos)) for g, x in zip(got, q))
+        torch.cuda.synchronize()
+        table.copy_(table.flip(0) if step % 2 else table.flip(1))
+
+
 def test_captured_verification():
     logits, drafts, u, probs = _drafts(5, 3, 9000, False, torch.float32, seed=10)
     verify_drafts(logits, drafts, u, probs)
