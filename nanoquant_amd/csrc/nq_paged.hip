@@ -258,12 +258,7 @@ __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least,
             sum += count(e) + kCharge;
         }
     }
-    int64_t incl = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t up = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += up;
-    }
+    const int64_t incl = static_cast<int64_t>(wave_scan(static_cast<double>(sum)));  // far below 2^53
     if (lane == 63) wave_total[wave] = incl;
     __syncthreads();
     int64_t before = incl - sum;
@@ -495,13 +490,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
 #pragma unroll
             for (int kt = 0; kt < D / 32; ++kt) qf[rt][kt] = *vec(src + 32 * kt);
         }
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) {
-            all_last = min(all_last, __shfl_xor(all_last, off, 64));
-            all_start = max(all_start, __shfl_xor(all_start, off, 64));
-        }
-        all_last = __builtin_amdgcn_readfirstlane(all_last);
-        all_start = __builtin_amdgcn_readfirstlane(all_start);
+        all_last = least_of<16>(all_last);
+        all_start = largest_of<16>(all_start);
 
         f32x4 o[RT][D / 16], lsum[RT];
         float m[RT];
@@ -1066,15 +1056,9 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                 // in accumulation registers, from which the products take them as they are: the vector registers hold the rest
                 if constexpr (RW == 2) asm volatile("" : "+a"(qf[rw][kt]));
             }
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            lo = min(lo, __shfl_xor(lo, off, 64));
-            hi = max(hi, __shfl_xor(hi, off, 64));
-            all_start = max(all_start, __shfl_xor(all_start, off, 64));
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
-        all_start = __builtin_amdgcn_readfirstlane(all_start);
+        lo = least_of<32>(lo);
+        hi = largest_of<32>(hi);
+        all_start = largest_of<32>(all_start);
         const int any_start = a.window > 0 ? max(0, lo == INT32_MAX ? 0 : lo - a.window + 1) : 0;  // the first key of some row
         if constexpr (!kShared) {
             if (lane == 0) {

@@ -18,6 +18,23 @@ __device__ inline float max_xor16(float v) {
     return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 
+// Smallest and largest over lanes 0 to kLanes - 1 (16 or 32), the same in the whole wave.
+template <int kControl>
+__device__ inline int dpp_or_own(int v) {  // of the lane that a DPP control names, the lane's own where there is none
+    return __builtin_amdgcn_update_dpp(v, v, kControl, 0xF, 0xF, false);
+}
+template <int kLanes>
+__device__ inline int least_of(int v) {
+    v = min(v, dpp_or_own<0x111>(v));  // row_shr:1
+    v = min(v, dpp_or_own<0x112>(v));
+    v = min(v, dpp_or_own<0x114>(v));
+    v = min(v, dpp_or_own<0x118>(v));
+    if (kLanes == 32) v = min(v, dpp_or_own<0x142>(v));  // row_bcast:15
+    return __builtin_amdgcn_readlane(v, kLanes - 1);
+}
+template <int kLanes>
+__device__ inline int largest_of(int v) { return ~least_of<kLanes>(~v); }
+
 // u of the lane that a DPP control names, 0 where there is none or the row is masked out.
 template <int kControl, int kRows>
 __device__ inline uint64_t dpp(uint64_t u) {
