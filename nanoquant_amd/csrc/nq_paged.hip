@@ -390,6 +390,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         u = shares.first;
     } else {
         entry = static_cast<int>(blockIdx.x) / a.kv_heads;
+        __syncthreads();  // s_tainted is cleared before any wave sets it (make_shares has barriers of its own)
     }
 
     uint32_t voff[Instr];

@@ -225,6 +225,22 @@ def test_values_that_a_token_does_not_see_do_not_reach_it(group, tokens, dtype):
     assert y[-1, 1].isnan().any()
 
 
+@pytest.mark.parametrize("dim,tokens,group", [(128, 4, 1), (64, 3, 4), (128, 16, 1)])
+def test_values_that_a_token_does_not_see_in_blocks_without_shares(dim, tokens, group):
+    """Sequences of two to five tiles of 32 keys, whose last one each of a block's four waves has in turn: a value there that
+    is not finite and that the last token alone sees leaves the others what they are without it."""
+    lengths = [60, 90, 120, 160]
+    q, k, v, table, pos = oracle.paged_case(2 * group, 2, dim, 16, lengths, tokens, torch.bfloat16, "cuda")
+    assert _lib.load().nq_paged_attention_workspace_bytes(4, tokens, 2 * group, 2, dim, table.shape[1], 16) == 0
+    ref, spread = oracle.attention(q, k, v, table, pos)
+    for bad in (math.nan, math.inf, -math.inf):
+        for b, n in enumerate(lengths):
+            v[int(table[b, (n - 1) // 16]), :, (n - 1) % 16] = bad
+        y = paged_attention(q, k, v, table, pos)
+        _check(y[:, :-1], ref[:, :-1], spread[:, :-1], torch.bfloat16, 160)
+        assert not torch.isfinite(y[:, -1]).any()
+
+
 def test_attention_of_large_scores():
     """Scores of some hundreds, of both signs, and a last key that beats all before it."""
     q, k, v, table, pos = oracle.paged_case(4, 1, 128, 16, [300, 150], 1, torch.float16, "cuda")
