@@ -244,7 +244,8 @@ std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Ten
         (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat))
         return {};
     const int64_t B = logits.size(0), n = logits.size(1) - 1, V = logits.size(2);
-    if (logits.stride(2) != 1 || logits.stride(1) < V || (B > 1 && logits.stride(0) != (n + 1) * logits.stride(1)) ||
+    const int64_t stride = n > 0 ? logits.stride(1) : B > 1 ? logits.stride(0) : V;  // between rows
+    if (logits.stride(2) != 1 || stride < V || (n > 0 && B > 1 && logits.stride(0) != (n + 1) * stride) ||
         !plain(drafts, logits, at::kLong) || drafts.size(0) != B || drafts.size(1) != n || !plain(uniforms, logits, at::kFloat) ||
         uniforms.size(0) != B || uniforms.size(1) != n + 1 || !(temperature >= 0.0) ||
         static_cast<float>(temperature) > 3.402823466e38f || (temperature > 0.0 && static_cast<float>(temperature) == 0.0f))
@@ -257,7 +258,7 @@ std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Ten
     const c10::DeviceGuard guard(logits.device());
     Tensor accepted = at::empty({B}, drafts.options()), tokens = at::empty({B, n + 1}, drafts.options());
     const Tensor ws = scratch(bytes, logits);
-    if (lib->verify(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), logits.stride(1),
+    if (lib->verify(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), stride,
                     static_cast<const int64_t*>(drafts.const_data_ptr()), static_cast<const float*>(data_of(draft_probs)),
                     static_cast<const float*>(uniforms.const_data_ptr()), static_cast<float>(temperature),
                     static_cast<int64_t*>(accepted.mutable_data_ptr()), static_cast<int64_t*>(tokens.mutable_data_ptr()), B, n, V,

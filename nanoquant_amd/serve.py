@@ -299,6 +299,17 @@ def paged_rotary_attention(shape, layer: int, q, k, v, cos, sin, positions, cach
 
 # ------------------------------------------------------------------------------------- drafted tokens
 
+def _logit_rows(x):
+    """x [batch, rows, vocab] as evenly spaced rows, and the elements between two: itself, or a copy. The stride of a dimension
+    of one element says nothing, and ``contiguous`` leaves it as it is."""
+    batch, rows, vocab = x.shape
+    stride = x.stride(1) if rows > 1 else x.stride(0) if batch > 1 else vocab
+    if x.stride(2) != 1 or stride < vocab or (rows > 1 and batch > 1 and x.stride(0) != rows * stride):
+        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+        stride = vocab
+    return x, stride
+
+
 def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float = 1.0):
     """Keep or turn down drafted tokens so that what comes out is distributed as the model's own tokens.
 
@@ -339,8 +350,7 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
         tokens = torch.empty(B, n + 1, dtype=torch.int64, device=logits.device)
         if B == 0:
             return accepted, tokens
-        if logits.stride(2) != 1 or logits.stride(1) < V or logits.stride(0) != (n + 1) * logits.stride(1):
-            logits = logits.contiguous()
+        logits, stride = _logit_rows(logits)
         drafts, uniforms = drafts.contiguous(), uniforms.contiguous()
         if draft_probs is not None:
             draft_probs = draft_probs.contiguous()
@@ -348,7 +358,7 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
         nbytes = lib.nq_verify_drafts_workspace_bytes(B, n, V)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
         code = _lib.NQ_F32 if logits.dtype == torch.float32 else _lib.dtype_code(logits.dtype)
-        _launch(what, lib.nq_verify_drafts, logits, code, logits.data_ptr(), logits.stride(1), drafts.data_ptr(),
+        _launch(what, lib.nq_verify_drafts, logits, code, logits.data_ptr(), stride, drafts.data_ptr(),
                 _lib.ptr(draft_probs), uniforms.data_ptr(), temperature, accepted.data_ptr(), tokens.data_ptr(), B, n, V,
                 ws.data_ptr(), nbytes)
         return accepted, tokens

@@ -421,6 +421,20 @@ def test_verify_takes_strided_rows():
     assert torch.equal(got[1], want[1])
 
 
+def test_verify_takes_single_rows_whatever_their_strides():
+    """No drafts: one row a sequence, as a view whose strides of dimensions of one element are any."""
+    logits, drafts, u, _ = _drafts(6, 0, 3001, True, torch.float32, seed=14)
+    want = verify_drafts(logits, drafts, u)
+    across = logits.view(1, 6, 3001).transpose(0, 1)
+    assert across.stride() == (3001, 18006, 1)
+    wide = torch.full((6, 2, 3100), 60.0, device="cuda")
+    wide[:, 1, :3001] = logits[:, 0]
+    close = torch.as_strided(logits, (1, 1, 3001), (1, 1, 1))
+    for x, n in ((across, 6), (wide[:, 1:, :3001], 6), (close, 1)):
+        got = verify_drafts(x, drafts[:n], u[:n])
+        assert torch.equal(got[0], want[0][:n]) and torch.equal(got[1], want[1][:n])
+
+
 def _together(cache, shape, tokens, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     draw = lambda n: torch.randn(cache.batch, tokens, n * 128, device="cuda", generator=g).half()  # noqa: E731

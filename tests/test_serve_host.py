@@ -89,6 +89,20 @@ def test_verify_rows_without_a_distribution():
     assert got[1][:3, 0].tolist() == [7, 9, 0]
 
 
+def test_rows_of_logits_whatever_the_strides():
+    """The rows that a kernel would read are the tensor's, also where a dimension has one element and any stride."""
+    from nanoquant_amd.serve import _logit_rows
+    x = torch.arange(4 * 7 * 10).view(4, 7, 10).float()
+    for t in (x, x[..., 1:9], x[:, :3], x[:, ::2], x[:, 2:3], x[2:3], x[2:3, 4:5], x[1:2].transpose(0, 1), x[..., 3:4], x[:1, :1, :1],
+              x.transpose(0, 1), x[:, 3].unsqueeze(1).expand(4, 5, 10), x[0, :, :1].t()[None], x[0, :, :1].t().unsqueeze(1)):
+        rows, stride = _logit_rows(t)
+        B, R, V = t.shape
+        at = rows.storage_offset() + (B * R - 1) * stride + V
+        assert stride >= V and at <= rows.untyped_storage().nbytes() // 4
+        assert torch.equal(torch.as_strided(rows, (B * R, V), (stride, 1), rows.storage_offset()).reshape(t.shape), t)
+    assert _logit_rows(x[1:2].transpose(0, 1))[0].data_ptr() == x[1:2].data_ptr()  # read in place
+
+
 def test_verified_tokens_have_the_models_distribution():
     """Over a fine grid of random numbers the first token's frequencies are the model's probabilities: of 400 x 400 pairs
     (accept, pick) a border moves a count by at most one a row of the grid, so each is within 2 / 400 of p."""
