@@ -85,8 +85,8 @@ struct Row {
 // exp(d) for d <= 0 as p t: n = round(128 d / ln2), t = 2^(n / 128) from a table, with n / 128's whole part added to its
 // exponent, and a polynomial p of |r| <= ln2 / 256 (table-driven exp, Tang 1989), whose first term left out is below 2^-49. n
 // comes as the low bits of a sum with 1.5 * 2^52. The copy in LDS has i << 13 taken from the upper word of entry i, so that
-// all of n << 13 is added to it (an exponent's one is 2^20). Below -700 exp(d) counts as exp(-700), which is nothing beside 1. A table of
-// 32 entries, a copy in every pair of LDS banks, and one term more cost 10%: the arithmetic bounds this, not the table's reads.
+// all of n << 13 is added to it (an exponent's one is 2^20). A table of 32 entries, a copy in every pair of LDS banks, and one
+// term more cost 10%: the arithmetic bounds this, not the table's reads.
 constexpr int kTable = 128;
 __device__ const double kPowers[kTable] = {  // 2^(i / 128)
     0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0, 0x1.059b0d3158574p+0,
@@ -120,25 +120,37 @@ __device__ inline void fill_table(double* table) {
     if (threadIdx.x < kTable)
         table[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, kPowers[threadIdx.x]) - (static_cast<uint64_t>(threadIdx.x) << 45));
 }
-__device__ inline void exp_parts(double d, const double* table, double& p, double& t) {
+__device__ inline uint32_t exp_reduce(double d, double& p) {  // n, p
     constexpr double kMagic = 6755399441055744.0;
-    d = fmax(d, -700.0);
     const double sum = fma(d, kTable * 1.4426950408889634, kMagic);
     const double r = fma(sum - kMagic, -0.6931471805599453 / kTable, d);
     p = fma(r, 1.0 / 24, 1.0 / 6);
     p = fma(r, p, 0.5);
     p = fma(r, p, 1.0);
     p = fma(r, p, 1.0);
-    const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
+    return static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum));
+}
+__device__ inline double exp_power(uint32_t n, uint32_t add, const double* table) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     u32x2 bits = __builtin_bit_cast(u32x2, table[n & (kTable - 1)]);
-    bits.y += n << 13;
-    t = __builtin_bit_cast(double, bits);
+    bits.y += add << 13;
+    return __builtin_bit_cast(double, bits);
+}
+// For sums in which there is a 1 as well: below -700 exp(d) counts as exp(-700), which is nothing beside it.
+__device__ inline void exp_parts(double d, const double* table, double& p, double& t) {
+    const uint32_t n = exp_reduce(fmax(d, -700.0), p);
+    t = exp_power(n, n, table);
 }
 __device__ inline double exp_of(double d, const double* table) {
     double p, t;
     exp_parts(d, table, p, t);
     return p * t;
+}
+// For what is compared with 0: subnormal where exp(d) is, and 0 below that (about -745). The whole part of n / 128 goes in last.
+__device__ inline double exp_or_zero(double d, const double* table) {
+    double p;
+    const uint32_t n = exp_reduce(fmax(d, -1100.0), p);
+    return __builtin_ldexp(p * exp_power(n, n & (kTable - 1), table), static_cast<int>(n) >> 7);
 }
 
 // (order of x, index) as one number whose maximum is torch.argmax's choice: the first largest, the first NaN if there is one.
@@ -317,7 +329,7 @@ __device__ inline Walk walk_of(const VerifyArgs& a, int64_t b, const double* tab
             const float m = rank_value(st.rank);
             double p = 0.0;
             if (a.inv_t == 0.0 || !finite(m)) p = finite(m) && rank_index(st.rank) == x ? 1.0 : 0.0;
-            else if (logit != -INFINITY) p = exp_of((static_cast<double>(logit) - m) * a.inv_t, table) / st.z;
+            else if (logit != -INFINITY) p = exp_or_zero((static_cast<double>(logit) - m) * a.inv_t, table) / st.z;
             const double q = a.inv_t != 0.0 ? qx : 1.0;
             if ((t & 15) == 0) {
                 stats[group] = st;
@@ -379,7 +391,7 @@ struct Part {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const bool none = x[i] == -INFINITY || !(inside || static_cast<unsigned>(first + i) < static_cast<unsigned>(src.vocab));
-            p[i] = none ? 0.0 : exp_of((static_cast<double>(x[i]) - top) * a.inv_t, table) * walk.inv_z;
+            p[i] = none ? 0.0 : exp_or_zero((static_cast<double>(x[i]) - top) * a.inv_t, table) * walk.inv_z;
             w[i] = walk.draft >= 0 ? (p[i] > q[i] ? p[i] - q[i] : 0.0) : p[i];
         }
     }

@@ -409,6 +409,47 @@ def test_verify_at_the_ends_of_the_random_numbers():
     assert int(got[1].max()) < 4990
 
 
+@pytest.mark.parametrize("dtype,mask", [(torch.float32, -1e4), (torch.float32, torch.finfo(torch.float32).min),
+                                        (torch.float16, -65504.0), (torch.bfloat16, -1e4)], ids=str)
+def test_verify_never_takes_a_token_masked_with_a_finite_number(dtype, mask):
+    """exp is 0 in float64 that far below the largest: at a random number of 0 neither the first index nor a draft is taken for
+    it, and where the drafter's probabilities cover the model's there is nothing left but p itself."""
+    logits, drafts, u, probs = _drafts(6, 2, 5000, False, dtype, seed=15)
+    logits[:, :, :10] = mask
+    logits[:, :, 4990:] = mask
+    u[:3] = 0.0
+    drafts[0], drafts[1] = 3, 4995   # masked drafts
+    u[3:, :2] = 1.0 - 2.0 ** -24
+    probs[:] = torch.softmax(logits[:, :2].float(), -1) * (1 + 1e-3)  # q > p wherever p is positive
+    for q in (probs, None):
+        for temperature in (1.0, 0.7):
+            want = oracle.verify(logits, drafts, u, q, temperature)
+            got = verify_drafts(logits, drafts, u, q, temperature)
+            assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+            kept = got[0].view(-1, 1) > torch.arange(3, device="cuda")
+            extra = got[1][(got[1] >= 0) & ~kept]
+            assert int(extra.min()) >= 10 and int(extra.max()) < 4990
+
+
+def test_verify_where_exponentials_are_subnormal():
+    """Weights down to 2^-1074 are weights, and those below are none: exponents of -728 and -768, whose exponentials are near
+    1e-316 and 1e-334, and the same by a small temperature."""
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.full((4, 2, 3000), -768.0, dtype=dtype, device="cuda")
+        logits[:, :, 2000] = 0.0
+        logits[1:, :, 700] = -728.0
+        drafts = torch.tensor([[5], [700], [1], [2000]], device="cuda")
+        u = torch.zeros(4, 2, device="cuda")
+        for x, temperature in ((logits, 1.0), (logits / 1024, 2.0 ** -10)):
+            got = verify_drafts(x, drafts, u, None, temperature)
+            want = oracle.verify(x, drafts, u, None, temperature)
+            assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+            assert got[1][:3, 0].tolist() == [2000, 700, 700]
+    x = torch.tensor([[[0.0, -10.0, 5.0]]], device="cuda")
+    got = verify_drafts(x, torch.zeros(1, 0, dtype=torch.int64, device="cuda"), torch.zeros(1, 1, device="cuda"), None, 0.005)
+    assert got[1].tolist() == [[2]]
+
+
 def test_verify_takes_strided_rows():
     logits, drafts, u, probs = _drafts(4, 3, 5003, False, torch.bfloat16, seed=9)
     want = verify_drafts(logits, drafts, u, probs)
