@@ -19,6 +19,7 @@ Hugging Face's static cache and samples one token a step (``src/nanoquant/kernel
 from __future__ import annotations
 
 import math
+import sys
 
 import torch
 
@@ -366,7 +367,9 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
     top = x.amax(dim=-1, keepdim=True)  # NaN where the row has one
     best = x.argmax(dim=-1, keepdim=True)
     plain = torch.isfinite(top) if temperature else torch.zeros_like(top, dtype=torch.bool)
-    e = torch.exp((x - torch.where(plain, top, 0.0)) * (1.0 / temperature if temperature else 1.0))
+    # finite, so that 0 stays 0: two logits that differ are 2^-149 apart at least, far enough for any such temperature
+    factor = min(1.0 / temperature, sys.float_info.max) if temperature else 1.0
+    e = torch.exp((x - torch.where(plain, top, 0.0)) * factor)
     p = torch.where(plain, e / e.sum(dim=-1, keepdim=True), torch.zeros_like(e).scatter_(2, best, 1.0))
     real = (drafts >= 0) & (drafts < V)
     at = torch.where(real, drafts, 0).unsqueeze(-1)

@@ -120,6 +120,19 @@ def test_verified_tokens_have_the_models_distribution():
     assert ((count / (n * n)) - p).abs().max() < 2.0 / n
 
 
+@pytest.mark.parametrize("temperature", [1e-310, 5e-324, 1e-46, 1e300])
+def test_verify_at_temperatures_whose_reciprocal_or_float_is_none(temperature):
+    """A positive temperature is not greedy, however small: two tokens that are equally likely share the draws."""
+    logits = torch.tensor([1.0, 1.0, 0.0]).expand(1, 2, 3)
+    for draft in (0, 1, 2):
+        for u in ([0.9, 0.3], [0.9, 0.7], [0.3, 0.99], [0.1, 0.0]):
+            drafts, us = torch.tensor([[draft]]), torch.tensor([u])
+            for probs in (None, torch.tensor([[[0.9, 0.1, 0.0]]])):
+                want = oracle.verify(logits, drafts, us, probs, temperature)
+                got = verify_drafts(logits, drafts, us, probs, temperature)
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_paged_model_equals_the_static_cache():
     """Prompts of two lengths in one padded batch, then single tokens, against each sequence alone on a static cache."""
     model = random_llama(TINY, device="cpu", seed=3)
