@@ -419,7 +419,8 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * Draft i is kept iff all before it are and uniforms[b][i] * q_i(x_i) < p_i(x_i). accepted[b] = their number n, and
  * tokens[b] (int64 [batch, drafts + 1]) the n drafts, one token more, and -1 behind. That token is the first index at which
  * the running sum of w passes uniforms[b][drafts] times its total: w = p_n where no draft was turned down, else
- * max(p_n - q_n, 0) (p_n where that is zero everywhere). temperature 0 takes p as 1 at the first largest logit.
+ * max(p_n - q_n, 0) (p_n where that is zero everywhere). temperature 0 takes p as 1 at the first largest logit;
+ * any other finite one is taken in fp64 as it is.
  * A row with a NaN or an infinite largest logit has no distribution: its draft is turned down and the token is its argmax
  * (the first NaN if there is one). Probabilities and sums in fp64. Three or four launches.
  *   workspace   nq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
@@ -429,7 +430,7 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * harness samples one token a step with torch ops (src/nanoquant/kernel/test_decode.py:350-353). */
 size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
-                     const float* uniforms, float temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
+                     const float* uniforms, double temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
                      int64_t drafts, int64_t vocab, void* workspace, size_t workspace_bytes, nq_stream_t stream);
 
 /* ---------------------------------------------------------------- norm and activation of many tokens */

@@ -95,7 +95,7 @@ SIGNATURES = {
     "nq_paged_attention": (_int, [_int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                   _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
     "nq_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64]),
-    "nq_verify_drafts": (_int, [_int, _vp, _i64, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
+    "nq_verify_drafts": (_int, [_int, _vp, _i64, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
     "nq_rms_norm": (_int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp]),
     "nq_silu_mul": (_int, [_int, _vp, _vp, _vp, _i64, _vp]),
     "nq_dense_gemv": (_int, [_int, _vp, _vp, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _i64, _i64, _vp]),

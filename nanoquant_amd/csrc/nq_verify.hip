@@ -12,6 +12,7 @@
 // Probabilities and their sums are fp64: the token is where a running sum over up to 10^5 terms passes a number, and fp32
 // rounding would move a visible share of the borders between tokens.
 #include <algorithm>
+#include <cfloat>
 
 #include "nq_common.h"
 #include "nq_wave.h"
@@ -567,13 +568,13 @@ size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
 }
 
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
-                     const float* uniforms, float temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
+                     const float* uniforms, double temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
                      int64_t drafts, int64_t vocab, void* workspace, size_t workspace_bytes, nq_stream_t stream) {
     const char* name = "nq_verify_drafts";
     if (dtype != NQ_F16 && dtype != NQ_BF16 && dtype != NQ_F32) return fail(NQ_ERR_DTYPE, "%s: unsupported dtype %d", name, dtype);
     if (batch < 0 || drafts < 0 || vocab <= 0) return fail(NQ_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
     if (row_stride < vocab) return fail(NQ_ERR_SHAPE, "%s: rows of logits overlap", name);
-    if (!(temperature >= 0.0f) || temperature > 3.402823466e38f)
+    if (!(temperature >= 0.0 && temperature <= DBL_MAX))
         return fail(NQ_ERR_INVALID_ARGUMENT, "%s: the temperature must be a finite number from 0", name);
     if (batch == 0) return NQ_OK;
     const size_t need = nq_verify_drafts_workspace_bytes(batch, drafts, vocab);
@@ -591,7 +592,8 @@ int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const in
     a.draft = draft;
     a.draft_probs = draft_probs;
     a.uniforms = uniforms;
-    a.inv_t = temperature > 0.0f ? 1.0 / static_cast<double>(temperature) : 0.0;
+    // finite, so that 0 stays 0: two logits that differ are 2^-149 apart at least, far enough for any such temperature
+    a.inv_t = temperature > 0.0 ? std::min(1.0 / temperature, DBL_MAX) : 0.0;
     a.accepted = accepted;
     a.tokens = tokens;
     a.vocab = vocab;

@@ -247,8 +247,7 @@ std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Ten
     const int64_t stride = n > 0 ? logits.stride(1) : B > 1 ? logits.stride(0) : V;  // between rows
     if (logits.stride(2) != 1 || stride < V || (n > 0 && B > 1 && logits.stride(0) != (n + 1) * stride) ||
         !plain(drafts, logits, at::kLong) || drafts.size(0) != B || drafts.size(1) != n || !plain(uniforms, logits, at::kFloat) ||
-        uniforms.size(0) != B || uniforms.size(1) != n + 1 || !(temperature >= 0.0) ||
-        static_cast<float>(temperature) > 3.402823466e38f || (temperature > 0.0 && static_cast<float>(temperature) == 0.0f))
+        uniforms.size(0) != B || uniforms.size(1) != n + 1 || !(temperature >= 0.0) || std::isinf(temperature))
         return {};
     if (draft_probs.has_value() && (!plain(*draft_probs, logits, at::kFloat) || draft_probs->dim() != 3 ||
                                     draft_probs->size(0) != B || draft_probs->size(1) != n || draft_probs->size(2) != V))
@@ -260,7 +259,7 @@ std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Ten
     const Tensor ws = scratch(bytes, logits);
     if (lib->verify(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), stride,
                     static_cast<const int64_t*>(drafts.const_data_ptr()), static_cast<const float*>(data_of(draft_probs)),
-                    static_cast<const float*>(uniforms.const_data_ptr()), static_cast<float>(temperature),
+                    static_cast<const float*>(uniforms.const_data_ptr()), temperature,
                     static_cast<int64_t*>(accepted.mutable_data_ptr()), static_cast<int64_t*>(tokens.mutable_data_ptr()), B, n, V,
                     ws.mutable_data_ptr(), bytes, stream_of(logits)) != NQ_OK)
         return {};

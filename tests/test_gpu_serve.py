@@ -450,6 +450,42 @@ def test_verify_where_exponentials_are_subnormal():
     assert got[1].tolist() == [[2]]
 
 
+@pytest.mark.parametrize("temperature", [0.6, 0.7, 1.3])
+def test_verify_takes_the_temperature_as_given(temperature):
+    """Accept tests u q < p whose two sides differ by less than rounding the temperature to float32 moves p, and by more than
+    1e-13 of it: float64's exponential and quotient are off by some 1e-15."""
+    g = torch.Generator().manual_seed(16)
+    logits = torch.randn(4000, 2, 3, generator=g) * 4
+    drafts = torch.randint(0, 3, (4000, 1), generator=g)
+    rounded = torch.tensor(temperature).double()  # float32
+    p, near = (torch.softmax(logits[:, 0].double() / t, -1).gather(1, drafts)[:, 0] for t in (temperature, rounded))
+    u = torch.rand(4000, 2, generator=g) * 0.5 + 0.5
+    q = ((p + near) / 2 / u[:, 0].double()).float()
+    sides = torch.stack((p, near)) - u[:, 0].double() * q.double()
+    pick = (sides[0] * sides[1] < 0) & (sides.abs() > 1e-13 * p).all(0)
+    assert int(pick.sum()) > 50
+    logits, drafts, u, q = logits[pick], drafts[pick], u[pick], q[pick]
+    probs = torch.zeros(len(q), 1, 3).scatter_(2, drafts.unsqueeze(1), q.view(-1, 1, 1))
+    want = oracle.verify(logits, drafts, u, probs, temperature)
+    assert 0 < int(want[0].sum()) < len(q)
+    for device in ("cpu", "cuda"):
+        got = verify_drafts(*(t.to(device) for t in (logits, drafts, u, probs)), temperature)
+        assert torch.equal(got[0].cpu(), want[0])
+
+
+@pytest.mark.parametrize("temperature", [1e-310, 5e-324, 1e-46, 1e-40, 1e300])
+def test_verify_at_temperatures_that_no_float32_holds(temperature):
+    """A positive temperature is not greedy, however small, and no finite one too large."""
+    logits = torch.tensor([1.0, 1.0, 0.0], device="cuda").expand(4, 2, 3)
+    u = torch.tensor([[0.9, 0.3], [0.9, 0.7], [0.3, 0.99], [0.1, 0.0]], device="cuda")
+    for draft in (0, 1, 2):
+        drafts = torch.full((4, 1), draft, device="cuda")
+        for probs in (None, torch.tensor([0.9, 0.1, 0.0], device="cuda").expand(4, 1, 3)):
+            want = oracle.verify(logits, drafts, u, probs, temperature)
+            got = verify_drafts(logits, drafts, u, probs, temperature)
+            assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 def test_verify_takes_strided_rows():
     logits, drafts, u, probs = _drafts(4, 3, 5003, False, torch.bfloat16, seed=9)
     want = verify_drafts(logits, drafts, u, probs)
