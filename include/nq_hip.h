@@ -425,9 +425,10 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * (the first NaN if there is one). Probabilities and sums in fp64. Three or four launches.
  *   workspace   nq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
  *               not overlap.
- * vocab <= 2^30, and at most 2^23 rows of logits and 2^23 pieces of 4096 of a row a sequence, else NQ_ERR_UNSUPPORTED (and a
- * workspace of 0 bytes). Logits aligned to their size, draft_probs and uniforms to 4 bytes, whole numbers to 8. The reference has no counterpart: its
- * harness samples one token a step with torch ops (src/nanoquant/kernel/test_decode.py:350-353). */
+ * vocab <= 2^30, at most 2^23 rows of logits, and batch * (pieces of 4096 logits of a row, ceil((vocab + 7) / 4096)) below 2^23
+ * (2^22 in NQ_F32), else NQ_ERR_UNSUPPORTED. Logits aligned to their size, draft_probs and uniforms to 4 bytes, whole numbers to
+ * 8. The reference has no counterpart: its harness samples one token a step with torch ops
+ * (src/nanoquant/kernel/test_decode.py:350-353). */
 size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab);
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
                      const float* uniforms, double temperature, int64_t* accepted, int64_t* tokens, int64_t batch,

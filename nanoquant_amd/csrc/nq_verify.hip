@@ -563,7 +563,7 @@ size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
     if (batch <= 0 || drafts < 0 || vocab <= 0 || vocab > (1 << 30) || batch > INT32_MAX || drafts > INT32_MAX / 2) return 0;
     if (batch > (int64_t{1} << 23) / (drafts + 1)) return 0;
     const int64_t chunks = chunks_of(batch * (drafts + 1), vocab);
-    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks || batch > (int64_t{1} << 23) / row_parts_of(vocab)) return 0;  // blocks of 256 threads
+    if (batch * (drafts + 1) > (int64_t{1} << 23) / chunks || batch > (int64_t{1} << 23) / row_parts_of(vocab)) return 0;
     return static_cast<size_t>(batch) * (((drafts + 1) * chunks + row_parts_of(vocab)) * 16 + 32);
 }
 
@@ -578,7 +578,9 @@ int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const in
         return fail(NQ_ERR_INVALID_ARGUMENT, "%s: the temperature must be a finite number from 0", name);
     if (batch == 0) return NQ_OK;
     const size_t need = nq_verify_drafts_workspace_bytes(batch, drafts, vocab);
-    if (need == 0) return fail(NQ_ERR_UNSUPPORTED, "%s: sizes too large", name);
+    const int64_t part_threads = dtype == NQ_F32 ? Part<F32>::kThreads : Part<F16>::kThreads;
+    if (need == 0 || batch * row_parts_of(vocab) > UINT32_MAX / part_threads)  // a launch's threads are counted in 32 bits
+        return fail(NQ_ERR_UNSUPPORTED, "%s: sizes too large", name);
     if (!logits || (!draft && drafts) || !uniforms || !accepted || !tokens || !workspace)
         return fail(NQ_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
     if (!aligned(logits, dtype == NQ_F32 ? 4 : 2) || !aligned(draft, 8) || !aligned(draft_probs, 4) || !aligned(uniforms, 4) ||

@@ -260,3 +260,18 @@ def test_c_abi_argument_errors_need_no_gpu():
     assert verify(batch=1 << 30, drafts=1 << 20) == verify(vocab=1 << 32, stride=1 << 32) == _lib.NQ_ERR_UNSUPPORTED
     assert verify(logits=p + 2) == verify(ws=p + 8) == _lib.NQ_ERR_ALIGNMENT
     assert verify(nbytes=lib.nq_verify_drafts_workspace_bytes(2, 3, 100) - 1) == _lib.NQ_ERR_WORKSPACE
+
+
+def test_c_abi_limits_of_the_verification_need_no_gpu():
+    """A launch has fewer than 2^32 threads, 1024 for a part of a row in float32 and 512 in the 16-bit types. Every call below
+    ends before its launch, for its workspace of no bytes if not for its size."""
+    lib, p = _lib.load(), 256
+
+    def verify(dtype, batch, vocab=4):
+        return lib.nq_verify_drafts(dtype, p, vocab, p, None, p, 1.0, p, p, batch, 0, vocab, p, 0, None)
+
+    assert verify(_lib.NQ_F32, 1 << 22) == verify(_lib.NQ_F16, 1 << 23) == verify(_lib.NQ_BF16, 1 << 23) == _lib.NQ_ERR_UNSUPPORTED
+    assert verify(_lib.NQ_F32, (1 << 22) - 1) == verify(_lib.NQ_F16, (1 << 23) - 1) == _lib.NQ_ERR_WORKSPACE
+    three = 2 * 4096 + 1  # logits, which lie in up to three parts
+    assert verify(_lib.NQ_F32, (1 << 22) // 3 + 1, three) == verify(_lib.NQ_BF16, (1 << 23) // 3 + 1, three) == _lib.NQ_ERR_UNSUPPORTED
+    assert verify(_lib.NQ_F32, (1 << 22) // 3, three) == verify(_lib.NQ_BF16, (1 << 23) // 3, three) == _lib.NQ_ERR_WORKSPACE
