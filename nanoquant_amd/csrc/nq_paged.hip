@@ -141,7 +141,7 @@ constexpr int kLeastTiles = 8;     // the same of rows_kernel's
 // sequences' next tokens 66 against 63.5; two chunks of 700 tokens, heads of 64, 147 against 145.
 constexpr int kFewStart = 8, kStart = 4;
 constexpr float kSlack = 8.0f;
-constexpr int64_t kMaxGrid = 1 << 23;  // blocks of 256 threads: their count stays in 32 bits
+constexpr int64_t kMaxThreads = int64_t{1} << 31;  // of a launch, which counts them in 32 bits
 
 struct PagedArgs {
     const uint16_t* q;
@@ -1497,10 +1497,11 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
         const int64_t entries = p.few ? kFewEntries : kEntries;
         if (p.row_groups > entries) p.shared = false;  // a prompt this long fills the card
         p.batch = std::min({batch, std::max<int64_t>(1, entries / p.row_groups),
-                            std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads * p.rows_kept))});
+                            std::max<int64_t>(1, kMaxThreads / 256 / (p.row_groups * kv_heads * p.rows_kept))});
     }
     if (!p.shared) {
-        p.batch = std::min(batch, std::max<int64_t>(1, kMaxGrid / (p.row_groups * kv_heads)));
+        const int threads = p.few || p.tiles == 2 ? 256 : 512;
+        p.batch = std::min(batch, std::max<int64_t>(1, kMaxThreads / threads / (p.row_groups * kv_heads)));
         return p;
     }
     p.part_o = static_cast<size_t>(p.blocks) * 2 * p.rows_kept * head_dim * sizeof(float);
@@ -1615,7 +1616,7 @@ int nq_paged_rope_write(int dtype, const void* q, int64_t q_stride, const void* 
         return fail(NQ_ERR_SHAPE, "%s: token strides must hold the heads and be multiples of 8", name);
     if (batch == 0 || tokens == 0) return NQ_OK;
     const int64_t slots = (heads + 2 * kv_heads) * (head_dim / 16);
-    if (batch * tokens > kMaxGrid * 256 / slots) return fail(NQ_ERR_UNSUPPORTED, "%s: sizes too large", name);
+    if (batch * tokens > kMaxThreads / slots) return fail(NQ_ERR_UNSUPPORTED, "%s: sizes too large", name);
     if (int st = check_pages(name, k_pages, v_pages, pages, page_size, table, table_stride, table_pages, positions)) return st;
     for (const void* p : {q, k, v, rope_cos, rope_sin, static_cast<const void*>(q_out)}) {
         if (!p) return fail(NQ_ERR_INVALID_ARGUMENT, "%s: null pointer", name);

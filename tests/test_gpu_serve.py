@@ -294,6 +294,25 @@ def test_attention_past_32_bit_offsets():
     assert torch.equal(paged_attention(q, k, v, moved, pos), want)
 
 
+def test_attention_of_more_blocks_than_a_launch_takes():
+    """2^17 sequences of 17 tokens and 64 kv heads are 2^23 blocks of 512 threads, one launch's threads and one more."""
+    batch, tokens, heads, dim = 1 << 17, 17, 64, 64
+    print("\n[case] paged attention", batch, tokens, heads, dim, flush=True)
+    k, v = (torch.randn(3, heads, 32, dim, device="cuda").half() for _ in range(2))
+    table = (torch.arange(batch, device="cuda") % 3).int().view(batch, 1)
+    pos = torch.arange(tokens, device="cuda").expand(batch, tokens).contiguous()
+    some = torch.randn(3, tokens, heads * dim, device="cuda").half()
+    q = torch.empty(batch, tokens, heads * dim, dtype=torch.float16, device="cuda")
+    q.view(-1)[:3 * (batch // 3) * tokens * heads * dim].view(batch // 3, 3, -1).copy_(some.view(1, 3, -1))
+    q[3 * (batch // 3):] = some[:batch % 3]
+    y = paged_attention(q, k, v, table, pos)
+    ref, spread = oracle.attention(some, k, v, table[:3], pos[:3])
+    _check(y[:3], ref, spread, torch.float16, tokens)
+    whole = y[:3 * (batch // 3)].view(batch // 3, 3, -1)
+    assert all(bool((part == whole[:1]).all()) for part in whole.split(2048))
+    assert torch.equal(y[3 * (batch // 3):], y[:batch % 3])
+
+
 WRITE = [(4, 4, 128, 16, [1, 17], 1), (8, 2, 64, 48, [100, 3, 50], 7), (5, 5, 128, 16, [65], 64), (4, 1, 32, 8, [20, 9], 12),
          (6, 3, 16, 5, [23], 11)]
 
