@@ -157,7 +157,10 @@ def _rows(x, batch, tokens):
 
 
 def _table_rows(table):
-    return table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
+    """The table with rows a kernel can read: itself, or a copy (``contiguous`` keeps the stride of a dimension of one element)."""
+    if table.stride(0) >= table.shape[1] and (table.stride(1) == 1 or table.shape[1] == 1):
+        return table
+    return torch.empty(table.shape, dtype=table.dtype, device=table.device).copy_(table)
 
 
 def _pool_fits(k_pages, v_pages):

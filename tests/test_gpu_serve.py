@@ -275,6 +275,17 @@ def test_attention_takes_strided_queries_and_tables():
     _check(paged_attention(one, k, v, table, pos[:, 1:2]), ref, spread, torch.float16, 130)
 
 
+def test_one_sequence_takes_a_table_of_any_stride():
+    q, k, v, table, pos = oracle.paged_case(4, 2, 128, 16, [90], 3, torch.float16, "cuda")
+    close = table.view(-1, 1).t()
+    assert close.shape == table.shape and close.stride() == (1, 1)
+    assert torch.equal(paged_attention(q, k, v, close, pos), paged_attention(q, k, v, table, pos))
+    cos, sin = torch.randn(2, 1, 3, 128, device="cuda").unbind(0)
+    heads, pools = q[..., :256].contiguous(), [(k.clone(), v.clone()) for _ in range(2)]
+    out = [paged_rope_write(q, heads, heads, cos, sin, pos, *pool, t) for pool, t in zip(pools, (close, table))]
+    assert torch.equal(*out) and all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(*pools))
+
+
 def test_attention_of_nothing():
     q, k, v, table, pos = oracle.paged_case(4, 2, 128, 16, [20], 1, torch.float16, "cuda")
     assert paged_attention(q[:0], k, v, table[:0], pos[:0]).shape == (0, 1, 512)

@@ -41,6 +41,17 @@ def test_values_that_a_token_does_not_see_do_not_reach_it():
     assert y[0, 3].isnan().all()
 
 
+def test_rows_of_the_table_whatever_the_strides():
+    """A table of one sequence has any stride between its rows, and is not refused for it."""
+    from nanoquant_amd.serve import _table_rows
+    x = torch.arange(24, dtype=torch.int32).view(4, 6)
+    for t in (x, x[:, 1:3], x[1:2], x[:, 2:3], x[:, 3:4].t(), x[0, :, None].t(), x.t(), x[2].expand(5, 6), x[:, ::2],
+              torch.as_strided(x, (1, 6), (0, 1))):
+        rows = _table_rows(t)
+        assert rows.stride(0) >= t.shape[1] and (rows.stride(1) == 1 or t.shape[1] == 1) and torch.equal(rows, t)
+    assert _table_rows(x[:, 1:3]).data_ptr() == x[:, 1:3].data_ptr()  # read in place
+
+
 def test_write_against_the_definition():
     _, k_pages, v_pages, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 30, 3], 5, torch.float32, "cpu")
     g = torch.Generator().manual_seed(1)
