@@ -277,6 +277,8 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     k = k_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
     v = v_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
     qg = q.reshape(B, T, KV, H // KV, D).permute(0, 2, 3, 1, 4).float()  # [B, KV, G, T, D]
+    if not _only_eager(q, k_pages, v_pages, table, positions):  # 0 * NaN in the keys' gradients
+        qg = torch.where(seen.any(dim=-1, keepdim=True), qg, 0.0)
     scores = torch.matmul(qg, k.transpose(-1, -2).contiguous()) * scale
     scores = scores.masked_fill(~seen, -math.inf)
     top = scores.amax(dim=-1, keepdim=True)
@@ -288,7 +290,7 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     o = torch.where(up, math.inf, torch.where(down, -math.inf, o))
     o = torch.where(nan | (up & down), math.nan, o)
     total = e.sum(dim=-1, keepdim=True)
-    o = torch.where(total == 0.0, 0.0, o / total)
+    o = torch.where(total == 0.0, 0.0, o / torch.where(total == 0.0, 1.0, total))  # 0 / 0 would have NaN for a gradient
     return o.permute(0, 3, 1, 2, 4).reshape(B, T, H * D).to(q.dtype)
 
 

@@ -52,6 +52,78 @@ def test_rows_of_the_table_whatever_the_strides():
     assert _table_rows(x[:, 1:3]).data_ptr() == x[:, 1:3].data_ptr()  # read in place
 
 
+def _gradients(q, k_pages, v_pages, table, positions, w, window=0, sinks=0):
+    """Of sum w out by q and the pages, from the formula in float64, and how far float32 ones may be off.
+
+    A score is off by (D + 1) u times its summed |q k| scale at most (u = 2^-24), so a probability by a factor of 1 +- e with e
+    twice the largest of that, and 8 u for the exponential and the division. With a_j = |w| . |v_j| the gradient of score j,
+    p_j (w . v_j - sum_i p_i w . v_i), is off by e p_j (a_j + 2 sum_i p_i a_i), and those of q, k and v by what that makes of
+    their terms, and half as much again for the sums' own roundings."""
+    q, k_pages, v_pages, w = (t.double() for t in (q, k_pages, v_pages, w))
+    N, KV, S, D = k_pages.shape
+    dq, dk, dv = (torch.zeros(2, *t.shape, dtype=torch.float64) for t in (q, k_pages, v_pages))
+    for b in range(q.shape[0]):
+        page = table[b].long().repeat_interleave(S)
+        row = torch.arange(page.shape[0]) % S
+        for t in range(q.shape[1]):
+            seen = oracle.visible(int(positions[b, t]), page.shape[0], window, sinks) & (page >= 0) & (page < N)
+            if not seen.any():
+                continue
+            at = (page[seen], slice(None), row[seen])
+            k, v = k_pages[at].transpose(0, 1), v_pages[at].transpose(0, 1)  # [KV, keys, D]
+            qt, wt = (x[b, t].view(KV, -1, D) for x in (q, w))
+            p = torch.softmax(qt @ k.transpose(1, 2) * D ** -0.5, -1)
+            e = 1.5 * (2 * (D + 1) * 2.0 ** -24 * float((qt.abs() @ k.abs().transpose(1, 2)).max()) * D ** -0.5 + 8 * 2.0 ** -24)
+            for i, (dp, sign, s, kk, qq, ww) in enumerate((
+                    (wt @ v.transpose(1, 2), -1.0, 1.0, k, qt, wt),
+                    (wt.abs() @ v.abs().transpose(1, 2), 2.0, e, k.abs(), qt.abs(), wt.abs()))):
+                ds = s * p * (dp + sign * (p * dp).sum(-1, keepdim=True)) * D ** -0.5
+                dq[i, b, t] += (ds @ kk).reshape(-1)
+                dk[i][at] += (ds.transpose(1, 2) @ qq).transpose(0, 1)
+                dv[i][at] += (s * p.transpose(1, 2) @ ww).transpose(0, 1)
+    return dq, dk, dv
+
+
+def _leaves(*tensors):
+    return [t.clone().requires_grad_(True) for t in tensors]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (7, 2)])
+def test_gradients_of_tokens_that_all_see_something(window, sinks):
+    """No padding, whole pages: the torch ops' gradients against the formula's and, in one direction, against differences."""
+    q, k, v, table, pos = oracle.paged_case(4, 2, 32, 8, [16, 32], 5, torch.float32, "cpu", window=window, sinks=sinks, spare=0)
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
+    w = torch.randn(q.shape, generator=torch.Generator().manual_seed(11))
+    leaves = _leaves(q, k, v)
+    (paged_attention(*leaves, table, pos, window, sinks) * w).sum().backward()
+    along = 0.0
+    step = [torch.randn(x.shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64) for i, x in enumerate((q, k, v))]
+    for leaf, want, d in zip(leaves, _gradients(q, k, v, table, pos, w, window, sinks), step):
+        assert ((leaf.grad.double() - want[0]).abs() <= want[1]).all()
+        along += float((want[0] * d).sum())
+    h = 1e-4  # the third derivative's part of the quotient is h^2 / 6 times it, far below 1e-4 of the sum
+    ends = [(oracle.attention(*(x.double() + f * h * d for x, d in zip((q, k, v), step)), table, pos, window, sinks)[0] * w).sum()
+            for f in (1.0, -1.0)]
+    assert abs(float(ends[0] - ends[1]) / (2 * h) - along) < 1e-4 * (1 + abs(along))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (5, 2)])
+def test_gradients_beside_tokens_that_see_nothing(window, sinks):
+    """Padding, a sequence without pages and a position past the table have no gradient and leave the others theirs."""
+    q, k, v, table, pos = oracle.paged_case(4, 2, 32, 8, [16, 3, 32], 5, torch.float32, "cpu", window=window, sinks=sinks)
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
+    pos[0, 1] = table.shape[1] * 8
+    table[2, :] = -1
+    q[pos < 0] = math.nan
+    w = torch.randn(q.shape, generator=torch.Generator().manual_seed(12))
+    leaves = _leaves(q, k, v)
+    y = paged_attention(*leaves, table, pos, window, sinks)
+    (y * w).sum().backward()
+    assert (y[pos < 0] == 0).all() and (y[2] == 0).all()
+    for leaf, want in zip(leaves, _gradients(q, k, v, table, pos, w, window, sinks)):
+        assert ((leaf.grad.double() - want[0]).abs() <= want[1]).all()
+
+
 def test_write_against_the_definition():
     _, k_pages, v_pages, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 30, 3], 5, torch.float32, "cpu")
     g = torch.Generator().manual_seed(1)
