@@ -277,9 +277,16 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     k = k_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
     v = v_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
     qg = q.reshape(B, T, KV, H // KV, D).permute(0, 2, 3, 1, 4).float()  # [B, KV, G, T, D]
-    if not _only_eager(q, k_pages, v_pages, table, positions):  # 0 * NaN in the keys' gradients
+    if _only_eager(q, k_pages, v_pages, table, positions):
+        scores = torch.matmul(qg, k.transpose(-1, -2).contiguous()) * scale
+    else:
+        # 0 * NaN again, in the gradients: queries of tokens that see nothing are none, and the products that are
+        # differentiated take the finite keys; scores of the others are constants, for the tokens that see them
         qg = torch.where(seen.any(dim=-1, keepdim=True), qg, 0.0)
-    scores = torch.matmul(qg, k.transpose(-1, -2).contiguous()) * scale
+        finite = torch.isfinite(k)
+        scores = torch.matmul(qg, torch.where(finite, k, 0.0).transpose(-1, -2).contiguous()) * scale
+        other = torch.matmul(qg.detach(), k.detach().transpose(-1, -2).contiguous()) * scale
+        scores = torch.where(finite.all(dim=-1).unsqueeze(-2), scores, other)
     scores = scores.masked_fill(~seen, -math.inf)
     top = scores.amax(dim=-1, keepdim=True)
     e = torch.exp(scores - torch.where(top == -math.inf, 0.0, top))

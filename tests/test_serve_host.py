@@ -124,6 +124,26 @@ def test_gradients_beside_tokens_that_see_nothing(window, sinks):
         assert ((leaf.grad.double() - want[0]).abs() <= want[1]).all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_beside_keys_that_are_not_finite(bad):
+    """Rows of the pages that hold nothing yet, or keys of later tokens, have no part in a token's gradient."""
+    q, k, v, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 21], 3, torch.float32, "cpu")
+    k, v = torch.where(k.isnan(), bad, k), torch.where(v.isnan(), bad, v)
+    w = torch.randn(q.shape, generator=torch.Generator().manual_seed(13))
+    want = _gradients(q, k, v, table, pos, w)
+    leaves = _leaves(q, k, v)
+    (paged_attention(*leaves, table, pos) * w).sum().backward()
+    for leaf, (grad, bound) in zip(leaves, want):
+        assert ((leaf.grad.double() - grad).abs() <= bound).all()
+    k[int(table[1, 2]), :, 4, 3] = math.nan  # position 20 of sequence 1, which its last token alone sees
+    leaves = _leaves(q, k, v)
+    y = paged_attention(*leaves, table, pos)
+    (y * w).sum().backward()
+    assert y[1, 2].isnan().all()
+    early = torch.tensor([[True, True, True], [True, True, False]])
+    assert ((leaves[0].grad.double() - want[0][0])[early].abs() <= want[0][1][early]).all()
+
+
 def test_write_against_the_definition():
     _, k_pages, v_pages, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 30, 3], 5, torch.float32, "cpu")
     g = torch.Generator().manual_seed(1)
