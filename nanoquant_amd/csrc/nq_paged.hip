@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteArgs a) {
 constexpr int kTile = 32;          // keys a wave of few_kernel takes at a time
 constexpr int kWaves = 4;          // of a block
 constexpr int kCUs = 256;
-// (sequence, row group) pairs of a launch, whose key counts every block adds up: two blocks of either kernel fit a CU's LDS
+// (sequence, row group) pairs of a launch, whose key counts every block adds up in LDS: 8 KB, with which two blocks still fit a
+// CU where its rings let them (FewShape; rows_kernel of 64 dimensions)
 constexpr int kFewEntries = 512, kEntries = 1024;
 constexpr int kLeastShare = 4;     // tiles a block of few_kernel takes at least: one a wave
 constexpr int kLeastTiles = 8;     // the same of rows_kernel's
@@ -724,7 +725,7 @@ __device__ inline Parts parts_of(const PagedArgs& a, int seg) {
 
 // Adds what the blocks left of one row of an (entry, kv head), for few rows of which many blocks may hold a part: the threads
 // in groups of D / 4, a group every Groups-th part. Bound by latency: where the parts lie, then the parts, then their sums;
-// 3.3 us for one token of 32 kv heads in eight parts each, 5.0 for 40 rows of 72 (sequence, kv head) pairs.
+// 3.3 to 3.9 us for one token of 32 kv heads in eight parts each, 5.0 for 40 rows of 72 (sequence, kv head) pairs.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_join_kernel(const PagedArgs a, int group) {
     constexpr int L4 = D / 4, Groups = 256 / L4, kAhead = 4;

@@ -398,7 +398,7 @@ struct Part {
     }
 };
 
-// Bound by latency too, of the statistics, of the tests, then of the part: 10 us for 64 sequences of 25 parts.
+// Bound by latency too, of the statistics, of the tests, then of the part: 12 us for 64 sequences of 25 parts.
 template <typename T, bool kTests>
 __global__ __launch_bounds__(Part<T>::kThreads) void part_sums_kernel(const VerifyArgs a) {
     constexpr int kWaves = Part<T>::kThreads / 64;
