@@ -13,8 +13,9 @@ is bound by its host path. What that does not take is checked, copied into place
 
 float16 and bfloat16 tensors on the GPU run the HIP library (``nq_paged_rope_write``, ``nq_paged_attention``,
 ``nq_verify_drafts``); CPU tensors, float32 models, head sizes other than 64 and 128 and page sizes that are no multiple of 16
-run torch ops with the same results but for rounding. The reference has no counterpart: its harness decodes one batch on
-Hugging Face's static cache and samples one token a step (``src/nanoquant/kernel/test_decode.py:350-422``).
+run torch ops with the same results but for rounding, in float32, or in float64 where the tensors are. The reference has no
+counterpart: its harness decodes one batch on Hugging Face's static cache and samples one token a step
+(``src/nanoquant/kernel/test_decode.py:350-422``).
 """
 from __future__ import annotations
 
@@ -209,10 +210,11 @@ def paged_rope_write(q, k, v, cos, sin, positions, k_pages, v_pages, table):
                 table.data_ptr(), table.stride(0), table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(), N, S, out.data_ptr(),
                 B, T, q.shape[2] // D, KV, D)
         return out
-    cos, sin = cos.reshape(B, T, 1, D).float(), sin.reshape(B, T, 1, D).float()
+    wide = torch.promote_types(q.dtype, torch.float32)
+    cos, sin = cos.reshape(B, T, 1, D).to(wide), sin.reshape(B, T, 1, D).to(wide)
 
     def rotate(x):
-        x = x.reshape(B, T, -1, D).float()
+        x = x.reshape(B, T, -1, D).to(wide)
         return (x * cos + torch.cat((-x[..., D // 2:], x[..., :D // 2]), dim=-1) * sin).to(q.dtype)
 
     real = (positions >= 0) & (positions < table.shape[1] * S)
@@ -264,6 +266,7 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
                 v_pages.data_ptr(), N, S, table.data_ptr(), table.stride(0), table.shape[1], positions.data_ptr(),
                 out.data_ptr(), B, T, H, KV, D, window, sinks, scale, _lib.ptr(ws), nbytes)
         return out
+    wide = torch.promote_types(q.dtype, torch.float32)
     P = table.shape[1]
     page = table.long()
     there = (page >= 0) & (page < N)
@@ -274,9 +277,9 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     if window:
         seen = seen & ((key > p - window) | (key < sinks))
     seen = seen.view(B, 1, 1, T, P * S)
-    k = k_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
-    v = v_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).float()
-    qg = q.reshape(B, T, KV, H // KV, D).permute(0, 2, 3, 1, 4).float()  # [B, KV, G, T, D]
+    k = k_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).to(wide)
+    v = v_pages[page].transpose(1, 2).reshape(B, KV, 1, P * S, D).to(wide)
+    qg = q.reshape(B, T, KV, H // KV, D).permute(0, 2, 3, 1, 4).to(wide)  # [B, KV, G, T, D]
     if _only_eager(q, k_pages, v_pages, table, positions):
         scores = torch.matmul(qg, k.transpose(-1, -2).contiguous()) * scale
     else:

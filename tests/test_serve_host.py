@@ -144,6 +144,22 @@ def test_gradients_beside_keys_that_are_not_finite(bad):
     assert ((leaves[0].grad.double() - want[0][0])[early].abs() <= want[0][1][early]).all()
 
 
+def test_float64_stays_float64():
+    """Results and gradients: differences of float64 results need them."""
+    q, k, v, table, pos = oracle.paged_case(2, 1, 8, 4, [3, 7], 3, torch.float64, "cpu", window=4, sinks=1)
+    ref, _ = oracle.attention(q, k, v, table, pos, 4, 1)
+    assert (paged_attention(q, k, v, table, pos, 4, 1) - ref).abs().max() < 1e-13
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
+    pos[0, 2] = -1
+    assert torch.autograd.gradcheck(lambda *x: paged_attention(*x, table, pos, 4, 1), _leaves(q, k, v))
+    g = torch.Generator().manual_seed(17)
+    q, heads = torch.randn(2, 3, 16, generator=g).double(), torch.randn(2, 3, 8, generator=g).double()
+    cos, sin = torch.randn(2, 2, 3, 8, generator=g).double().unbind(0)
+    want = oracle.write(q, heads, heads, cos, sin, pos, k, v, table)
+    out = paged_rope_write(q, heads, heads, cos, sin, pos, k, v, table)
+    assert all((a - b).abs().max() < 1e-13 for a, b in zip((out, k, v), want))
+
+
 def test_write_against_the_definition():
     _, k_pages, v_pages, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 30, 3], 5, torch.float32, "cpu")
     g = torch.Generator().manual_seed(1)
