@@ -266,6 +266,9 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
                 v_pages.data_ptr(), N, S, table.data_ptr(), table.stride(0), table.shape[1], positions.data_ptr(),
                 out.data_ptr(), B, T, H, KV, D, window, sinks, scale, _lib.ptr(ws), nbytes)
         return out
+    if q.device.type in ("cpu", "cuda") and torch.is_autocast_enabled(q.device.type):  # which would round the products' operands
+        with torch.autocast(q.device.type, enabled=False):
+            return paged_attention(q, k_pages, v_pages, table, positions, window, sinks, scale)
     wide = torch.promote_types(q.dtype, torch.float32)
     P = table.shape[1]
     page = table.long()

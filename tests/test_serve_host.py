@@ -160,6 +160,18 @@ def test_float64_stays_float64():
     assert all((a - b).abs().max() < 1e-13 for a, b in zip((out, k, v), want))
 
 
+def test_torch_ops_keep_their_precision_under_autocast():
+    q, k, v, table, pos = oracle.paged_case(4, 2, 32, 8, [17, 30], 3, torch.float32, "cpu")
+    leaves = _leaves(q, k, v)
+    want = paged_attention(*leaves, table, pos)
+    want.sum().backward()
+    again = _leaves(q, k, v)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = paged_attention(*again, table, pos)
+    got.sum().backward()
+    assert torch.equal(got, want) and all(torch.equal(a.grad, b.grad) for a, b in zip(again, leaves))
+
+
 def test_write_against_the_definition():
     _, k_pages, v_pages, table, pos = oracle.paged_case(4, 2, 32, 8, [9, 30, 3], 5, torch.float32, "cpu")
     g = torch.Generator().manual_seed(1)
