@@ -60,7 +60,8 @@ class PagedKVCache:
     positions and the first ``sinks``.
 
     ``reserve`` gives a sequence the pages that its next tokens need, ``trim`` takes back those that no later token will see,
-    ``release`` all of them. A program may also fill the table itself.
+    ``release`` all of them. A program may also fill the table itself, and then uses none of these: they write a sequence's row
+    as they know it. Serve under ``torch.no_grad``, or what a model with gradients writes makes the pools part of its graph.
     """
 
     def __init__(self, shape, batch: int, pages: int, page_size: int, max_len: int, device, dtype, window: int = 0,
