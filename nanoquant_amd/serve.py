@@ -12,10 +12,10 @@ Calls of well-laid-out tensors on the GPU go through the C++ of ``libnq_ops.so``
 is bound by its host path. What that does not take is checked, copied into place or refused here.
 
 float16 and bfloat16 tensors on the GPU run the HIP library (``nq_paged_rope_write``, ``nq_paged_attention``,
-``nq_verify_drafts``); CPU tensors, float32 models, head sizes other than 64 and 128 and page sizes that are no multiple of 16
-run torch ops with the same results but for rounding, in float32, or in float64 where the tensors are. The reference has no
-counterpart: its harness decodes one batch on Hugging Face's static cache and samples one token a step
-(``src/nanoquant/kernel/test_decode.py:350-422``).
+``nq_verify_drafts``); CPU tensors, float32 models, calls that are differentiated, head sizes other than 64 and 128 and page
+sizes that are no multiple of 16 run torch ops with the same results but for rounding, in float32, or in float64 where the
+tensors are. The reference has no counterpart: its harness decodes one batch on Hugging Face's static cache and samples one
+token a step (``src/nanoquant/kernel/test_decode.py:350-422``).
 """
 from __future__ import annotations
 
