@@ -406,6 +406,38 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
                        int64_t head_dim, int64_t window, int64_t sinks, float scaling, void* workspace,
                        size_t workspace_bytes, nq_stream_t stream);
 
+/* nq_paged_attention for sequences of which groups have their leading pages in common (answers to one prompt): those keys and
+ * values are read once a group, and take part in one product with the queries of all its members.
+ *   members   device int32 [groups, most], contiguous: the sequences of each group in any order; entries outside [0, batch) are
+ *             nobody. A sequence in no group is on its own; of one that is named twice the last place counts.
+ *   shared    device int32 [groups]: the first shared[g] entries of the table are the same in the rows of group g's members
+ *             (none where it is not positive, all where it is more). Where they are not, the results of those sequences mean
+ *             nothing; no memory outside the pool is read.
+ * Everything else, the result but for rounding too, is as for nq_paged_attention.
+ *   workspace nq_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one
+ *             must not overlap.
+ * Past what nq_paged_attention takes, NQ_ERR_UNSUPPORTED where one launch cannot list the work: see the workspace function,
+ * which returns 0 for such a call. Call nq_paged_attention then. */
+size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t groups, int64_t most);
+int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                              int64_t pages, int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_pages,
+                              const int64_t* positions, const int32_t* members, const int32_t* shared, int64_t groups,
+                              int64_t most, void* out, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, int64_t window, int64_t sinks, float scaling, void* workspace,
+                              size_t workspace_bytes, nq_stream_t stream);
+
+/* Pages copied within each of `count` pools (the keys' and the values' of every layer, say): page target[i] becomes page
+ * source[i] for i < moves, whatever the pages hold.
+ *   pools     host array of `count` device addresses, read before the function returns; each pool holds `pages` pages of
+ *             page_bytes bytes, one after the other
+ *   source, target  device int32 [moves]; a pair with a page outside [0, pages) is passed over
+ * No page may be the target of two pairs, or the target of one and the source of another (what such pages hold then is open).
+ * One launch for 256 pools and 2^31 threads' worth of pages. Addresses and page_bytes that are multiples of 16 move 16 bytes a
+ * lane, others one. */
+int nq_copy_pages(void* const* pools, int64_t count, int64_t pages, int64_t page_bytes, const int32_t* source,
+                  const int32_t* target, int64_t moves, nq_stream_t stream);
+
 /* ---------------------------------------------------------------- drafted tokens */
 
 /* Verification of drafted tokens against the model's distributions, from given random numbers, so that the tokens that come
@@ -433,6 +465,28 @@ size_t nq_verify_drafts_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
 int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const int64_t* draft, const float* draft_probs,
                      const float* uniforms, double temperature, int64_t* accepted, int64_t* tokens, int64_t batch,
                      int64_t drafts, int64_t vocab, void* workspace, size_t workspace_bytes, nq_stream_t stream);
+
+/* ---------------------------------------------------------------- scored tokens */
+
+/* What the model's distributions p = softmax(logits / temperature) say of given tokens, for batch x rows rows of logits:
+ *   logits    dtype (NQ_F16, NQ_BF16 or NQ_F32): row r of sequence b, `vocab` values, begins b * batch_stride + r * row_stride
+ *             elements from here
+ *   tokens    device int64, that of row (b, r) at b * token_batch_stride + r * token_stride
+ *   logprobs  float [batch, rows] = log p[token]; 0 for a token outside [0, vocab) (-1 for padding)
+ *   entropy   float [batch, rows] = - sum p log p, where a p of 0 (a logit of -inf) adds nothing
+ *   top_tokens, top_logprobs  int64 and float [batch, rows, top]: the indexes of the `top` largest logits, the lowest first of
+ *             equal ones, and their log p. Not touched where top is 0.
+ * In a row with a NaN, or whose largest logit is infinite, log p and the entropy are NaN and NaNs are the largest logits.
+ * Exponentials and sums in fp32. Every logit is read once where none is NaN.
+ *   workspace nq_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
+ *             not overlap.
+ * vocab <= 2^30, top <= 64 and <= vocab, fewer than 2^23 rows, temperature from 2^-64 to 2^64, else NQ_ERR_UNSUPPORTED. Tensors
+ * aligned to their elements. The reference has no kernel of this kind. */
+size_t nq_token_logprobs_workspace_bytes(int64_t batch, int64_t rows, int64_t vocab, int64_t top);
+int nq_token_logprobs(int dtype, const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens,
+                      int64_t token_batch_stride, int64_t token_stride, double temperature, int64_t top, float* logprobs,
+                      float* entropy, int64_t* top_tokens, float* top_logprobs, int64_t batch, int64_t rows, int64_t vocab,
+                      void* workspace, size_t workspace_bytes, nq_stream_t stream);
 
 /* ---------------------------------------------------------------- norm and activation of many tokens */
 

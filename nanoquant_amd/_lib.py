@@ -96,6 +96,13 @@ SIGNATURES = {
                                   _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
     "nq_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "nq_verify_drafts": (_int, [_int, _vp, _i64, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
+    "nq_paged_shared_attention_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "nq_paged_shared_attention": (_int, [_int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
+                                         _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
+    "nq_copy_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "nq_token_logprobs_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
+    "nq_token_logprobs": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, ctypes.c_double, _i64, _vp, _vp, _vp, _vp, _i64, _i64,
+                                 _i64, _vp, _size, _vp]),
     "nq_rms_norm": (_int, [_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp]),
     "nq_silu_mul": (_int, [_int, _vp, _vp, _vp, _i64, _vp]),
     "nq_dense_gemv": (_int, [_int, _vp, _vp, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
@@ -120,7 +127,8 @@ SIGNATURES = {
 OPS_FUNCTIONS = ("nq_gemv_workspace_bytes", "nq_gemv", "nq_gemm_onebit_workspace_bytes", "nq_gemm_onebit",
                  "nq_gemm_nanoquant_workspace_bytes", "nq_gemm_nanoquant", "nq_paged_rope_write",
                  "nq_paged_attention_workspace_bytes", "nq_paged_attention", "nq_verify_drafts_workspace_bytes",
-                 "nq_verify_drafts")
+                 "nq_verify_drafts", "nq_paged_shared_attention_workspace_bytes", "nq_paged_shared_attention", "nq_copy_pages",
+                 "nq_token_logprobs_workspace_bytes", "nq_token_logprobs")
 
 _lock = threading.Lock()
 _lib = None

@@ -37,8 +37,13 @@ struct Library {
     decltype(&nq_paged_attention) paged_attention;
     decltype(&nq_verify_drafts_workspace_bytes) verify_bytes;
     decltype(&nq_verify_drafts) verify;
+    decltype(&nq_paged_shared_attention_workspace_bytes) shared_attention_bytes;
+    decltype(&nq_paged_shared_attention) shared_attention;
+    decltype(&nq_copy_pages) copy_pages;
+    decltype(&nq_token_logprobs_workspace_bytes) logprobs_bytes;
+    decltype(&nq_token_logprobs) logprobs;
 };
-constexpr int kFunctions = 11;
+constexpr int kFunctions = 16;
 std::atomic<const Library*> g_library{nullptr};
 
 int dtype_code(at::ScalarType t) { return t == at::kHalf ? NQ_F16 : NQ_BF16; }
@@ -235,6 +240,85 @@ OptTensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& 
     return out;
 }
 
+OptTensor shared_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                           const Tensor& positions, const Tensor& members, const Tensor& shared, int64_t window, int64_t sinks,
+                           std::optional<double> scale) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    if (!pages_ok(lib, q, k_pages, v_pages, table, positions)) return std::nullopt;
+    const int64_t B = q.size(0), T = q.size(1), KV = k_pages.size(1), S = k_pages.size(2), D = k_pages.size(3), H = q.size(2) / D;
+    const int64_t qs = row_stride(q, B, T);
+    if ((D != 64 && D != 128) || S % 16 || qs == 0 || window < 0 || sinks < 0 || members.dim() != 2 || shared.dim() != 1 ||
+        members.numel() == 0 || members.size(0) != shared.size(0) || !plain(members, q, at::kInt) || !plain(shared, q, at::kInt))
+        return std::nullopt;
+    const int64_t groups = members.size(0), most = members.size(1);
+    const size_t bytes = lib->shared_attention_bytes(B, T, H, KV, D, groups, most);
+    if (bytes == 0) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty(q.sizes(), q.options());
+    const Tensor ws = scratch(bytes, q);
+    const float factor = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D)));
+    if (lib->shared_attention(dtype_code(q.scalar_type()), q.const_data_ptr(), qs, k_pages.const_data_ptr(),
+                              v_pages.const_data_ptr(), k_pages.size(0), S, static_cast<const int32_t*>(table.const_data_ptr()),
+                              table.stride(0), table.size(1), static_cast<const int64_t*>(positions.const_data_ptr()),
+                              static_cast<const int32_t*>(members.const_data_ptr()),
+                              static_cast<const int32_t*>(shared.const_data_ptr()), groups, most, out.mutable_data_ptr(), B, T, H,
+                              KV, D, window, sinks, factor, ws.mutable_data_ptr(), bytes, stream_of(q)) != NQ_OK)
+        return std::nullopt;
+    return out;
+}
+
+bool copy_pages(const std::vector<Tensor>& pools, const Tensor& source, const Tensor& target) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    if (!lib || pools.empty() || !source.is_cuda() || source.dim() != 1 || source.numel() == 0 || target.sizes() != source.sizes() ||
+        !plain(source, source, at::kInt) || !plain(target, source, at::kInt))
+        return false;
+    const Tensor& first = pools[0];
+    std::vector<void*> at;
+    at.reserve(pools.size());
+    for (const Tensor& pool : pools) {
+        if (!plain(pool, source, first.scalar_type()) || pool.dim() < 1 || pool.numel() == 0 || pool.sizes() != first.sizes())
+            return false;
+        at.push_back(pool.mutable_data_ptr());
+    }
+    const c10::DeviceGuard guard(source.device());
+    const int64_t pages = first.size(0), bytes = first.numel() / pages * static_cast<int64_t>(first.element_size());
+    return lib->copy_pages(at.data(), static_cast<int64_t>(at.size()), pages, bytes,
+                           static_cast<const int32_t*>(source.const_data_ptr()),
+                           static_cast<const int32_t*>(target.const_data_ptr()), source.numel(), stream_of(source)) == NQ_OK;
+}
+
+// {logprobs, entropy, top_tokens, top_logprobs}, or an empty list.
+std::vector<Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature) {
+    const Library* lib = g_library.load(std::memory_order_acquire);
+    const auto type = logits.scalar_type();
+    const int64_t dims = logits.dim() - 1;
+    if (!lib || !logits.is_cuda() || (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) || dims < 1 || dims > 2 ||
+        logits.numel() == 0 || tokens.dim() != dims || tokens.scalar_type() != at::kLong || tokens.device() != logits.device())
+        return {};
+    const int64_t V = logits.size(dims), R = logits.size(dims - 1), B = dims == 2 ? logits.size(0) : 1;
+    const int64_t row = logits.stride(dims - 1), batch = dims == 2 ? logits.stride(0) : 0;
+    if (tokens.sizes() != logits.sizes().slice(0, dims) || (V > 1 && logits.stride(dims) != 1) || (R > 1 && row < V) ||
+        (B > 1 && batch < V) || top < 0 || top > V)
+        return {};
+    const size_t bytes = lib->logprobs_bytes(B, R, V, top);
+    if (bytes == 0) return {};
+    const c10::DeviceGuard guard(logits.device());
+    const auto shape = tokens.sizes();
+    std::vector<int64_t> wide = shape.vec();
+    wide.push_back(top);
+    Tensor logprobs = at::empty(shape, logits.options().dtype(at::kFloat)), entropy = at::empty_like(logprobs);
+    Tensor top_tokens = at::empty(wide, tokens.options()), top_logprobs = at::empty(wide, logprobs.options());
+    const Tensor ws = scratch(bytes, logits);
+    if (lib->logprobs(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), batch, row,
+                      static_cast<const int64_t*>(tokens.const_data_ptr()), dims == 2 ? tokens.stride(0) : 0,
+                      tokens.stride(dims - 1), temperature, top, static_cast<float*>(logprobs.mutable_data_ptr()),
+                      static_cast<float*>(entropy.mutable_data_ptr()), static_cast<int64_t*>(top_tokens.mutable_data_ptr()),
+                      static_cast<float*>(top_logprobs.mutable_data_ptr()), B, R, V, ws.mutable_data_ptr(), bytes,
+                      stream_of(logits)) != NQ_OK)
+        return {};
+    return {logprobs, entropy, top_tokens, top_logprobs};
+}
+
 // {accepted, tokens}, or an empty list.
 std::vector<Tensor> verify(const Tensor& logits, const Tensor& drafts, const Tensor& uniforms, const OptTensor& draft_probs,
                            double temperature) {
@@ -284,6 +368,11 @@ extern "C" int nq_ops_bind(void* const* functions, int count) {
     library.paged_attention = reinterpret_cast<decltype(library.paged_attention)>(functions[8]);
     library.verify_bytes = reinterpret_cast<decltype(library.verify_bytes)>(functions[9]);
     library.verify = reinterpret_cast<decltype(library.verify)>(functions[10]);
+    library.shared_attention_bytes = reinterpret_cast<decltype(library.shared_attention_bytes)>(functions[11]);
+    library.shared_attention = reinterpret_cast<decltype(library.shared_attention)>(functions[12]);
+    library.copy_pages = reinterpret_cast<decltype(library.copy_pages)>(functions[13]);
+    library.logprobs_bytes = reinterpret_cast<decltype(library.logprobs_bytes)>(functions[14]);
+    library.logprobs = reinterpret_cast<decltype(library.logprobs)>(functions[15]);
     g_library.store(&library, std::memory_order_release);
     return 0;
 }
@@ -301,4 +390,7 @@ TORCH_LIBRARY_IMPL(nanoquant_amd, CUDA, m) {
     m.impl("paged_rope_write", &paged_write);
     m.impl("paged_attention", &paged_attention);
     m.impl("verify_drafts", &verify);
+    m.impl("paged_shared_attention", &shared_attention);
+    m.impl("copy_pages", &copy_pages);
+    m.impl("token_logprobs", &token_logprobs);
 }

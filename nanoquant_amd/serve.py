@@ -1,24 +1,30 @@
 """What serving many sequences at once needs beyond one static cache: a KV cache in pages, each sequence at a length of its
-own, and the check of drafted tokens.
+own, several answers to one prompt, the check of drafted tokens and the scores of given ones.
 
 * :class:`PagedKVCache` holds the pools and the page table; ``NanoQuantLlama.forward`` takes it in place of a
   ``StaticKVCache``, with positions [B, T].
 * :func:`paged_rope_write` rotates the new tokens' queries and keys and writes keys and values into the pages.
 * :func:`paged_attention` is causal attention over the pages, for one new token a sequence, drafted tokens, prompts and
   chunks of prompts, optionally under a sliding window with a few first tokens that stay visible.
+* :func:`paged_shared_attention` is the same for sequences of which groups have their leading pages in common, which
+  :meth:`PagedKVCache.fork` makes; those keys and values are read once a group.
+* :func:`copy_pages` copies pages within the pools of every layer.
 * :func:`verify_drafts` keeps or turns down drafted tokens by the model's logits and given random numbers.
+* :func:`token_logprobs` gives the log probabilities of given tokens, the entropy and the most probable alternatives.
 
 Calls of well-laid-out tensors on the GPU go through the C++ of ``libnq_ops.so`` (``csrc/torch_ops/nq_ops.cpp``): a small call
 is bound by its host path. What that does not take is checked, copied into place or refused here.
 
 float16 and bfloat16 tensors on the GPU run the HIP library (``nq_paged_rope_write``, ``nq_paged_attention``,
-``nq_verify_drafts``); CPU tensors, float32 models, calls that are differentiated, head sizes other than 64 and 128 and page
-sizes that are no multiple of 16 run torch ops with the same results but for rounding, in float32, or in float64 where the
-tensors are. The reference has no counterpart: its harness decodes one batch on Hugging Face's static cache and samples one
+``nq_verify_drafts``, ``nq_paged_shared_attention``, ``nq_copy_pages``, ``nq_token_logprobs``); CPU tensors, float32 models,
+calls that are differentiated, head sizes other than 64 and 128 and page sizes that are no multiple of 16 run torch ops with the
+same results but for rounding, in float32, or in float64 where the tensors are. Pages of any type are copied by the library,
+and logits in float32 scored and verified by it. The reference has no counterpart: its harness decodes one batch on Hugging Face's static cache and samples one
 token a step (``src/nanoquant/kernel/test_decode.py:350-422``).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import sys
 
@@ -35,7 +41,11 @@ for _schema in (
         "Tensor(b!) v_pages, Tensor table) -> Tensor?",
         "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor positions, int window, int sinks, "
         "float? scale) -> Tensor?",
-        "verify_drafts(Tensor logits, Tensor drafts, Tensor uniforms, Tensor? draft_probs, float temperature) -> Tensor[]"):
+        "verify_drafts(Tensor logits, Tensor drafts, Tensor uniforms, Tensor? draft_probs, float temperature) -> Tensor[]",
+        "paged_shared_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor positions, Tensor members, "
+        "Tensor shared, int window, int sinks, float? scale) -> Tensor?",
+        "copy_pages(Tensor(a!)[] pools, Tensor source, Tensor target) -> bool",
+        "token_logprobs(Tensor logits, Tensor tokens, int top, float temperature) -> Tensor[]"):
     _OPS.define(_schema)
 
 
@@ -47,6 +57,7 @@ def _native(name):
 
 
 _native_write, _native_attention, _native_verify = (_native(n) for n in ("paged_rope_write", "paged_attention", "verify_drafts"))
+_native_shared, _native_copy, _native_score = (_native(n) for n in ("paged_shared_attention", "copy_pages", "token_logprobs"))
 
 
 class PagedKVCache:
@@ -60,8 +71,15 @@ class PagedKVCache:
     positions and the first ``sinks``.
 
     ``reserve`` gives a sequence the pages that its next tokens need, ``trim`` takes back those that no later token will see,
-    ``release`` all of them. A program may also fill the table itself, and then uses none of these: they write a sequence's row
-    as they know it. Serve under ``torch.no_grad``, or what a model with gradients writes makes the pools part of its graph.
+    ``release`` all of them. ``fork`` lets sequences go on where another stands: they share its whole pages, which are counted
+    and go back to the pool with the last that has them, and ``own`` gives a sequence copies of shared pages before something is
+    written there. ``compact`` moves the pages that are in use to the front of the pools. A program may also fill the table
+    itself, and then uses none of these: they write a sequence's row as they know it. Serve under ``torch.no_grad``, or what a
+    model with gradients writes makes the pools part of its graph.
+
+    ``members`` and ``shared`` (None before the first fork) say which sequences have their leading pages in common, as
+    :func:`paged_shared_attention` takes it, and ``groups`` how many such groups there are. Their memory stays as long as no
+    more groups and no larger ones come up than ever before, so a graph captured with the largest follows their changes.
     """
 
     def __init__(self, shape, batch: int, pages: int, page_size: int, max_len: int, device, dtype, window: int = 0,
@@ -79,6 +97,9 @@ class PagedKVCache:
         self.table = torch.full((batch, self.max_pages), -1, device=device, dtype=torch.int32)
         self._host = [[-1] * self.max_pages for _ in range(batch)]  # the table as the methods below left it
         self._free = list(range(pages - 1, -1, -1))
+        self._owners = [0] * pages  # sequences that have a page
+        self.members = self.shared = None
+        self.groups = 0
 
     def _row(self, sequence: int):
         if not 0 <= sequence < self.batch:
@@ -87,6 +108,51 @@ class PagedKVCache:
 
     def _store(self, sequence: int):
         self.table[sequence].copy_(torch.tensor(self._host[sequence], dtype=torch.int32))
+
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._owners[page] = 1
+        return page
+
+    def _drop(self, page: int) -> None:
+        self._owners[page] -= 1
+        if self._owners[page] == 0:
+            self._free.append(page)
+
+    def _copy(self, moves) -> None:
+        source, target = torch.tensor(moves, dtype=torch.int32).t().contiguous().to(self.table.device).unbind(0)
+        copy_pages([*self.k, *self.v], source, target)
+
+    def _regroup(self) -> None:
+        """``members`` and ``shared`` of the sequences whose first page is the same: what all of their rows begin with."""
+        if self.members is None and max(self._owners) < 2:
+            return
+        alike = {}
+        for b, row in enumerate(self._host):
+            first = next(((i, page) for i, page in enumerate(row) if page >= 0), None)
+            if first is not None and self._owners[first[1]] > 1:
+                alike.setdefault(first, []).append(b)
+        lists, shared = [], []
+        for sequences in alike.values():
+            rows = [self._host[b] for b in sequences]
+            low, high = min(rows), max(rows)  # what these two begin with all begin with
+            common = next((i for i, (x, y) in enumerate(zip(low, high)) if x != y), self.max_pages)
+            while common and low[common - 1] < 0:
+                common -= 1
+            if len(sequences) > 1 and common:
+                lists.append(sequences)
+                shared.append(common)
+        self.groups = len(lists)
+        most = max(map(len, lists), default=0)
+        if self.members is None or self.members.shape[0] < len(lists) or self.members.shape[1] < most:
+            old = (0, 0) if self.members is None else self.members.shape
+            shape = (max(old[0], len(lists)), max(old[1], most))
+            self.members = torch.empty(shape, dtype=torch.int32, device=self.table.device)
+            self.shared = torch.empty(shape[0], dtype=torch.int32, device=self.table.device)
+        groups, most = self.members.shape
+        lists += [[]] * (groups - len(lists))
+        self.members.copy_(torch.tensor([x + [-1] * (most - len(x)) for x in lists], dtype=torch.int32).view(groups, most))
+        self.shared.copy_(torch.tensor(shared + [0] * (groups - len(shared)), dtype=torch.int32))
 
     def reserve(self, sequence: int, length: int, start: int = 0) -> None:
         """Pages for the sequence's positions ``start`` to ``length - 1`` (those it has stay). RuntimeError, and no change,
@@ -98,18 +164,20 @@ class PagedKVCache:
         if len(need) > len(self._free):
             raise RuntimeError(f"the paged cache has {len(self._free)} pages left, sequence {sequence} needs {len(need)}")
         for i in need:
-            row[i] = self._free.pop()
+            row[i] = self._take()
         if need:
             self._store(sequence)
+            self._regroup()
 
     def _take_back(self, sequence: int, slots) -> int:
         row = self._row(sequence)
         gone = [i for i in slots if row[i] >= 0]
         for i in gone:
-            self._free.append(row[i])
+            self._drop(row[i])
             row[i] = -1
         if gone:
             self._store(sequence)
+            self._regroup()
         return len(gone)
 
     def trim(self, sequence: int, position: int) -> int:
@@ -121,8 +189,75 @@ class PagedKVCache:
         return self._take_back(sequence, range(-(-self.sinks // self.page_size), first))
 
     def release(self, sequence: int) -> int:
-        """Take back all pages of a sequence; returns their number. Calls in flight on other streams must have ended."""
+        """Take back all pages of a sequence (those that others share stay theirs); returns their number. Calls in flight on
+        other streams must have ended."""
         return self._take_back(sequence, range(self.max_pages))
+
+    def fork(self, source: int, targets, length: int) -> None:
+        """The sequences ``targets``, which have no pages, get the first ``length`` positions of ``source``: its whole pages as
+        they are, shared from now on, and a copy each of the page that ``length`` ends in. What is shared is only read: see
+        ``own``. RuntimeError, and no change, where the pool has too few pages left."""
+        row, targets = self._row(source), list(targets)
+        if not 0 <= length <= self.max_len:
+            raise ValueError(f"{length} positions do not fit max_len {self.max_len}")
+        if len(set(targets)) != len(targets) or source in targets or any(page >= 0 for b in targets for page in self._row(b)):
+            raise ValueError(f"sequences {targets} must be others than {source}, named once and without pages")
+        whole = length // self.page_size
+        split = length % self.page_size > 0 and row[whole] >= 0
+        if split and len(targets) > len(self._free):
+            raise RuntimeError(f"the paged cache has {len(self._free)} pages left, {len(targets)} forks need one each")
+        moves = []
+        for b in targets:
+            self._host[b][:whole] = row[:whole]
+            for page in row[:whole]:
+                if page >= 0:
+                    self._owners[page] += 1
+            if split:
+                self._host[b][whole] = self._take()
+                moves.append((row[whole], self._host[b][whole]))
+        if moves:
+            self._copy(moves)
+        for b in targets:
+            self._store(b)
+        self._regroup()
+
+    def own(self, sequence: int, length: int, start: int) -> int:
+        """Pages of the sequence alone, with the same contents, in place of those of positions ``start`` to ``length - 1`` that
+        others have too, so that it may write there (a sequence set back before the position that it was forked at); returns
+        their number. RuntimeError, and no change, where the pool has too few pages left."""
+        row = self._row(sequence)
+        if not 0 <= start <= length <= self.max_len:
+            raise ValueError(f"positions {start} to {length} do not fit max_len {self.max_len}")
+        slots = range(start // self.page_size, -(-length // self.page_size))
+        shared = [i for i in slots if row[i] >= 0 and self._owners[row[i]] > 1]
+        if len(shared) > len(self._free):
+            raise RuntimeError(f"the paged cache has {len(self._free)} pages left, sequence {sequence} needs {len(shared)}")
+        moves = []
+        for i in shared:
+            moves.append((row[i], self._take()))
+            self._drop(row[i])
+            row[i] = moves[-1][1]
+        if moves:
+            self._copy(moves)
+            self._store(sequence)
+            self._regroup()
+        return len(moves)
+
+    def compact(self) -> int:
+        """Move the pages that are in use to the front of the pools; returns their number, which is the first page that is not.
+        Calls in flight on other streams must have ended."""
+        used = self.pages - len(self._free)
+        holes = [page for page in range(used) if self._owners[page] == 0]
+        moved = dict(zip((page for page in range(used, self.pages) if self._owners[page]), holes))
+        if moved:
+            self._copy(list(moved.items()))
+            for page, to in moved.items():
+                self._owners[to], self._owners[page] = self._owners[page], 0
+            for row in self._host:
+                row[:] = [moved.get(page, page) for page in row]
+            self._free = list(range(self.pages - 1, used - 1, -1))
+            self.table.copy_(torch.tensor(self._host, dtype=torch.int32))
+        return used
 
 
 # ------------------------------------------------------------------------------------- arguments
@@ -308,12 +443,98 @@ def paged_attention(q, k_pages, v_pages, table, positions, window: int = 0, sink
     return o.permute(0, 3, 1, 2, 4).reshape(B, T, H * D).to(q.dtype)
 
 
+def paged_shared_attention(q, k_pages, v_pages, table, positions, members, shared, window: int = 0, sinks: int = 0,
+                           scale: float | None = None):
+    """:func:`paged_attention` of sequences of which groups have their leading pages in common (answers to one prompt):
+    ``members`` int32 [groups, most] are the sequences of each group (entries outside the batch, as -1, are nobody), whose rows
+    of the table begin with the same ``shared`` (int32 [groups]) entries; see :meth:`PagedKVCache.fork`. Those pages are read
+    once a group. A sequence in no group is on its own; of one that is named twice the last place counts. Where members' rows
+    do not begin alike, their results mean nothing.
+
+    Other arguments and the result, but for rounding, are :func:`paged_attention`'s, which also takes the calls that the kernel
+    does not: those that run torch ops, and more than 1024 sequences and groups of 64 rows at once."""
+    what = "paged_shared_attention"
+    given = (q, k_pages, v_pages, table, positions, members, shared)
+    if _native_shared is not None and q.is_cuda and _only_eager(*given):
+        out = _native_shared(*given, window, sinks, scale)
+        if out is not None:
+            return out
+    if members.dim() != 2 or shared.dim() != 1 or members.shape[0] != shared.shape[0]:
+        raise ValueError(f"{what}: members must be [groups, most] and shared [groups], got {tuple(members.shape)} and "
+                         f"{tuple(shared.shape)}")
+    if members.dtype != torch.int32 or shared.dtype != torch.int32:
+        raise TypeError(f"{what}: members and shared must be int32, got {members.dtype} and {shared.dtype}")
+    for t in (members, shared):
+        if t.device != q.device:
+            raise ValueError(f"{what}: tensors on {t.device} and {q.device}")
+    B, T, N, KV, S, D = _check_pages(what, k_pages, v_pages, table, positions, q.dtype, q.device)
+    if q.dim() != 3 or q.shape[:2] != positions.shape or q.shape[2] % (KV * D) or q.shape[2] == 0:
+        raise ValueError(f"{what}: q {tuple(q.shape)} does not fit {B} x {T} tokens and pages of {KV} heads of {D}")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"{what}: negative window ({window}) or sinks ({sinks})")
+    if (q.is_cuda and q.dtype in _HALF and (D == 128 or D == 64) and S % 16 == 0 and members.numel() and q.numel()
+            and _only_eager(*given) and _pool_fits(k_pages, v_pages) and table.shape[1] * S <= 1 << 30):
+        lib = _lib.load()
+        nbytes = lib.nq_paged_shared_attention_workspace_bytes(B, T, q.shape[2] // D, KV, D, *members.shape)
+        if nbytes:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q, qs = _rows(q, B, T)
+            table, positions = _table_rows(table), positions.contiguous()
+            members, shared = members.contiguous(), shared.contiguous()
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            _launch(what, lib.nq_paged_shared_attention, q, _lib.dtype_code(q.dtype), q.data_ptr(), qs, k_pages.data_ptr(),
+                    v_pages.data_ptr(), N, S, table.data_ptr(), table.stride(0), table.shape[1], positions.data_ptr(),
+                    members.data_ptr(), shared.data_ptr(), *members.shape, out.data_ptr(), B, T, q.shape[2] // D, KV, D, window,
+                    sinks, D ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
+            return out
+    return paged_attention(q, k_pages, v_pages, table, positions, window, sinks, scale)
+
+
+def copy_pages(pools, source, target) -> None:
+    """Copy page ``source[i]`` over page ``target[i]`` in each of ``pools``, tensors [pages, ...] alike in shape and type (the
+    keys' and values' of every layer). source and target are int32 [moves] on the pools' device; a pair with a page that is not
+    there (-1) is passed over. No page may be the target of two pairs, or the target of one and the source of another."""
+    what = "copy_pages"
+    pools = list(pools)
+    eager = _only_eager(*pools, source, target)
+    if _native_copy is not None and eager and source.is_cuda and _native_copy(pools, source, target):
+        return
+    if source.dim() != 1 or target.shape != source.shape:
+        raise ValueError(f"{what}: source and target must be [moves], got {tuple(source.shape)} and {tuple(target.shape)}")
+    if source.dtype != torch.int32 or target.dtype != torch.int32:
+        raise TypeError(f"{what}: source and target must be int32, got {source.dtype} and {target.dtype}")
+    for t in (target, *pools):
+        if t.device != source.device:
+            raise ValueError(f"{what}: tensors on {t.device} and {source.device}")
+    for pool in pools:
+        if pool.dim() == 0 or pool.shape != pools[0].shape or pool.dtype != pools[0].dtype:
+            raise ValueError(f"{what}: pools must be alike, got {tuple(pool.shape)} of {pool.dtype} and "
+                             f"{tuple(pools[0].shape)} of {pools[0].dtype}")
+    if not pools or pools[0].numel() == 0 or source.numel() == 0:
+        return
+    pages = pools[0].shape[0]
+    if source.is_cuda and eager and all(pool.is_contiguous() for pool in pools):
+        source, target = source.contiguous(), target.contiguous()
+        at = (ctypes.c_void_p * len(pools))(*(pool.data_ptr() for pool in pools))
+        _launch(what, _lib.load().nq_copy_pages, source, at, len(pools), pages, pools[0].nbytes // pages, source.data_ptr(),
+                target.data_ptr(), source.shape[0])
+        return
+    there = ((source >= 0) & (source < pages) & (target >= 0) & (target < pages)).nonzero()[:, 0]
+    source, target = source[there].long(), target[there].long()
+    for pool in pools:
+        pool[target] = pool[source]
+
+
 def paged_rotary_attention(shape, layer: int, q, k, v, cos, sin, positions, cache: PagedKVCache):
     """A layer's attention between the q, k and v projections and o_proj: rotary embedding, write into the pages and
-    attention over them under the cache's window and sinks. Arguments as :func:`paged_rope_write`; returns [B, T, H * D]."""
+    attention over them under the cache's window and sinks, shared pages read once a group. Arguments as
+    :func:`paged_rope_write`; returns [B, T, H * D]."""
     k_pages, v_pages = cache.k[layer], cache.v[layer]
     dtype = k_pages.dtype
     q = paged_rope_write(q.to(dtype), k.to(dtype), v.to(dtype), cos, sin, positions, k_pages, v_pages, cache.table)
+    if cache.groups:
+        return paged_shared_attention(q, k_pages, v_pages, cache.table, positions, cache.members, cache.shared, cache.window,
+                                      cache.sinks, shape.head_dim ** -0.5)
     return paged_attention(q, k_pages, v_pages, cache.table, positions, cache.window, cache.sinks, shape.head_dim ** -0.5)
 
 
@@ -412,3 +633,70 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature: float
     index = torch.arange(n + 1, device=logits.device)
     tokens = torch.cat((drafts, torch.full_like(token, -1)), dim=1)
     return accepted, torch.where(index < row[:, 0], tokens, torch.where(index == row[:, 0], token, -1))
+
+
+# ------------------------------------------------------------------------------------- scored tokens
+
+_TEMPERATURES = (2.0 ** -64, 2.0 ** 64)  # that float32 exponents have room for
+
+
+def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
+    """What p = softmax(logits / temperature) says of given tokens.
+
+    logits [rows, vocab] or [B, T, vocab] (any strides with the vocabulary's elements side by side, as of ``logits[:, :-1]``;
+    float32, float16, bfloat16, or float64 by torch ops), tokens int64 [rows] or [B, T]. Returns ``(logprobs, entropy,
+    top_tokens, top_logprobs)``: log p of the given token, 0 for one outside the vocabulary (-1 for padding); -sum p log p; the
+    ``top`` largest logits' indexes [..., top], the lowest first of equal ones, and their log p. In float32 (float64 for float64
+    logits). A logit of -inf has no part in the sums. In a row with a NaN, or whose largest logit is infinite, log p and the
+    entropy are NaN, and a NaN counts as the largest logit."""
+    what = "token_logprobs"
+    if _native_score is not None and logits.is_cuda and _only_eager(logits, tokens):
+        out = _native_score(logits, tokens, top, temperature)
+        if out:
+            return tuple(out)
+    if logits.dim() not in (2, 3) or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"{what}: logits must be [rows, vocab] or [B, T, vocab] and tokens like them without vocab, got "
+                         f"{tuple(logits.shape)} and {tuple(tokens.shape)}")
+    if logits.dtype not in (torch.float32, torch.float64, *_HALF) or tokens.dtype != torch.int64:
+        raise TypeError(f"{what}: logits float32, float64, float16 or bfloat16 and tokens int64, got {logits.dtype} and "
+                        f"{tokens.dtype}")
+    if tokens.device != logits.device:
+        raise ValueError(f"{what}: tensors on {tokens.device} and {logits.device}")
+    V = logits.shape[-1]
+    if V == 0 or not 0 <= top <= V:
+        raise ValueError(f"{what}: {top} alternatives of {V} tokens")
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"{what}: the temperature must be a finite number above 0, got {temperature}")
+    shape, kind = tokens.shape, torch.promote_types(logits.dtype, torch.float32)
+    usual = _TEMPERATURES[0] <= temperature <= _TEMPERATURES[1]
+    if (logits.is_cuda and kind == torch.float32 and top <= 64 and V <= 1 << 30 and usual and tokens.numel()
+            and _only_eager(logits, tokens)):
+        rows = logits if logits.dim() == 3 else logits.unsqueeze(0)
+        B, T = rows.shape[:2]
+        if (V > 1 and rows.stride(2) != 1) or (T > 1 and rows.stride(1) < V) or (B > 1 and rows.stride(0) < V):
+            rows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device).copy_(rows)
+        at = tokens if tokens.dim() == 2 else tokens.unsqueeze(0)
+        lib = _lib.load()
+        nbytes = lib.nq_token_logprobs_workspace_bytes(B, T, V, top)
+        if nbytes:
+            logprobs, entropy = torch.empty(2, *shape, dtype=kind, device=logits.device).unbind(0)
+            top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=logits.device)
+            top_logprobs = torch.empty(*shape, top, dtype=kind, device=logits.device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+            code = _lib.NQ_F32 if logits.dtype == torch.float32 else _lib.dtype_code(logits.dtype)
+            _launch(what, lib.nq_token_logprobs, logits, code, rows.data_ptr(), rows.stride(0), rows.stride(1), at.data_ptr(),
+                    at.stride(0), at.stride(1), temperature, top, logprobs.data_ptr(), entropy.data_ptr(),
+                    top_tokens.data_ptr(), top_logprobs.data_ptr(), B, T, V, ws.data_ptr(), nbytes)
+            return logprobs, entropy, top_tokens, top_logprobs
+    x = logits.to(kind if usual else torch.float64)
+    d = (x - x.detach().amax(dim=-1, keepdim=True)) / temperature
+    e = torch.exp(d)
+    total = e.sum(dim=-1)
+    log_total = torch.log(total)
+    there = (tokens >= 0) & (tokens < V)
+    given = d.gather(-1, torch.where(there, tokens, 0).unsqueeze(-1))[..., 0] - log_total
+    entropy = log_total - (e * torch.where(d == -math.inf, 0.0, d)).sum(dim=-1) / total
+    # an order that is stable gives the lowest index of equal logits, and a NaN comes first in it
+    order = torch.sort(logits.detach(), dim=-1, descending=True, stable=True).indices[..., :top].contiguous()
+    best = d.gather(-1, order) - log_total.unsqueeze(-1)
+    return torch.where(there, given, 0.0).to(kind), entropy.to(kind), order, best.to(kind)

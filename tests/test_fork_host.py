@@ -1,0 +1,404 @@
+"""Forked sequences, attention over shared pages and scored tokens on the CPU (the torch ops), their refusals, and the C ABI's."""
+import math
+
+import pytest
+import torch
+
+import fork_oracle
+import serve_oracle as oracle
+from nanoquant_amd import (PagedKVCache, _lib, copy_pages, paged_attention, paged_shared_attention, token_logprobs)
+from nanoquant_amd.decode import LlamaShape, random_llama
+
+TINY = LlamaShape(hidden=128, layers=2, heads=4, kv_heads=2, ffn=320, vocab=500)
+
+
+def test_shared_attention_is_attention():
+    case = fork_oracle.shared_case(4, 2, 32, 8, [(3, [1, 9, 4]), (1, [2, 30])], [5, 17], 3, torch.float32, "cpu")
+    q, k, v, table, pos, members, shared = case
+    ref, _ = oracle.attention(q, k, v, table, pos, 9, 2)
+    y = paged_shared_attention(*case, window=9, sinks=2)
+    assert (y.double() - ref).abs().max() < 1e-5
+    assert torch.equal(y, paged_attention(q, k, v, table, pos, 9, 2))
+
+
+def test_copy_pages():
+    pools = [torch.randn(7, 2, 3, 5) for _ in range(3)]
+    want = [p.clone() for p in pools]
+    source, target = torch.tensor([0, 5, -1, 2, 9, 3], dtype=torch.int32), torch.tensor([4, 1, 6, 7, 0, -2], dtype=torch.int32)
+    for p in want:
+        p[4], p[1] = p[0], p[5]
+    copy_pages(pools, source, target)
+    assert all(torch.equal(a, b) for a, b in zip(pools, want))
+    copy_pages(pools, source[:0], target[:0])
+    copy_pages([], source, target)
+    copy_pages((p for p in pools), source, target)
+    assert all(torch.equal(a, b) for a, b in zip(pools, want))
+
+
+def _cache(batch=6, pages=12, page=4, max_len=30, **kw):
+    cache = PagedKVCache(TINY, batch, pages, page, max_len, "cpu", torch.float32, **kw)
+    for pool in (*cache.k, *cache.v):
+        pool.normal_()
+    return cache
+
+
+def _contents(cache, b, length):
+    """What the sequence's positions hold, by the device's table."""
+    j = torch.arange(length)
+    page = cache.table[b].long()[j // cache.page_size]
+    assert (page >= 0).all()
+    return [pool[page, :, j % cache.page_size].clone() for pool in (*cache.k, *cache.v)]
+
+
+def _sound(cache):
+    """Every page is free, or counted as often as rows of the table have it; the table is what the host has."""
+    assert cache.table.tolist() == cache._host
+    held = [0] * cache.pages
+    for row in cache._host:
+        for page in row:
+            if page >= 0:
+                held[page] += 1
+    assert held == cache._owners
+    assert sorted(cache._free) == [p for p in range(cache.pages) if held[p] == 0]
+    if cache.members is None:
+        return
+    for i in range(cache.members.shape[0]):
+        sequences = [b for b in cache.members[i].tolist() if b >= 0]
+        n = int(cache.shared[i])
+        assert (len(sequences) > 1 and n > 0) if i < cache.groups else (not sequences and n == 0)
+        assert len({tuple(cache._host[b][:n]) for b in sequences}) <= 1
+
+
+def test_forks_share_whole_pages_and_copy_the_last():
+    cache = _cache()
+    cache.reserve(0, 10)
+    want = _contents(cache, 0, 10)
+    cache.fork(0, [2, 5], 10)
+    _sound(cache)
+    assert cache._host[2][:2] == cache._host[0][:2] == cache._host[5][:2] and len({cache._host[b][2] for b in (0, 2, 5)}) == 3
+    assert cache.groups == 1 and sorted(b for b in cache.members[0].tolist() if b >= 0) == [0, 2, 5] and int(cache.shared[0]) == 2
+    assert len(cache._free) == 12 - 5
+    for b in (0, 2, 5):
+        assert all(torch.equal(x, y) for x, y in zip(_contents(cache, b, 10), want))
+    cache.reserve(2, 20)
+    cache.fork(2, [1], 17)  # a fork of a fork
+    _sound(cache)
+    assert cache.release(0) == 3 and len(cache._free) == 12 - 5 - 2 - 1 + 1
+    _sound(cache)
+    assert all(torch.equal(x, y) for x, y in zip(_contents(cache, 5, 10), want))
+    for b in (1, 2, 5):
+        cache.release(b)
+        _sound(cache)
+    assert cache.groups == 0 and len(cache._free) == 12
+
+
+def test_forks_at_the_end_of_a_page_and_of_nothing():
+    cache = _cache()
+    cache.reserve(0, 8)
+    cache.fork(0, [1], 8)   # no page to copy
+    assert cache._host[1] == cache._host[0]
+    cache.fork(0, [2], 0)   # nothing in common
+    assert cache._host[2] == [-1] * cache.max_pages
+    cache.fork(0, [3], 6)
+    cache.fork(0, [], 8)
+    _sound(cache)
+    assert cache._host[3][0] == cache._host[0][0] and cache._host[3][1] not in cache._host[0]
+    assert int(cache.shared[0]) == 1  # what all three begin with
+    cache.fork(2, [4], 20)  # of a sequence without pages
+    _sound(cache)
+
+
+def test_pages_of_its_own_before_a_sequence_writes():
+    cache = _cache()
+    cache.reserve(0, 12)
+    cache.fork(0, [1, 2], 12)
+    want = _contents(cache, 0, 12)
+    assert cache.own(1, 11, 5) == 2
+    _sound(cache)
+    assert cache._host[1][0] == cache._host[0][0] and not set(cache._host[1][1:3]) & set(cache._host[0])
+    assert cache.own(1, 11, 5) == 0
+    assert int(cache.shared[0]) == 1
+    for pool in (*cache.k, *cache.v):
+        pool[cache._host[1][1]] = 7.0
+    for b in (0, 2):
+        assert all(torch.equal(x, y) for x, y in zip(_contents(cache, b, 12), want))
+    cache.release(0), cache.release(1)
+    assert cache.own(2, 12, 0) == 0  # nobody else has them any more
+    _sound(cache)
+
+
+def test_compaction_keeps_what_sequences_hold():
+    cache = _cache(pages=15)
+    for b, n in enumerate((9, 20, 5)):
+        cache.reserve(b, n)
+    cache.fork(1, [3, 4], 18)
+    cache.release(0)
+    held = {b: _contents(cache, b, n) for b, n in ((1, 20), (2, 5), (3, 18), (4, 18))}
+    used = cache.compact()
+    _sound(cache)
+    assert used == 15 - len(cache._free) == 9 and max(map(max, cache._host)) == used - 1
+    for b, want in held.items():
+        assert all(torch.equal(x, y) for x, y in zip(_contents(cache, b, want[0].shape[0]), want))
+    assert cache.compact() == used
+    cache.reserve(0, 24)
+    _sound(cache)
+    assert _cache().compact() == 0
+
+
+def test_groups_under_a_window():
+    """Sequences that have dropped pages of the prompt: grouped by what their rows still begin with."""
+    cache = _cache(window=6, sinks=2, pages=20)
+    cache.reserve(0, 20)
+    cache.fork(0, [1, 2], 20)
+    cache.reserve(1, 28)
+    cache.trim(1, 27)
+    _sound(cache)
+    assert int(cache.shared[0]) == 1  # the sinks' page
+    cache.trim(0, 27), cache.trim(2, 27)
+    _sound(cache)
+    assert cache.groups == 1 and int(cache.shared[0]) == 1
+
+
+def test_many_forks_at_random():
+    import random
+    rng = random.Random(4)
+    cache = _cache(batch=7, pages=30, max_len=32)
+    length, text = [0] * 7, [None] * 7
+    for step in range(300):
+        b = rng.randrange(7)
+        try:
+            what = rng.choice(["reserve", "fork", "release", "own", "compact"])
+            if what == "reserve":
+                n = rng.randint(length[b], 32)
+                cache.reserve(b, n)
+                length[b] = n
+            elif what == "fork":
+                targets = [c for c in range(7) if c != b and cache._host[c] == [-1] * cache.max_pages][:rng.randint(1, 3)]
+                cache.fork(b, targets, rng.randint(0, length[b]))
+                for c in targets:
+                    length[c] = sum(page >= 0 for page in cache._host[c]) * 4
+            elif what == "release":
+                cache.release(b)
+                length[b] = 0
+            elif what == "own":
+                start = rng.randint(0, length[b])
+                cache.own(b, length[b], start)
+                assert all(cache._owners[p] == 1 for p in cache._host[b][start // 4:-(-length[b] // 4)] if p >= 0)
+            else:
+                text = [_contents(cache, c, length[c]) for c in range(7)]
+                cache.compact()
+                for c in range(7):
+                    assert all(torch.equal(x, y) for x, y in zip(_contents(cache, c, length[c]), text[c]))
+        except RuntimeError:
+            assert len(cache._free) < 9
+        _sound(cache)
+
+
+def _score_case(shape, V, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(*shape, V, generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, V, shape, generator=g)
+    tokens.view(-1)[1::4] = torch.tensor([-1, V, 1 << 40]).repeat(tokens.numel())[:tokens.view(-1)[1::4].numel()]
+    return logits, tokens
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("shape,V,top,temperature", [((5,), 33, 4, 1.0), ((2, 3), 500, 7, 0.7), ((4,), 1, 1, 1.0), ((3, 1), 9, 9, 2.5),
+                                                     ((6,), 200, 0, 1.0)])
+def test_score_against_the_definition(shape, V, top, temperature, dtype):
+    logits, tokens = _score_case(shape, V, dtype)
+    got = token_logprobs(logits, tokens, top, temperature)
+    assert got[0].dtype == (torch.float64 if dtype == torch.float64 else torch.float32)
+    fork_oracle.check_score(got, fork_oracle.score(logits, tokens, top, temperature))
+
+
+def odd_rows(V, dtype):
+    """Rows with masks, equal logits, infinities and NaN, and a token for each."""
+    x = torch.randn(12, V, generator=torch.Generator().manual_seed(5)).to(dtype)
+    x[0, 1:] = -math.inf                  # one token left: log p 0, no entropy
+    x[1, ::2] = -math.inf
+    x[2] = 1.5                            # all alike
+    x[3] = -math.inf
+    x[4, V // 2] = math.nan
+    x[5, 3], x[5, V - 1] = math.inf, math.nan
+    x[6, 4] = math.inf
+    x[7, V // 3:] = torch.finfo(dtype).min
+    x[8, V - 2:] = 60.0                   # two far above the others
+    x[9, :] = 0.0
+    x[9, 1::2] = -0.0
+    x[10, 2], x[10, 5] = math.nan, -math.nan
+    x[11, :] = -20000.0
+    return x, torch.tensor([0, 0, V - 1, 1, 0, 3, 4, V - 1, V - 1, 2, 0, 7])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_score_of_odd_rows(dtype):
+    logits, tokens = odd_rows(41, dtype)
+    for top in (0, 3, 41):
+        fork_oracle.check_score(token_logprobs(logits, tokens, top), fork_oracle.score(logits, tokens, top, 1.0))
+
+
+@pytest.mark.parametrize("temperature", [5e-324, 1e-300, 1e-30, 1e30, 1e300])
+def test_score_at_extreme_temperatures(temperature):
+    logits, tokens = _score_case((6,), 50, torch.float32)
+    logits[0, 3:9] = -math.inf
+    fork_oracle.check_score(token_logprobs(logits, tokens, 3, temperature), fork_oracle.score(logits, tokens, 3, temperature))
+
+
+def test_gradients_of_scores():
+    """log p's and the entropy's, against the formulas: (1[j = token] - p_j) / T, and -p_j (log p_j + H) / T."""
+    logits, tokens = _score_case((5,), 30, torch.float32)
+    logits[1, 4:9] = -math.inf
+    w, z = torch.randn(2, 5, generator=torch.Generator().manual_seed(1))
+    T = 0.8
+    x = logits.clone().requires_grad_(True)
+    given, entropy, _, best = token_logprobs(x, tokens, 2, T)
+    (given * w + entropy * z).sum().backward()
+    d = logits.double()
+    logp = torch.log_softmax(d / T, -1)
+    p = logp.exp()
+    there = (tokens >= 0) & (tokens < 30)
+    one = torch.nn.functional.one_hot(torch.where(there, tokens, 0), 30).double()
+    H = -(p * torch.where(p > 0, logp, 0.0)).sum(-1, keepdim=True)
+    want = torch.where(there, w, 0.0).double().unsqueeze(1) * (one - p) / T
+    want -= z.double().unsqueeze(1) * p * (torch.where(p > 0, logp, 0.0) + H) / T
+    # every factor is a float32 result off by a few of its roundings, of sums over 30 terms: 2^-24 * 64 of terms up to 10
+    assert (x.grad.double() - want).abs().max() < 64 * 2.0 ** -24 * 10
+    assert torch.autograd.gradcheck(lambda y: token_logprobs(y, tokens[2:], 0, T)[:2], (logits[2:].double().requires_grad_(True),))
+
+
+def test_a_model_answers_a_prompt_several_times():
+    """Forked, then decoded together: every answer is what a sequence of its own says, and its score what its logits say."""
+    torch.manual_seed(0)
+    model = random_llama(TINY, bpw=2.0, device="cpu", dtype=torch.float32).eval()
+    answers, P, page = 3, 11, 4
+    prompt = torch.randint(0, TINY.vocab, (P,))
+    texts = torch.randint(0, TINY.vocab, (answers, 6))
+    with torch.no_grad():
+        alone = PagedKVCache(TINY, answers, 40, page, 40, "cpu", torch.float32)
+        forked = PagedKVCache(TINY, answers, 40, page, 40, "cpu", torch.float32)
+        for b in range(answers):
+            alone.reserve(b, P + 6)
+        model(prompt.expand(answers, -1), torch.arange(P).expand(answers, -1), alone)
+        forked.reserve(0, P)
+        ids, pos = torch.zeros(answers, P, dtype=torch.int64), torch.full((answers, P), -1)
+        ids[0], pos[0] = prompt, torch.arange(P)
+        model(ids, pos, forked)
+        forked.fork(0, [1, 2], P)
+        for b in range(answers):
+            forked.reserve(b, P + 6, P)
+        assert forked.groups == 1 and int(forked.shared[0]) == 2
+        for t in range(6):
+            at = torch.full((answers, 1), P + t)
+            want, got = model(texts[:, t:t + 1], at, alone), model(texts[:, t:t + 1], at, forked)
+            assert torch.allclose(got, want, rtol=0, atol=1e-4)
+            chosen = texts[:, t + 1:t + 2] if t < 5 else texts[:, :1]
+            a, b = token_logprobs(want, chosen, 3), token_logprobs(got, chosen, 3)
+            assert torch.allclose(a[0], b[0], rtol=0, atol=1e-3) and a[3].shape == (answers, 1, 3)
+        forked.compact()
+
+
+def test_refusals():
+    case = fork_oracle.shared_case(4, 2, 32, 8, [(3, [1, 9])], [5], 1, torch.float32, "cpu")
+    q, k, v, table, pos, members, shared = case
+    with pytest.raises(ValueError, match="members"):
+        paged_shared_attention(*case[:5], members[0], shared)
+    with pytest.raises(ValueError, match="members"):
+        paged_shared_attention(*case[:5], members, torch.cat((shared, shared)))
+    with pytest.raises(TypeError, match="int32"):
+        paged_shared_attention(*case[:5], members.long(), shared)
+    with pytest.raises(TypeError, match="int32"):
+        paged_shared_attention(*case[:5], members, shared.long())
+    with pytest.raises(ValueError, match="window"):
+        paged_shared_attention(*case, window=-1)
+    with pytest.raises(ValueError, match="does not fit"):
+        paged_shared_attention(q[..., :24], *case[1:])
+    pools = [torch.zeros(4, 2, 3), torch.zeros(4, 2, 3)]
+    one = torch.tensor([1], dtype=torch.int32)
+    with pytest.raises(ValueError, match="alike"):
+        copy_pages([pools[0], torch.zeros(4, 3, 2)], one, one)
+    with pytest.raises(ValueError, match="alike"):
+        copy_pages([pools[0], pools[1].half()], one, one)
+    with pytest.raises(ValueError, match="moves"):
+        copy_pages(pools, one, torch.cat((one, one)))
+    with pytest.raises(TypeError, match="int32"):
+        copy_pages(pools, one.long(), one)
+    cache = _cache(pages=4)
+    cache.reserve(0, 10)
+    with pytest.raises(RuntimeError, match="pages left"):
+        cache.fork(0, [1, 2], 10)
+    _sound(cache)
+    for targets in ([0], [1, 1]):
+        with pytest.raises(ValueError, match="without pages"):
+            cache.fork(0, targets, 8)
+    cache.fork(0, [1], 8)
+    with pytest.raises(ValueError, match="without pages"):
+        cache.fork(0, [1], 8)
+    with pytest.raises(IndexError):
+        cache.fork(0, [6], 8)
+    with pytest.raises(ValueError, match="max_len"):
+        cache.fork(0, [2], 31)
+    with pytest.raises(ValueError, match="max_len"):
+        cache.own(0, 4, 5)
+    with pytest.raises(RuntimeError, match="pages left"):
+        cache.own(1, 8, 0)
+    _sound(cache)
+    logits, tokens = _score_case((5,), 30, torch.float32)
+    with pytest.raises(ValueError, match="vocab"):
+        token_logprobs(logits, tokens[:4])
+    with pytest.raises(ValueError, match="vocab"):
+        token_logprobs(logits[0], tokens[0])
+    with pytest.raises(TypeError, match="int64"):
+        token_logprobs(logits, tokens.int())
+    with pytest.raises(TypeError, match="float32"):
+        token_logprobs(logits.int(), tokens)
+    for top in (-1, 31):
+        with pytest.raises(ValueError, match="alternatives"):
+            token_logprobs(logits, tokens, top)
+    for bad in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            token_logprobs(logits, tokens, temperature=bad)
+    assert [tuple(x.shape) for x in token_logprobs(logits[:0], tokens[:0], 2)] == [(0,), (0,), (0, 2), (0, 2)]
+
+
+def test_c_abi_argument_errors_need_no_gpu():
+    import ctypes
+    lib = _lib.load()
+    p = 256  # a pointer that is never followed: every call below ends before its launch
+
+    def attn(dtype=0, q=p, stride=128 * 4, pages=4, page_size=16, table_stride=8, table_pages=8, members=p, groups=2, most=3, batch=1,
+             tokens=1, heads=4, kv=2, dim=128, window=0, sinks=0, ws=p, nbytes=1 << 40, k=p):
+        return lib.nq_paged_shared_attention(dtype, q, stride, k, p, pages, page_size, p, table_stride, table_pages, p, members, p,
+                                             groups, most, p, batch, tokens, heads, kv, dim, window, sinks, 1.0, ws, nbytes, None)
+
+    assert attn(dtype=2) == _lib.NQ_ERR_DTYPE
+    assert attn(batch=0) == attn(tokens=0) == 0
+    assert attn(batch=-1) == attn(pages=0) == attn(window=-1) == attn(sinks=-1) == attn(groups=-1) == attn(most=-1) == \
+        attn(q=None) == attn(k=None) == attn(members=None) == _lib.NQ_ERR_INVALID_ARGUMENT
+    assert attn(heads=3) == attn(table_stride=7) == attn(stride=504) == attn(stride=516) == _lib.NQ_ERR_SHAPE
+    assert attn(dim=96, stride=4096) == attn(page_size=24) == attn(batch=1 << 20, tokens=1 << 20) == _lib.NQ_ERR_UNSUPPORTED
+    assert attn(q=p + 8) == attn(k=p + 2) == attn(members=p + 2) == attn(ws=p + 8) == _lib.NQ_ERR_ALIGNMENT
+
+    def copy(pools=(p, p), pages=4, nbytes=64, source=p, moves=2):
+        at = (ctypes.c_void_p * 2)(*pools)
+        return lib.nq_copy_pages(at, 2, pages, nbytes, source, p, moves, None)
+
+    assert copy(moves=0) == 0
+    assert copy(moves=-1) == copy(pages=0) == copy(nbytes=0) == copy(source=None) == copy(pools=(p, None)) == \
+        _lib.NQ_ERR_INVALID_ARGUMENT
+    assert copy(source=p + 2) == _lib.NQ_ERR_ALIGNMENT
+    assert copy(pages=1 << 31) == copy(nbytes=(1 << 33) + 1) == _lib.NQ_ERR_UNSUPPORTED
+
+    def score(dtype=2, row=100, batch_stride=300, temperature=1.0, top=3, batch=2, rows=3, vocab=100, ws=p, nbytes=1 << 40, logits=p,
+              best=p):
+        return lib.nq_token_logprobs(dtype, logits, batch_stride, row, p, 3, 1, temperature, top, p, p, best, p, batch, rows, vocab,
+                                     ws, nbytes, None)
+
+    assert score(dtype=3) == _lib.NQ_ERR_DTYPE
+    assert score(batch=0) == score(rows=0) == 0
+    assert score(row=99) == score(batch_stride=99) == _lib.NQ_ERR_SHAPE
+    assert score(temperature=0.0) == score(temperature=math.nan) == score(temperature=math.inf) == score(vocab=0) == \
+        score(top=-1) == score(top=101) == score(logits=None) == score(best=None) == _lib.NQ_ERR_INVALID_ARGUMENT
+    assert score(batch=1 << 20, rows=1 << 20) == score(vocab=1 << 31, row=1 << 31, batch_stride=1 << 33) == score(top=65) == \
+        score(temperature=2.0 ** -65) == score(temperature=2.0 ** 65) == _lib.NQ_ERR_UNSUPPORTED
+    assert score(logits=p + 2) == score(best=p + 4) == _lib.NQ_ERR_ALIGNMENT
