@@ -42,6 +42,7 @@ FILE_FLAGS = {
     "nq_gemv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     # the same in the paged attention: its outputs are rescaled now and then, and went through both files for it
     "nq_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "nq_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],  # few_kernel again
 }
 
 

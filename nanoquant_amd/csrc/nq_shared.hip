@@ -3,67 +3,138 @@
 #include <cmath>
 
 #include "nq_common.h"
-#include "nq_paged.h"
+#include "nq_paged_few.h"
 
 namespace nq {
 namespace {
 
-constexpr int kEntries = 1024;  // pieces of work that a launch lists
-
-struct SharedArgs {
-    const uint16_t* q;
-    int64_t q_stride;
-    const uint16_t* k_pages;
-    const uint16_t* v_pages;
-    Pages pages;
-    const int64_t* positions;
-    const int32_t* members;  // [groups][most]
-    const int32_t* shared;   // [groups]: pages
-    int groups, most;
-    uint16_t* out;
-    int batch, tokens, heads, kv_heads;
-    int window, sinks;
-    float scale;  // times log2(e)
-};
-
-// A wave a row, a key at a time, lane l at dimensions l and, of 128, l + 64.
+// Adds up what few_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave a row, D / 4 lanes a
+// part.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void shared_kernel(const SharedArgs a) {
-    constexpr int N = D / 64;
+__global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int rows, int64_t count) {
+    constexpr int L4 = D / 4, Groups = 64 / L4, kAhead = 4;
     const int lane = threadIdx.x & 63;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);  // (sequence, token, head)
-    if (row >= static_cast<int64_t>(a.batch) * a.tokens * a.heads) return;
+    if (row >= count) return;
     const int64_t token = row / a.heads;
-    const int head = static_cast<int>(row - token * a.heads), kvh = head / (a.heads / a.kv_heads);
+    const int head = static_cast<int>(row - token * a.heads), kvh = head / a.groups;
     const int b = static_cast<int>(token / a.tokens);
-    const int64_t p = a.positions[token];
-    const int last = p >= 0 && p < a.pages.capacity() ? static_cast<int>(p) : -1;
-    const int start = a.window > 0 ? max(0, last - a.window + 1) : 0;
-    const uint16_t* q = a.q + token * a.q_stride + static_cast<int64_t>(head) * D + lane;
-    float o[N], m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
-    for (int key = 0; key <= last; ++key) {
-        const int page = a.pages.page(b, key / a.pages.page_size);
-        if (!(key >= start || key < a.sinks) || page < 0) continue;
-        const int64_t at = ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D + lane;
-        float s = 0.0f;
-        for (int i = 0; i < N; ++i) s = fmaf(T::to_float(q[64 * i]), T::to_float(a.k_pages[at + 64 * i]), s);
-        s = wave_sum(s) * a.scale;
-        const float top = fmaxf(m, s);
-        const float keep = __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(s - top);
-        const bool none = top == -INFINITY && s == s;  // scores of -inf so far
-        m = top;
-        l = none ? 0.0f : fmaf(l, keep, e);
-        for (int i = 0; i < N; ++i) o[i] = none ? 0.0f : fmaf(e, T::to_float(a.v_pages[at + 64 * i]), o[i] * keep);
+    const int r = static_cast<int>(token - static_cast<int64_t>(b) * a.tokens) * a.groups + head - kvh * a.groups;
+    const int at = a.place[b];
+    struct Parts {
+        int64_t first, later;  // rows of the first part and, were it one of the later ones, of the first block's
+        int n;
+    };
+    auto parts_of = [&](int entry, int in_entry) {
+        const int2 d = a.desc[entry * a.kv_heads + kvh];
+        return Parts{first_part(a, entry, kvh) + in_entry, later_part(a, d.x >> 1, rows) + in_entry, d.y - (d.x >> 1) + 1};
+    };
+    Parts common{0, 0, 0};
+    if (at >= 0) {
+        const int g = at / a.most, in_group = (at - g * a.most) * a.tokens * a.groups + r;
+        common = parts_of(g * a.group_rows + in_group / rows, in_group % rows);
     }
-    for (int i = 0; i < N; ++i) a.out[row * D + lane + 64 * i] = T::from_float(l == 0.0f ? 0.0f : o[i] / l);
+    const Parts own = parts_of(a.entries_of_groups() + b * a.row_groups + r / rows, r % rows);
+    const int n = common.n + own.n, grp = lane / L4, d0 = 4 * (lane % L4);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = grp; i0 < n; i0 += kAhead * Groups) {
+        float2 ml[kAhead];
+        f32x4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {  // those past the last read it again
+            const int part = min(i0 + i * Groups, n - 1);
+            const bool of_common = part < common.n;
+            const int k = of_common ? part : part - common.n;
+            const int64_t from = k == 0 ? (of_common ? common.first : own.first)
+                                        : (of_common ? common.later : own.later) + static_cast<int64_t>(k) * rows;
+            ml[i] = a.part_ml[from];
+            x[i] = *reinterpret_cast<const f32x4*>(a.part_o + from * D + d0);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(M - mu);
+        M = top;
+        L *= keep;
+        o *= keep;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mu);
+            const bool in = i0 + i * Groups < n;
+            L = in ? fmaf(f, ml[i].y, L) : L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = in ? fmaf(f, x[i][e], o[e]) : o[e];
+        }
+    }
+#pragma unroll
+    for (int off = L4; off < 64; off <<= 1) {
+        const float other = __shfl_xor(M, off, 64), top = fmaxf(M, other);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(M - mu), f1 = __builtin_amdgcn_exp2f(other - mu);
+        L = f0 * L + f1 * __shfl_xor(L, off, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = f0 * o[e] + f1 * __shfl_xor(o[e], off, 64);
+        M = top;
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    if (grp == 0) *reinterpret_cast<uint2*>(a.out + row * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
-template <typename T>
-void launch_shared(const SharedArgs& a, int64_t head_dim, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.batch) * a.tokens * a.heads, 4)));
-    if (head_dim == 64) shared_kernel<T, 64><<<grid, 256, 0, st>>>(a);
-    else shared_kernel<T, 128><<<grid, 256, 0, st>>>(a);
+// Row tiles of a launch, its list of work and what it needs of the workspace; tiles 0: more than a launch lists.
+struct Plan {
+    int tiles = 0;  // of 16 rows
+    int64_t group_rows, row_groups, group_kept, rows_kept;
+    size_t part_o, part_ml, desc, place, bytes;
+};
+
+Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t sharing, int64_t most) {
+    Plan p{};
+    const int64_t each = tokens * groups, together = most * each;
+    const int tiles = together <= 16 ? 1 : together <= 32 ? 2 : 4;
+    p.group_rows = ceil_div(together, 16 * tiles);
+    p.row_groups = ceil_div(each, 16 * tiles);
+    p.group_kept = std::min<int64_t>(together, 16 * tiles);
+    p.rows_kept = std::min<int64_t>(each, 16 * tiles);
+    const bool wide = tiles > 2 && head_dim == 128;
+    const int64_t entries = sharing * p.group_rows + batch * p.row_groups;
+    if (entries > (wide ? 2 : 1) * kFewEntries) return p;
+    const int64_t parts = kv_heads * (sharing * p.group_rows * p.group_kept + batch * p.row_groups * p.rows_kept) +
+                          static_cast<int64_t>(wide ? 1 : 2) * kCUs * 16 * tiles;
+    p.tiles = tiles;
+    p.part_o = static_cast<size_t>(parts * head_dim) * sizeof(float);
+    p.part_ml = static_cast<size_t>(ceil_div(parts, 2) * 2) * sizeof(float2);
+    p.desc = static_cast<size_t>(ceil_div(entries * kv_heads, 2) * 2) * sizeof(int2);
+    p.place = static_cast<size_t>(batch) * sizeof(int);
+    p.bytes = p.part_o + p.part_ml + p.desc + p.place;
+    return p;
+}
+
+template <typename T, int D>
+void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
+    a.row_groups = static_cast<int>(p.row_groups);
+    a.rows_kept = static_cast<int>(p.rows_kept);
+    a.group_rows = static_cast<int>(p.group_rows);
+    a.group_kept = static_cast<int>(p.group_kept);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.part_o);
+    a.desc = reinterpret_cast<int2*>(ws + p.part_o + p.part_ml);
+    a.place = reinterpret_cast<int*>(ws + p.part_o + p.part_ml + p.desc);
+    if (p.tiles == 1) few_kernel<T, D, 1, true, GroupArgs><<<dim3(FewShape<D, 1>::kBlocks), 64 * kWaves, 0, st>>>(a);
+    else if (p.tiles == 2) few_kernel<T, D, 2, true, GroupArgs><<<dim3(FewShape<D, 2>::kBlocks), 64 * kWaves, 0, st>>>(a);
+    else few_kernel<T, D, 4, true, GroupArgs><<<dim3(FewShape<D, 4>::kBlocks), 64 * kWaves, 0, st>>>(a);
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
+    group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, 16 * p.tiles, rows);
+}
+
+// A call's plan; tiles 0 where there is none.
+Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t sharing, int64_t most) {
+    if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65536 || batch > INT32_MAX ||
+        tokens > INT32_MAX || batch * tokens > INT32_MAX / heads || sharing <= 0 || most <= 0 || sharing > INT32_MAX ||
+        most > INT32_MAX / sharing || most > INT32_MAX / (tokens * heads) || (head_dim != 64 && head_dim != 128))
+        return Plan{};
+    return make_plan(batch, tokens, heads / kv_heads, kv_heads, head_dim, sharing, most);
 }
 
 }  // namespace
@@ -75,11 +146,7 @@ extern "C" {
 
 size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t groups, int64_t most) {
-    if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65536 || batch > INT32_MAX ||
-        tokens > INT32_MAX || batch * tokens > INT32_MAX / heads || groups <= 0 || most <= 0 || groups > kEntries || most > INT32_MAX / (tokens * heads))
-        return 0;
-    const int64_t rows = tokens * (heads / kv_heads);
-    return groups * ceil_div(most * rows, 64) + batch * ceil_div(rows, 64) <= kEntries ? 16 : 0;
+    return plan_of(batch, tokens, heads, kv_heads, head_dim, groups, most).bytes;
 }
 
 int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -100,10 +167,14 @@ int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const 
     if (batch == 0 || tokens == 0) return NQ_OK;
     if (batch * tokens > INT32_MAX / heads) return fail(NQ_ERR_UNSUPPORTED, "%s: sizes too large", name);
     if (int st = check_pages(name, k_pages, v_pages, pages, page_size, table, table_stride, table_pages, positions)) return st;
-    if (!q || !out || (groups * most && (!members || !shared))) return fail(NQ_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+    if (!q || !out || !members || !shared) return fail(NQ_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(members, 4) || !aligned(shared, 4))
         return fail(NQ_ERR_ALIGNMENT, "%s: q, out and the workspace must be 16-byte aligned, the groups 4-byte", name);
-    SharedArgs a{};
+    const Plan plan = plan_of(batch, tokens, heads, kv_heads, head_dim, groups, most);
+    if (plan.tiles == 0) return fail(NQ_ERR_UNSUPPORTED, "%s: no groups, or more work than a launch lists", name);
+    if (!workspace || workspace_bytes < plan.bytes)
+        return fail(NQ_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", name, workspace ? workspace_bytes : size_t{0}, plan.bytes);
+    GroupArgs a{};
     a.q = static_cast<const uint16_t*>(q);
     a.q_stride = q_stride;
     a.k_pages = static_cast<const uint16_t*>(k_pages);
@@ -112,18 +183,26 @@ int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const 
     a.positions = positions;
     a.members = members;
     a.shared = shared;
-    a.groups = static_cast<int>(groups);
+    a.sharing = static_cast<int>(groups);
     a.most = static_cast<int>(most);
     a.out = static_cast<uint16_t*>(out);
     a.batch = static_cast<int>(batch);
     a.tokens = static_cast<int>(tokens);
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
+    a.groups = static_cast<int>(heads / kv_heads);
     a.window = static_cast<int>(std::min(window, kMaxKeys));
     a.sinks = static_cast<int>(std::min(sinks, kMaxKeys));
     a.scale = scaling * 1.44269504088896340736f;  // exp(x) = exp2(x log2(e))
-    if (dtype == NQ_F16) launch_shared<F16>(a, head_dim, as_stream(stream));
-    else launch_shared<BF16>(a, head_dim, as_stream(stream));
+    char* ws = static_cast<char*>(workspace);
+    hipStream_t st = as_stream(stream);
+    if (dtype == NQ_F16) {
+        if (head_dim == 64) launch_shared<F16, 64>(a, plan, ws, st);
+        else launch_shared<F16, 128>(a, plan, ws, st);
+    } else {
+        if (head_dim == 64) launch_shared<BF16, 64>(a, plan, ws, st);
+        else launch_shared<BF16, 128>(a, plan, ws, st);
+    }
     return check_launch(name);
 }
 
