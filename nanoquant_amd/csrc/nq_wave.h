@@ -35,6 +35,18 @@ __device__ inline int least_of(int v) {
 template <int kLanes>
 __device__ inline int largest_of(int v) { return ~least_of<kLanes>(~v); }
 
+// Largest over the wave, the same in all of it.
+__device__ inline float wave_max(float v) {
+    auto larger = [](float x, int y) { return fmaxf(x, __builtin_bit_cast(float, y)); };
+    v = larger(v, dpp_or_own<0x111>(__builtin_bit_cast(int, v)));
+    v = larger(v, dpp_or_own<0x112>(__builtin_bit_cast(int, v)));
+    v = larger(v, dpp_or_own<0x114>(__builtin_bit_cast(int, v)));
+    v = larger(v, dpp_or_own<0x118>(__builtin_bit_cast(int, v)));
+    v = larger(v, dpp_or_own<0x142>(__builtin_bit_cast(int, v)));
+    v = larger(v, dpp_or_own<0x143>(__builtin_bit_cast(int, v)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // u of the lane that a DPP control names, 0 where there is none or the row is masked out.
 template <int kControl, int kRows>
 __device__ inline uint64_t dpp(uint64_t u) {
