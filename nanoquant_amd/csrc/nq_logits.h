@@ -12,6 +12,7 @@ struct F32 {};
 template <typename T>
 struct Elem {
     static constexpr int N = 8;
+    static constexpr uint32_t kNone = T::ONE_PAIR == 0x3C003C00u ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
     __device__ static float get(const void* p, int64_t i) { return T::to_float(static_cast<const uint16_t*>(p)[i]); }
     __device__ static void unpack(const u32x4& v, float* x) {
 #pragma unroll
@@ -21,6 +22,7 @@ struct Elem {
 template <>
 struct Elem<F32> {
     static constexpr int N = 4;
+    static constexpr uint32_t kNone = 0xFF800000u;
     __device__ static float get(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
     __device__ static void unpack(const u32x4& v, float* x) {
 #pragma unroll
@@ -54,11 +56,27 @@ struct LogitRow {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) v[i] = pieces[min((k * kPieces + i) * kThreads + static_cast<int>(threadIdx.x), last)];
     }
+    __device__ bool at_edge(int k) const { return k == 0 || (k + 1) * (kBatch * kThreads) - lead > vocab; }
+    // Piece p of this thread's in part k with -inf for what lies outside the row
+    __device__ u32x4 cleared(int k, int p, u32x4 v) const {
+        constexpr int each = N / 4;  // logits of a word
+        const int first = element(k, N * p);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t keep = 0;
+#pragma unroll
+            for (int i = 0; i < each; ++i)
+                if (static_cast<unsigned>(first + each * w + i) < static_cast<unsigned>(vocab))
+                    keep |= (each == 1 ? 0xFFFFFFFFu : 0xFFFFu) << (16 * i);
+            v[w] = bit_select(keep, v[w], Elem<T>::kNone);
+        }
+        return v;
+    }
     // -inf for what lies outside the row
     __device__ void unpack(int k, const u32x4* v, float* x) const {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) Elem<T>::unpack(v[i], x + N * i);
-        if (k == 0 || (k + 1) * (kBatch * kThreads) - lead > vocab) {
+        if (at_edge(k)) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) x[i] = static_cast<unsigned>(element(k, i)) < static_cast<unsigned>(vocab) ? x[i] : -INFINITY;
         }

@@ -2,8 +2,8 @@
 //
 // All rows' chunks (32 or 16 logits a thread of a block, in the 16-bit types and in fp32) are one line of units, cut into equal
 // shares for the blocks. A block goes through its share once: sums of e = 2^d and e d, d = (x - ref) log2(e) / T, with each
-// wave's ref moved up to its largest logit wherever that is 8 octaves above it; and the `top` largest logits so far, as keys
-// that order them. A row that lies in one share is finished by its block, parts of others are joined by join_kernel.
+// wave's ref moved up to its largest logit wherever that is 8 octaves above it; and the `top` largest logits so far, each wave's
+// in its lanes. A row that lies in one share is finished by its block, parts of others are joined by join_kernel.
 #include <algorithm>
 #include <cmath>
 
@@ -16,35 +16,36 @@ namespace nq {
 namespace {
 
 constexpr int kCUs = 256;
-constexpr int kMaxTop = 64, kGroups = 64;  // of threads
-constexpr int kHeld = 2048;                // keys that a block holds
+constexpr int kMaxTop = 64;  // a wave's lanes
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// Keys that order logits as torch.argmax does: a NaN before everything, equal ones by their index. 0 is no key.
-__device__ inline uint64_t order_key(float x, int at) {
+// Keys that order logits as torch.argmax does: a NaN before everything, equal ones by their index. Below 2^32 is no key.
+__device__ inline uint32_t order_bits(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);  // -0 becomes 0
-    const uint32_t k = x != x ? 0xFFFFFFFFu : u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
-    return static_cast<uint64_t>(k) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(at));
+    return x != x ? 0xFFFFFFFFu : u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ inline float from_order_bits(uint32_t k) { return __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ inline uint64_t order_key(float x, int at) {
+    return static_cast<uint64_t>(order_bits(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(at));
+}
+__device__ inline bool is_key(uint64_t key) { return key >> 32 != 0; }
 __device__ inline int key_index(uint64_t key) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)); }
-__device__ inline float key_logit(uint64_t key) {  // -inf of no key
-    const uint32_t k = static_cast<uint32_t>(key >> 32);
-    return key == 0 ? -INFINITY : __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
-}
+__device__ inline float key_logit(uint64_t key) { return is_key(key) ? from_order_bits(static_cast<uint32_t>(key >> 32)) : -INFINITY; }
 
+// Of e = 2^d and e d, d = x scale - ref: what ref has of a rounding, all d have in common, and log p = x scale - ref - log2 s.
 struct Sums {
-    float ref, s, d;  // sum of e and of e d
+    float ref, s, d;
     // the same of two sets of logits; a set whose logits are all -inf has s = 0
-    __device__ void join(const Sums& o, float scale) {
+    __device__ void join(const Sums& o) {
         const float top = fmaxf(ref, o.ref);
-        move(top, scale);
+        move(top);
         Sums other = o;
-        other.move(top, scale);
+        other.move(top);
         s += other.s;
         d += other.d;
     }
-    __device__ void move(float to, float scale) {
-        const float by = (ref - to) * scale, f = __builtin_amdgcn_exp2f(by);
+    __device__ void move(float to) {
+        const float by = ref - to, f = __builtin_amdgcn_exp2f(by);
         if (s != 0.0f) {  // also where it is NaN
             d = f == 0.0f ? 0.0f : f * fmaf(by, s, d);
             s *= f;
@@ -52,6 +53,14 @@ struct Sums {
         ref = to;
     }
 };
+
+// Of all lanes' sums, the same in the whole wave.
+__device__ inline Sums joined(Sums sums) {
+    sums.move(wave_max(sums.ref));
+    sums.s = wave_add(sums.s);
+    sums.d = wave_add(sums.d);
+    return sums;
+}
 
 struct ScoreArgs {
     const void* logits;
@@ -62,13 +71,12 @@ struct ScoreArgs {
     float* entropy;
     int64_t* top_tokens;
     float* top_logprobs;
-    float scale;        // log2(e) / temperature
-    double per_degree;  // 1 / temperature
+    float scale;  // log2(e) / temperature
     int rows, vocab, top;
     int chunks;      // of a row
     int64_t share;   // chunks of a block
     int64_t units;   // of all rows
-    float4* sums;    // [blocks][2]: ref, s, d, 1 where the keys are not all there
+    float4* sums;    // [blocks][2]: ref, s, d
     uint64_t* keys;  // [blocks][2][top]
     __device__ int64_t first(int64_t row) const {  // element
         const int64_t b = row / rows;
@@ -76,20 +84,29 @@ struct ScoreArgs {
     }
 };
 
-// A row's results but for its alternatives; log p of a logit.
+// A row's given token and its logit, read before the row is.
 template <typename T>
-struct Scored {
-    float ref, log_sum;
-    double per_degree;
-    __device__ Scored(const ScoreArgs& a, const Sums& sums) : ref(sums.ref), log_sum(log2f(sums.s)), per_degree(a.per_degree) {}
-    // in fp64: the difference of two fp32 logits may be more than fp32 holds
-    __device__ float logprob(float x) const {
-        return static_cast<float>((static_cast<double>(x) - ref) * per_degree - static_cast<double>(kLn2) * log_sum);
-    }
-    __device__ void store(const ScoreArgs& a, int64_t row, const Sums& sums) const {  // one thread
+struct Given {
+    bool there = false;
+    float x = 0.0f;
+    __device__ Given(const ScoreArgs& a, int64_t row, bool wanted) {
+        if (!wanted) return;
         const int64_t b = row / a.rows, token = a.tokens[b * a.token_batch_stride + (row - b * a.rows) * a.token_stride];
-        const bool there = token >= 0 && token < a.vocab;
-        a.logprobs[row] = there ? logprob(Elem<T>::get(a.logits, a.first(row) + token)) : 0.0f;
+        there = token >= 0 && token < a.vocab;
+        if (there) x = Elem<T>::get(a.logits, a.first(row) + token);
+    }
+};
+
+// A row's results from its sums, whose ref is given apart: twice as wide where it has to be.
+struct Scored {
+    double scale, ref;
+    float log_sum;
+    __device__ Scored(const ScoreArgs& a, const Sums& sums, double ref_) : scale(a.scale), ref(ref_), log_sum(log2f(sums.s)) {}
+    // in fp64: x scale and ref may be large and nearly the same, and their difference more than fp32 holds
+    __device__ float logprob(float x) const { return static_cast<float>((x * scale - ref - log_sum) * 0.69314718055994530942); }
+    template <typename T>
+    __device__ void store(const ScoreArgs& a, int64_t row, const Sums& sums, const Given<T>& given) const {  // one thread
+        a.logprobs[row] = given.there ? logprob(given.x) : 0.0f;
         a.entropy[row] = kLn2 * (log_sum - sums.d / sums.s);
     }
     __device__ void store_top(const ScoreArgs& a, int64_t row, int k, uint64_t key) const {
@@ -114,9 +131,9 @@ __device__ inline uint64_t block_largest(uint64_t bound, int n, uint64_t* red, K
     return best;
 }
 
-// The alternatives of a row, one after the other: where there is a NaN, or more keys were met than a block holds.
+// The alternatives of a row, one after the other: where there is a NaN.
 template <typename T, int kThreads>
-__device__ inline void slow_top(const ScoreArgs& a, int64_t row, const Scored<T>& scored, uint64_t* red) {
+__device__ inline void slow_top(const ScoreArgs& a, int64_t row, const Scored& scored, uint64_t* red) {
     uint64_t key = ~uint64_t{0};
     const int64_t first = a.first(row);
     for (int k = 0; k < a.top; ++k) {
@@ -125,231 +142,280 @@ __device__ inline void slow_top(const ScoreArgs& a, int64_t row, const Scored<T>
     }
 }
 
-// The `top` largest keys among those held, sorted, and the last of them as a bound for what comes.
-struct Held {
-    uint64_t keys[kHeld], best[kMaxTop], group[kGroups];
-    uint64_t bound;  // keys below it are none of the largest; 0 at first
-    int count;
+// The `top` largest keys that a wave has met, the largest in lane 0, and a logit below which none is one of them.
+struct TopList {
+    uint64_t key = 0;
+    float least = -INFINITY;
+    __device__ void insert(uint64_t k, int top) {  // the same for the wave
+        const int place = __popcll(__ballot(key > k)), lane = threadIdx.x & 63;
+        if (place >= top) return;
+        const uint64_t before = dpp<0x138, 0xF>(key);  // wave_shr:1
+        key = lane < place ? key : lane == place ? k : before;
+        least = fmaxf(least, key_logit(read_lane(key, top - 1)));
+    }
+    // Each lane has the largest of some logits: at least the upper half of the top-th largest's bits, a bit at a time
+    __device__ void sharpen(float largest, int top) {
+        const uint32_t mine = order_bits(largest);
+        uint32_t bound = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t more = bound | 1u << bit;
+            bound = __popcll(__ballot(mine >= more)) >= top ? more : bound;
+        }
+        if (bound >= 0x00800000u) least = fmaxf(least, from_order_bits(bound));  // else -inf, or no number
+    }
 };
-template <int kThreads>
-__device__ inline void keep_largest(Held& held, int n, int top) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t key = held.keys[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += held.keys[j] > key ? 1 : 0;
-        if (rank < top) held.best[rank] = key;
+
+// A row's sums where logits times the scale are too large for fp32, and ref, the scaled largest logit.
+template <typename T, int kThreads>
+__device__ inline Sums slow_sums(const ScoreArgs& a, int64_t row, uint64_t* red, Sums* wave_sums, double& ref) {
+    const int64_t first = a.first(row);
+    auto at = [&](int i) { return Elem<T>::get(a.logits, first + i); };
+    const float most = key_logit(block_largest<kThreads>(~uint64_t{0}, a.vocab, red, [&](int i) { return order_key(at(i), i); }));
+    Sums sums{0.0f, 0.0f, 0.0f};
+    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
+        const float d = (at(i) - most) * a.scale, e = __builtin_amdgcn_exp2f(d);
+        sums.s += e;
+        sums.d = fmaf(e, fmaxf(d, -1000.0f), sums.d);
     }
+    sums.s = wave_add(sums.s);
+    sums.d = wave_add(sums.d);
     __syncthreads();
-    for (int i = threadIdx.x; i < min(n, top); i += kThreads) held.keys[i] = held.best[i];
-    if (threadIdx.x == 0) {
-        held.count = min(n, top);
-        if (n >= top) held.bound = held.best[top - 1];
-    }
+    if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = sums;
     __syncthreads();
+    sums = wave_sums[0];
+    for (int w = 1; w < kThreads / 64; ++w) sums.join(wave_sums[w]);
+    ref = static_cast<double>(most) * a.scale;
+    return sums;
 }
+// Beyond this what ref is rounded by moves the exponentials by an octave and more. Infinities too.
+__device__ inline bool leaves_fp32(const Sums& sums) { return fabsf(sums.ref) > 0x1p24f; }
 
 template <typename T, int kThreads>
-__global__ __launch_bounds__(kThreads, kThreads == 256 ? 5 : 4) void score_kernel(const ScoreArgs a) {
+__global__ __launch_bounds__(kThreads, kThreads == 256 ? 6 : 4) void score_kernel(const ScoreArgs a) {
     constexpr int N = Elem<T>::N, kBatch = 4 * N, kWaves = kThreads / 64;
     using Row = LogitRow<T, kThreads, kBatch>;
-    __shared__ Held held;
+    static_assert(Row::kPieces == 4, "a chunk is four pieces a thread");
+    __shared__ uint64_t keys[kWaves * kMaxTop];
+    __shared__ float lane_most[kWaves][64];
+    __shared__ int key_count[2];  // of this segment, of the next
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t red[kWaves];
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int64_t u = blockIdx.x * a.share;
     const int64_t end = min(u + a.share, a.units);
+    if (t == 0) key_count[0] = 0;
     for (int segment = 0; u < end; ++segment) {
         const int64_t at_row = u / a.chunks;
         const int c0 = static_cast<int>(u - at_row * a.chunks), c1 = static_cast<int>(min<int64_t>(a.chunks, c0 + end - u));
         u += c1 - c0;
+        const bool whole = c0 == 0 && c1 == a.chunks;
         const Row row(a.logits, a.first(at_row), a.vocab);
+        u32x4 next[4];
+        row.load(c0, next);
+        const Given<T> given(a, at_row, whole && t == 0);
         Sums sums{-INFINITY, 0.0f, 0.0f};
         float limit = -INFINITY;
-        bool spilled = false;
-        if (a.top) {
-            __syncthreads();  // the segment before has been read
-            if (t == 0) {
-                held.bound = 0;
-                held.count = 0;
-            }
-            __syncthreads();
-        }
-        int had = 0;  // keys held before this chunk
+        TopList list;
         for (int c = c0; c < c1; ++c) {
-            u32x4 v[Row::kPieces];
-            row.load(c, v);
-            float x[kBatch];
-            row.unpack(c, v, x);
-            float piece_most[Row::kPieces];
+            u32x4 v[4];
 #pragma unroll
-            for (int p = 0; p < Row::kPieces; ++p) {
-                piece_most[p] = x[N * p];
+            for (int p = 0; p < 4; ++p) v[p] = next[p];
+            if (c + 1 < c1) row.load(c + 1, next);
+            const bool edge = row.at_edge(c);
+            if (edge) {
 #pragma unroll
-                for (int i = 1; i < N; ++i) piece_most[p] = fmaxf(piece_most[p], x[N * p + i]);
+                for (int p = 0; p < 4; ++p) v[p] = row.cleared(c, p, v[p]);
             }
-            static_assert(Row::kPieces == 4, "a chunk is four pieces a thread");
+            // nothing unpacked is kept from here to there: what that would take in registers costs more than unpacking again
+            auto forget = [&] {
+#pragma unroll
+                for (int p = 0; p < 4; ++p) asm volatile("" : "+v"(v[p]));
+            };
+            float piece_most[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                float x[N];
+                Elem<T>::unpack(v[p], x);
+                piece_most[p] = x[0];
+#pragma unroll
+                for (int i = 1; i < N; ++i) piece_most[p] = fmaxf(piece_most[p], x[i]);
+            }
             const float most = fmaxf(fmaxf(piece_most[0], piece_most[1]), fmaxf(piece_most[2], piece_most[3]));
             if (__any(most > limit)) {
-                sums.move(wave_max(fmaxf(most, sums.ref)), a.scale);
-                limit = sums.ref + 8.0f / a.scale;
+                sums.move(fmaxf(wave_max(most) * a.scale, sums.ref));
+                limit = (sums.ref + 8.0f) / a.scale;
             }
             const float ref = sums.ref == -INFINITY ? 0.0f : sums.ref;
+            float s = 0.0f, d = NAN;
+            if (!edge) {
+                d = 0.0f;
+                forget();
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const float d = (x[i] - ref) * a.scale, e = __builtin_amdgcn_exp2f(d);
-                sums.s += e;
-                sums.d = fmaf(e, fmaxf(d, -1000.0f), sums.d);  // 0 of a logit of -inf
+                for (int p = 0; p < 4; ++p) {
+                    float x[N];
+                    Elem<T>::unpack(v[p], x);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float by = fmaf(x[i], a.scale, -ref), e = __builtin_amdgcn_exp2f(by);
+                        s += e;
+                        d = fmaf(e, by, d);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-            if (a.top == 0 || spilled) continue;
+            if (__any(d != d)) {  // a logit of -inf adds nothing, but 0 times it does
+                s = d = 0.0f;
+                forget();
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    float x[N];
+                    Elem<T>::unpack(v[p], x);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float by = fmaf(x[i], a.scale, -ref), e = __builtin_amdgcn_exp2f(by);
+                        s += e;
+                        d = fmaf(e, fmaxf(by, -1000.0f), d);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            sums.s += s;
+            sums.d += d;
+            if (a.top == 0) continue;
+            if (c == c0) {
+                // the block's lanes in 64 groups, one of each wave a group
+                lane_most[wave][lane] = most;
+                __syncthreads();
+                float x = lane_most[0][lane];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) x = fmaxf(x, lane_most[w][lane]);
+                list.sharpen(x, a.top);
+            }
+            const uint64_t some = __ballot(most >= list.least);
+            if (some == 0) continue;
+            if (c != c0 && __popcll(some) > 8) list.sharpen(most, a.top);  // as long as a few insertions
+            forget();
             // logit e of a piece, e known to nobody before: these parts run seldom, and unrolled their compares would take the
             // scalar registers of everything
-            auto pick = [&](const u32x4& w, int e) {
+            auto pick = [](u32x4 w, int e) {
                 const int word = 4 * e / N;
-                const uint32_t u = word & 2 ? (word & 1 ? w[3] : w[2]) : (word & 1 ? w[1] : w[0]);
-                if constexpr (N == 4) return __builtin_bit_cast(float, u);
-                else return T::to_float(static_cast<uint16_t>(u >> (16 * (e & 1))));
+                const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+                const uint32_t x = word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : w3;
+                if constexpr (N == 4) return __builtin_bit_cast(float, x);
+                else return T::to_float(static_cast<uint16_t>(x >> (16 * (e & 1))));
             };
-            auto inside = [&](int at) { return static_cast<unsigned>(at) < static_cast<unsigned>(a.vocab); };
-            // a bound from this chunk: the top-th largest of 64 groups of threads' largest
-            auto sharpen = [&] {
-                uint64_t key = 0;
-                const int p = piece_most[0] == most ? 0 : piece_most[1] == most ? 1 : piece_most[2] == most ? 2 : 3;
-                const u32x4 w = p & 2 ? (p & 1 ? v[3] : v[2]) : (p & 1 ? v[1] : v[0]);
-#pragma unroll 1
-                for (int e = 0; e < N; ++e) {
-                    const int at = row.element(c, N * p + e);
-                    if (pick(w, e) == most && inside(at) && key == 0) key = order_key(most, at);
-                }
 #pragma unroll
-                for (int off = 1; off < kThreads / kGroups; off <<= 1) {
-                    const uint64_t other = static_cast<uint64_t>(__shfl_xor(static_cast<long long>(key), off, 64));
-                    key = other > key ? other : key;
-                }
-                if (t % (kThreads / kGroups) == 0) held.group[t / (kThreads / kGroups)] = key;
-                __syncthreads();
-                if (t < kGroups) {
-                    key = held.group[t];
-                    int rank = 0;
-                    for (int j = 0; j < kGroups; ++j) rank += held.group[j] > key ? 1 : 0;
-                    if (rank == a.top - 1 && key > held.bound) held.bound = key;  // keys are different but for 0
-                }
-                __syncthreads();
-            };
-            auto hold = [&] {  // returns how many are held with this chunk's
-                const uint64_t bound = held.bound;
-                const float least = key_logit(bound);
-#pragma unroll
-                for (int p = 0; p < Row::kPieces; ++p) {
-                    if (!__any(piece_most[p] >= least)) continue;
+            for (int p = 0; p < 4; ++p) {
+                if (__any(piece_most[p] >= list.least)) {
+                    const u32x4 w = v[p];
+                    const int first = row.element(c, N * p);
 #pragma unroll 1
                     for (int e = 0; e < N; ++e) {
-                        const float y = pick(v[p], e);
-                        const int at = row.element(c, N * p + e);
-                        if (y >= least && inside(at) && order_key(y, at) >= bound) {
-                            const int place = atomicAdd(&held.count, 1);
-                            if (place < kHeld) held.keys[place] = order_key(y, at);
+                        const float y = pick(w, e);
+                        uint64_t todo = __ballot(y >= list.least);
+                        if (todo == 0) continue;
+                        const uint64_t key = order_key(y, first + e);
+                        todo &= __ballot(static_cast<unsigned>(first + e) < static_cast<unsigned>(a.vocab) && key > read_lane(list.key, a.top - 1));
+                        while (todo != 0) {
+                            list.insert(read_lane(key, __builtin_ctzll(todo)), a.top);
+                            todo &= todo - 1;
                         }
                     }
                 }
-                __syncthreads();
-                return held.count;
-            };
-            if (c == c0) sharpen();
-            int n = hold();
-            if (n > kHeld && c > c0) {
-                __syncthreads();
-                if (t == 0) held.count = had;
-                sharpen();
-                n = hold();
             }
-            spilled = n > kHeld;
-            if (!spilled && (c == c0 || c + 1 == c1 || n > 2 * a.top + 32)) {
-                keep_largest<kThreads>(held, n, a.top);
-                n = min(n, a.top);
-            }
-            had = n;
-            __syncthreads();
         }
-        // the block's sums
-        sums.s = wave_sum(sums.s);
-        sums.d = wave_sum(sums.d);
-        if ((t & 63) == 0) wave_sums[t >> 6] = sums;
+        // the waves' sums and lists
+        sums.s = wave_add(sums.s);
+        sums.d = wave_add(sums.d);
+        if (segment > 0 && a.top == 0) __syncthreads();  // the ones before have been read; with lists the first chunk saw to that
+        if (lane == 0) wave_sums[wave] = sums;
+        if (a.top) {
+            const int n = __popcll(__ballot(is_key(list.key)));  // the first n lanes'
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&key_count[segment & 1], n);
+            at = __builtin_amdgcn_readfirstlane(at);
+            if (lane < n) keys[at + lane] = list.key;
+        }
         __syncthreads();
-        Sums all = wave_sums[0];
-        for (int w = 1; w < kWaves; ++w) all.join(wave_sums[w], a.scale);
-        if (c0 == 0 && c1 == a.chunks) {
-            const Scored<T> scored(a, all);
-            if (t == 0) scored.store(a, at_row, all);
-            if (a.top == 0) {
-            } else if (spilled || all.s != all.s) {
-                slow_top<T, kThreads>(a, at_row, scored, red);
-            } else if (t < a.top) {
-                scored.store_top(a, at_row, t, held.keys[t]);
-            }
-        } else {
-            const int64_t part = static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0);
-            if (t == 0) a.sums[part] = float4{all.ref, all.s, all.d, spilled ? 1.0f : 0.0f};
-            if (t < a.top) a.keys[part * a.top + t] = !spilled && t < had ? held.keys[t] : 0;
+        if (t == 0) key_count[(segment + 1) & 1] = 0;
+        Sums all = joined(lane < kWaves ? wave_sums[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+        const int64_t part = static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0);
+        double ref = all.ref;
+        if (whole) {
+            if (leaves_fp32(all)) all = slow_sums<T, kThreads>(a, at_row, red, wave_sums, ref);
+        } else if (t == 0) {
+            a.sums[part] = float4{all.ref, all.s, all.d, 0.0f};
         }
-        __syncthreads();  // wave_sums
+        const Scored scored(a, all, ref);
+        if (whole && t == 0) scored.store(a, at_row, all, given);
+        if (whole && a.top && all.s != all.s) {
+            slow_top<T, kThreads>(a, at_row, scored, red);
+            continue;
+        }
+        if (a.top == 0) continue;
+        const int n = key_count[segment & 1];
+        for (int i = t; i < n; i += kThreads) {
+            const uint64_t key = keys[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) rank += keys[j] > key ? 1 : 0;
+            if (rank >= a.top) continue;
+            if (whole) scored.store_top(a, at_row, rank, key);
+            else a.keys[part * a.top + rank] = key;
+        }
+        if (!whole && n + t < a.top) a.keys[part * a.top + n + t] = 0;
     }
 }
 
 // A block a row: joins the parts that several blocks left of it.
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const ScoreArgs a) {
-    constexpr int kFew = 1024;
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads) void join_kernel(const ScoreArgs a) {
+    constexpr int kFew = kThreads * 4;
     __shared__ uint64_t keys[kFew];
-    __shared__ uint64_t red[4];
+    __shared__ uint64_t red[kThreads / 64];
+    __shared__ Sums wave_sums[kThreads / 64];
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x, first = row * a.chunks;
     const int64_t b0 = first / a.share, b1 = (first + a.chunks - 1) / a.share;
     if (b0 == b1) return;
-    const int n = static_cast<int>(b1 - b0) + 1;
+    const Given<T> given(a, row, t == 0);
+    const int n = static_cast<int>(b1 - b0) + 1, count = n * a.top;
     auto part = [&](int i) { return (b0 + i) * 2 + ((b0 + i) * a.share < first ? 1 : 0); };
+    auto key_of = [&](int i) { return a.keys[part(i / a.top) * a.top + i % a.top]; };
+    if (count <= kFew)
+        for (int i = t; i < count; i += kThreads) keys[i] = key_of(i);
     // every wave joins all the parts, a lane every 64th
     Sums all{-INFINITY, 0.0f, 0.0f};
-    bool lost = false;
     for (int i = t & 63; i < n; i += 64) {
         const float4 p = a.sums[part(i)];
-        all.join(Sums{p.x, p.y, p.z}, a.scale);
-        lost |= p.w != 0.0f;
+        all.join(Sums{p.x, p.y, p.z});
     }
-    for (int off = 1; off < 64; off <<= 1) {
-        // joined in the same order by both lanes
-        const Sums other{__shfl_xor(all.ref, off, 64), __shfl_xor(all.s, off, 64), __shfl_xor(all.d, off, 64)};
-        if (t & off) {
-            Sums low = other;
-            low.join(all, a.scale);
-            all = low;
-        } else {
-            all.join(other, a.scale);
-        }
-    }
-    const Scored<T> scored(a, all);
-    if (t == 0) scored.store(a, row, all);
+    all = joined(all);
+    double ref = all.ref;
+    if (leaves_fp32(all)) all = slow_sums<T, kThreads>(a, row, red, wave_sums, ref);
+    const Scored scored(a, all, ref);
+    if (t == 0) scored.store(a, row, all, given);
     if (a.top == 0) return;
-    if (__any(lost) || all.s != all.s) {
-        slow_top<T, 256>(a, row, scored, red);
+    if (all.s != all.s) {
+        slow_top<T, kThreads>(a, row, scored, red);
         return;
     }
-    const int count = n * a.top;
-    auto key_of = [&](int i) { return a.keys[part(i / a.top) * a.top + i % a.top]; };
     if (count > kFew) {
         uint64_t key = ~uint64_t{0};
         for (int k = 0; k < a.top; ++k) {
-            key = block_largest<256>(key, count, red, key_of);
+            key = block_largest<kThreads>(key, count, red, key_of);
             if (t == 0) scored.store_top(a, row, k, key);
         }
         return;
     }
-    for (int i = t; i < count; i += 256) keys[i] = key_of(i);
     __syncthreads();
-    for (int i = t; i < count; i += 256) {
+    for (int i = t; i < count; i += kThreads) {
         const uint64_t key = keys[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < count; ++j) rank += keys[j] > key ? 1 : 0;
-        if (key != 0 && rank < a.top) scored.store_top(a, row, rank, key);
+        if (is_key(key) && rank < a.top) scored.store_top(a, row, rank, key);
     }
 }
 
@@ -390,7 +456,11 @@ void launch_score(const ScoreArgs& a, const Plan& p, int64_t rows, hipStream_t s
     const dim3 grid(static_cast<unsigned>(p.blocks));
     if (p.wide) score_kernel<T, 1024><<<grid, 1024, 0, st>>>(a);
     else score_kernel<T, 256><<<grid, 256, 0, st>>>(a);
-    if (p.joined()) join_kernel<T><<<dim3(static_cast<unsigned>(rows)), 256, 0, st>>>(a);
+    if (!p.joined()) return;
+    // of few parts a wave a row
+    const dim3 all(static_cast<unsigned>(rows));
+    if ((ceil_div(p.chunks, p.share) + 1) * a.top <= 128) join_kernel<T, 64><<<all, 64, 0, st>>>(a);
+    else join_kernel<T, 256><<<all, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -438,7 +508,6 @@ int nq_token_logprobs(int dtype, const void* logits, int64_t batch_stride, int64
     a.top_tokens = top_tokens;
     a.top_logprobs = top_logprobs;
     a.scale = static_cast<float>(1.44269504088896340736 / temperature);
-    a.per_degree = 1.0 / temperature;
     a.rows = static_cast<int>(rows);
     a.vocab = static_cast<int>(vocab);
     a.top = static_cast<int>(top);

@@ -87,6 +87,17 @@ __device__ inline uint64_t wave_largest(uint64_t v) {
     v = larger(v, dpp<0x143, 0xC>(v));
     return read_lane(v, 63);
 }
+// Sum over the wave, the same in all of it.
+__device__ inline float wave_add(float v) {
+    auto add = [](float x, int y) { return x + __builtin_bit_cast(float, y); };
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x111, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x112, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x114, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x118, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x142, 0xA, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x143, 0xC, 0xF, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 __device__ inline double wave_total(double v) { return read_lane(wave_scan(v), 63); }
 
 }  // namespace nq
