@@ -56,7 +56,12 @@ struct LogitRow {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) v[i] = pieces[min((k * kPieces + i) * kThreads + static_cast<int>(threadIdx.x), last)];
     }
-    __device__ bool at_edge(int k) const { return k == 0 || (k + 1) * (kBatch * kThreads) - lead > vocab; }
+    __device__ void load_once(int k, u32x4* v) const {  // the same of what is not read again
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            v[i] = __builtin_nontemporal_load(pieces + min((k * kPieces + i) * kThreads + static_cast<int>(threadIdx.x), last));
+    }
+    __device__ bool at_edge(int k) const { return (k == 0 && lead > 0) || (k + 1) * (kBatch * kThreads) - lead > vocab; }
     // Piece p of this thread's in part k with -inf for what lies outside the row
     __device__ u32x4 cleared(int k, int p, u32x4 v) const {
         constexpr int each = N / 4;  // logits of a word

@@ -16,6 +16,7 @@ namespace nq {
 namespace {
 
 constexpr int kCUs = 256;
+constexpr int kPerCU = 5;    // blocks of 256 threads: registers for more would go to scratch
 constexpr int kMaxTop = 64;  // a wave's lanes
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -192,12 +193,12 @@ __device__ inline Sums slow_sums(const ScoreArgs& a, int64_t row, uint64_t* red,
 __device__ inline bool leaves_fp32(const Sums& sums) { return fabsf(sums.ref) > 0x1p24f; }
 
 template <typename T, int kThreads>
-__global__ __launch_bounds__(kThreads, kThreads == 256 ? 6 : 4) void score_kernel(const ScoreArgs a) {
+__global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_kernel(const ScoreArgs a) {
     constexpr int N = Elem<T>::N, kBatch = 4 * N, kWaves = kThreads / 64;
     using Row = LogitRow<T, kThreads, kBatch>;
     static_assert(Row::kPieces == 4, "a chunk is four pieces a thread");
     __shared__ uint64_t keys[kWaves * kMaxTop];
-    __shared__ float lane_most[kWaves][64];
+    __shared__ float lane_most[2][kWaves][64];
     __shared__ int key_count[2];  // of this segment, of the next
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t red[kWaves];
@@ -212,16 +213,18 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 6 : 4) void score_kerne
         const bool whole = c0 == 0 && c1 == a.chunks;
         const Row row(a.logits, a.first(at_row), a.vocab);
         u32x4 next[4];
-        row.load(c0, next);
+        row.load_once(c0, next);
         const Given<T> given(a, at_row, whole && t == 0);
         Sums sums{-INFINITY, 0.0f, 0.0f};
         float limit = -INFINITY;
         TopList list;
+        float most_yet = -INFINITY;
+        int turn = 0;
         for (int c = c0; c < c1; ++c) {
             u32x4 v[4];
 #pragma unroll
             for (int p = 0; p < 4; ++p) v[p] = next[p];
-            if (c + 1 < c1) row.load(c + 1, next);
+            if (c + 1 < c1) row.load_once(c + 1, next);
             const bool edge = row.at_edge(c);
             if (edge) {
 #pragma unroll
@@ -283,18 +286,19 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 6 : 4) void score_kerne
             sums.s += s;
             sums.d += d;
             if (a.top == 0) continue;
-            if (c == c0) {
-                // the block's lanes in 64 groups, one of each wave a group
-                lane_most[wave][lane] = most;
+            most_yet = fmaxf(most_yet, most);
+            if (((c - c0) & (c - c0 - 1)) == 0) {  // a bound from all waves, the block's lanes in 64 groups: chunks 0, 1, 2, 4, 8 ...
+                lane_most[turn][wave][lane] = most_yet;
                 __syncthreads();
-                float x = lane_most[0][lane];
+                float x = lane_most[turn][0][lane];
 #pragma unroll
-                for (int w = 1; w < kWaves; ++w) x = fmaxf(x, lane_most[w][lane]);
+                for (int w = 1; w < kWaves; ++w) x = fmaxf(x, lane_most[turn][w][lane]);
                 list.sharpen(x, a.top);
+                turn ^= 1;
             }
             const uint64_t some = __ballot(most >= list.least);
             if (some == 0) continue;
-            if (c != c0 && __popcll(some) > 8) list.sharpen(most, a.top);  // as long as a few insertions
+            if (__popcll(some) > 16) list.sharpen(most, a.top);  // which takes as long as a few insertions
             forget();
             // logit e of a piece, e known to nobody before: these parts run seldom, and unrolled their compares would take the
             // scalar registers of everything
@@ -430,13 +434,16 @@ struct Plan {
 
 Plan make_plan(int64_t rows, int64_t vocab, int64_t top, int piece) {
     Plan p;
-    p.wide = rows < 128 && vocab >= 16384;
+    // Rows that leave CUs idle are cut up wide, a block a CU: 150 rows of 32000 9.1 us a block of 256 threads for 8192 logits, 7.0 a
+    // block of 1024 a row; 300 rows 9.0 and 12.3. (fp16 without alternatives)
+    p.wide = rows <= kCUs && vocab >= 16384;
     const int64_t chunk = (p.wide ? 1024 : 256) * 4 * piece;
     p.chunks = ceil_div(vocab + piece - 1, chunk);
     const int64_t units = rows * p.chunks;
-    if (p.wide) p.share = p.chunks <= 2 ? p.chunks : ceil_div(units, 2 * kCUs);
-    else if (rows >= kCUs && rows <= 8 * kCUs) p.share = p.chunks;
-    else p.share = ceil_div(units, 8 * kCUs);
+    // Whole rows need no second launch to join their parts, 5 us
+    if (p.wide) p.share = p.chunks <= 2 ? p.chunks : ceil_div(units, kCUs);
+    else if (rows >= kCUs && rows <= kPerCU * kCUs) p.share = p.chunks;
+    else p.share = ceil_div(units, kPerCU * kCUs);
     p.blocks = ceil_div(units, p.share);
     p.sums = static_cast<size_t>(p.blocks) * 2 * sizeof(float4);
     p.bytes = p.joined() ? p.sums + static_cast<size_t>(p.blocks) * 2 * top * sizeof(uint64_t) : 16;
