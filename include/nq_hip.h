@@ -478,8 +478,8 @@ int nq_verify_drafts(int dtype, const void* logits, int64_t row_stride, const in
  *             equal ones, and their log p. Not touched where top is 0.
  * In a row with a NaN, or whose largest logit is infinite, log p and the entropy are NaN and NaNs are the largest logits.
  * Exponentials and sums in fp32. Every logit is read once where none is NaN.
- *   workspace nq_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one must
- *             not overlap.
+ *   workspace nq_token_logprobs_workspace_bytes(...) bytes (none where rows are not cut up), 16-byte aligned, no initial
+ *             contents; calls that share one must not overlap.
  * vocab <= 2^30, top <= 64 and <= vocab, fewer than 2^23 rows, temperature from 2^-64 to 2^64, else NQ_ERR_UNSUPPORTED. Tensors
  * aligned to their elements. The reference has no kernel of this kind. */
 size_t nq_token_logprobs_workspace_bytes(int64_t batch, int64_t rows, int64_t vocab, int64_t top);

@@ -446,11 +446,11 @@ Plan make_plan(int64_t rows, int64_t vocab, int64_t top, int piece) {
     else p.share = ceil_div(units, kPerCU * kCUs);
     p.blocks = ceil_div(units, p.share);
     p.sums = static_cast<size_t>(p.blocks) * 2 * sizeof(float4);
-    p.bytes = p.joined() ? p.sums + static_cast<size_t>(p.blocks) * 2 * top * sizeof(uint64_t) : 16;
+    p.bytes = p.joined() ? p.sums + static_cast<size_t>(p.blocks) * 2 * top * sizeof(uint64_t) : 0;
     return p;
 }
 
-// A call's plan; no bytes where there is none. The pieces of fp32 rows are shorter: whatever the type, it is given theirs.
+// A call's plan; no blocks where there is none.
 Plan plan_of(int64_t batch, int64_t rows, int64_t vocab, int64_t top, int piece) {
     if (batch <= 0 || rows <= 0 || vocab <= 0 || top < 0 || top > vocab || vocab > kMaxVocab || top > kMaxTop ||
         rows > kMaxThreads / 256 / batch)
@@ -501,7 +501,7 @@ int nq_token_logprobs(int dtype, const void* logits, int64_t batch_stride, int64
         return fail(NQ_ERR_ALIGNMENT, "%s: tensors must be aligned to their elements", name);
     const Plan plan = plan_of(batch, rows, vocab, top, dtype == NQ_F32 ? Elem<F32>::N : Elem<F16>::N);
     if (!aligned(workspace, 16)) return fail(NQ_ERR_ALIGNMENT, "%s: the workspace must be 16-byte aligned", name);
-    if (!workspace || workspace_bytes < plan.bytes)
+    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
         return fail(NQ_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", name, workspace ? workspace_bytes : size_t{0}, plan.bytes);
     ScoreArgs a{};
     a.logits = logits;

@@ -301,19 +301,18 @@ std::vector<Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, i
         (B > 1 && batch < V) || top < 0 || top > V)
         return {};
     const size_t bytes = lib->logprobs_bytes(B, R, V, top);
-    if (bytes == 0) return {};
     const c10::DeviceGuard guard(logits.device());
     const auto shape = tokens.sizes();
     std::vector<int64_t> wide = shape.vec();
     wide.push_back(top);
     Tensor logprobs = at::empty(shape, logits.options().dtype(at::kFloat)), entropy = at::empty_like(logprobs);
     Tensor top_tokens = at::empty(wide, tokens.options()), top_logprobs = at::empty(wide, logprobs.options());
-    const Tensor ws = scratch(bytes, logits);
+    const Tensor ws = bytes ? scratch(bytes, logits) : Tensor();
     if (lib->logprobs(type == at::kFloat ? NQ_F32 : dtype_code(type), logits.const_data_ptr(), batch, row,
                       static_cast<const int64_t*>(tokens.const_data_ptr()), dims == 2 ? tokens.stride(0) : 0,
                       tokens.stride(dims - 1), temperature, top, static_cast<float*>(logprobs.mutable_data_ptr()),
                       static_cast<float*>(entropy.mutable_data_ptr()), static_cast<int64_t*>(top_tokens.mutable_data_ptr()),
-                      static_cast<float*>(top_logprobs.mutable_data_ptr()), B, R, V, ws.mutable_data_ptr(), bytes,
+                      static_cast<float*>(top_logprobs.mutable_data_ptr()), B, R, V, bytes ? ws.mutable_data_ptr() : nullptr, bytes,
                       stream_of(logits)) != NQ_OK)
         return {};
     return {logprobs, entropy, top_tokens, top_logprobs};

@@ -31,7 +31,7 @@ import sys
 import torch
 
 from . import _lib
-from ._dispatch import launch as _launch, only_eager as _only_eager
+from ._dispatch import launch as _launch, only_eager as _only_eager, only_eager_many as _only_eager_many
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -496,7 +496,7 @@ def copy_pages(pools, source, target) -> None:
     there (-1) is passed over. No page may be the target of two pairs, or the target of one and the source of another."""
     what = "copy_pages"
     pools = list(pools)
-    eager = _only_eager(*pools, source, target)
+    eager = _only_eager_many(pools, source, target)
     if _native_copy is not None and eager and source.is_cuda and _native_copy(pools, source, target):
         return
     if source.dim() != 1 or target.shape != source.shape:
@@ -669,7 +669,7 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
         raise ValueError(f"{what}: the temperature must be a finite number above 0, got {temperature}")
     shape, kind = tokens.shape, torch.promote_types(logits.dtype, torch.float32)
     usual = _TEMPERATURES[0] <= temperature <= _TEMPERATURES[1]
-    if (logits.is_cuda and kind == torch.float32 and top <= 64 and V <= 1 << 30 and usual and tokens.numel()
+    if (logits.is_cuda and kind == torch.float32 and top <= 64 and V <= 1 << 30 and usual and 0 < tokens.numel() < 1 << 23
             and _only_eager(logits, tokens)):
         rows = logits if logits.dim() == 3 else logits.unsqueeze(0)
         B, T = rows.shape[:2]
@@ -678,16 +678,15 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
         at = tokens if tokens.dim() == 2 else tokens.unsqueeze(0)
         lib = _lib.load()
         nbytes = lib.nq_token_logprobs_workspace_bytes(B, T, V, top)
-        if nbytes:
-            logprobs, entropy = torch.empty(2, *shape, dtype=kind, device=logits.device).unbind(0)
-            top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=logits.device)
-            top_logprobs = torch.empty(*shape, top, dtype=kind, device=logits.device)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-            code = _lib.NQ_F32 if logits.dtype == torch.float32 else _lib.dtype_code(logits.dtype)
-            _launch(what, lib.nq_token_logprobs, logits, code, rows.data_ptr(), rows.stride(0), rows.stride(1), at.data_ptr(),
-                    at.stride(0), at.stride(1), temperature, top, logprobs.data_ptr(), entropy.data_ptr(),
-                    top_tokens.data_ptr(), top_logprobs.data_ptr(), B, T, V, ws.data_ptr(), nbytes)
-            return logprobs, entropy, top_tokens, top_logprobs
+        logprobs, entropy = torch.empty(2, *shape, dtype=kind, device=logits.device).unbind(0)
+        top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=logits.device)
+        top_logprobs = torch.empty(*shape, top, dtype=kind, device=logits.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        code = _lib.NQ_F32 if logits.dtype == torch.float32 else _lib.dtype_code(logits.dtype)
+        _launch(what, lib.nq_token_logprobs, logits, code, rows.data_ptr(), rows.stride(0), rows.stride(1), at.data_ptr(),
+                at.stride(0), at.stride(1), temperature, top, logprobs.data_ptr(), entropy.data_ptr(), top_tokens.data_ptr(),
+                top_logprobs.data_ptr(), B, T, V, _lib.ptr(ws), nbytes)
+        return logprobs, entropy, top_tokens, top_logprobs
     x = logits.to(kind if usual else torch.float64)
     d = (x - x.detach().amax(dim=-1, keepdim=True)) / temperature
     e = torch.exp(d)
