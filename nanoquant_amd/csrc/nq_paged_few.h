@@ -50,12 +50,24 @@ struct GroupArgs : PagedArgs {
     const int32_t* members;  // [sharing][most]
     const int32_t* shared;   // [sharing]: pages in common
     int sharing, most;       // groups, and places of one
-    int group_rows;          // row groups of a group; row_groups and rows_kept are a sequence's
-    int group_kept;          // rows of one that there are
-    int* place;              // [batch]: out, where a sequence stands in `members`; -1: nowhere
+    // Of a group's entries and of the sequences': row groups (a sequence's are row_groups), rows of one, and those that there
+    // are. Each entry's first part has a place of its own among the workspace's parts, the later ones their block's.
+    int group_rows, group_tile, group_kept, own_tile;  // rows_kept: a sequence's
+    int64_t own_first, group_later, own_later;         // rows
+    bool apart;              // groups' entries are another launch's, which has left `place`
+    int* place;              // [batch]: where a sequence stands in `members`; -1: nowhere
     __device__ int entries_of_groups() const { return sharing * group_rows; }
     // the keys that the members of place's group share
     __device__ int end_of(int at) const { return min(max(shared[at / most], 0), pages.table_pages) * pages.page_size; }
+    __device__ int64_t first_part(int entry, int kvh) const {
+        const int own = entry - entries_of_groups();
+        if (own < 0) return (static_cast<int64_t>(entry) * kv_heads + kvh) * group_kept;
+        return own_first + (static_cast<int64_t>(own) * kv_heads + kvh) * rows_kept;
+    }
+    __device__ int64_t later_part(int entry, int block) const {
+        const bool of_group = entry < entries_of_groups();
+        return (of_group ? group_later : own_later) + static_cast<int64_t>(block) * (of_group ? group_tile : own_tile);
+    }
 };
 
 // A position that the table holds, -1 for any other.
@@ -109,10 +121,8 @@ __device__ inline Tiles tiles_within(const PagedArgs& a, int lo, int hi, int fro
 }
 
 // Row groups of `group` rows (token t, query head g of a kv head's G: row t G + g); entry = (sequence, row group).
-__device__ inline int2 span_of_few(const PagedArgs& a, int entry, int group) {  // the least and the largest position
-    const int b = entry / a.row_groups;
-    const int first = (entry - b * a.row_groups) * group;
-    const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + group - 1) / a.groups);
+__device__ inline int2 span_of_few(const PagedArgs& a, int b, int first, int rows) {  // the least and the largest position
+    const int t0 = first / a.groups, t1 = min(a.tokens - 1, (first + rows - 1) / a.groups);
     int lo = INT32_MAX, hi = -1;
     for (int t = t0; t <= t1; t += 8) {
         int p[8];
@@ -127,7 +137,8 @@ __device__ inline int2 span_of_few(const PagedArgs& a, int entry, int group) {  
     return int2{lo, hi};
 }
 __device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
-    const int2 span = span_of_few(a, entry, group);
+    const int b = entry / a.row_groups;
+    const int2 span = span_of_few(a, b, (entry - b * a.row_groups) * group, group);
     return tiles_between<kTile>(a, span.x, span.y);
 }
 
@@ -138,10 +149,10 @@ struct GroupPlan {
     int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found, INT32_MAX: nobody
     int2 spans[kEntries];
 };
-// Entries' positions, members' and shared pages' among them; `rows` of a row group. All threads of the block.
-template <int kThreads, int kEntries>
+// All threads of the block; `rows` of a row group. kOwn: the sequences' entries as well, behind the groups'.
+template <int kThreads, int kEntries, bool kOwn = false>
 __device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntries>& plan) {
-    const int t = threadIdx.x, first = a.entries_of_groups(), own = a.batch * a.row_groups, each = a.tokens * a.groups;
+    const int t = threadIdx.x, first = a.entries_of_groups(), each = a.tokens * a.groups;
     for (int b = t; b < a.batch; b += kThreads) plan.place[b] = -1;
     for (int e = t; e < first; e += kThreads) {
         plan.spans[e] = int2{INT32_MAX, -1};
@@ -153,14 +164,18 @@ __device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntr
         if (b >= 0 && b < a.batch && a.shared[at / a.most] > 0) atomicMax(&plan.place[b], at);
     }
     __syncthreads();
-    for (int e = t; e < own; e += kThreads) {
-        const int b = e / a.row_groups, at = plan.place[b];
-        const int2 span = span_of_few(a, e, rows);
-        plan.spans[first + e] = span;
-        plan.lead[first + e] = b;
+    const int own = (each + rows - 1) / rows;  // row groups of a sequence
+    for (int e = t; e < a.batch * own; e += kThreads) {
+        const int b = e / own, at = plan.place[b];
+        if (!kOwn && at < 0) continue;
+        const int row = (e - b * own) * rows;
+        const int2 span = span_of_few(a, b, row, min(rows, each - row));
+        if constexpr (kOwn) {
+            plan.spans[first + e] = span;
+            plan.lead[first + e] = b;
+        }
         if (at < 0) continue;
-        const int g = at / a.most, row0 = (at - g * a.most) * each + (e - b * a.row_groups) * rows;
-        const int row1 = min(row0 + rows, (at - g * a.most + 1) * each) - 1;
+        const int g = at / a.most, row0 = (at - g * a.most) * each + row, row1 = min(row0 + rows, (at - g * a.most + 1) * each) - 1;
         for (int i = row0 / rows; i <= row1 / rows; ++i) {
             atomicMin(&plan.spans[g * a.group_rows + i].x, span.x);
             atomicMax(&plan.spans[g * a.group_rows + i].y, span.y);
@@ -170,6 +185,18 @@ __device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntr
     __syncthreads();
     if (blockIdx.x == 0)
         for (int b = t; b < a.batch; b += kThreads) a.place[b] = plan.place[b];
+}
+// The sequences' entries alone, where another launch has left their places.
+template <int kThreads, int kEntries>
+__device__ inline void plan_own(const GroupArgs& a, int rows, GroupPlan<kEntries>& plan) {
+    const int each = a.tokens * a.groups;
+    for (int b = threadIdx.x; b < a.batch; b += kThreads) plan.place[b] = a.place[b];
+    for (int e = threadIdx.x; e < a.batch * a.row_groups; e += kThreads) {
+        const int b = e / a.row_groups, row = (e - b * a.row_groups) * rows;
+        plan.spans[e] = span_of_few(a, b, row, min(rows, each - row));
+        plan.lead[e] = b;
+    }
+    __syncthreads();
 }
 
 // Which keys of a tile a row sees, a bit a key: arithmetic on words, since compares of every key with every row would each
@@ -252,17 +279,6 @@ __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least,
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-// Where an entry's parts lie in the workspace of a launch with groups, in rows: the first, then those of the blocks behind.
-__device__ inline int64_t first_part(const GroupArgs& a, int entry, int kvh) {
-    const int of_groups = a.entries_of_groups(), own = entry - of_groups;
-    if (own < 0) return (static_cast<int64_t>(entry) * a.kv_heads + kvh) * a.group_kept;
-    return static_cast<int64_t>(of_groups) * a.kv_heads * a.group_kept + (static_cast<int64_t>(own) * a.kv_heads + kvh) * a.rows_kept;
-}
-__device__ inline int64_t later_part(const GroupArgs& a, int block, int rows) {
-    const int64_t all = static_cast<int64_t>(a.entries_of_groups()) * a.group_kept + static_cast<int64_t>(a.batch) * a.row_groups * a.rows_kept;
-    return all * a.kv_heads + static_cast<int64_t>(block) * rows;
-}
-
 // Rows row0 on of an entry's row group, of which `rows` there are: where a row's query lies, and which keys it sees.
 struct RowAt {
     int64_t q_row;  // (sequence, token)
@@ -394,20 +410,25 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     const int c = lane & 15, g = lane >> 4;
     if (t < 2) s_tainted[t] = 0;
     Shares shares{};
-    int entry;
+    int entry, of_groups = 0;  // entries, which come first
     int64_t u = 0;
     if constexpr (kShared) {
         int entries = a.batch * a.row_groups;
         if constexpr (kGroups) {
-            plan_groups<64 * kWaves>(a, 16 * RT, plan);
-            entries += a.entries_of_groups();
+            if (a.apart) {
+                plan_own<64 * kWaves>(a, 16 * RT, plan);
+            } else {
+                plan_groups<64 * kWaves, kEntries, true>(a, 16 * RT, plan);
+                of_groups = a.entries_of_groups();
+            }
+            entries += of_groups;
         }
         shares = make_shares<64 * kWaves, Shape::kBlocks>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
             Tiles r;
             if constexpr (kGroups) {
                 if (plan.lead[e] == INT32_MAX) return 0;  // nobody's
-                const int g = e / a.group_rows, at = e < a.entries_of_groups() ? -1 : plan.place[plan.lead[e]];
-                const int from = at < 0 ? 0 : a.end_of(at), to = e < a.entries_of_groups() ? a.end_of(g * a.most) : INT32_MAX;
+                const int at = e < of_groups ? -1 : plan.place[plan.lead[e]];
+                const int from = at < 0 ? 0 : a.end_of(at), to = e < of_groups ? a.end_of(e / a.group_rows * a.most) : INT32_MAX;
                 r = tiles_within<kTile>(a, spans[e].x, spans[e].y, from, to);
             } else {
                 r = tiles_of_few(a, e, 16 * RT);
@@ -431,7 +452,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         voff[j] = static_cast<uint32_t>(row * D * 2 + 16 * ((lane % C) ^ (swz & (C - 1))));
     }
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(&ring[wave][0][0][0]));
-    int slot = 0, turn = 0;
+    int slot = 0, turn = 0, all_of_groups = 0;
+    if constexpr (kGroups) all_of_groups = a.entries_of_groups();
     while (true) {
         int kvh, first = 0, n, units = 0;
         Rows<Args> rows{};
@@ -450,7 +472,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             if constexpr (kGroups) {
                 rows.place = plan.place;
                 rows.b = __builtin_amdgcn_readfirstlane(plan.lead[entry]);
-                if (entry < a.entries_of_groups()) {
+                if (entry < of_groups) {
                     rows.group = entry / a.group_rows;
                     rows.to = __builtin_amdgcn_readfirstlane(a.end_of(rows.group * a.most));
                 } else {
@@ -468,7 +490,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         const int count = tiles.count;
         if constexpr (kGroups) {
             const bool of_group = rows.group >= 0;
-            const int e = of_group ? entry : entry - a.entries_of_groups(), many = of_group ? a.group_rows : a.row_groups;
+            const int e = of_group ? entry : entry - of_groups, many = of_group ? a.group_rows : a.row_groups;
             rows.row0 = (e - e / many * many) * (16 * RT);
             rows.rows = min(16 * RT, (of_group ? a.most : 1) * a.tokens * a.groups - rows.row0);
         } else {
@@ -696,8 +718,9 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
 
         // the waves' sums, joined through the rings a row group at a time
         const bool done = !kGroups && first == 0 && n == count;
+        const int listed = kGroups ? entry - of_groups + all_of_groups : entry;  // among the entries of all launches
         int64_t part;
-        if constexpr (kGroups) part = first == 0 ? first_part(a, entry, kvh) : later_part(a, static_cast<int>(blockIdx.x), 16 * RT);
+        if constexpr (kGroups) part = first == 0 ? a.first_part(listed, kvh) : a.later_part(listed, static_cast<int>(blockIdx.x));
         else part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept;
         float* red = reinterpret_cast<float*>(&ring[0][0][0][0]);
         __syncthreads();
@@ -748,7 +771,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         }
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
-            a.desc[entry * a.kv_heads + kvh] =
+            a.desc[listed * a.kv_heads + kvh] =
                 int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + units - 1) / shares.share)};
         if (u >= shares.end) return;
         slot = 1;  // a share's first and last (entry, kv head) are the ones that it may not finish

@@ -4,6 +4,7 @@
 
 #include "nq_common.h"
 #include "nq_paged_few.h"
+#include "nq_paged_rows.h"
 
 namespace nq {
 namespace {
@@ -11,7 +12,7 @@ namespace {
 // Adds up what few_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave a row, D / 4 lanes a
 // part.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int rows, int64_t count) {
+__global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int64_t count) {
     constexpr int L4 = D / 4, Groups = 64 / L4, kAhead = 4;
     const int lane = threadIdx.x & 63;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);  // (sequence, token, head)
@@ -23,18 +24,19 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int 
     const int at = a.place[b];
     struct Parts {
         int64_t first, later;  // rows of the first part and, were it one of the later ones, of the first block's
-        int n;
+        int n, step;
     };
     auto parts_of = [&](int entry, int in_entry) {
         const int2 d = a.desc[entry * a.kv_heads + kvh];
-        return Parts{first_part(a, entry, kvh) + in_entry, later_part(a, d.x >> 1, rows) + in_entry, d.y - (d.x >> 1) + 1};
+        return Parts{a.first_part(entry, kvh) + in_entry, a.later_part(entry, d.x >> 1) + in_entry, d.y - (d.x >> 1) + 1,
+                     entry < a.entries_of_groups() ? a.group_tile : a.own_tile};
     };
-    Parts common{0, 0, 0};
+    Parts common{0, 0, 0, 0};
     if (at >= 0) {
         const int g = at / a.most, in_group = (at - g * a.most) * a.tokens * a.groups + r;
-        common = parts_of(g * a.group_rows + in_group / rows, in_group % rows);
+        common = parts_of(g * a.group_rows + in_group / a.group_tile, in_group % a.group_tile);
     }
-    const Parts own = parts_of(a.entries_of_groups() + b * a.row_groups + r / rows, r % rows);
+    const Parts own = parts_of(a.entries_of_groups() + b * a.row_groups + r / a.own_tile, r % a.own_tile);
     const int n = common.n + own.n, grp = lane / L4, d0 = 4 * (lane % L4);
     float M = -INFINITY, L = 0.0f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -47,7 +49,7 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int 
             const bool of_common = part < common.n;
             const int k = of_common ? part : part - common.n;
             const int64_t from = k == 0 ? (of_common ? common.first : own.first)
-                                        : (of_common ? common.later : own.later) + static_cast<int64_t>(k) * rows;
+                                        : (of_common ? common.later : own.later) + static_cast<int64_t>(k) * (of_common ? common.step : own.step);
             ml[i] = a.part_ml[from];
             x[i] = *reinterpret_cast<const f32x4*>(a.part_o + from * D + d0);
         }
@@ -82,30 +84,44 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int 
     if (grp == 0) *reinterpret_cast<uint2*>(a.out + row * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
-// Row tiles of a launch, its list of work and what it needs of the workspace; tiles 0: more than a launch lists.
+// What a call's launches list, and what they need of the workspace; tiles 0: more than they list.
 struct Plan {
-    int tiles = 0;  // of 16 rows
-    int64_t group_rows, row_groups, group_kept, rows_kept;
+    int tiles = 0;   // of 16 rows a wave of few_kernel
+    int many = 0;    // of 32 rows a wave of rows_kernel, which then takes the groups; 0: few_kernel takes them too
+    int64_t group_rows, row_groups, group_tile, own_tile, group_kept, rows_kept;
+    int64_t own_first, group_later, own_later;  // rows of parts
     size_t part_o, part_ml, desc, place, bytes;
 };
 
 Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t sharing, int64_t most) {
     Plan p{};
     const int64_t each = tokens * groups, together = most * each;
-    const int tiles = together <= 16 ? 1 : together <= 32 ? 2 : 4;
-    p.group_rows = ceil_div(together, 16 * tiles);
-    p.row_groups = ceil_div(each, 16 * tiles);
-    p.group_kept = std::min<int64_t>(together, 16 * tiles);
-    p.rows_kept = std::min<int64_t>(each, 16 * tiles);
+    auto tiles_of = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
+    int many = 0, tiles = tiles_of(together);
+    if (together > 64) {
+        // two row tiles a wave where the rows fill them, as for a sequence of many rows
+        many = 2 * ceil_div(together, 256) * 15 <= ceil_div(together, 128) * 16 ? 2 : 1;
+        tiles = tiles_of(each);
+    }
+    p.own_tile = 16 * tiles;
+    p.group_tile = many ? 128 * many : p.own_tile;
+    p.group_rows = ceil_div(together, p.group_tile);
+    p.row_groups = ceil_div(each, p.own_tile);
+    p.group_kept = std::min(together, p.group_tile);
+    p.rows_kept = std::min(each, p.own_tile);
     const bool wide = tiles > 2 && head_dim == 128;
-    const int64_t entries = sharing * p.group_rows + batch * p.row_groups;
-    if (entries > (wide ? 2 : 1) * kFewEntries) return p;
-    const int64_t parts = kv_heads * (sharing * p.group_rows * p.group_kept + batch * p.row_groups * p.rows_kept) +
-                          static_cast<int64_t>(wide ? 1 : 2) * kCUs * 16 * tiles;
+    const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups, listed = (wide ? 2 : 1) * kFewEntries;
+    if (many ? of_groups > kEntries || own > listed : of_groups + own > listed) return p;
+    const int64_t blocks = wide ? kCUs : 2 * kCUs;
+    p.own_first = kv_heads * of_groups * p.group_kept;
+    p.own_later = p.own_first + kv_heads * own * p.rows_kept;
+    p.group_later = many ? p.own_later + blocks * p.own_tile : p.own_later;
+    const int64_t parts = p.group_later + (many ? kCUs : blocks) * p.group_tile;
     p.tiles = tiles;
+    p.many = many;
     p.part_o = static_cast<size_t>(parts * head_dim) * sizeof(float);
     p.part_ml = static_cast<size_t>(ceil_div(parts, 2) * 2) * sizeof(float2);
-    p.desc = static_cast<size_t>(ceil_div(entries * kv_heads, 2) * 2) * sizeof(int2);
+    p.desc = static_cast<size_t>(ceil_div((of_groups + own) * kv_heads, 2) * 2) * sizeof(int2);
     p.place = static_cast<size_t>(batch) * sizeof(int);
     p.bytes = p.part_o + p.part_ml + p.desc + p.place;
     return p;
@@ -116,16 +132,24 @@ void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
     a.row_groups = static_cast<int>(p.row_groups);
     a.rows_kept = static_cast<int>(p.rows_kept);
     a.group_rows = static_cast<int>(p.group_rows);
+    a.group_tile = static_cast<int>(p.group_tile);
     a.group_kept = static_cast<int>(p.group_kept);
+    a.own_tile = static_cast<int>(p.own_tile);
+    a.own_first = p.own_first;
+    a.group_later = p.group_later;
+    a.own_later = p.own_later;
+    a.apart = p.many > 0;
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + p.part_o);
     a.desc = reinterpret_cast<int2*>(ws + p.part_o + p.part_ml);
     a.place = reinterpret_cast<int*>(ws + p.part_o + p.part_ml + p.desc);
+    if (p.many == 1) rows_kernel<T, D, 1, true, GroupArgs><<<dim3(kCUs), 512, 0, st>>>(a);
+    else if (p.many == 2) rows_kernel<T, D, 2, true, GroupArgs><<<dim3(kCUs), 256, 0, st>>>(a);
     if (p.tiles == 1) few_kernel<T, D, 1, true, GroupArgs><<<dim3(FewShape<D, 1>::kBlocks), 64 * kWaves, 0, st>>>(a);
     else if (p.tiles == 2) few_kernel<T, D, 2, true, GroupArgs><<<dim3(FewShape<D, 2>::kBlocks), 64 * kWaves, 0, st>>>(a);
     else few_kernel<T, D, 4, true, GroupArgs><<<dim3(FewShape<D, 4>::kBlocks), 64 * kWaves, 0, st>>>(a);
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
-    group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, 16 * p.tiles, rows);
+    group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, rows);
 }
 
 // A call's plan; tiles 0 where there is none.
