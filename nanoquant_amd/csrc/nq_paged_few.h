@@ -54,7 +54,6 @@ struct GroupArgs : PagedArgs {
     // are. Each entry's first part has a place of its own among the workspace's parts, the later ones their block's.
     int group_rows, group_tile, group_kept, own_tile;  // rows_kept: a sequence's
     int64_t own_first, group_later, own_later;         // rows
-    bool apart;              // groups' entries are another launch's, which has left `place`
     int* place;              // [batch]: where a sequence stands in `members`; -1: nowhere
     __device__ int entries_of_groups() const { return sharing * group_rows; }
     // the keys that the members of place's group share
@@ -149,9 +148,9 @@ struct GroupPlan {
     int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found, INT32_MAX: nobody
     int2 spans[kEntries];
 };
-// All threads of the block; `rows` of a row group. kOwn: the sequences' entries as well, behind the groups'.
-template <int kThreads, int kEntries, bool kOwn = false>
-__device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntries>& plan) {
+// All threads of the block.
+template <int kThreads, int kEntries>
+__device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan) {
     const int t = threadIdx.x, first = a.entries_of_groups(), each = a.tokens * a.groups;
     for (int b = t; b < a.batch; b += kThreads) plan.place[b] = -1;
     for (int e = t; e < first; e += kThreads) {
@@ -164,19 +163,15 @@ __device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntr
         if (b >= 0 && b < a.batch && a.shared[at / a.most] > 0) atomicMax(&plan.place[b], at);
     }
     __syncthreads();
-    const int own = (each + rows - 1) / rows;  // row groups of a sequence
-    for (int e = t; e < a.batch * own; e += kThreads) {
-        const int b = e / own, at = plan.place[b];
-        if (!kOwn && at < 0) continue;
-        const int row = (e - b * own) * rows;
-        const int2 span = span_of_few(a, b, row, min(rows, each - row));
-        if constexpr (kOwn) {
-            plan.spans[first + e] = span;
-            plan.lead[first + e] = b;
-        }
+    for (int e = t; e < a.batch * a.row_groups; e += kThreads) {
+        const int b = e / a.row_groups, at = plan.place[b], row = (e - b * a.row_groups) * a.own_tile;
+        const int rows = min(a.own_tile, each - row);
+        const int2 span = span_of_few(a, b, row, rows);
+        plan.spans[first + e] = span;
+        plan.lead[first + e] = b;
         if (at < 0) continue;
-        const int g = at / a.most, row0 = (at - g * a.most) * each + row, row1 = min(row0 + rows, (at - g * a.most + 1) * each) - 1;
-        for (int i = row0 / rows; i <= row1 / rows; ++i) {
+        const int g = at / a.most, row0 = (at - g * a.most) * each + row;
+        for (int i = row0 / a.group_tile; i <= (row0 + rows - 1) / a.group_tile; ++i) {
             atomicMin(&plan.spans[g * a.group_rows + i].x, span.x);
             atomicMax(&plan.spans[g * a.group_rows + i].y, span.y);
             atomicMin(&plan.lead[g * a.group_rows + i], b);
@@ -186,17 +181,15 @@ __device__ inline void plan_groups(const GroupArgs& a, int rows, GroupPlan<kEntr
     if (blockIdx.x == 0)
         for (int b = t; b < a.batch; b += kThreads) a.place[b] = plan.place[b];
 }
-// The sequences' entries alone, where another launch has left their places.
-template <int kThreads, int kEntries>
-__device__ inline void plan_own(const GroupArgs& a, int rows, GroupPlan<kEntries>& plan) {
-    const int each = a.tokens * a.groups;
-    for (int b = threadIdx.x; b < a.batch; b += kThreads) plan.place[b] = a.place[b];
-    for (int e = threadIdx.x; e < a.batch * a.row_groups; e += kThreads) {
-        const int b = e / a.row_groups, row = (e - b * a.row_groups) * rows;
-        plan.spans[e] = span_of_few(a, b, row, min(rows, each - row));
-        plan.lead[e] = b;
-    }
-    __syncthreads();
+// The tiles of kKeys keys of an entry, whose span turns into their places. 0: nobody's
+template <int kKeys, int kEntries>
+__device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e) {
+    if (plan.lead[e] == INT32_MAX) return 0;
+    const int of_groups = a.entries_of_groups(), at = e < of_groups ? -1 : plan.place[plan.lead[e]];
+    const int from = at < 0 ? 0 : a.end_of(at), to = e < of_groups ? a.end_of(e / a.group_rows * a.most) : INT32_MAX;
+    const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, from, to);
+    plan.spans[e] = int2{r.sink_tiles, r.window_tile};
+    return r.count;
 }
 
 // Which keys of a tile a row sees, a bit a key: arithmetic on words, since compares of every key with every row would each
@@ -230,14 +223,16 @@ __device__ inline uint32_t pack2<BF16>(float a, float b) {
 // before it.
 struct Shares {
     int64_t share, first, end;  // units a block, and this block's
-    int entry;                  // of the first; -1: nothing to do
+    int64_t base;               // the first unit of all
+    int block;                  // this one, of those that have shares
+    int entry;                  // of the first unit; -1: nothing to do
+    __device__ int block_of(int64_t unit) const { return static_cast<int>((unit - base) / share); }
 };
 // a / b for 0 <= a < 2^42 and b < 2^26: the quotient in fp64 is off by less than its distance from the next integer.
 __device__ inline int quotient(int64_t a, int b) { return static_cast<int>(static_cast<double>(a) / b); }
 
-template <int kThreads, int kBlocks, typename Count>
-__device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
-                                     int* s_entry, Count count) {
+template <int kThreads, typename Count>
+__device__ inline void prefix_sums(int entries, int64_t* pre, int64_t* wave_total, Count count) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int per = (entries + kThreads - 1) / kThreads;
     int64_t sum = 0;
@@ -262,20 +257,32 @@ __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least,
     for (int w = 0; w < kThreads / 64; ++w) all += wave_total[w];
     if (t == 0) pre[entries] = all;
     __syncthreads();
+}
+// The share of one of `blocks` blocks in the units of entries e0 to e1 - 1.
+template <int kThreads>
+__device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre, int* s_entry) {
     Shares r;
-    const int64_t total = all * a.kv_heads;
-    r.share = max<int64_t>((total + kBlocks - 1) / kBlocks, least);
-    r.first = blockIdx.x * r.share;
-    r.end = min(r.first + r.share, total);
+    r.base = pre[e0] * a.kv_heads;
+    r.block = block;
+    const int64_t total = pre[e1] * a.kv_heads - r.base;
+    r.share = max<int64_t>((total + blocks - 1) / blocks, least);
+    r.first = r.base + block * r.share;
+    r.end = min(r.first + r.share, r.base + total);
     if (r.first >= r.end) {
         r.entry = -1;
         return r;
     }
-    for (int e = t; e < entries; e += kThreads)
+    for (int e = e0 + static_cast<int>(threadIdx.x); e < e1; e += kThreads)
         if (pre[e] * a.kv_heads <= r.first && r.first < pre[e + 1] * a.kv_heads) *s_entry = e;
     __syncthreads();
     r.entry = __builtin_amdgcn_readfirstlane(*s_entry);
     return r;
+}
+template <int kThreads, int kBlocks, typename Count>
+__device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
+                                     int* s_entry, Count count) {
+    prefix_sums<kThreads>(entries, pre, wave_total, count);
+    return take_share<kThreads>(a, 0, entries, static_cast<int>(blockIdx.x), kBlocks, least, pre, s_entry);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -380,70 +387,34 @@ template <int D, int RT>
 struct FewShape {
     static constexpr bool kWide = RT >= 3 && D == 128;  // too many registers for two blocks on a CU
     static constexpr int kPerCU = kWide ? 1 : 2, kBlocks = kPerCU * kCUs;
-    static constexpr int kGroupEntries = kWide ? 2 * kFewEntries : kFewEntries;  // of a launch with groups
     static constexpr int kStages = kWide || D == 64 ? 2 : 1;  // tiles in a wave's ring: 16 KB, 32 where a block has the CU
 };
 
-template <typename T, int D, int RT, bool kShared, typename Args = PagedArgs>
-__global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_kernel(const Args a) {
+template <int W>
+struct FewMarks {
+    float stat_m[W][16], stat_l[W][16];
+    int tainted[2];  // a value that is not finite in a tile that the rows see in part: this (entry, kv head)'s, the next's
+};
+
+// What a block of W waves does with its share; without shares, with `entry`.
+template <typename T, int D, int RT, bool kShared, int W, typename Args, int kPlanned>
+__device__ __forceinline__ void few_segments(const Args& a, const Shares& shares, int entry,
+                                             uint16_t (&ring)[W][FewShape<D, RT>::kStages][2][kTile * D], const int64_t* pre,
+                                             const int2* spans, const GroupPlan<kPlanned>& plan, FewMarks<W>& marks) {
     using Shape = FewShape<D, RT>;
     constexpr bool kGroups = Args::kGroups;
-    constexpr int kEntries = kGroups ? Shape::kGroupEntries : kShared ? kFewEntries : 0;
-    static_assert(kShared || !kGroups, "entries with groups are shared out");
     constexpr int C = D / 8;                  // 16-byte chunks of a row
     constexpr int RowsPer = 64 / C;           // rows of one DMA instruction
     constexpr int Instr = 16 / RowsPer;       // instructions for 16 rows
     constexpr int Half = 2 * Instr;           // for a tile's keys, or its values
     constexpr int S = Shape::kStages, TileElems = kTile * D;
-    __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][S][2][TileElems];
-    __shared__ int64_t pre[kEntries + 1];
-    __shared__ int2 own_spans[kShared && !kGroups ? kEntries : 1];  // {sink_tiles, window_tile}
-    __shared__ GroupPlan<kGroups ? kEntries : 1> plan;
-    int2* const spans = kGroups ? plan.spans : own_spans;
-    __shared__ int64_t wave_total[kWaves];
-    __shared__ float stat_m[kWaves][16], stat_l[kWaves][16];
-    __shared__ int s_entry;
-    __shared__ int s_tainted[2];  // a value that is not finite in a tile that the rows see in part: this (entry, kv head)'s, the next's
-    static_assert(sizeof(ring) >= sizeof(float) * kWaves * 16 * D, "the rings hold the waves' sums of 16 rows");
+    static_assert(sizeof(ring) >= sizeof(float) * W * 16 * D, "the rings hold the waves' sums of 16 rows");
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
-    if (t < 2) s_tainted[t] = 0;
-    Shares shares{};
-    int entry, of_groups = 0;  // entries, which come first
-    int64_t u = 0;
-    if constexpr (kShared) {
-        int entries = a.batch * a.row_groups;
-        if constexpr (kGroups) {
-            if (a.apart) {
-                plan_own<64 * kWaves>(a, 16 * RT, plan);
-            } else {
-                plan_groups<64 * kWaves, kEntries, true>(a, 16 * RT, plan);
-                of_groups = a.entries_of_groups();
-            }
-            entries += of_groups;
-        }
-        shares = make_shares<64 * kWaves, Shape::kBlocks>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
-            Tiles r;
-            if constexpr (kGroups) {
-                if (plan.lead[e] == INT32_MAX) return 0;  // nobody's
-                const int at = e < of_groups ? -1 : plan.place[plan.lead[e]];
-                const int from = at < 0 ? 0 : a.end_of(at), to = e < of_groups ? a.end_of(e / a.group_rows * a.most) : INT32_MAX;
-                r = tiles_within<kTile>(a, spans[e].x, spans[e].y, from, to);
-            } else {
-                r = tiles_of_few(a, e, 16 * RT);
-            }
-            spans[e] = int2{r.sink_tiles, r.window_tile};
-            return r.count + kFewStart;
-        });
-        if (shares.entry < 0) return;
-        entry = shares.entry;
-        u = shares.first;
-    } else {
-        entry = static_cast<int>(blockIdx.x) / a.kv_heads;
-        __syncthreads();  // s_tainted is cleared before any wave sets it (make_shares has barriers of its own)
-    }
-
+    int64_t u = kShared ? shares.first : 0;
+    int of_groups = 0;  // entries, which come first
+    if constexpr (kGroups) of_groups = a.entries_of_groups();
     uint32_t voff[Instr];
 #pragma unroll
     for (int j = 0; j < Instr; ++j) {
@@ -452,8 +423,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         voff[j] = static_cast<uint32_t>(row * D * 2 + 16 * ((lane % C) ^ (swz & (C - 1))));
     }
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_addr(&ring[wave][0][0][0]));
-    int slot = 0, turn = 0, all_of_groups = 0;
-    if constexpr (kGroups) all_of_groups = a.entries_of_groups();
+    int slot = 0, turn = 0;
     while (true) {
         int kvh, first = 0, n, units = 0;
         Rows<Args> rows{};
@@ -514,7 +484,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             int there;      // bit h: half h's page is there
         };
         auto places_of = [&](int i) {
-            const int key0 = tiles.at(first + wave + kWaves * i) * kTile;
+            const int key0 = tiles.at(first + wave + W * i) * kTile;
             Places p;
             p.there = 0;
 #pragma unroll
@@ -534,7 +504,28 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
                 for (int j = 0; j < Instr; ++j) dma16_lds(from, voff[j], lds + static_cast<uint32_t>(h * 16 * D) * 2u + 1024u * j);
             }
         };
-        const int mine = n > wave ? (n - wave + kWaves - 1) / kWaves : 0;
+        u32x4 qf[RT][D / 32];
+        int last[RT], start[RT];
+        int all_last = INT32_MAX, all_start = 0;  // what every row sees
+        auto fetch_queries = [&] {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const RowAt row = rows.at(a, min(16 * rt + c, rows.rows - 1));
+                last[rt] = 16 * rt + c < rows.rows ? row.last : -1;
+                start[rt] = a.window > 0 ? max(0, row.position - a.window + 1) : 0;
+                if (last[rt] >= 0) {
+                    all_last = min(all_last, last[rt]);
+                    all_start = max(all_start, start[rt]);
+                }
+                const uint16_t* src = a.q + row.q_row * a.q_stride + static_cast<int64_t>(kvh * a.groups + row.head) * D + 8 * g;
+#pragma unroll
+                for (int kt = 0; kt < D / 32; ++kt) qf[rt][kt] = *vec(src + 32 * kt);
+            }
+        };
+        // loads come back in the order in which they went out: of a group, where the rows lie is loaded before the queries are,
+        // and the tiles would have to come first
+        if constexpr (kGroups) fetch_queries();
+        const int mine = n > wave ? (n - wave + W - 1) / W : 0;
         int there[S] = {};  // of the tiles that are out, the oldest first
 #pragma unroll
         for (int st = 0; st < S; ++st)
@@ -545,22 +536,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
                 issue(a.v_pages, p, st, 1);
             }
 
-        u32x4 qf[RT][D / 32];
-        int last[RT], start[RT];
-        int all_last = INT32_MAX, all_start = 0;  // what every row sees
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const RowAt row = rows.at(a, min(16 * rt + c, rows.rows - 1));
-            last[rt] = 16 * rt + c < rows.rows ? row.last : -1;
-            start[rt] = a.window > 0 ? max(0, row.position - a.window + 1) : 0;
-            if (last[rt] >= 0) {
-                all_last = min(all_last, last[rt]);
-                all_start = max(all_start, start[rt]);
-            }
-            const uint16_t* src = a.q + row.q_row * a.q_stride + static_cast<int64_t>(kvh * a.groups + row.head) * D + 8 * g;
-#pragma unroll
-            for (int kt = 0; kt < D / 32; ++kt) qf[rt][kt] = *vec(src + 32 * kt);
-        }
+        if constexpr (!kGroups) fetch_queries();
         all_last = least_of<16>(all_last);
         all_start = largest_of<16>(all_start);
 
@@ -587,7 +563,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             const int stage = S == 1 ? 0 : i & 1, ahead = min(mine - 1 - i, S - 1);  // tiles out behind this one
             const uint16_t* kb = ring[wave][stage][0];
             const uint16_t* vb = ring[wave][stage][1];
-            const int key0 = tiles.at(first + wave + kWaves * i) * kTile;
+            const int key0 = tiles.at(first + wave + W * i) * kTile;
             const bool more = i + S < mine;
             Places next{};
             if (more) next = places_of(i + S);
@@ -706,7 +682,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) o[rt][d0 + e] = mfma16x16x32<T>(vf[e], pf[rt], o[rt][d0 + e]);
             }
-            if (zero != zero) s_tainted[turn] = 1;
+            if (zero != zero) marks.tainted[turn] = 1;
             if (more) {
                 reads_ended();
                 issue(a.v_pages, next, stage, 1);
@@ -718,13 +694,12 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
 
         // the waves' sums, joined through the rings a row group at a time
         const bool done = !kGroups && first == 0 && n == count;
-        const int listed = kGroups ? entry - of_groups + all_of_groups : entry;  // among the entries of all launches
         int64_t part;
-        if constexpr (kGroups) part = first == 0 ? a.first_part(listed, kvh) : a.later_part(listed, static_cast<int>(blockIdx.x));
-        else part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept;
+        if constexpr (kGroups) part = first == 0 ? a.first_part(entry, kvh) : a.later_part(entry, shares.block);
+        else part = (static_cast<int64_t>(shares.block) * 2 + slot) * a.rows_kept;
         float* red = reinterpret_cast<float*>(&ring[0][0][0][0]);
         __syncthreads();
-        const bool tainted = s_tainted[turn] != 0;
+        const bool tainted = marks.tainted[turn] != 0;
         if (tainted) slow_rows<T, D>(a, rows, kvh, tiles, kTile, first, n, done, part);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -734,24 +709,24 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             for (int dt = 0; dt < D / 16; ++dt)
                 *reinterpret_cast<f32x4*>(red + (wave * 16 + c) * D + 4 * ((4 * dt + g) ^ c)) = o[rt][dt];
             if (g == 0) {  // a row of padding took part where the tile was whole: its sums are none
-                stat_m[wave][c] = last[rt] < 0 ? -INFINITY : m[rt];
-                stat_l[wave][c] = last[rt] < 0 ? 0.0f : lsum[rt][0];
+                marks.stat_m[wave][c] = last[rt] < 0 ? -INFINITY : m[rt];
+                marks.stat_l[wave][c] = last[rt] < 0 ? 0.0f : lsum[rt][0];
             }
             __syncthreads();
-            for (int id = t; id < 16 * C; id += 64 * kWaves) {
+            for (int id = t; id < 16 * C; id += 64 * W) {
                 const int row = id / C, ch = id % C;
                 if (16 * rt + row >= rows.rows) continue;
-                float M = stat_m[0][row];
+                float M = marks.stat_m[0][row];
 #pragma unroll
-                for (int w = 1; w < kWaves; ++w) M = fmaxf(M, stat_m[w][row]);
+                for (int w = 1; w < W; ++w) M = fmaxf(M, marks.stat_m[w][row]);
                 const float mu = M == -INFINITY ? 0.0f : M;
                 float L = 0.0f;
                 f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    if (stat_l[w][row] == 0.0f) continue;
-                    const float f = __builtin_amdgcn_exp2f(stat_m[w][row] - mu);
-                    L += f * stat_l[w][row];
+                for (int w = 0; w < W; ++w) {
+                    if (marks.stat_l[w][row] == 0.0f) continue;
+                    const float f = __builtin_amdgcn_exp2f(marks.stat_m[w][row] - mu);
+                    L += f * marks.stat_l[w][row];
                     lo += f * *reinterpret_cast<const f32x4*>(red + (w * 16 + row) * D + 4 * ((2 * ch) ^ row));
                     hi += f * *reinterpret_cast<const f32x4*>(red + (w * 16 + row) * D + 4 * ((2 * ch + 1) ^ row));
                 }
@@ -771,8 +746,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
         }
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
-            a.desc[listed * a.kv_heads + kvh] =
-                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + units - 1) / shares.share)};
+            a.desc[entry * a.kv_heads + kvh] = int2{shares.block * 2 + slot, shares.block_of(seg + units - 1)};
         if (u >= shares.end) return;
         slot = 1;  // a share's first and last (entry, kv head) are the ones that it may not finish
         if (kvh + 1 == a.kv_heads) {
@@ -780,10 +754,53 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             if constexpr (kGroups)
                 while (pre[entry + 1] == pre[entry]) ++entry;  // nobody's; another one holds the unit u
         }
-        if (t == 0) s_tainted[turn ^ 1] = 0;
+        if (t == 0) marks.tainted[turn ^ 1] = 0;
         turn ^= 1;
         __syncthreads();
     }
+}
+
+template <typename T, int D, int RT, bool kShared, typename Args = PagedArgs>
+__global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_kernel(const Args a) {
+    using Shape = FewShape<D, RT>;
+    constexpr bool kGroups = Args::kGroups;
+    constexpr int kEntries = kShared ? kFewEntries : 0;
+    static_assert(kShared || !kGroups, "entries with groups are shared out");
+    __shared__ __attribute__((aligned(16))) uint16_t ring[kWaves][Shape::kStages][2][kTile * D];
+    __shared__ int64_t pre[kEntries + 1];
+    __shared__ int2 own_spans[kShared && !kGroups ? kEntries : 1];  // {sink_tiles, window_tile}
+    __shared__ GroupPlan<kGroups ? kEntries : 1> plan;
+    __shared__ int64_t wave_total[kWaves];
+    __shared__ FewMarks<kWaves> marks;
+    __shared__ int s_entry;
+    if (threadIdx.x < 2) marks.tainted[threadIdx.x] = 0;
+    Shares shares{};
+    int entry;
+    if constexpr (kShared) {
+        int entries = a.batch * a.row_groups;
+        if constexpr (kGroups) {
+            plan_groups<64 * kWaves>(a, plan);
+            entries += a.entries_of_groups();
+        }
+        shares = make_shares<64 * kWaves, Shape::kBlocks>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
+            if constexpr (kGroups) {
+                const int n = tiles_of_plan<kTile>(a, plan, e);
+                return n == 0 ? 0 : n + kFewStart;
+            } else {
+                const Tiles r = tiles_of_few(a, e, 16 * RT);
+                own_spans[e] = int2{r.sink_tiles, r.window_tile};
+                return r.count + kFewStart;
+            }
+        });
+        if (shares.entry < 0) return;
+        entry = shares.entry;
+    } else {
+        entry = static_cast<int>(blockIdx.x) / a.kv_heads;
+        __syncthreads();  // the marks are cleared before any wave sets one (make_shares has barriers of its own)
+    }
+    const int2* spans = own_spans;
+    if constexpr (kGroups) spans = plan.spans;
+    few_segments<T, D, RT, kShared, kWaves>(a, shares, entry, ring, pre, spans, plan, marks);
 }
 
 }  // namespace

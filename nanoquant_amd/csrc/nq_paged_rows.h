@@ -55,56 +55,34 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
 // kShared: the work of all row groups in equal shares over the grid, as few_kernel's; otherwise a block takes a row group,
 // the last ones (the longest of a prompt) first.
 // With GroupArgs: the entries of groups only, each over the keys that its members share; every part goes to the workspace.
-template <typename T, int D, int RW, bool kShared, typename Args = PagedArgs>
-__global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_kernel(const Args a) {
+template <int D>
+struct RowsRings {
+    uint16_t k[4][kKeys * D], v[4][kKeys * D];
+};
+struct RowsMarks {
+    int spans[2][4];
+    int tainted[2];  // as few_kernel's
+};
+
+// What a block does with its share; without shares, with `entry`.
+template <typename T, int D, int RW, bool kShared, typename Args, int kPlanned>
+__device__ __forceinline__ void rows_segments(const Args& a, const Shares& shares, int entry, RowsRings<D>& rings, const int64_t* pre,
+                                              const GroupPlan<kPlanned>& plan, RowsMarks& marks) {
     constexpr bool kGroups = Args::kGroups;
-    static_assert(kShared || !kGroups, "entries of groups are shared out");
-    constexpr int NW = RW == 1 ? 8 : 4;  // waves
     constexpr int C = D / 8;             // 16-byte chunks of a row
     constexpr int RowsPer = 64 / C;      // rows of one DMA instruction
     constexpr int Instr = 16 / RowsPer;  // instructions for 16 rows
     constexpr int Group = 128 * RW;
     constexpr int KT = D / 16, DT = D / 32, KG = KT / 2;
     constexpr int TileElems = kKeys * D, kStep = RW == 1 ? 2 : 1;  // tiles from one of a wave's to its next
-    __shared__ __attribute__((aligned(16))) uint16_t kring[4][TileElems], vring[4][TileElems];
-    __shared__ int spans[2][4];
-    __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
-    __shared__ int64_t wave_total[NW];
-    __shared__ int s_entry;
-    __shared__ int s_tainted[2];  // as few_kernel's
-    __shared__ GroupPlan<kGroups ? kEntries : 1> plan;
+    auto& kring = rings.k;
+    auto& vring = rings.v;
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int rwave = wave & 3, grp = wave >> 2;  // its rows, and of the two halves of RW 1
     const int c = lane & 31, kg = lane >> 5;
-    if (t < 2) s_tainted[t] = 0;
-    Shares shares{};
-    int entry, slot = 0, turn = 0;
-    int64_t u = 0;
-    if constexpr (kShared) {
-        int entries = a.batch * a.row_groups;
-        if constexpr (kGroups) {
-            entries = a.entries_of_groups();
-            plan_groups<64 * NW>(a, Group, plan);
-        }
-        shares = make_shares<64 * NW, kCUs>(a, entries, kLeastTiles, pre, wave_total, &s_entry, [&](int e) {
-            if constexpr (kGroups) {
-                if (plan.lead[e] == INT32_MAX) return 0;  // nobody's
-                const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, 0, a.end_of(e / a.group_rows * a.most));
-                plan.spans[e] = int2{r.sink_tiles, r.window_tile};
-                return r.count + kStart;
-            } else {
-                return a.spans[e].z + kStart;
-            }
-        });
-        if (shares.entry < 0) return;
-        entry = shares.entry;
-        u = shares.first;
-    } else {
-        const int order = static_cast<int>(blockIdx.x) / (a.batch * a.kv_heads);
-        const int rest = static_cast<int>(blockIdx.x) - order * a.batch * a.kv_heads;
-        entry = rest / a.kv_heads * a.row_groups + a.row_groups - 1 - order;
-    }
+    int slot = 0, turn = 0;
+    int64_t u = kShared ? shares.first : 0;
 
     uint32_t koff[Instr], voff[Instr];
 #pragma unroll
@@ -225,7 +203,9 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         auto begin = [&] {
             for (int it = grp; it < (RW == 1 ? 4 : 3) && it < n; it += kStep) issue(it);
         };
-        if constexpr (kShared) begin();  // while the queries come
+        // loads come back in the order in which they went out: of a group, where the rows lie is loaded before the queries are,
+        // and the tiles would have to come first
+        if constexpr (kShared && !kGroups) begin();  // while the queries come
 
         u32x4 qf[RW][KT];
         int last[RW], start[RW];
@@ -246,6 +226,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) qf[rw][kt] = *vec(src + 16 * kt);
         }
+        if constexpr (kGroups) begin();
 #pragma unroll
         for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
@@ -262,15 +243,15 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         if constexpr (kGroups) any_start = least_of<32>(any_of);  // lo is no position where the shared keys end before
         if constexpr (!kShared) {
             if (lane == 0) {
-                spans[0][rwave] = lo;
-                spans[1][rwave] = hi;
+                marks.spans[0][rwave] = lo;
+                marks.spans[1][rwave] = hi;
             }
             __syncthreads();
             int blo = INT32_MAX, bhi = -1;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                blo = min(blo, spans[0][w]);
-                bhi = max(bhi, spans[1][w]);
+                blo = min(blo, marks.spans[0][w]);
+                bhi = max(bhi, marks.spans[1][w]);
             }
             tiles = tiles_between<kKeys>(a, blo, bhi);
             tiles.sink_tiles = __builtin_amdgcn_readfirstlane(tiles.sink_tiles);
@@ -405,7 +386,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
                     for (int rw = 0; rw < RW; ++rw) o[rw][dt] = mfma32x32x16<T>(vf[k2][dt], p[rw][k2], o[rw][dt]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (zero != zero) s_tainted[turn] = 1;
+            if (zero != zero) marks.tainted[turn] = 1;
         };
         u32x4 kf[2][KG];
         // S^T = K Q^T of 32 keys, operands read ahead of the products that run, the first half of them by `come` if `begun`
@@ -548,10 +529,10 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
 
         const bool done = !kGroups && first == 0 && n == count;
         __syncthreads();
-        const bool tainted = s_tainted[turn] != 0;
+        const bool tainted = marks.tainted[turn] != 0;
         int64_t parts;
-        if constexpr (kGroups) parts = first == 0 ? a.first_part(entry, kvh) : a.later_part(entry, static_cast<int>(blockIdx.x));
-        else parts = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * a.rows_kept;
+        if constexpr (kGroups) parts = first == 0 ? a.first_part(entry, kvh) : a.later_part(entry, shares.block);
+        else parts = (static_cast<int64_t>(shares.block) * 2 + slot) * a.rows_kept;
         if (tainted) {
             Rows<Args> these = rows;
             these.row0 = group0;
@@ -635,7 +616,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{static_cast<int>(blockIdx.x) * 2 + slot, static_cast<int>((seg + count + kStart - 1) / shares.share)};
+                int2{shares.block * 2 + slot, shares.block_of(seg + count + kStart - 1)};
         if (u >= shares.end) return;
         slot = 1;
         if (kvh + 1 == a.kv_heads) {
@@ -643,10 +624,35 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
             if constexpr (kGroups)
                 while (pre[entry + 1] == pre[entry]) ++entry;  // nobody's; another one holds the unit u
         }
-        if (t == 0) s_tainted[turn ^ 1] = 0;
+        if (t == 0) marks.tainted[turn ^ 1] = 0;
         turn ^= 1;
         __syncthreads();
     }
+}
+
+template <typename T, int D, int RW, bool kShared>
+__global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_kernel(const PagedArgs a) {
+    constexpr int NW = RW == 1 ? 8 : 4;  // waves
+    __shared__ __attribute__((aligned(16))) RowsRings<D> rings;
+    __shared__ RowsMarks marks;
+    __shared__ int64_t pre[kShared ? kEntries + 1 : 1];
+    __shared__ int64_t wave_total[NW];
+    __shared__ int s_entry;
+    __shared__ GroupPlan<1> plan;
+    if (threadIdx.x < 2) marks.tainted[threadIdx.x] = 0;
+    Shares shares{};
+    int entry;
+    if constexpr (kShared) {
+        shares = make_shares<64 * NW, kCUs>(a, a.batch * a.row_groups, kLeastTiles, pre, wave_total, &s_entry,
+                                            [&](int e) { return a.spans[e].z + kStart; });
+        if (shares.entry < 0) return;
+        entry = shares.entry;
+    } else {
+        const int order = static_cast<int>(blockIdx.x) / (a.batch * a.kv_heads);
+        const int rest = static_cast<int>(blockIdx.x) - order * a.batch * a.kv_heads;
+        entry = rest / a.kv_heads * a.row_groups + a.row_groups - 1 - order;
+    }
+    rows_segments<T, D, RW, kShared>(a, shares, entry, rings, pre, plan, marks);
 }
 
 }  // namespace

@@ -84,10 +84,53 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
     if (grp == 0) *reinterpret_cast<uint2*>(a.out + row * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
-// What a call's launches list, and what they need of the workspace; tiles 0: more than they list.
+// Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as few_kernel
+// does with eight waves, each in equal shares; all of them work out the same list. How many blocks either gets goes by what its
+// units take of a CU, a tile of 64 keys and 128 rows or one of 32 keys: kGroupCost to kOwnCost.
+constexpr int kGroupCost = 3, kOwnCost = 1, kGroupTile = 128;
+constexpr int kLeastGroupTiles = 6;  // of a block's share, a segment's start among them
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
+    constexpr int kThreads = 512, W = kThreads / 64;
+    __shared__ __attribute__((aligned(16))) union {
+        uint16_t few[W][FewShape<D, RT>::kStages][2][kTile * D];
+        RowsRings<D> rows;
+    } rings;
+    __shared__ int64_t pre[kEntries + 1];
+    __shared__ GroupPlan<kEntries> plan;
+    __shared__ int64_t wave_total[W];
+    __shared__ union {
+        FewMarks<W> few;
+        RowsMarks rows;
+    } marks;
+    __shared__ int s_entry;
+    const int of_groups = a.entries_of_groups(), entries = of_groups + a.batch * a.row_groups;
+    plan_groups<kThreads>(a, plan);
+    prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
+        if (e >= of_groups) return tiles_of_plan<kTile>(a, plan, e) + kFewStart;
+        const int n = tiles_of_plan<kKeys>(a, plan, e);
+        return n == 0 ? 0 : n + kStart;
+    });
+    const int blocks = static_cast<int>(gridDim.x), block = static_cast<int>(blockIdx.x);
+    const int64_t group_cost = pre[of_groups] * kGroupCost, cost = group_cost + (pre[entries] - pre[of_groups]) * kOwnCost;
+    int for_groups = 0;
+    if (group_cost > 0) for_groups = min(max(static_cast<int>((group_cost * blocks + cost / 2) / cost), 1), blocks - 1);
+    if (block < for_groups) {
+        if (threadIdx.x < 2) marks.rows.tainted[threadIdx.x] = 0;
+        const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, &s_entry);
+        if (shares.entry >= 0) rows_segments<T, D, 1, true>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
+    } else {
+        if (threadIdx.x < 2) marks.few.tainted[threadIdx.x] = 0;
+        const Shares shares = take_share<kThreads>(a, of_groups, entries, block - for_groups, blocks - for_groups, W, pre, &s_entry);
+        if (shares.entry >= 0) few_segments<T, D, RT, true, W>(a, shares, shares.entry, rings.few, pre, plan.spans, plan, marks.few);
+    }
+}
+
+// What a call's launch lists, and what it needs of the workspace; tiles 0: more than it lists.
 struct Plan {
-    int tiles = 0;   // of 16 rows a wave of few_kernel
-    int many = 0;    // of 32 rows a wave of rows_kernel, which then takes the groups; 0: few_kernel takes them too
+    int tiles = 0;      // of 16 rows a wave
+    bool apart;         // shared_kernel, else few_kernel takes the groups' entries too
     int64_t group_rows, row_groups, group_tile, own_tile, group_kept, rows_kept;
     int64_t own_first, group_later, own_later;  // rows of parts
     size_t part_o, part_ml, desc, place, bytes;
@@ -96,29 +139,22 @@ struct Plan {
 Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t sharing, int64_t most) {
     Plan p{};
     const int64_t each = tokens * groups, together = most * each;
-    auto tiles_of = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
-    int many = 0, tiles = tiles_of(together);
-    if (together > 64) {
-        // two row tiles a wave where the rows fill them, as for a sequence of many rows
-        many = 2 * ceil_div(together, 256) * 15 <= ceil_div(together, 128) * 16 ? 2 : 1;
-        tiles = tiles_of(each);
-    }
+    p.apart = together > 32;
+    const int tiles = (p.apart ? each : together) > 16 ? 2 : 1;
     p.own_tile = 16 * tiles;
-    p.group_tile = many ? 128 * many : p.own_tile;
+    p.group_tile = p.apart ? kGroupTile : p.own_tile;
     p.group_rows = ceil_div(together, p.group_tile);
     p.row_groups = ceil_div(each, p.own_tile);
     p.group_kept = std::min(together, p.group_tile);
     p.rows_kept = std::min(each, p.own_tile);
-    const bool wide = tiles > 2 && head_dim == 128;
-    const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups, listed = (wide ? 2 : 1) * kFewEntries;
-    if (many ? of_groups > kEntries || own > listed : of_groups + own > listed) return p;
-    const int64_t blocks = wide ? kCUs : 2 * kCUs;
+    const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
+    if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
+    const int64_t blocks = p.apart ? kCUs : 2 * kCUs;
     p.own_first = kv_heads * of_groups * p.group_kept;
     p.own_later = p.own_first + kv_heads * own * p.rows_kept;
-    p.group_later = many ? p.own_later + blocks * p.own_tile : p.own_later;
-    const int64_t parts = p.group_later + (many ? kCUs : blocks) * p.group_tile;
+    p.group_later = p.apart ? p.own_later + blocks * p.own_tile : p.own_later;
+    const int64_t parts = p.group_later + blocks * p.group_tile;
     p.tiles = tiles;
-    p.many = many;
     p.part_o = static_cast<size_t>(parts * head_dim) * sizeof(float);
     p.part_ml = static_cast<size_t>(ceil_div(parts, 2) * 2) * sizeof(float2);
     p.desc = static_cast<size_t>(ceil_div((of_groups + own) * kv_heads, 2) * 2) * sizeof(int2);
@@ -138,16 +174,17 @@ void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
     a.own_first = p.own_first;
     a.group_later = p.group_later;
     a.own_later = p.own_later;
-    a.apart = p.many > 0;
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + p.part_o);
     a.desc = reinterpret_cast<int2*>(ws + p.part_o + p.part_ml);
     a.place = reinterpret_cast<int*>(ws + p.part_o + p.part_ml + p.desc);
-    if (p.many == 1) rows_kernel<T, D, 1, true, GroupArgs><<<dim3(kCUs), 512, 0, st>>>(a);
-    else if (p.many == 2) rows_kernel<T, D, 2, true, GroupArgs><<<dim3(kCUs), 256, 0, st>>>(a);
-    if (p.tiles == 1) few_kernel<T, D, 1, true, GroupArgs><<<dim3(FewShape<D, 1>::kBlocks), 64 * kWaves, 0, st>>>(a);
-    else if (p.tiles == 2) few_kernel<T, D, 2, true, GroupArgs><<<dim3(FewShape<D, 2>::kBlocks), 64 * kWaves, 0, st>>>(a);
-    else few_kernel<T, D, 4, true, GroupArgs><<<dim3(FewShape<D, 4>::kBlocks), 64 * kWaves, 0, st>>>(a);
+    if (p.apart) {
+        if (p.tiles == 1) shared_kernel<T, D, 1><<<dim3(kCUs), 512, 0, st>>>(a);
+        else shared_kernel<T, D, 2><<<dim3(kCUs), 512, 0, st>>>(a);
+    } else {
+        if (p.tiles == 1) few_kernel<T, D, 1, true, GroupArgs><<<dim3(FewShape<D, 1>::kBlocks), 64 * kWaves, 0, st>>>(a);
+        else few_kernel<T, D, 2, true, GroupArgs><<<dim3(FewShape<D, 2>::kBlocks), 64 * kWaves, 0, st>>>(a);
+    }
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
     group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, rows);
 }
