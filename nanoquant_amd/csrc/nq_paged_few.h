@@ -56,8 +56,6 @@ struct GroupArgs : PagedArgs {
     int64_t own_first, group_later, own_later;         // rows
     int* place;              // [batch]: where a sequence stands in `members`; -1: nowhere
     __device__ int entries_of_groups() const { return sharing * group_rows; }
-    // the keys that the members of place's group share
-    __device__ int end_of(int at) const { return min(max(shared[at / most], 0), pages.table_pages) * pages.page_size; }
     __device__ int64_t first_part(int entry, int kvh) const {
         const int own = entry - entries_of_groups();
         if (own < 0) return (static_cast<int64_t>(entry) * kv_heads + kvh) * group_kept;
@@ -146,12 +144,23 @@ template <int kEntries>
 struct GroupPlan {
     int place[kEntries];  // of a sequence: the last place that names it, -1
     int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found, INT32_MAX: nobody
+    int ends[kEntries];   // of a group: the shared keys
     int2 spans[kEntries];
+    __device__ int from(int b, int most) const { return place[b] < 0 ? 0 : ends[place[b] / most]; }  // of a sequence's own keys
 };
 // All threads of the block.
 template <int kThreads, int kEntries>
 __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan) {
-    const int t = threadIdx.x, first = a.entries_of_groups(), each = a.tokens * a.groups;
+    const int t = threadIdx.x, first = a.entries_of_groups(), each = a.tokens * a.groups, own = a.batch * a.row_groups;
+    auto span_of = [&](int e) {
+        const int b = e / a.row_groups, row = (e - b * a.row_groups) * a.own_tile;
+        return span_of_few(a, b, row, min(a.own_tile, each - row));
+    };
+    // what all threads load first, together
+    int2 span = {0, 0};
+    if (t < own) span = span_of(t);
+    const int member = t < a.sharing * a.most ? a.members[t] : -1;
+    for (int g = t; g < a.sharing; g += kThreads) plan.ends[g] = min(max(a.shared[g], 0), a.pages.table_pages) * a.pages.page_size;
     for (int b = t; b < a.batch; b += kThreads) plan.place[b] = -1;
     for (int e = t; e < first; e += kThreads) {
         plan.spans[e] = int2{INT32_MAX, -1};
@@ -159,14 +168,14 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
     }
     __syncthreads();
     for (int at = t; at < a.sharing * a.most; at += kThreads) {
-        const int b = a.members[at];
-        if (b >= 0 && b < a.batch && a.shared[at / a.most] > 0) atomicMax(&plan.place[b], at);
+        const int b = at == t ? member : a.members[at];
+        if (b >= 0 && b < a.batch && plan.ends[at / a.most] > 0) atomicMax(&plan.place[b], at);
     }
     __syncthreads();
-    for (int e = t; e < a.batch * a.row_groups; e += kThreads) {
+    for (int e = t; e < own; e += kThreads) {
         const int b = e / a.row_groups, at = plan.place[b], row = (e - b * a.row_groups) * a.own_tile;
         const int rows = min(a.own_tile, each - row);
-        const int2 span = span_of_few(a, b, row, rows);
+        if (e != t) span = span_of(e);
         plan.spans[first + e] = span;
         plan.lead[first + e] = b;
         if (at < 0) continue;
@@ -185,8 +194,8 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
 template <int kKeys, int kEntries>
 __device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e) {
     if (plan.lead[e] == INT32_MAX) return 0;
-    const int of_groups = a.entries_of_groups(), at = e < of_groups ? -1 : plan.place[plan.lead[e]];
-    const int from = at < 0 ? 0 : a.end_of(at), to = e < of_groups ? a.end_of(e / a.group_rows * a.most) : INT32_MAX;
+    const int of_groups = a.entries_of_groups();
+    const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.most), to = e < of_groups ? plan.ends[e / a.group_rows] : INT32_MAX;
     const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, from, to);
     plan.spans[e] = int2{r.sink_tiles, r.window_tile};
     return r.count;
@@ -226,10 +235,11 @@ struct Shares {
     int64_t base;               // the first unit of all
     int block;                  // this one, of those that have shares
     int entry;                  // of the first unit; -1: nothing to do
-    __device__ int block_of(int64_t unit) const { return static_cast<int>((unit - base) / share); }
+    __device__ int block_of(int64_t unit) const;
 };
 // a / b for 0 <= a < 2^42 and b < 2^26: the quotient in fp64 is off by less than its distance from the next integer.
-__device__ inline int quotient(int64_t a, int b) { return static_cast<int>(static_cast<double>(a) / b); }
+__device__ inline int64_t quotient(int64_t a, int64_t b) { return static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b)); }
+__device__ inline int Shares::block_of(int64_t unit) const { return static_cast<int>(quotient(unit - base, share)); }
 
 template <int kThreads, typename Count>
 __device__ inline void prefix_sums(int entries, int64_t* pre, int64_t* wave_total, Count count) {
@@ -265,7 +275,7 @@ __device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int bloc
     r.base = pre[e0] * a.kv_heads;
     r.block = block;
     const int64_t total = pre[e1] * a.kv_heads - r.base;
-    r.share = max<int64_t>((total + blocks - 1) / blocks, least);
+    r.share = max<int64_t>(quotient(total + blocks - 1, blocks), least);
     r.first = r.base + block * r.share;
     r.end = min(r.first + r.share, r.base + total);
     if (r.first >= r.end) {
@@ -397,7 +407,7 @@ struct FewMarks {
 };
 
 // What a block of W waves does with its share; without shares, with `entry`.
-template <typename T, int D, int RT, bool kShared, int W, typename Args, int kPlanned>
+template <typename T, int D, int RT, bool kShared, int W, int kCharge, typename Args, int kPlanned>
 __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares, int entry,
                                              uint16_t (&ring)[W][FewShape<D, RT>::kStages][2][kTile * D], const int64_t* pre,
                                              const int2* spans, const GroupPlan<kPlanned>& plan, FewMarks<W>& marks) {
@@ -432,22 +442,21 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
         if constexpr (kShared) {
             const int64_t seg0 = pre[entry] * a.kv_heads;
             units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
-            kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
+            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(u - seg0, units)));
             seg = seg0 + static_cast<int64_t>(kvh) * units;
-            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart);
+            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge);
             u = min(shares.end, seg + units);
-            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kFewStart - first;
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge - first;
             if (n <= 0) return;  // the share ended before its first tile
-            tiles = Tiles{__builtin_amdgcn_readfirstlane(spans[entry].x), __builtin_amdgcn_readfirstlane(spans[entry].y), units - kFewStart};
+            tiles = Tiles{__builtin_amdgcn_readfirstlane(spans[entry].x), __builtin_amdgcn_readfirstlane(spans[entry].y), units - kCharge};
             if constexpr (kGroups) {
                 rows.place = plan.place;
                 rows.b = __builtin_amdgcn_readfirstlane(plan.lead[entry]);
                 if (entry < of_groups) {
                     rows.group = entry / a.group_rows;
-                    rows.to = __builtin_amdgcn_readfirstlane(a.end_of(rows.group * a.most));
+                    rows.to = __builtin_amdgcn_readfirstlane(plan.ends[rows.group]);
                 } else {
-                    const int at = __builtin_amdgcn_readfirstlane(plan.place[rows.b]);
-                    rows.from = at < 0 ? 0 : __builtin_amdgcn_readfirstlane(a.end_of(at));
+                    rows.from = __builtin_amdgcn_readfirstlane(plan.from(rows.b, a.most));
                 }
                 tiles.front = rows.from / kTile;
             }
@@ -800,7 +809,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     }
     const int2* spans = own_spans;
     if constexpr (kGroups) spans = plan.spans;
-    few_segments<T, D, RT, kShared, kWaves>(a, shares, entry, ring, pre, spans, plan, marks);
+    few_segments<T, D, RT, kShared, kWaves, kFewStart>(a, shares, entry, ring, pre, spans, plan, marks);
 }
 
 }  // namespace

@@ -65,7 +65,7 @@ struct RowsMarks {
 };
 
 // What a block does with its share; without shares, with `entry`.
-template <typename T, int D, int RW, bool kShared, typename Args, int kPlanned>
+template <typename T, int D, int RW, bool kShared, int kCharge, typename Args, int kPlanned>
 __device__ __forceinline__ void rows_segments(const Args& a, const Shares& shares, int entry, RowsRings<D>& rings, const int64_t* pre,
                                               const GroupPlan<kPlanned>& plan, RowsMarks& marks) {
     constexpr bool kGroups = Args::kGroups;
@@ -125,7 +125,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             rows.b = __builtin_amdgcn_readfirstlane(plan.lead[entry]);
             rows.group = entry / a.group_rows;
             rows.place = plan.place;
-            rows.to = __builtin_amdgcn_readfirstlane(a.end_of(rows.group * a.most));
+            rows.to = __builtin_amdgcn_readfirstlane(plan.ends[rows.group]);
             rows.rows = a.most * a.tokens * a.groups;
             row0 = (entry - rows.group * a.group_rows) * Group;
         } else {
@@ -141,12 +141,12 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
         if constexpr (kShared) {
             const int64_t seg0 = pre[entry] * a.kv_heads;
             const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
-            count = units - kStart;
-            kvh = __builtin_amdgcn_readfirstlane(quotient(u - seg0, units));
+            count = units - kCharge;
+            kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(u - seg0, units)));
             seg = seg0 + static_cast<int64_t>(kvh) * units;
-            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart);
+            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge);
             u = min(shares.end, seg + units);
-            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kStart - first;
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge - first;
             if (n <= 0) return;  // the share ended before its first tile
             if constexpr (kGroups) {
                 tiles = Tiles{__builtin_amdgcn_readfirstlane(plan.spans[entry].x), __builtin_amdgcn_readfirstlane(plan.spans[entry].y), count};
@@ -177,7 +177,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             }
         };
         auto place = [&](int it) {
-            if ((it & 63) < kStep) look_up(it & ~63);
+            if ((it & 63) < kStep && !(kGroups && it < kStep)) look_up(it & ~63);
             const int at = it & 63, by = 4 * (it & 3);
             there = (there & ~(15u << by)) | static_cast<uint32_t>(__builtin_amdgcn_readlane(my_there, at)) << by;
             const int page = __builtin_amdgcn_readlane(my_page, at), rest = __builtin_amdgcn_readlane(my_rest, at);
@@ -204,8 +204,9 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             for (int it = grp; it < (RW == 1 ? 4 : 3) && it < n; it += kStep) issue(it);
         };
         // loads come back in the order in which they went out: of a group, where the rows lie is loaded before the queries are,
-        // and the tiles would have to come first
-        if constexpr (kShared && !kGroups) begin();  // while the queries come
+        // and the tiles would have to come first; and the pages are looked up before
+        if constexpr (kGroups) look_up(0);
+        else if constexpr (kShared) begin();  // while the queries come
 
         u32x4 qf[RW][KT];
         int last[RW], start[RW];
@@ -616,7 +617,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{shares.block * 2 + slot, shares.block_of(seg + count + kStart - 1)};
+                int2{shares.block * 2 + slot, shares.block_of(seg + count + kCharge - 1)};
         if (u >= shares.end) return;
         slot = 1;
         if (kvh + 1 == a.kv_heads) {
@@ -652,7 +653,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
         const int rest = static_cast<int>(blockIdx.x) - order * a.batch * a.kv_heads;
         entry = rest / a.kv_heads * a.row_groups + a.row_groups - 1 - order;
     }
-    rows_segments<T, D, RW, kShared>(a, shares, entry, rings, pre, plan, marks);
+    rows_segments<T, D, RW, kShared, kStart>(a, shares, entry, rings, pre, plan, marks);
 }
 
 }  // namespace

@@ -85,10 +85,26 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
 }
 
 // Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as few_kernel
-// does with eight waves, each in equal shares; all of them work out the same list. How many blocks either gets goes by what its
-// units take of a CU, a tile of 64 keys and 128 rows or one of 32 keys: kGroupCost to kOwnCost.
-constexpr int kGroupCost = 3, kOwnCost = 1, kGroupTile = 128;
-constexpr int kLeastGroupTiles = 6;  // of a block's share, a segment's start among them
+// does with eight waves, each in equal shares; all of them work out the same list. How many blocks either gets goes by what a
+// unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how much longer the groups' blocks take
+// for their beginning and their end.
+constexpr float kGroupTime = 1200.0f, kOwnTime = 400.0f, kGroupMore = 8000.0f;
+constexpr int kGroupStart = 8, kOwnStart = 12;  // what a segment costs on top of its tiles, in tiles
+constexpr int kGroupTile = 128;
+constexpr int kLeastGroupTiles = kGroupStart + 2;  // of a block's share
+
+// Blocks of `blocks` for groups' work such that both parts end together.
+__device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units, int blocks) {
+    if (group_units == 0) return 0;
+    const float g = static_cast<float>(group_units) * kGroupTime, s = static_cast<float>(own_units) * kOwnTime;
+    int lo = 1, hi = blocks - 1;
+    while (lo < hi) {  // the first number at which the groups' part ends first
+        const int n = (lo + hi) / 2;
+        if (g / static_cast<float>(n) + kGroupMore <= s / static_cast<float>(blocks - n)) hi = n;
+        else lo = n + 1;
+    }
+    return lo;
+}
 
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
@@ -108,22 +124,20 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
     const int of_groups = a.entries_of_groups(), entries = of_groups + a.batch * a.row_groups;
     plan_groups<kThreads>(a, plan);
     prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
-        if (e >= of_groups) return tiles_of_plan<kTile>(a, plan, e) + kFewStart;
+        if (e >= of_groups) return tiles_of_plan<kTile>(a, plan, e) + kOwnStart;
         const int n = tiles_of_plan<kKeys>(a, plan, e);
-        return n == 0 ? 0 : n + kStart;
+        return n == 0 ? 0 : n + kGroupStart;
     });
     const int blocks = static_cast<int>(gridDim.x), block = static_cast<int>(blockIdx.x);
-    const int64_t group_cost = pre[of_groups] * kGroupCost, cost = group_cost + (pre[entries] - pre[of_groups]) * kOwnCost;
-    int for_groups = 0;
-    if (group_cost > 0) for_groups = min(max(static_cast<int>((group_cost * blocks + cost / 2) / cost), 1), blocks - 1);
+    const int for_groups = blocks_for_groups(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads, blocks);
     if (block < for_groups) {
         if (threadIdx.x < 2) marks.rows.tainted[threadIdx.x] = 0;
         const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, &s_entry);
-        if (shares.entry >= 0) rows_segments<T, D, 1, true>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
+        if (shares.entry >= 0) rows_segments<T, D, 1, true, kGroupStart>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
     } else {
         if (threadIdx.x < 2) marks.few.tainted[threadIdx.x] = 0;
         const Shares shares = take_share<kThreads>(a, of_groups, entries, block - for_groups, blocks - for_groups, W, pre, &s_entry);
-        if (shares.entry >= 0) few_segments<T, D, RT, true, W>(a, shares, shares.entry, rings.few, pre, plan.spans, plan, marks.few);
+        if (shares.entry >= 0) few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few, pre, plan.spans, plan, marks.few);
     }
 }
 
