@@ -88,22 +88,20 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
 // does with eight waves, each in equal shares; all of them work out the same list. How many blocks either gets goes by what a
 // unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how much longer the groups' blocks take
 // for their beginning and their end.
-constexpr float kGroupTime = 1200.0f, kOwnTime = 400.0f, kGroupMore = 8000.0f;
+constexpr float kGroupTime = 1200.0f, kGroupTime64 = 700.0f, kOwnTime = 400.0f, kGroupMore = 4000.0f;
 constexpr int kGroupStart = 8, kOwnStart = 12;  // what a segment costs on top of its tiles, in tiles
 constexpr int kGroupTile = 128;
-constexpr int kLeastGroupTiles = kGroupStart + 2;  // of a block's share
+constexpr int kLeastGroupTiles = 6;  // of a block's share, starts among them
 
-// Blocks of `blocks` for groups' work such that both parts end together.
-__device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units, int blocks) {
+// Blocks of kCUs for groups' work such that both parts end together, of the numbers 4 lane + 2.
+template <int D>
+__device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units) {
     if (group_units == 0) return 0;
-    const float g = static_cast<float>(group_units) * kGroupTime, s = static_cast<float>(own_units) * kOwnTime;
-    int lo = 1, hi = blocks - 1;
-    while (lo < hi) {  // the first number at which the groups' part ends first
-        const int n = (lo + hi) / 2;
-        if (g / static_cast<float>(n) + kGroupMore <= s / static_cast<float>(blocks - n)) hi = n;
-        else lo = n + 1;
-    }
-    return lo;
+    const int n = 4 * (static_cast<int>(threadIdx.x) & 63) + 2;
+    const float g = static_cast<float>(group_units) * (D == 128 ? kGroupTime : kGroupTime64) * __builtin_amdgcn_rcpf(static_cast<float>(n));
+    const float s = static_cast<float>(own_units) * kOwnTime * __builtin_amdgcn_rcpf(static_cast<float>(kCUs - n));
+    const int late = __popcll(__ballot(g + kGroupMore > s));  // the lanes at which the groups' part ends last: the first ones
+    return min(4 * late + 2, kCUs - 2);
 }
 
 template <typename T, int D, int RT>
@@ -128,15 +126,15 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
         const int n = tiles_of_plan<kKeys>(a, plan, e);
         return n == 0 ? 0 : n + kGroupStart;
     });
-    const int blocks = static_cast<int>(gridDim.x), block = static_cast<int>(blockIdx.x);
-    const int for_groups = blocks_for_groups(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads, blocks);
+    const int block = static_cast<int>(blockIdx.x);
+    const int for_groups = blocks_for_groups<D>(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads);
     if (block < for_groups) {
         if (threadIdx.x < 2) marks.rows.tainted[threadIdx.x] = 0;
         const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, &s_entry);
         if (shares.entry >= 0) rows_segments<T, D, 1, true, kGroupStart>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
     } else {
         if (threadIdx.x < 2) marks.few.tainted[threadIdx.x] = 0;
-        const Shares shares = take_share<kThreads>(a, of_groups, entries, block - for_groups, blocks - for_groups, W, pre, &s_entry);
+        const Shares shares = take_share<kThreads>(a, of_groups, entries, block - for_groups, kCUs - for_groups, W, pre, &s_entry);
         if (shares.entry >= 0) few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few, pre, plan.spans, plan, marks.few);
     }
 }
