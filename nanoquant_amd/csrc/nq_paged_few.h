@@ -664,8 +664,7 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
             };
             u32x4 keep;
             if (!whole) {
-#pragma unroll
-                for (int off = 1; off < 16; off <<= 1) some |= __shfl_xor(some, off, 64);
+                some = or_row16(some);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) keep[w] = pair_mask(some, 16 * (w >> 1) + 2 * (w & 1));
             }

@@ -290,8 +290,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[rw][i] = or_minus_inf(s[rw][i], seen, 8 * (i >> 2) + (i & 3));
                 }
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) some |= __shfl_xor(some, off, 64);
+                some = or_half32(some);
             }
             return whole;
         };

@@ -18,6 +18,23 @@ __device__ inline float max_xor16(float v) {
     return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 
+// Bits of any lane of the row of 16; of any lane of the half of 32.
+template <int kControl>
+__device__ inline uint32_t or_dpp(uint32_t v) {
+    return v | static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, 0xF, 0xF, false));
+}
+__device__ inline uint32_t or_row16(uint32_t v) {
+    v = or_dpp<0x121>(v);  // row_ror:1
+    v = or_dpp<0x122>(v);
+    v = or_dpp<0x124>(v);
+    return or_dpp<0x128>(v);
+}
+__device__ inline uint32_t or_half32(uint32_t v) {
+    v = or_row16(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // the even rows of 16 lanes twice, the odd ones twice
+    return static_cast<uint32_t>(r[0]) | static_cast<uint32_t>(r[1]);
+}
+
 // Smallest and largest over lanes 0 to kLanes - 1 (16 or 32), the same in the whole wave.
 template <int kControl>
 __device__ inline int dpp_or_own(int v) {  // of the lane that a DPP control names, the lane's own where there is none
