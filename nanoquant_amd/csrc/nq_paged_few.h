@@ -146,6 +146,7 @@ struct GroupPlan {
     int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found, INT32_MAX: nobody
     int ends[kEntries];   // of a group: the shared keys
     int2 spans[kEntries];
+    uint8_t slow[kEntries];  // of a group's entry: the tiles in which some member's window begins
     __device__ int from(int b, int most) const { return place[b] < 0 ? 0 : ends[place[b] / most]; }  // of a sequence's own keys
 };
 // All threads of the block.
@@ -197,6 +198,10 @@ __device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& pla
     const int of_groups = a.entries_of_groups();
     const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.most), to = e < of_groups ? plan.ends[e / a.group_rows] : INT32_MAX;
     const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, from, to);
+    int slow = 0;
+    if (e < of_groups && a.window > 0 && r.count > r.sink_tiles)
+        slow = min(max(0, plan.spans[e].y - a.window + 1), to - 1) / kKeys - r.window_tile + 1;
+    plan.slow[e] = static_cast<uint8_t>(min(max(slow, 0), 255));
     plan.spans[e] = int2{r.sink_tiles, r.window_tile};
     return r.count;
 }

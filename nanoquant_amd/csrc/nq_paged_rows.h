@@ -135,18 +135,20 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
         }
         const int group0 = row0;
         row0 += rwave * (32 * RW);
-        int kvh, first = 0, n, count;
+        int kvh, first = 0, n, count, units = 0;
         int64_t seg = 0;
         Tiles tiles;
         if constexpr (kShared) {
             const int64_t seg0 = pre[entry] * a.kv_heads;
-            const int units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
-            count = units - kCharge;
+            units = __builtin_amdgcn_readfirstlane(static_cast<int>(pre[entry + 1] - pre[entry]));
+            int charge = kCharge;
+            if constexpr (kGroups) charge += __builtin_amdgcn_readfirstlane(static_cast<int>(plan.slow[entry]));
+            count = units - charge;
             kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(u - seg0, units)));
             seg = seg0 + static_cast<int64_t>(kvh) * units;
-            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge);
+            first = max(0, __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - charge);
             u = min(shares.end, seg + units);
-            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - kCharge - first;
+            n = __builtin_amdgcn_readfirstlane(static_cast<int>(u - seg)) - charge - first;
             if (n <= 0) return;  // the share ended before its first tile
             if constexpr (kGroups) {
                 tiles = Tiles{__builtin_amdgcn_readfirstlane(plan.spans[entry].x), __builtin_amdgcn_readfirstlane(plan.spans[entry].y), count};
@@ -616,7 +618,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
         if constexpr (!kShared) return;
         if (first == 0 && t == 0)
             a.desc[entry * a.kv_heads + kvh] =
-                int2{shares.block * 2 + slot, shares.block_of(seg + count + kCharge - 1)};
+                int2{shares.block * 2 + slot, shares.block_of(seg + units - 1)};
         if (u >= shares.end) return;
         slot = 1;
         if (kvh + 1 == a.kv_heads) {

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
     prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
         if (e >= of_groups) return tiles_of_plan<kTile>(a, plan, e) + kOwnStart;
         const int n = tiles_of_plan<kKeys>(a, plan, e);
-        return n == 0 ? 0 : n + kGroupStart;
+        return n == 0 ? 0 : n + kGroupStart + plan.slow[e];  // a tile that is masked takes twice as long
     });
     const int block = static_cast<int>(blockIdx.x);
     const int for_groups = blocks_for_groups<D>(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads);
