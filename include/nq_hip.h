@@ -416,8 +416,9 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * Everything else, the result but for rounding too, is as for nq_paged_attention.
  *   workspace nq_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one
  *             must not overlap.
- * Past what nq_paged_attention takes, NQ_ERR_UNSUPPORTED where one launch cannot list the work: see the workspace function,
- * which returns 0 for such a call. Call nq_paged_attention then. */
+ * NQ_ERR_UNSUPPORTED also where there is no group, or more work than a launch lists: with rows = tokens * heads / kv_heads,
+ * groups * ceil(most * rows / 128) + batch * ceil(rows / (rows > 16 ? 32 : 16)) entries beyond 1024, or, where most * rows is 32
+ * at most, groups + batch beyond 512. The workspace function returns 0 for such a call; nq_paged_attention takes it. */
 size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t groups, int64_t most);
 int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,

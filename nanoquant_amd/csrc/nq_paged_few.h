@@ -139,11 +139,13 @@ __device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
     return tiles_between<kTile>(a, span.x, span.y);
 }
 
+constexpr int kNobody = INT32_MAX, kIdle = 1 << 30;  // a sequence without tokens leads only where no other does
+
 // What the blocks of a launch with groups work out before they take their shares, in LDS.
 template <int kEntries>
 struct GroupPlan {
     int place[kEntries];  // of a sequence: the last place that names it, -1
-    int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found, INT32_MAX: nobody
+    int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found; kNobody
     int ends[kEntries];   // of a group: the shared keys
     int2 spans[kEntries];
     uint8_t slow[kEntries];  // of a group's entry: the tiles in which some member's window begins
@@ -165,7 +167,7 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
     for (int b = t; b < a.batch; b += kThreads) plan.place[b] = -1;
     for (int e = t; e < first; e += kThreads) {
         plan.spans[e] = int2{INT32_MAX, -1};
-        plan.lead[e] = INT32_MAX;
+        plan.lead[e] = kNobody;
     }
     __syncthreads();
     for (int at = t; at < a.sharing * a.most; at += kThreads) {
@@ -184,7 +186,7 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
         for (int i = row0 / a.group_tile; i <= (row0 + rows - 1) / a.group_tile; ++i) {
             atomicMin(&plan.spans[g * a.group_rows + i].x, span.x);
             atomicMax(&plan.spans[g * a.group_rows + i].y, span.y);
-            atomicMin(&plan.lead[g * a.group_rows + i], b);
+            atomicMin(&plan.lead[g * a.group_rows + i], span.y < 0 ? b | kIdle : b);
         }
     }
     __syncthreads();
@@ -194,7 +196,8 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
 // The tiles of kKeys keys of an entry, whose span turns into their places. 0: nobody's
 template <int kKeys, int kEntries>
 __device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e) {
-    if (plan.lead[e] == INT32_MAX) return 0;
+    if (plan.lead[e] == kNobody) return 0;
+    plan.lead[e] &= ~kIdle;
     const int of_groups = a.entries_of_groups();
     const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.most), to = e < of_groups ? plan.ends[e / a.group_rows] : INT32_MAX;
     const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, from, to);

@@ -100,6 +100,7 @@ class PagedKVCache:
         self._owners = [0] * pages  # sequences that have a page
         self.members = self.shared = None
         self.groups = 0
+        self._common = [0] * batch  # entries that a sequence's row has in common with its group's
 
     def _row(self, sequence: int):
         if not 0 <= sequence < self.batch:
@@ -125,14 +126,13 @@ class PagedKVCache:
 
     def _regroup(self) -> None:
         """``members`` and ``shared`` of the sequences whose first page is the same: what all of their rows begin with."""
-        if self.members is None and max(self._owners) < 2:
-            return
         alike = {}
         for b, row in enumerate(self._host):
             first = next(((i, page) for i, page in enumerate(row) if page >= 0), None)
             if first is not None and self._owners[first[1]] > 1:
                 alike.setdefault(first, []).append(b)
         lists, shared = [], []
+        self._common = [0] * self.batch
         for sequences in alike.values():
             rows = [self._host[b] for b in sequences]
             low, high = min(rows), max(rows)  # what these two begin with all begin with
@@ -142,6 +142,8 @@ class PagedKVCache:
             if len(sequences) > 1 and common:
                 lists.append(sequences)
                 shared.append(common)
+                for b in sequences:
+                    self._common[b] = common
         self.groups = len(lists)
         most = max(map(len, lists), default=0)
         if self.members is None or self.members.shape[0] < len(lists) or self.members.shape[1] < most:
@@ -167,7 +169,8 @@ class PagedKVCache:
             row[i] = self._take()
         if need:
             self._store(sequence)
-            self._regroup()
+            if need[0] < self._common[sequence]:
+                self._regroup()
 
     def _take_back(self, sequence: int, slots) -> int:
         row = self._row(sequence)
@@ -177,7 +180,8 @@ class PagedKVCache:
             row[i] = -1
         if gone:
             self._store(sequence)
-            self._regroup()
+            if gone[0] < self._common[sequence]:
+                self._regroup()
         return len(gone)
 
     def trim(self, sequence: int, position: int) -> int:
@@ -207,6 +211,9 @@ class PagedKVCache:
         if split and len(targets) > len(self._free):
             raise RuntimeError(f"the paged cache has {len(self._free)} pages left, {len(targets)} forks need one each")
         moves = []
+        pages = [self._free[-1 - i] for i in range(len(targets))] if split else []  # those that will be taken
+        if pages:
+            self._copy([(row[whole], page) for page in pages])
         for b in targets:
             self._host[b][:whole] = row[:whole]
             for page in row[:whole]:
@@ -214,10 +221,6 @@ class PagedKVCache:
                     self._owners[page] += 1
             if split:
                 self._host[b][whole] = self._take()
-                moves.append((row[whole], self._host[b][whole]))
-        if moves:
-            self._copy(moves)
-        for b in targets:
             self._store(b)
         self._regroup()
 
@@ -232,16 +235,16 @@ class PagedKVCache:
         shared = [i for i in slots if row[i] >= 0 and self._owners[row[i]] > 1]
         if len(shared) > len(self._free):
             raise RuntimeError(f"the paged cache has {len(self._free)} pages left, sequence {sequence} needs {len(shared)}")
-        moves = []
-        for i in shared:
-            moves.append((row[i], self._take()))
-            self._drop(row[i])
-            row[i] = moves[-1][1]
-        if moves:
-            self._copy(moves)
+        if shared:
+            self._copy([(row[i], self._free[-1 - k]) for k, i in enumerate(shared)])  # those that will be taken
+            for i in shared:
+                page = self._take()
+                self._drop(row[i])
+                row[i] = page
             self._store(sequence)
-            self._regroup()
-        return len(moves)
+            if shared[0] < self._common[sequence]:
+                self._regroup()
+        return len(shared)
 
     def compact(self) -> int:
         """Move the pages that are in use to the front of the pools; returns their number, which is the first page that is not.
@@ -452,7 +455,7 @@ def paged_shared_attention(q, k_pages, v_pages, table, positions, members, share
     do not begin alike, their results mean nothing.
 
     Other arguments and the result, but for rounding, are :func:`paged_attention`'s, which also takes the calls that the kernel
-    does not: those that run torch ops, and more than 1024 sequences and groups of 64 rows at once."""
+    does not: those that run torch ops, and batches past about a thousand sequences (``nq_paged_shared_attention``)."""
     what = "paged_shared_attention"
     given = (q, k_pages, v_pages, table, positions, members, shared)
     if _native_shared is not None and q.is_cuda and _only_eager(*given):

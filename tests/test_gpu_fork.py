@@ -180,6 +180,30 @@ def test_attention_takes_strided_tensors_and_a_scale():
     _check(y, ref, spread, torch.float16, _keys(table, k))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.07])
+@pytest.mark.parametrize("members", [3, 20])
+def test_attention_with_scales_that_are_not_positive(members, scale):
+    q, k, v, table, pos, lists, shared = fork_oracle.shared_case(8, 2, 128, 16, [(9, [30, 4, 70][:members] + [5] * (members - 3))], [40],
+                                                                 1, torch.bfloat16, "cuda")
+    y = paged_shared_attention(q, k, v, table, pos, lists, shared, scale=scale)
+    ref, spread = oracle.attention(q, k, v, table, pos, scale=scale)
+    _check(y, ref, spread, torch.bfloat16, _keys(table, k))
+
+
+@pytest.mark.parametrize("members", [3, 20])
+def test_members_that_have_ended(members):
+    """A sequence without tokens whose row of the table is gone leaves the others theirs, wherever it stands."""
+    case = fork_oracle.shared_case(8, 2, 64, 16, [(5, [9] * members)], [], 1, torch.float16, "cuda")
+    q, k, v, table, pos, lists, shared = case
+    for gone in (0, 1, members - 1):
+        pos[gone], table[gone] = -1, -1
+        y = paged_shared_attention(q, k, v, table, pos, lists, shared)
+        ref, spread = oracle.attention(q, k, v, table, pos)
+        _check(y, ref, spread, torch.float16, _keys(table, k))
+    pos[:], table[:] = -1, -1
+    assert not paged_shared_attention(q, k, v, table, pos, lists, shared).any()
+
+
 def test_attention_of_nothing_and_of_other_types():
     q, k, v, table, pos, members, shared = fork_oracle.shared_case(4, 2, 128, 16, [(4, [5, 9])], [], 1, torch.float16, "cuda")
     assert paged_shared_attention(q[:0], k, v, table[:0], pos[:0], members, shared).shape == (0, 1, 512)
@@ -401,6 +425,16 @@ def test_the_largest_wherever_they_lie(dtype):
     for top in (1, 20, 64):
         got = token_logprobs(logits.cuda(), tokens.cuda(), top)
         fork_oracle.check_score(got, fork_oracle.score(logits, tokens, top, 1.0))
+
+
+def test_score_of_one_long_row():
+    """More parts with more alternatives than the join keeps at hand."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    logits = torch.randn(2, 1 << 22, device="cuda", generator=g).half()
+    logits[1, 5::7] = -math.inf
+    tokens = torch.tensor([7, -1], device="cuda")
+    for top in (2, 64):
+        fork_oracle.check_score(token_logprobs(logits, tokens, top), fork_oracle.score(logits, tokens, top, 1.0))
 
 
 def test_score_takes_strided_rows():
