@@ -49,8 +49,9 @@ struct LogitRow {
         last = (vocab + lead - 1) / N;
     }
     // Part k of a row is its elements k kBatch kThreads - lead on; element i of this thread's is element(k, i).
-    __device__ int element(int k, int i) const {
-        return (k * (kPieces * kThreads) + (i / N) * kThreads + static_cast<int>(threadIdx.x)) * N - lead + i % N;
+    __device__ int element(int k, int i) const { return element_of(k, static_cast<int>(threadIdx.x), i); }
+    __device__ int element_of(int k, int thread, int i) const {
+        return (k * (kPieces * kThreads) + (i / N) * kThreads + thread) * N - lead + i % N;
     }
     __device__ void load(int k, u32x4* v) const {  // past the last piece, which is not used, the last
 #pragma unroll

@@ -199,6 +199,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
     static_assert(Row::kPieces == 4, "a chunk is four pieces a thread");
     __shared__ uint64_t keys[kWaves * kMaxTop];
     __shared__ float lane_most[2][kWaves][64];
+    __shared__ uint32_t lane_words[kWaves][16];
     __shared__ int key_count[2];  // of this segment, of the next
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t red[kWaves];
@@ -296,35 +297,51 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
                 list.sharpen(x, a.top);
                 turn ^= 1;
             }
-            const uint64_t some = __ballot(most >= list.least);
+            uint64_t some = __ballot(most >= list.least);
+            if (__popcll(some) > 16) {  // which takes as long as a few insertions
+                list.sharpen(most, a.top);
+                some = __ballot(most >= list.least);
+            }
             if (some == 0) continue;
-            if (__popcll(some) > 16) list.sharpen(most, a.top);  // which takes as long as a few insertions
             forget();
-            // logit e of a piece, e known to nobody before: these parts run seldom, and unrolled their compares would take the
-            // scalar registers of everything
-            auto pick = [](u32x4 w, int e) {
-                const int word = 4 * e / N;
-                const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
-                const uint32_t x = word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : w3;
-                if constexpr (N == 4) return __builtin_bit_cast(float, x);
-                else return T::to_float(static_cast<uint16_t>(x >> (16 * (e & 1))));
+            auto hold = [&](float y, int at, bool here) {  // of each lane a logit
+                uint64_t todo = __ballot(here && y >= list.least);
+                if (todo == 0) return;
+                const uint64_t key = order_key(y, at);
+                todo &= __ballot(static_cast<unsigned>(at) < static_cast<unsigned>(a.vocab) && key > read_lane(list.key, a.top - 1));
+                while (todo != 0) {
+                    list.insert(read_lane(key, __builtin_ctzll(todo)), a.top);
+                    todo &= todo - 1;
+                }
             };
+            constexpr int kEach = N / 4;  // logits of a word
+            auto logit_of = [](uint32_t word, int i) {
+                if constexpr (kEach == 1) return __builtin_bit_cast(float, word);
+                else return T::to_float(static_cast<uint16_t>(word >> (16 * i)));
+            };
+            if (__popcll(some) <= 8) {
+                // a lane's logits go through LDS to as many lanes
+                for (; some != 0; some &= some - 1) {
+                    const int from = __builtin_ctzll(some);
+                    if (lane == from) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) lane_words[wave][i] = v[i / 4][i % 4];
+                    }
+                    const int i = lane % kBatch;
+                    hold(logit_of(lane_words[wave][i / kEach], i % kEach), row.element_of(c, 64 * wave + from, i), lane < kBatch);
+                }
+                continue;
+            }
+            // logit e of every lane's piece in turn; unrolled the compares would take the scalar registers of everything
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 if (__any(piece_most[p] >= list.least)) {
-                    const u32x4 w = v[p];
+                    const uint32_t w0 = v[p][0], w1 = v[p][1], w2 = v[p][2], w3 = v[p][3];
                     const int first = row.element(c, N * p);
 #pragma unroll 1
                     for (int e = 0; e < N; ++e) {
-                        const float y = pick(w, e);
-                        uint64_t todo = __ballot(y >= list.least);
-                        if (todo == 0) continue;
-                        const uint64_t key = order_key(y, first + e);
-                        todo &= __ballot(static_cast<unsigned>(first + e) < static_cast<unsigned>(a.vocab) && key > read_lane(list.key, a.top - 1));
-                        while (todo != 0) {
-                            list.insert(read_lane(key, __builtin_ctzll(todo)), a.top);
-                            todo &= todo - 1;
-                        }
+                        const int word = e / kEach;
+                        hold(logit_of(word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : w3, e % kEach), first + e, true);
                     }
                 }
             }
