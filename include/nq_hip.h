@@ -418,7 +418,8 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  *             must not overlap.
  * NQ_ERR_UNSUPPORTED also where there is no group, or more work than a launch lists: with rows = tokens * heads / kv_heads,
  * groups * ceil(most * rows / 128) + batch * ceil(rows / (rows > 16 ? 32 : 16)) entries beyond 1024, or, where most * rows is 32
- * at most, groups + batch beyond 512. The workspace function returns 0 for such a call; nq_paged_attention takes it. */
+ * at most, groups + batch beyond 512; and beyond 2^25 output rows of heads. The workspace function returns 0 for such a call;
+ * nq_paged_attention takes it. */
 size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t groups, int64_t most);
 int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,

@@ -161,6 +161,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     p.rows_kept = std::min(each, p.own_tile);
     const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
     if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
+    if (batch * each * kv_heads > kMaxThreads / 64) return p;  // rows of group_join_kernel, a wave each
     const int64_t blocks = p.apart ? kCUs : 2 * kCUs;
     p.own_first = kv_heads * of_groups * p.group_kept;
     p.own_later = p.own_first + kv_heads * own * p.rows_kept;

@@ -361,6 +361,27 @@ def test_refusals():
     assert [tuple(x.shape) for x in token_logprobs(logits[:0], tokens[:0], 2)] == [(0,), (0,), (0, 2), (0, 2)]
 
 
+def test_c_abi_limits_of_shared_pages_need_no_gpu():
+    """What a launch lists: row groups of groups and of sequences, and a wave for each row of the output in 32-bit threads."""
+    lib, p = _lib.load(), 256
+
+    def nbytes(batch, tokens=1, heads=8, kv=2, groups=1, most=9):
+        return lib.nq_paged_shared_attention_workspace_bytes(batch, tokens, heads, kv, 128, groups, most)
+
+    assert nbytes(1023) > 0 and nbytes(1024) == 0                      # 36 rows a group: one entry, and one a sequence
+    assert nbytes(1015, most=32 * 9) > 0 and nbytes(1016, most=32 * 9) == 0  # 1152 rows, nine entries
+    assert nbytes(511, most=8) > 0 and nbytes(512, most=8) == 0        # up to 32 rows
+    assert nbytes(100, tokens=20) > 0 and nbytes(500, tokens=20) == 0  # 80 rows a sequence, three entries
+    assert nbytes(500, heads=65536, kv=65536, most=64) > 0 and nbytes(600, heads=65536, kv=65536, most=64) == 0
+    assert nbytes(0) == nbytes(4, groups=0) == nbytes(4, most=0) == nbytes(4, heads=7) == nbytes(4, most=1 << 31) == 0
+    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 8, 8, p, p, p, 1, 9, p, 1024, 1, 8, 2, 128, 0, 0, 1.0, p,
+                                         1 << 40, None) == _lib.NQ_ERR_UNSUPPORTED
+    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 8, 8, p, p, p, 1, 9, p, 10, 1, 8, 2, 128, 0, 0, 1.0, p,
+                                         nbytes(10) - 1, None) == _lib.NQ_ERR_WORKSPACE
+    assert lib.nq_token_logprobs_workspace_bytes(1, 1, 1000, 5) == 0 < lib.nq_token_logprobs_workspace_bytes(1, 64, 100003, 5)
+    assert lib.nq_token_logprobs(2, p, 0, 100003, p, 0, 1, 1.0, 3, p, p, p, p, 1, 64, 100003, p, 100, None) == _lib.NQ_ERR_WORKSPACE
+
+
 def test_c_abi_argument_errors_need_no_gpu():
     import ctypes
     lib = _lib.load()
