@@ -276,9 +276,8 @@ __device__ inline void prefix_sums(int entries, int64_t* pre, int64_t* wave_tota
     if (t == 0) pre[entries] = all;
     __syncthreads();
 }
-// The share of one of `blocks` blocks in the units of entries e0 to e1 - 1.
-template <int kThreads>
-__device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre, int* s_entry) {
+// The share of one of `blocks` blocks in the units of entries e0 to e1 - 1, but for its first entry; `end` <= `first`: nothing.
+__device__ inline Shares share_of(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre) {
     Shares r;
     r.base = pre[e0] * a.kv_heads;
     r.block = block;
@@ -286,12 +285,18 @@ __device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int bloc
     r.share = max<int64_t>(quotient(total + blocks - 1, blocks), least);
     r.first = r.base + block * r.share;
     r.end = min(r.first + r.share, r.base + total);
-    if (r.first >= r.end) {
-        r.entry = -1;
-        return r;
-    }
+    r.entry = -1;
+    return r;
+}
+__device__ inline bool holds_unit(const PagedArgs& a, const int64_t* pre, int e, int64_t unit) {
+    return pre[e] * a.kv_heads <= unit && unit < pre[e + 1] * a.kv_heads;
+}
+template <int kThreads>
+__device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre, int* s_entry) {
+    Shares r = share_of(a, e0, e1, block, blocks, least, pre);
+    if (r.first >= r.end) return r;
     for (int e = e0 + static_cast<int>(threadIdx.x); e < e1; e += kThreads)
-        if (pre[e] * a.kv_heads <= r.first && r.first < pre[e + 1] * a.kv_heads) *s_entry = e;
+        if (holds_unit(a, pre, e, r.first)) *s_entry = e;
     __syncthreads();
     r.entry = __builtin_amdgcn_readfirstlane(*s_entry);
     return r;
@@ -351,10 +356,10 @@ __device__ inline uint2 read_transposed(const uint16_t* p) {
 // with lane l at dimensions l and, of 128, l + 64. For data of which no speed is asked.
 template <typename T, int D, typename Args>
 __device__ inline void slow_rows(const Args& a, const Rows<Args>& rows, int kvh, const Tiles& tiles, int keys, int first, int n,
-                                 bool done, int64_t part) {
+                                 bool done, int64_t part, int wave, int waves) {
     constexpr int N = D / 64;
     const int lane = threadIdx.x & 63;
-    for (int row = threadIdx.x >> 6; row < rows.rows; row += static_cast<int>(blockDim.x) >> 6) {
+    for (int row = wave; row < rows.rows; row += waves) {
         const RowAt at_row = rows.at(a, row);
         const int last = at_row.last, start = a.window > 0 ? max(0, at_row.position - a.window + 1) : 0;
         const uint16_t* q = a.q + at_row.q_row * a.q_stride + static_cast<int64_t>(kvh * a.groups + at_row.head) * D + lane;
@@ -414,11 +419,27 @@ struct FewMarks {
     int tainted[2];  // a value that is not finite in a tile that the rows see in part: this (entry, kv head)'s, the next's
 };
 
-// What a block of W waves does with its share; without shares, with `entry`.
-template <typename T, int D, int RT, bool kShared, int W, int kCharge, typename Args, int kPlanned>
+// Barriers of the waves that work together: of a whole block, or of kWaves of its waves among others. All of a block's waves
+// are on their CU until the last has ended, so those that wait do not keep the others out.
+struct BlockSync {
+    __device__ void operator()() const { __syncthreads(); }
+};
+template <int kWaves_>
+struct WavesSync {
+    int* arrived;  // in LDS, 0 at first
+    int due = 0;
+    __device__ void operator()() {
+        due += kWaves_;
+        if ((threadIdx.x & 63) == 0) __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
+        while (__hip_atomic_load(arrived, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) < due) __builtin_amdgcn_s_sleep(1);
+    }
+};
+
+// What W waves do with their share, thread t of them; without shares, with `entry`.
+template <typename T, int D, int RT, bool kShared, int W, int kCharge, typename Args, int kPlanned, typename Sync>
 __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares, int entry,
                                              uint16_t (&ring)[W][FewShape<D, RT>::kStages][2][kTile * D], const int64_t* pre,
-                                             const int2* spans, const GroupPlan<kPlanned>& plan, FewMarks<W>& marks) {
+                                             const int2* spans, const GroupPlan<kPlanned>& plan, FewMarks<W>& marks, int t, Sync sync) {
     using Shape = FewShape<D, RT>;
     constexpr bool kGroups = Args::kGroups;
     constexpr int C = D / 8;                  // 16-byte chunks of a row
@@ -427,7 +448,7 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
     constexpr int Half = 2 * Instr;           // for a tile's keys, or its values
     constexpr int S = Shape::kStages, TileElems = kTile * D;
     static_assert(sizeof(ring) >= sizeof(float) * W * 16 * D, "the rings hold the waves' sums of 16 rows");
-    const int t = threadIdx.x, lane = t & 63;
+    const int lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4;
     int64_t u = kShared ? shares.first : 0;
@@ -714,13 +735,13 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
         if constexpr (kGroups) part = first == 0 ? a.first_part(entry, kvh) : a.later_part(entry, shares.block);
         else part = (static_cast<int64_t>(shares.block) * 2 + slot) * a.rows_kept;
         float* red = reinterpret_cast<float*>(&ring[0][0][0][0]);
-        __syncthreads();
+        sync();
         const bool tainted = marks.tainted[turn] != 0;
-        if (tainted) slow_rows<T, D>(a, rows, kvh, tiles, kTile, first, n, done, part);
+        if (tainted) slow_rows<T, D>(a, rows, kvh, tiles, kTile, first, n, done, part, wave, W);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             if (tainted) break;
-            if (rt > 0) __syncthreads();
+            if (rt > 0) sync();
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt)
                 *reinterpret_cast<f32x4*>(red + (wave * 16 + c) * D + 4 * ((4 * dt + g) ^ c)) = o[rt][dt];
@@ -728,7 +749,7 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
                 marks.stat_m[wave][c] = last[rt] < 0 ? -INFINITY : m[rt];
                 marks.stat_l[wave][c] = last[rt] < 0 ? 0.0f : lsum[rt][0];
             }
-            __syncthreads();
+            sync();
             for (int id = t; id < 16 * C; id += 64 * W) {
                 const int row = id / C, ch = id % C;
                 if (16 * rt + row >= rows.rows) continue;
@@ -772,7 +793,7 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
         }
         if (t == 0) marks.tainted[turn ^ 1] = 0;
         turn ^= 1;
-        __syncthreads();
+        sync();
     }
 }
 
@@ -816,7 +837,7 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     }
     const int2* spans = own_spans;
     if constexpr (kGroups) spans = plan.spans;
-    few_segments<T, D, RT, kShared, kWaves, kFewStart>(a, shares, entry, ring, pre, spans, plan, marks);
+    few_segments<T, D, RT, kShared, kWaves, kFewStart>(a, shares, entry, ring, pre, spans, plan, marks, static_cast<int>(threadIdx.x), BlockSync{});
 }
 
 }  // namespace

@@ -539,7 +539,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             Rows<Args> these = rows;
             these.row0 = group0;
             these.rows = min(Group, rows.rows - group0);
-            slow_rows<T, D>(a, these, kvh, tiles, kKeys, first, n, done, parts);
+            slow_rows<T, D>(a, these, kvh, tiles, kKeys, first, n, done, parts, wave, static_cast<int>(blockDim.x) >> 6);
         }
         // the halves' sums: the second group's through the key ring, its statistics through the value ring's first 2 KB
         if (RW == 1 && !tainted) {

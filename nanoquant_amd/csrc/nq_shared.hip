@@ -85,11 +85,11 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
 }
 
 // Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as few_kernel
-// does with eight waves, each in equal shares; all of them work out the same list. How many blocks either gets goes by what a
+// does, half a block each, in equal shares; all of them work out the same list. How many blocks either gets goes by what a
 // unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how much longer the groups' blocks take
 // for their beginning and their end.
 constexpr float kGroupTime = 1200.0f, kGroupTime64 = 700.0f, kOwnTime = 400.0f, kGroupMore = 4000.0f;
-constexpr int kGroupStart = 8, kOwnStart = 12;  // what a segment costs on top of its tiles, in tiles
+constexpr int kGroupStart = 8, kOwnStart = 6;  // what a segment costs on top of its tiles, in tiles
 constexpr int kGroupTile = 128;
 constexpr int kLeastGroupTiles = 6;  // of a block's share, starts among them
 
@@ -106,19 +106,19 @@ __device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units) 
 
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
-    constexpr int kThreads = 512, W = kThreads / 64;
+    constexpr int kThreads = 512, W = kThreads / 128;  // waves of a half
     __shared__ __attribute__((aligned(16))) union {
-        uint16_t few[W][FewShape<D, RT>::kStages][2][kTile * D];
+        uint16_t few[2][W][FewShape<D, RT>::kStages][2][kTile * D];
         RowsRings<D> rows;
     } rings;
     __shared__ int64_t pre[kEntries + 1];
     __shared__ GroupPlan<kEntries> plan;
-    __shared__ int64_t wave_total[W];
+    __shared__ int64_t wave_total[kThreads / 64];
     __shared__ union {
-        FewMarks<W> few;
+        FewMarks<W> few[2];
         RowsMarks rows;
     } marks;
-    __shared__ int s_entry;
+    __shared__ int first_entry[2], arrived[2];
     const int of_groups = a.entries_of_groups(), entries = of_groups + a.batch * a.row_groups;
     plan_groups<kThreads>(a, plan);
     prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
@@ -130,12 +130,25 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
     const int for_groups = blocks_for_groups<D>(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads);
     if (block < for_groups) {
         if (threadIdx.x < 2) marks.rows.tainted[threadIdx.x] = 0;
-        const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, &s_entry);
+        const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, first_entry);
         if (shares.entry >= 0) rows_segments<T, D, 1, true, kGroupStart>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
     } else {
-        if (threadIdx.x < 2) marks.few.tainted[threadIdx.x] = 0;
-        const Shares shares = take_share<kThreads>(a, of_groups, entries, block - for_groups, kCUs - for_groups, W, pre, &s_entry);
-        if (shares.entry >= 0) few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few, pre, plan.spans, plan, marks.few);
+        // the halves of the block go their own ways, so that one's first tiles come and its waves' sums are joined among the
+        // other's products
+        const int half = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 8), at = 2 * (block - for_groups);
+        if (threadIdx.x < 4) marks.few[threadIdx.x >> 1].tainted[threadIdx.x & 1] = 0;
+        if (threadIdx.x < 2) arrived[threadIdx.x] = 0;
+        Shares shares = share_of(a, of_groups, entries, at + half, 2 * (kCUs - for_groups), W, pre);
+        const int64_t next = shares.first + (half == 0 ? shares.share : -shares.share);  // the other half's first unit
+        for (int e = of_groups + static_cast<int>(threadIdx.x); e < entries; e += kThreads) {
+            if (holds_unit(a, pre, e, shares.first)) first_entry[half] = e;
+            if (holds_unit(a, pre, e, next)) first_entry[1 - half] = e;
+        }
+        __syncthreads();
+        if (shares.first >= shares.end) return;
+        shares.entry = __builtin_amdgcn_readfirstlane(first_entry[half]);
+        few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few[half], pre, plan.spans, plan, marks.few[half],
+                                                   static_cast<int>(threadIdx.x) & 255, WavesSync<W>{&arrived[half]});
     }
 }
 
@@ -162,11 +175,11 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
     if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
     if (batch * each * kv_heads > kMaxThreads / 64) return p;  // rows of group_join_kernel, a wave each
-    const int64_t blocks = p.apart ? kCUs : 2 * kCUs;
+    constexpr int64_t kHalves = 2 * kCUs;  // or blocks, two on a CU
     p.own_first = kv_heads * of_groups * p.group_kept;
     p.own_later = p.own_first + kv_heads * own * p.rows_kept;
-    p.group_later = p.apart ? p.own_later + blocks * p.own_tile : p.own_later;
-    const int64_t parts = p.group_later + blocks * p.group_tile;
+    p.group_later = p.apart ? p.own_later + kHalves * p.own_tile : p.own_later;
+    const int64_t parts = p.group_later + (p.apart ? kCUs : kHalves) * p.group_tile;
     p.tiles = tiles;
     p.part_o = static_cast<size_t>(parts * head_dim) * sizeof(float);
     p.part_ml = static_cast<size_t>(ceil_div(parts, 2) * 2) * sizeof(float2);
