@@ -416,12 +416,15 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  * Everything else, the result but for rounding too, is as for nq_paged_attention.
  *   workspace nq_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one
  *             must not overlap.
- * NQ_ERR_UNSUPPORTED also where there is no group, or more work than a launch lists: with rows = tokens * heads / kv_heads,
- * groups * ceil(most * rows / 128) + batch * ceil(rows / (rows > 16 ? 32 : 16)) entries beyond 1024, or, where most * rows is 32
- * at most, groups + batch beyond 512; and beyond 2^25 output rows of heads. The workspace function returns 0 for such a call;
- * nq_paged_attention takes it. */
+ * NQ_ERR_UNSUPPORTED also for the calls that are nq_paged_attention's, for which the workspace function returns 0:
+ *   no group;
+ *   keys and values of batch tables (table_pages * page_size * kv_heads * head_dim * 4 bytes each) below 2^27 bytes, or 2^26 where
+ *     most * rows is 32 at most (rows = tokens * heads / kv_heads), and rows beyond 64: where sharing saves less than it costs;
+ *   more work than a launch lists: groups * ceil(most * rows / 128) + batch * ceil(rows / (rows > 16 ? 32 : 16)) entries beyond
+ *     1024, or, where most * rows is 32 at most, groups + batch beyond 512; batch * tokens * heads beyond 2^25. */
 size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
-                                                 int64_t head_dim, int64_t groups, int64_t most);
+                                                 int64_t head_dim, int64_t table_pages, int64_t page_size, int64_t groups,
+                                                 int64_t most);
 int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                               int64_t pages, int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_pages,
                               const int64_t* positions, const int32_t* members, const int32_t* shared, int64_t groups,

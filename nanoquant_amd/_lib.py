@@ -96,7 +96,7 @@ SIGNATURES = {
                                   _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
     "nq_verify_drafts_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "nq_verify_drafts": (_int, [_int, _vp, _i64, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _i64, _i64, _i64, _vp, _size, _vp]),
-    "nq_paged_shared_attention_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "nq_paged_shared_attention_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "nq_paged_shared_attention": (_int, [_int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
                                          _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _size, _vp]),
     "nq_copy_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),

@@ -251,7 +251,7 @@ OptTensor shared_attention(const Tensor& q, const Tensor& k_pages, const Tensor&
         members.numel() == 0 || members.size(0) != shared.size(0) || !plain(members, q, at::kInt) || !plain(shared, q, at::kInt))
         return std::nullopt;
     const int64_t groups = members.size(0), most = members.size(1);
-    const size_t bytes = lib->shared_attention_bytes(B, T, H, KV, D, groups, most);
+    const size_t bytes = lib->shared_attention_bytes(B, T, H, KV, D, table.size(1), S, groups, most);
     if (bytes == 0) return std::nullopt;
     const c10::DeviceGuard guard(q.device());
     Tensor out = at::empty(q.sizes(), q.options());

@@ -78,8 +78,9 @@ class PagedKVCache:
     model with gradients writes makes the pools part of its graph.
 
     ``members`` and ``shared`` (None before the first fork) say which sequences have their leading pages in common, as
-    :func:`paged_shared_attention` takes it, and ``groups`` how many such groups there are. Their memory stays as long as no
-    more groups and no larger ones come up than ever before, so a graph captured with the largest follows their changes.
+    :func:`paged_shared_attention` takes it, and ``groups`` how many such groups there are; ``saved`` is what reading each
+    group's pages once saves in a layer, in bytes. Their memory stays as long as no more groups and no larger ones come up than
+    ever before, so a graph captured with the largest follows their changes. The model's layers use them from 64 MB saved on.
     """
 
     def __init__(self, shape, batch: int, pages: int, page_size: int, max_len: int, device, dtype, window: int = 0,
@@ -99,7 +100,7 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._owners = [0] * pages  # sequences that have a page
         self.members = self.shared = None
-        self.groups = 0
+        self.groups = self.saved = 0
         self._common = [0] * batch  # entries that a sequence's row has in common with its group's
 
     def _row(self, sequence: int):
@@ -145,6 +146,8 @@ class PagedKVCache:
                 for b in sequences:
                     self._common[b] = common
         self.groups = len(lists)
+        page = 2 * self.k[0][0].numel() * self.k[0].element_size() if self.k else 0
+        self.saved = sum((len(sequences) - 1) * common * page for sequences, common in zip(lists, shared))
         most = max(map(len, lists), default=0)
         if self.members is None or self.members.shape[0] < len(lists) or self.members.shape[1] < most:
             old = (0, 0) if self.members is None else self.members.shape
@@ -455,7 +458,8 @@ def paged_shared_attention(q, k_pages, v_pages, table, positions, members, share
     do not begin alike, their results mean nothing.
 
     Other arguments and the result, but for rounding, are :func:`paged_attention`'s, which also takes the calls that the kernel
-    does not: those that run torch ops, and batches past about a thousand sequences (``nq_paged_shared_attention``)."""
+    does not: those that run torch ops, small ones, many tokens a sequence (prompts), and batches past about a thousand sequences
+    (``nq_paged_shared_attention`` says where). It pays from about 64 MB of keys and values that are not read again."""
     what = "paged_shared_attention"
     given = (q, k_pages, v_pages, table, positions, members, shared)
     if _native_shared is not None and q.is_cuda and _only_eager(*given):
@@ -478,7 +482,7 @@ def paged_shared_attention(q, k_pages, v_pages, table, positions, members, share
     if (q.is_cuda and q.dtype in _HALF and (D == 128 or D == 64) and S % 16 == 0 and members.numel() and q.numel()
             and _only_eager(*given) and _pool_fits(k_pages, v_pages) and table.shape[1] * S <= 1 << 30):
         lib = _lib.load()
-        nbytes = lib.nq_paged_shared_attention_workspace_bytes(B, T, q.shape[2] // D, KV, D, *members.shape)
+        nbytes = lib.nq_paged_shared_attention_workspace_bytes(B, T, q.shape[2] // D, KV, D, table.shape[1], S, *members.shape)
         if nbytes:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             q, qs = _rows(q, B, T)
@@ -528,6 +532,9 @@ def copy_pages(pools, source, target) -> None:
         pool[target] = pool[source]
 
 
+_WORTH_SHARING = 1 << 26  # bytes: what the longer beginning and the join of the attention over shared pages take, 10 us
+
+
 def paged_rotary_attention(shape, layer: int, q, k, v, cos, sin, positions, cache: PagedKVCache):
     """A layer's attention between the q, k and v projections and o_proj: rotary embedding, write into the pages and
     attention over them under the cache's window and sinks, shared pages read once a group. Arguments as
@@ -535,7 +542,7 @@ def paged_rotary_attention(shape, layer: int, q, k, v, cos, sin, positions, cach
     k_pages, v_pages = cache.k[layer], cache.v[layer]
     dtype = k_pages.dtype
     q = paged_rope_write(q.to(dtype), k.to(dtype), v.to(dtype), cos, sin, positions, k_pages, v_pages, cache.table)
-    if cache.groups:
+    if cache.groups and cache.saved >= _WORTH_SHARING:
         return paged_shared_attention(q, k_pages, v_pages, cache.table, positions, cache.members, cache.shared, cache.window,
                                       cache.sinks, shape.head_dim ** -0.5)
     return paged_attention(q, k_pages, v_pages, cache.table, positions, cache.window, cache.sinks, shape.head_dim ** -0.5)

@@ -4,15 +4,16 @@ import math
 import torch
 
 
-def shared_case(heads, kv, dim, page, groups, alone, tokens, dtype, device, seed=0, spare=2):
+def shared_case(heads, kv, dim, page, groups, alone, tokens, dtype, device, seed=0, spare=2, read=0):
     """(q, k_pages, v_pages, table, positions, members, shared): ``groups`` are (pages in common, [positions of each member
     behind them]), ``alone`` lengths of sequences in no group. Sequences come in random order, pages too; rows of the pages that
-    hold no position, and pages of nobody, are NaN. The last ``tokens`` positions of a sequence are new, -1 behind them."""
+    hold no position, and pages of nobody, are NaN. The last ``tokens`` positions of a sequence are new, -1 behind them. The
+    table is as wide as ``read`` bytes of keys and values in all its rows would take: calls are told apart by that."""
     g = torch.Generator().manual_seed(seed)
     whole = [(i, n, n * page + own) for i, (n, owns) in enumerate(groups) for own in owns] + [(-1, 0, n) for n in alone]
     B = len(whole)
     place = torch.randperm(B, generator=g).tolist()
-    slots = max(-(-n // page) for _, _, n in whole) + 1
+    slots = max(max(-(-n // page) for _, _, n in whole) + 1, -(-read // (B * page * kv * dim * 4)))
     prompts = [n for n, _ in groups]
     used = sum(prompts) + sum(-(-n // page) - m for _, m, n in whole)
     pool = used + spare

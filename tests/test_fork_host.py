@@ -77,6 +77,7 @@ def test_forks_share_whole_pages_and_copy_the_last():
     _sound(cache)
     assert cache._host[2][:2] == cache._host[0][:2] == cache._host[5][:2] and len({cache._host[b][2] for b in (0, 2, 5)}) == 3
     assert cache.groups == 1 and sorted(b for b in cache.members[0].tolist() if b >= 0) == [0, 2, 5] and int(cache.shared[0]) == 2
+    assert cache.saved == 2 * 2 * 4 * (2 * 2 * 32 * 4)  # twice two pages of four positions' keys and values
     assert len(cache._free) == 12 - 5
     for b in (0, 2, 5):
         assert all(torch.equal(x, y) for x, y in zip(_contents(cache, b, 10), want))
@@ -362,21 +363,27 @@ def test_refusals():
 
 
 def test_c_abi_limits_of_shared_pages_need_no_gpu():
-    """What a launch lists: row groups of groups and of sequences, and a wave for each row of the output in 32-bit threads."""
+    """What a launch lists: row groups of groups and of sequences, and a wave for each row of the output in 32-bit threads; and
+    what is left to the plain attention."""
     lib, p = _lib.load(), 256
 
-    def nbytes(batch, tokens=1, heads=8, kv=2, groups=1, most=9):
-        return lib.nq_paged_shared_attention_workspace_bytes(batch, tokens, heads, kv, 128, groups, most)
+    def nbytes(batch, tokens=1, heads=8, kv=2, groups=1, most=9, keys=1 << 24, page=16):
+        return lib.nq_paged_shared_attention_workspace_bytes(batch, tokens, heads, kv, 128, keys // page, page, groups, most)
 
     assert nbytes(1023) > 0 and nbytes(1024) == 0                      # 36 rows a group: one entry, and one a sequence
     assert nbytes(1015, most=32 * 9) > 0 and nbytes(1016, most=32 * 9) == 0  # 1152 rows, nine entries
     assert nbytes(511, most=8) > 0 and nbytes(512, most=8) == 0        # up to 32 rows
-    assert nbytes(100, tokens=20) > 0 and nbytes(500, tokens=20) == 0  # 80 rows a sequence, three entries
+    assert nbytes(500, tokens=16) > 0 and nbytes(512, tokens=16) == 0  # 64 rows a sequence, two entries
+    assert nbytes(100, tokens=17) == 0                                 # 68
     assert nbytes(500, heads=65536, kv=65536, most=64) > 0 and nbytes(600, heads=65536, kv=65536, most=64) == 0
     assert nbytes(0) == nbytes(4, groups=0) == nbytes(4, most=0) == nbytes(4, heads=7) == nbytes(4, most=1 << 31) == 0
-    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 8, 8, p, p, p, 1, 9, p, 1024, 1, 8, 2, 128, 0, 0, 1.0, p,
+    assert nbytes(4, keys=1 << 31) == nbytes(4, page=0x7FFFFFFF) == nbytes(4, keys=0) == 0
+    # 2^27 bytes of the tables' keys and values, 2^26 with few rows a group: 8 sequences of 2 kv heads of 128, 8 KB a position
+    assert nbytes(8, keys=1 << 14) > 0 and nbytes(8, keys=(1 << 14) - 16) == 0
+    assert nbytes(8, keys=1 << 13, most=8) > 0 and nbytes(8, keys=(1 << 13) - 16, most=8) == 0
+    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 1 << 20, 1 << 20, p, p, p, 1, 9, p, 1024, 1, 8, 2, 128, 0, 0, 1.0, p,
                                          1 << 40, None) == _lib.NQ_ERR_UNSUPPORTED
-    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 8, 8, p, p, p, 1, 9, p, 10, 1, 8, 2, 128, 0, 0, 1.0, p,
+    assert lib.nq_paged_shared_attention(0, p, 1024, p, p, 4, 16, p, 1 << 20, 1 << 20, p, p, p, 1, 9, p, 10, 1, 8, 2, 128, 0, 0, 1.0, p,
                                          nbytes(10) - 1, None) == _lib.NQ_ERR_WORKSPACE
     assert lib.nq_token_logprobs_workspace_bytes(1, 1, 1000, 5) == 0 < lib.nq_token_logprobs_workspace_bytes(1, 64, 100003, 5)
     assert lib.nq_token_logprobs(2, p, 0, 100003, p, 0, 1, 1.0, 3, p, p, p, p, 1, 64, 100003, p, 100, None) == _lib.NQ_ERR_WORKSPACE

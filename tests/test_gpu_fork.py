@@ -36,6 +36,9 @@ SHARED = [
     (24, 1, 64, 64, [(8, [4, 9])], [], 3, 0, 0),
     (6, 2, 128, 16, [(20, [21, 22, 23, 24, 25, 26])], [], 8, 0, 0),
     (8, 4, 64, 16, [(3, [80, 90])], [], 33, 0, 0),
+    # the most rows of a sequence that this kernel takes
+    (24, 1, 64, 64, [(8, [4, 9])], [], 2, 0, 0),
+    (8, 4, 64, 16, [(3, [80, 90])], [], 32, 0, 0),
     # windows: over the prompt's end, past it, with sinks in the prompt, through all of it, and behind it
     (8, 2, 128, 16, [(20, [5, 60, 140])], [90], 1, 100, 4),
     (4, 4, 64, 32, [(10, [33, 1, 200])], [], 1, 33, 40),
@@ -54,19 +57,35 @@ def _check(y, ref, spread, dtype, keys):
 
 
 def _keys(table, k):
-    return table.shape[1] * k.shape[2]
+    """The most keys of a sequence."""
+    return int((table >= 0).sum(dim=1).max()) * k.shape[2]
+
+
+def shared_case(*sizes, **kw):
+    """A case whose table is wide enough for the kernel of shared pages: smaller calls are the plain attention's."""
+    return fork_oracle.shared_case(*sizes, **kw, read=1 << 27)
+
+
+def attend(q, k, v, table, pos, members, shared, *args, **kw):
+    """paged_shared_attention, of a call that its kernel takes unless a sequence has more than 64 rows a kv head."""
+    B, T = pos.shape
+    KV, S, D = k.shape[1:]
+    H = q.shape[2] // D
+    nbytes = _lib.load().nq_paged_shared_attention_workspace_bytes(B, T, H, KV, D, table.shape[1], S, *members.shape)
+    assert (nbytes > 0) == (T * H // KV <= 64)
+    return paged_shared_attention(q, k, v, table, pos, members, shared, *args, **kw)
 
 
 @pytest.mark.parametrize("dtype", HALF, ids=IDS)
 @pytest.mark.parametrize("case", SHARED, ids=ids)
 def test_attention(case, dtype):
     *sizes, window, sinks = case
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(*sizes, dtype, "cuda")
-    y = paged_shared_attention(q, k, v, table, pos, members, shared, window, sinks)
+    q, k, v, table, pos, members, shared = shared_case(*sizes, dtype, "cuda")
+    y = attend(q, k, v, table, pos, members, shared, window, sinks)
     ref, spread = oracle.attention(q, k, v, table, pos, window, sinks)
     _check(y, ref, spread, dtype, _keys(table, k))
     assert torch.equal(y[pos < 0], torch.zeros_like(y[pos < 0]))
-    again = paged_shared_attention(q, k, v, table, pos, members, shared, window, sinks)
+    again = attend(q, k, v, table, pos, members, shared, window, sinks)
     assert torch.equal(y, again)
 
 
@@ -74,15 +93,15 @@ def test_attention(case, dtype):
 @pytest.mark.parametrize("case", [(8, 2, 128, 16, [(500, [30, 700])], [], 1), (16, 2, 64, 64, [(90, [2000] + [11] * 20)], [4000], 1),
                                   (8, 8, 128, 32, [(100, [900, 40, 7]), (40, [3, 3])], [], 4)], ids=ids)
 def test_attention_over_long_prompts(case):
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(*case, torch.bfloat16, "cuda")
-    y = paged_shared_attention(q, k, v, table, pos, members, shared)
+    q, k, v, table, pos, members, shared = shared_case(*case, torch.bfloat16, "cuda")
+    y = attend(q, k, v, table, pos, members, shared)
     ref, spread = oracle.attention(q, k, v, table, pos)
     _check(y, ref, spread, torch.bfloat16, _keys(table, k))
 
 
 def test_groups_as_a_caller_may_give_them():
     """Members named twice, in two groups, that are nobody; counts below zero and past the table; tables without padding."""
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(8, 2, 128, 16, [(6, [5, 40, 9])], [30, 7], 1, torch.float16, "cuda")
+    q, k, v, table, pos, members, shared = shared_case(8, 2, 128, 16, [(6, [5, 40, 9])], [30, 7], 1, torch.float16, "cuda")
     ref, spread = oracle.attention(q, k, v, table, pos)
     of = [b for b in members[0].tolist() if b >= 0]
     no = [b for b in range(5) if b not in of]
@@ -97,20 +116,20 @@ def test_groups_as_a_caller_may_give_them():
         ([[-1]], [4]),
     ]
     for lists, counts in rows:
-        y = paged_shared_attention(q, k, v, table, pos, torch.tensor(lists, dtype=torch.int32, device="cuda"),
+        y = attend(q, k, v, table, pos, torch.tensor(lists, dtype=torch.int32, device="cuda"),
                                    torch.tensor(counts, dtype=torch.int32, device="cuda"))
         _check(y, ref, spread, torch.float16, _keys(table, k))
     strided = torch.stack((members, members), 2)[..., 0]
     assert not strided.is_contiguous()
-    first = paged_shared_attention(q, k, v, table, pos, members, shared)
-    assert torch.equal(paged_shared_attention(q, k, v, table, pos, strided, torch.stack((shared, shared), 1)[:, 0]), first)
+    first = attend(q, k, v, table, pos, members, shared)
+    assert torch.equal(attend(q, k, v, table, pos, strided, torch.stack((shared, shared), 1)[:, 0]), first)
     none = members[:, :0]
     assert torch.equal(paged_shared_attention(q, k, v, table, pos, none, shared), paged_attention(q, k, v, table, pos))
 
 
 def test_tokens_before_the_end_of_the_shared_pages():
     """Set back into the prompt, not yet begun, past the table; pages that are not there in the prompt and behind it."""
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(8, 2, 128, 16, [(6, [5, 40, 9, 20])], [30], 2, torch.bfloat16, "cuda")
+    q, k, v, table, pos, members, shared = shared_case(8, 2, 128, 16, [(6, [5, 40, 9, 20])], [30], 2, torch.bfloat16, "cuda")
     of = [b for b in members[0].tolist() if b >= 0]
     pos[of[0]] = torch.tensor([3, 90], device="cuda")
     pos[of[1]] = torch.tensor([-1, 17], device="cuda")
@@ -119,11 +138,11 @@ def test_tokens_before_the_end_of_the_shared_pages():
     table[of, 4] = 1 << 30
     table[of[3], 7] = -1
     for window, sinks in ((0, 0), (20, 5)):
-        y = paged_shared_attention(q, k, v, table, pos, members, shared, window, sinks)
+        y = attend(q, k, v, table, pos, members, shared, window, sinks)
         ref, spread = oracle.attention(q, k, v, table, pos, window, sinks)
         _check(y, ref, spread, torch.bfloat16, _keys(table, k))
     table[of] = -1
-    y = paged_shared_attention(q, k, v, table, pos, members, shared)
+    y = attend(q, k, v, table, pos, members, shared)
     assert torch.equal(y[of], torch.zeros_like(y[of]))
 
 
@@ -131,7 +150,7 @@ def test_tokens_before_the_end_of_the_shared_pages():
 @pytest.mark.parametrize("dim", [64, 128])
 def test_values_that_a_token_does_not_see_do_not_reach_it(dim, tokens):
     """An infinity or NaN in shared pages for the members that see it and no others, whatever rows are computed together."""
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(8, 2, dim, 16, [(6, [30, 40, 29])], [30], tokens, torch.bfloat16, "cuda")
+    q, k, v, table, pos, members, shared = shared_case(8, 2, dim, 16, [(6, [30, 40, 29])], [30], tokens, torch.bfloat16, "cuda")
     of = [b for b in members[0].tolist() if b >= 0]
     page = int(table[of[0], 3])  # positions 48 to 63
     v[page, 0, 5] = math.inf
@@ -142,7 +161,7 @@ def test_values_that_a_token_does_not_see_do_not_reach_it(dim, tokens):
     pos[of[2]] = 52              # sees none of them
     window, sinks = 70, 0        # member 0 is past the first with 126 - 69 = 57 on, member 1 with 67 on
     for w in (0, window):
-        y = paged_shared_attention(q, k, v, table, pos, members, shared, w, sinks)
+        y = attend(q, k, v, table, pos, members, shared, w, sinks)
         ref, spread = oracle.attention(q, k, v, table, pos, w, sinks)
         odd = ~torch.isfinite(ref)
         assert odd.any() and not odd[of[2]].any()
@@ -153,9 +172,9 @@ def test_values_that_a_token_does_not_see_do_not_reach_it(dim, tokens):
 
 
 def test_attention_of_large_scores():
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(8, 2, 128, 16, [(9, [30, 4])], [3], 1, torch.float16, "cuda")
+    q, k, v, table, pos, members, shared = shared_case(8, 2, 128, 16, [(9, [30, 4])], [3], 1, torch.float16, "cuda")
     q, k = q * 20, k.nan_to_num(0.0) * 20  # scores of thousands: one key takes all
-    y = paged_shared_attention(q, k, v, table, pos, members, shared)
+    y = attend(q, k, v, table, pos, members, shared)
     ref, _ = oracle.attention(q, k, v, table, pos)
     # scores up to 9000 in fp32 are off by 128 * 9000 * 2^-24 = 0.07 at most: weights by 15% where two are near
     top = (y.double().cpu() - ref).abs()
@@ -163,8 +182,8 @@ def test_attention_of_large_scores():
 
 
 def test_attention_takes_strided_tensors_and_a_scale():
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(8, 2, 128, 16, [(4, [5, 9])], [70], 3, torch.float16, "cuda")
-    want = paged_shared_attention(q, k, v, table, pos, members, shared, scale=0.05)
+    q, k, v, table, pos, members, shared = shared_case(8, 2, 128, 16, [(4, [5, 9])], [70], 3, torch.float16, "cuda")
+    want = attend(q, k, v, table, pos, members, shared, scale=0.05)
     ref, spread = oracle.attention(q, k, v, table, pos, scale=0.05)
     _check(want, ref, spread, torch.float16, _keys(table, k))
     wide = torch.full((3, 3, q.shape[2] + 24), math.nan, dtype=q.dtype, device="cuda")
@@ -174,18 +193,18 @@ def test_attention_takes_strided_tensors_and_a_scale():
     odd = torch.empty(q.numel() + 3, dtype=q.dtype, device="cuda")[3:].view(q.shape).copy_(q)
     for qq, tt, pp in ((wide[..., 8:8 + q.shape[2]], broad[:, 1:1 + table.shape[1]], pos), (odd, table.t().contiguous().t(), pos),
                        (q.transpose(0, 1).contiguous().transpose(0, 1), table, torch.stack((pos, pos), 2)[..., 0])):
-        assert torch.equal(paged_shared_attention(qq, k, v, tt, pp, members, shared, scale=0.05), want)
+        assert torch.equal(attend(qq, k, v, tt, pp, members, shared, scale=0.05), want)
     spread_out = torch.stack((k, k), 1)[:, 0]  # pools that are not contiguous run torch ops
-    y = paged_shared_attention(q, spread_out, v, table, pos, members, shared, scale=0.05)
+    y = attend(q, spread_out, v, table, pos, members, shared, scale=0.05)
     _check(y, ref, spread, torch.float16, _keys(table, k))
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.07])
 @pytest.mark.parametrize("members", [3, 20])
 def test_attention_with_scales_that_are_not_positive(members, scale):
-    q, k, v, table, pos, lists, shared = fork_oracle.shared_case(8, 2, 128, 16, [(9, [30, 4, 70][:members] + [5] * (members - 3))], [40],
+    q, k, v, table, pos, lists, shared = shared_case(8, 2, 128, 16, [(9, [30, 4, 70][:members] + [5] * (members - 3))], [40],
                                                                  1, torch.bfloat16, "cuda")
-    y = paged_shared_attention(q, k, v, table, pos, lists, shared, scale=scale)
+    y = attend(q, k, v, table, pos, lists, shared, scale=scale)
     ref, spread = oracle.attention(q, k, v, table, pos, scale=scale)
     _check(y, ref, spread, torch.bfloat16, _keys(table, k))
 
@@ -193,15 +212,15 @@ def test_attention_with_scales_that_are_not_positive(members, scale):
 @pytest.mark.parametrize("members", [3, 20])
 def test_members_that_have_ended(members):
     """A sequence without tokens whose row of the table is gone leaves the others theirs, wherever it stands."""
-    case = fork_oracle.shared_case(8, 2, 64, 16, [(5, [9] * members)], [], 1, torch.float16, "cuda")
+    case = shared_case(8, 2, 64, 16, [(5, [9] * members)], [], 1, torch.float16, "cuda")
     q, k, v, table, pos, lists, shared = case
     for gone in (0, 1, members - 1):
         pos[gone], table[gone] = -1, -1
-        y = paged_shared_attention(q, k, v, table, pos, lists, shared)
+        y = attend(q, k, v, table, pos, lists, shared)
         ref, spread = oracle.attention(q, k, v, table, pos)
         _check(y, ref, spread, torch.float16, _keys(table, k))
     pos[:], table[:] = -1, -1
-    assert not paged_shared_attention(q, k, v, table, pos, lists, shared).any()
+    assert not attend(q, k, v, table, pos, lists, shared).any()
 
 
 def test_attention_of_nothing_and_of_other_types():
@@ -218,16 +237,18 @@ def test_attention_of_nothing_and_of_other_types():
     assert q.grad is not None and torch.isfinite(q.grad).all()
 
 
-def test_more_sequences_than_a_launch_lists():
-    """Past the kernel's list of work the call is paged_attention's."""
-    q, k, v, table, pos, members, shared = fork_oracle.shared_case(2, 1, 64, 16, [(2, [1] * 1100)], [], 1, torch.float16, "cuda", spare=1)
-    y = paged_shared_attention(q, k, v, table, pos, members, shared)
-    assert torch.equal(y, paged_attention(q, k, v, table, pos))
+def test_calls_that_are_the_plain_attentions():
+    """Past the kernel's list of work, with many tokens a sequence, and small."""
+    q, k, v, table, pos, members, shared = fork_oracle.shared_case(2, 1, 64, 16, [(2, [1] * 1100)], [], 1, torch.float16, "cuda", spare=1, read=1 << 28)
+    assert torch.equal(paged_shared_attention(q, k, v, table, pos, members, shared), paged_attention(q, k, v, table, pos))
     some = torch.arange(900, device="cuda")
     keep = torch.where((members >= 0) & (members < 900), members, -1)
-    y = paged_shared_attention(q[some], k, v, table[some], pos[some], keep, shared)
+    y = attend(q[some], k, v, table[some], pos[some], keep, shared)
     ref, spread = oracle.attention(q[some], k, v, table[some], pos[some])
     _check(y, ref, spread, torch.float16, _keys(table, k))
+    for case in (shared_case(8, 1, 64, 16, [(2, [9, 30])], [], 9, torch.float16, "cuda"),
+                 fork_oracle.shared_case(8, 1, 64, 16, [(2, [9, 30])], [], 1, torch.float16, "cuda")):
+        assert torch.equal(paged_shared_attention(*case), paged_attention(*case[:5]))
 
 
 def test_attention_past_32_bit_offsets():
@@ -238,10 +259,11 @@ def test_attention_past_32_bit_offsets():
     far = 2 * pages - 4
     k[far:].normal_(generator=g)
     v[far:].normal_(generator=g)
-    table = torch.tensor([[far, far + 1, far + 2], [far, far + 1, far + 3]], dtype=torch.int32, device="cuda")
+    table = torch.full((2, 1024), -1, dtype=torch.int32, device="cuda")
+    table[:, :3] = torch.tensor([[far, far + 1, far + 2], [far, far + 1, far + 3]])
     pos = torch.tensor([[40], [45]], device="cuda")
     q = torch.randn(2, 1, 8 * D, device="cuda", generator=g).half()
-    y = paged_shared_attention(q, k, v, table, pos, torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"),
+    y = attend(q, k, v, table, pos, torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"),
                                torch.tensor([2], dtype=torch.int32, device="cuda"))
     ref, spread = oracle.attention(q, k[far:], v[far:], torch.where(table >= 0, table - far, -1), pos)
     _check(y, ref, spread, torch.float16, 48)
@@ -253,7 +275,7 @@ def test_captured_calls_follow_their_tensors(native, monkeypatch):
     if not native:
         for name in ("_native_shared", "_native_copy", "_native_score"):
             monkeypatch.setattr(serve, name, None)
-    cases = [fork_oracle.shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [100, 7], 1, torch.float16, "cuda", seed=i) for i in range(2)]
+    cases = [shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [100, 7], 1, torch.float16, "cuda", seed=i) for i in range(2)]
     logits = torch.randn(5, 5001, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).half()
     tokens = torch.arange(5, device="cuda")
     source, target = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (0, 1))
@@ -263,12 +285,12 @@ def test_captured_calls_follow_their_tensors(native, monkeypatch):
         stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(stream):
             for _ in range(2):
-                paged_shared_attention(*case)
+                attend(*case)
                 token_logprobs(logits, tokens, 4)
         torch.cuda.current_stream().wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            y = paged_shared_attention(*case)
+            y = attend(*case)
             s = token_logprobs(logits, tokens, 4)
         graphs.append(graph)
         outs.append((y, s))
@@ -299,21 +321,21 @@ def test_captured_calls_follow_their_tensors(native, monkeypatch):
             _check(y, ref, spread, torch.float16, _keys(table, k))
             fork_oracle.check_score(s, fork_oracle.score(logits, tokens, 4, 1.0))
             assert torch.equal(spare[step % 4], spare[(step + 1) % 4])
-            assert torch.equal(y, paged_shared_attention(*case))
+            assert torch.equal(y, attend(*case))
 
 
 def test_calls_on_two_streams():
-    cases = [fork_oracle.shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [600, 7], 1, torch.bfloat16, "cuda", seed=i) for i in range(2)]
+    cases = [shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [600, 7], 1, torch.bfloat16, "cuda", seed=i) for i in range(2)]
     logits = [torch.randn(40, 20011, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)) for i in range(2)]
     tokens = torch.arange(40, device="cuda")
-    want = [(paged_shared_attention(*c), token_logprobs(x, tokens, 5)) for c, x in zip(cases, logits)]
+    want = [(attend(*c), token_logprobs(x, tokens, 5)) for c, x in zip(cases, logits)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in cases]
     got = [[], []]
     for _ in range(10):
         for i, stream in enumerate(streams):
             with torch.cuda.stream(stream):
-                got[i].append((paged_shared_attention(*cases[i]), token_logprobs(logits[i], tokens, 5)))
+                got[i].append((attend(*cases[i]), token_logprobs(logits[i], tokens, 5)))
     torch.cuda.synchronize()
     for i in range(2):
         for y, s in got[i]:
@@ -322,7 +344,7 @@ def test_calls_on_two_streams():
 
 def test_calls_through_python_equal_those_through_the_library_of_operators(monkeypatch):
     assert None not in (serve._native_shared, serve._native_copy, serve._native_score)
-    case = fork_oracle.shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [100, 7], 2, torch.float16, "cuda")
+    case = shared_case(8, 2, 128, 16, [(30, [5, 40, 9])], [100, 7], 2, torch.float16, "cuda")
     logits, tokens = torch.randn(2, 7, 3001, device="cuda").bfloat16(), torch.randint(-1, 3001, (2, 7), device="cuda")
     pools = [torch.randn(9, 33, device="cuda") for _ in range(3)]
     source, target = torch.tensor([[0, 3, 8, 9], [1, 2, -1, 4]], dtype=torch.int32, device="cuda").unbind(0)
@@ -330,7 +352,7 @@ def test_calls_through_python_equal_those_through_the_library_of_operators(monke
     def everything():
         mine = [p.clone() for p in pools]
         copy_pages(mine, source, target)
-        return [paged_shared_attention(*case), *token_logprobs(logits[:, :-1], tokens[:, 1:], 6, 0.9), *mine]
+        return [attend(*case), *token_logprobs(logits[:, :-1], tokens[:, 1:], 6, 0.9), *mine]
 
     native = everything()
     for name in ("_native_shared", "_native_copy", "_native_score"):
@@ -493,7 +515,7 @@ def test_score_past_32_bit_offsets():
 
 # ---------------------------------------------------------------------------------------- together
 
-def test_a_model_answers_a_prompt_several_times():
+def test_a_model_answers_a_prompt_several_times(monkeypatch):
     """A prompt, its forks, their tokens decoded together in a captured step and scored; pages written after a fork are each
     sequence's own, and the cache moved together keeps what it holds."""
     shape = LlamaShape(hidden=1024, layers=3, heads=8, kv_heads=2, ffn=1408, vocab=1003)
@@ -503,8 +525,11 @@ def test_a_model_answers_a_prompt_several_times():
     answers, P, page, more = 5, 75, 16, 8
     prompt = torch.randint(0, shape.vocab, (P,), device="cuda", generator=g)
     texts = torch.randint(0, shape.vocab, (answers, more), device="cuda", generator=g)
+    calls = []
+    monkeypatch.setattr(serve, "_WORTH_SHARING", 1)
+    monkeypatch.setattr(serve, "paged_shared_attention", lambda *x: calls.append(1) or attend(*x))
     with torch.no_grad():
-        caches = [PagedKVCache(shape, answers, 60, page, 120, "cuda", torch.float16) for _ in range(2)]
+        caches = [PagedKVCache(shape, answers, 60, page, 40000, "cuda", torch.float16) for _ in range(2)]
         alone, forked = caches
         for b in range(answers):
             alone.reserve(b, P + more)
@@ -544,3 +569,4 @@ def test_a_model_answers_a_prompt_several_times():
             # the two ways round the probabilities' sums apart: fp16 steps of the hidden states, some layers of them
             assert (logits[live] - want[live]).abs().max() < 0.05 * want.abs().max()
             fork_oracle.check_score([s[live] for s in scores], fork_oracle.score(logits[live], ids[live], 4, 1.0))
+    assert len(calls) >= 2 * shape.layers and forked.saved == 3 * 4 * page * 2 * 2 * 128 * 2  # of four members, four pages
