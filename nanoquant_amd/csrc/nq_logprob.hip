@@ -1,9 +1,16 @@
 // Log probabilities of given tokens, the entropy and the most probable alternatives.
 //
 // All rows' chunks (32 or 16 logits a thread of a block, in the 16-bit types and in fp32) are one line of units, cut into equal
-// shares for the blocks. A block goes through its share once: sums of e = 2^d and e d, d = (x - ref) log2(e) / T, with each
+// shares for the blocks. A block goes through its share once: sums of e = 2^d and e d, d = x log2(e) / T - ref, with each
 // wave's ref moved up to its largest logit wherever that is 8 octaves above it; and the `top` largest logits so far, each wave's
 // in its lanes. A row that lies in one share is finished by its block, parts of others are joined by join_kernel.
+//
+// Bound by the read: 2111 rows of 100003 bf16 logits with the largest, 422 MB, 84 us (5.0 TB/s, a
+// large copy's rate); 777 rows of 32000 in fp16, 50 MB, 14.5 us in one launch. Few rows by latency: one row of 32000 in
+// fp32 with five alternatives 8.6 us, of which the launch and the first chunk's way, the sums and the lists' join are one chain;
+// 64 rows of 100003 with twenty alternatives 11.8 and 5.8 the join's. The 2111 rows
+// with several passes over each row 589 us; in one pass with the alternatives in LDS 143; with them in lanes and bounds from
+// ballots 102; with five blocks a CU 93.
 #include <algorithm>
 #include <cmath>
 

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void spans_kernel(const PagedArgs a, int group
 // fill each other's waits; they read each operand twice as often as RW 2's for the same rows. Their sums are joined through
 // LDS. (A half of each tile's keys to either, in step at every barrier: a prompt of 1000 tokens 28.5 us against 25.3.)
 // Bound by products and exponentials of a wave in turn: 4001 tokens of 64 heads of 8 kv heads under a window of 2047, RW 2,
-// 329 us (822 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
+// 319 us (848 TFLOP/s, where a large matrix product runs at 1345): of a tile's 5500 cycles 2050 are products, 2000 vector
 // instructions, of which about half overlap, 1100 waits for LDS and barriers, 480 scalar instructions. A prompt of 1000 tokens,
 // 32 heads, RW 1: 25.3 us, of which the longest row group's 16 tiles take 16.
 // kShared: the work of all row groups in equal shares over the grid, as few_kernel's; otherwise a block takes a row group,
