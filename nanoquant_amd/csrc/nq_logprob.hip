@@ -81,7 +81,8 @@ struct ScoreArgs {
     float* top_logprobs;
     float scale;  // log2(e) / temperature
     int rows, vocab, top;
-    int chunks;      // of a row
+    int chunks;      // of a row, up to a whole number of shares where its parts are blocks'
+    int full;        // those that it has
     int64_t share;   // chunks of a block
     int64_t units;   // of all rows
     float4* sums;    // [blocks][2]: ref, s, d
@@ -219,6 +220,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
         const int c0 = static_cast<int>(u - at_row * a.chunks), c1 = static_cast<int>(min<int64_t>(a.chunks, c0 + end - u));
         u += c1 - c0;
         const bool whole = c0 == 0 && c1 == a.chunks;
+        const int last = min(c1, a.full);
         const Row row(a.logits, a.first(at_row), a.vocab);
         u32x4 next[4];
         row.load_once(c0, next);
@@ -228,11 +230,11 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
         TopList list;
         float most_yet = -INFINITY;
         int turn = 0;
-        for (int c = c0; c < c1; ++c) {
+        for (int c = c0; c < last; ++c) {
             u32x4 v[4];
 #pragma unroll
             for (int p = 0; p < 4; ++p) v[p] = next[p];
-            if (c + 1 < c1) row.load_once(c + 1, next);
+            if (c + 1 < last) row.load_once(c + 1, next);
             const bool edge = row.at_edge(c);
             if (edge) {
 #pragma unroll
@@ -451,24 +453,25 @@ constexpr int64_t kMaxVocab = int64_t{1} << 30;
 
 struct Plan {
     bool wide = false;  // blocks of 1024 threads, else of 256
-    int64_t chunks = 0, share = 0, blocks = 0;
+    int64_t chunks = 0, full = 0, share = 0, blocks = 0;
     size_t sums = 0, bytes = 0;
     bool joined() const { return share % chunks != 0; }
 };
 
 Plan make_plan(int64_t rows, int64_t vocab, int64_t top, int piece) {
     Plan p;
-    // Rows that leave CUs idle are cut up wide, a block a CU: 150 rows of 32000 9.1 us a block of 256 threads for 8192 logits, 7.0 a
-    // block of 1024 a row; 300 rows 9.0 and 12.3. (fp16 without alternatives)
-    p.wide = rows <= kCUs && vocab >= 16384;
+    // Rows that leave CUs idle are for wide blocks, one a CU: 150 rows of 32000 9.1 us a block of 256 threads for 8192 logits, 7.0 a
+    // block of 1024 a row; 300 rows 9.0 and 12.3. (fp16 without alternatives) Each row in as many alike parts as there are CUs for
+    // it, so that no block has parts of two: 180 rows of 128000 in fp32 with the largest 20.9 us, 26.5 in equal shares of all.
+    p.wide = rows <= kCUs && vocab >= 8192;
     const int64_t chunk = (p.wide ? 1024 : 256) * 4 * piece;
-    p.chunks = ceil_div(vocab + piece - 1, chunk);
-    const int64_t units = rows * p.chunks;
-    // Whole rows need no second launch to join their parts, 5 us
-    if (p.wide) p.share = p.chunks <= 2 ? p.chunks : ceil_div(units, kCUs);
-    else if (rows >= kCUs && rows <= kPerCU * kCUs) p.share = p.chunks;
-    else p.share = ceil_div(units, kPerCU * kCUs);
-    p.blocks = ceil_div(units, p.share);
+    p.full = ceil_div(vocab + piece - 1, chunk);
+    // Whole rows need no second launch to join their parts, 5 us: 777 rows of 32000 14.4 us, 19.5 cut; 100 of 16000 11.2 and 15.0
+    if (p.wide) p.share = p.full <= 2 ? p.full : ceil_div(p.full, kCUs / rows);
+    else if (rows <= kPerCU * kCUs) p.share = p.full;
+    else p.share = ceil_div(rows * p.full, kPerCU * kCUs);
+    p.chunks = p.wide ? ceil_div(p.full, p.share) * p.share : p.full;
+    p.blocks = ceil_div(rows * p.chunks, p.share);
     p.sums = static_cast<size_t>(p.blocks) * 2 * sizeof(float4);
     p.bytes = p.joined() ? p.sums + static_cast<size_t>(p.blocks) * 2 * top * sizeof(uint64_t) : 0;
     return p;
@@ -543,6 +546,7 @@ int nq_token_logprobs(int dtype, const void* logits, int64_t batch_stride, int64
     a.vocab = static_cast<int>(vocab);
     a.top = static_cast<int>(top);
     a.chunks = static_cast<int>(plan.chunks);
+    a.full = static_cast<int>(plan.full);
     a.share = plan.share;
     a.units = batch * rows * plan.chunks;
     a.sums = static_cast<float4*>(workspace);

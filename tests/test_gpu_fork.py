@@ -426,6 +426,17 @@ def test_score(shape, V, top, temperature, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, *HALF], ids=["f32", *IDS])
+@pytest.mark.parametrize("rows,V,top", [(70, 100003, 3), (37, 128000, 64), (129, 70001, 2), (256, 8192, 1), (257, 8192, 4), (1280, 4097, 2),
+                                        (1281, 8193, 5), (1301, 20011, 40), (1500, 3000, 0)])
+def test_score_of_rows_in_parts(rows, V, top, dtype):
+    """Parts that end with a row and those that do not, rows whole, on both sides of where the kernel cuts otherwise."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    logits = (torch.randn(rows, V, device="cuda", generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, V, (rows,), device="cuda", generator=g)
+    fork_oracle.check_score(token_logprobs(logits, tokens, top), fork_oracle.score(logits, tokens, top, 1.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF], ids=["f32", *IDS])
 @pytest.mark.parametrize("V", [41, 9001, 70000])
 def test_score_of_odd_rows(V, dtype):
     logits, tokens = odd_rows(V, dtype)
