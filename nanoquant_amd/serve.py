@@ -19,8 +19,8 @@ float16 and bfloat16 tensors on the GPU run the HIP library (``nq_paged_rope_wri
 ``nq_verify_drafts``, ``nq_paged_shared_attention``, ``nq_copy_pages``, ``nq_token_logprobs``); CPU tensors, float32 models,
 calls that are differentiated, head sizes other than 64 and 128 and page sizes that are no multiple of 16 run torch ops with the
 same results but for rounding, in float32, or in float64 where the tensors are. Pages of any type are copied by the library,
-and logits in float32 scored and verified by it. The reference has no counterpart: its harness decodes one batch on Hugging Face's static cache and samples one
-token a step (``src/nanoquant/kernel/test_decode.py:350-422``).
+and logits in float32 scored and verified by it. The reference has no counterpart: its harness decodes one batch on Hugging
+Face's static cache and samples one token a step (``src/nanoquant/kernel/test_decode.py:350-422``).
 """
 from __future__ import annotations
 
@@ -80,7 +80,8 @@ class PagedKVCache:
     ``members`` and ``shared`` (None before the first fork) say which sequences have their leading pages in common, as
     :func:`paged_shared_attention` takes it, and ``groups`` how many such groups there are; ``saved`` is what reading each
     group's pages once saves in a layer, in bytes. Their memory stays as long as no more groups and no larger ones come up than
-    ever before, so a graph captured with the largest follows their changes. The model's layers use them from 64 MB saved on.
+    ever before, so a graph captured with the largest follows their changes; one captured before reads groups of nobody from
+    then on, which is right, but reads each sequence's pages for itself. The model's layers use them from 64 MB saved on.
     """
 
     def __init__(self, shape, batch: int, pages: int, page_size: int, max_len: int, device, dtype, window: int = 0,
@@ -100,6 +101,7 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._owners = [0] * pages  # sequences that have a page
         self.members = self.shared = None
+        self._outgrown = []  # those that graphs captured earlier read
         self.groups = self.saved = 0
         self._common = [0] * batch  # entries that a sequence's row has in common with its group's
 
@@ -146,12 +148,16 @@ class PagedKVCache:
                 for b in sequences:
                     self._common[b] = common
         self.groups = len(lists)
-        page = 2 * self.k[0][0].numel() * self.k[0].element_size() if self.k else 0
-        self.saved = sum((len(sequences) - 1) * common * page for sequences, common in zip(lists, shared))
+        position = 2 * self.k[0][0, :, 0].numel() * self.k[0].element_size() if self.k else 0
+        most = self.window + self.sinks if self.window else self.max_len
+        seen = [min(common * self.page_size, most) for common in shared]
+        self.saved = sum((len(sequences) - 1) * n * position for sequences, n in zip(lists, seen))
         most = max(map(len, lists), default=0)
         if self.members is None or self.members.shape[0] < len(lists) or self.members.shape[1] < most:
             old = (0, 0) if self.members is None else self.members.shape
             shape = (max(old[0], len(lists)), max(old[1], most))
+            if self.members is not None:
+                self._outgrown.append((self.members.fill_(-1), self.shared.zero_()))
             self.members = torch.empty(shape, dtype=torch.int32, device=self.table.device)
             self.shared = torch.empty(shape[0], dtype=torch.int32, device=self.table.device)
         groups, most = self.members.shape

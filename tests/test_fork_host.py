@@ -78,6 +78,9 @@ def test_forks_share_whole_pages_and_copy_the_last():
     assert cache._host[2][:2] == cache._host[0][:2] == cache._host[5][:2] and len({cache._host[b][2] for b in (0, 2, 5)}) == 3
     assert cache.groups == 1 and sorted(b for b in cache.members[0].tolist() if b >= 0) == [0, 2, 5] and int(cache.shared[0]) == 2
     assert cache.saved == 2 * 2 * 4 * (2 * 2 * 32 * 4)  # twice two pages of four positions' keys and values
+    cache.window, cache.sinks = 4, 1
+    cache._regroup()
+    assert cache.saved == 2 * 5 * (2 * 2 * 32 * 4)
     assert len(cache._free) == 12 - 5
     for b in (0, 2, 5):
         assert all(torch.equal(x, y) for x, y in zip(_contents(cache, b, 10), want))
@@ -360,6 +363,22 @@ def test_refusals():
         with pytest.raises(ValueError, match="temperature"):
             token_logprobs(logits, tokens, temperature=bad)
     assert [tuple(x.shape) for x in token_logprobs(logits[:0], tokens[:0], 2)] == [(0,), (0,), (0, 2), (0, 2)]
+
+
+def test_groups_that_outgrow_their_tensors_leave_nobody_in_the_old_ones():
+    """A graph captured before reads the old tensors on."""
+    cache = _cache()
+    cache.reserve(0, 9)
+    cache.fork(0, [1], 9)
+    members, shared = cache.members, cache.shared
+    assert members.tolist() == [[0, 1]] and shared.tolist() == [2]
+    cache.release(1)
+    cache.fork(0, [3], 9)
+    assert cache.members is members and members.tolist() == [[0, 3]]
+    cache.fork(0, [4, 5], 9)
+    assert cache.members is not members and cache.members.tolist() == [[0, 3, 4, 5]]
+    assert members.tolist() == [[-1, -1]] and shared.tolist() == [0]
+    assert any(a is members and b is shared for a, b in cache._outgrown)  # their memory is nobody else's
 
 
 def test_c_abi_limits_of_shared_pages_need_no_gpu():
