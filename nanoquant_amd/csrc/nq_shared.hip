@@ -11,7 +11,7 @@ namespace {
 
 // Adds up what few_kernel or shared_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave a row,
 // D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 4.1 us for 128 rows, 9.3 for 8192 of
-// 128 dimensions, with several parts a row on their way at once.
+// 128 dimensions, with several parts a row on their way at once (with half or twice as many 3 us more).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int64_t count) {
     constexpr int L4 = D / 4, Groups = 64 / L4, kAhead = 4;
@@ -85,20 +85,20 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
     if (grp == 0) *reinterpret_cast<uint2*>(a.out + row * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
-// Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as few_kernel
-// does, half a block each, in equal shares; all of them work out the same list. One launch, since the sequences' part is bound by
-// the read of keys and values and the groups' by products: in two launches, each on all CUs, 16 sequences with 8000 shared keys
-// 47 us against 36, 60 conversations 179 against 152, 128 samples under a window 221 against 161.
-// Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 25 us, bound by latency (the list,
-// the first tiles' way, the waves' join); 60 in five groups with 100 to 4000 of their own 146, bound by the read (5.0 TB/s, a
-// large copy's rate); 128 under a window of 12011 keys 155, bound by rows_segments' products and exponentials, of which
-// the tiles in which windows begin take twice. 11 sequences of 5 tokens, heads of 64, 5000 shared keys: 23 us.
-// How many blocks either gets goes by what a
-// unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how much longer the groups' blocks take
-// for their beginning and their end.
-constexpr float kGroupTime = 1200.0f, kGroupTime64 = 700.0f, kOwnTime = 400.0f, kGroupMore = 4000.0f;
-constexpr int kGroupStart = 8, kOwnStart = 6;  // what a segment costs on top of its tiles, in tiles
+// Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as
+// few_kernel does, a team of two waves each, in equal shares; all of them work out the same list. One launch, since the
+// sequences' part is bound by the read of keys and values and the groups' by products: in two launches, each on all CUs, 16
+// sequences with 8000 shared keys 47 us against 36, 60 conversations 179 against 152, 128 samples under a window 221 against
+// 161. Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 25 us, bound by latency
+// (the list, the first tiles' way, the waves' join); 60 in five groups with 100 to 4000 of their own 146, bound by the read
+// (5.0 TB/s, a large copy's rate); 128 under a window of 12011 keys 155, bound by rows_segments' products and exponentials, of
+// which the tiles in which windows begin take twice. 11 sequences of 5 tokens, heads of 64, 5000 shared keys: 23 us. How many
+// blocks either gets goes by what a unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how
+// much longer the groups' blocks take for their beginning and their end.
+constexpr float kGroupTime = 1200.0f, kGroupTime64 = 700.0f, kOwnTime = 400.0f, kOwnTime64 = 350.0f, kGroupMore = 4000.0f;
+constexpr int kGroupStart = 8, kOwnStart = 4;  // what a segment costs on top of its tiles, in tiles
 constexpr int kGroupTile = 128;
+constexpr int kTeams = 4;  // of a block's waves, for sequences' own keys: 40 samples of a prompt, 32 kv heads, 48.0 us, two teams 49.8
 constexpr int kLeastGroupTiles = 6;  // of a block's share, starts among them
 
 // Blocks of kCUs for groups' work such that both parts end together, of the numbers 4 lane + 2.
@@ -107,26 +107,26 @@ __device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units) 
     if (group_units == 0) return 0;
     const int n = 4 * (static_cast<int>(threadIdx.x) & 63) + 2;
     const float g = static_cast<float>(group_units) * (D == 128 ? kGroupTime : kGroupTime64) * __builtin_amdgcn_rcpf(static_cast<float>(n));
-    const float s = static_cast<float>(own_units) * kOwnTime * __builtin_amdgcn_rcpf(static_cast<float>(kCUs - n));
+    const float s = static_cast<float>(own_units) * (D == 128 ? kOwnTime : kOwnTime64) * __builtin_amdgcn_rcpf(static_cast<float>(kCUs - n));
     const int late = __popcll(__ballot(g + kGroupMore > s));  // the lanes at which the groups' part ends last: the first ones
     return min(4 * late + 2, kCUs - 2);
 }
 
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
-    constexpr int kThreads = 512, W = kThreads / 128;  // waves of a half
+    constexpr int kThreads = 512, W = kThreads / 64 / kTeams;  // waves of a team
     __shared__ __attribute__((aligned(16))) union {
-        uint16_t few[2][W][FewShape<D, RT>::kStages][2][kTile * D];
+        uint16_t few[kTeams][W][FewShape<D, RT>::kStages][2][kTile * D];
         RowsRings<D> rows;
     } rings;
     __shared__ int64_t pre[kEntries + 1];
     __shared__ GroupPlan<kEntries> plan;
     __shared__ int64_t wave_total[kThreads / 64];
     __shared__ union {
-        FewMarks<W> few[2];
+        FewMarks<W> few[kTeams];
         RowsMarks rows;
     } marks;
-    __shared__ int first_entry[2], arrived[2];
+    __shared__ int first_entry[kTeams], arrived[kTeams];
     const int of_groups = a.entries_of_groups(), entries = of_groups + a.batch * a.row_groups;
     plan_groups<kThreads>(a, plan);
     prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
@@ -141,22 +141,22 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
         const Shares shares = take_share<kThreads>(a, 0, of_groups, block, for_groups, kLeastGroupTiles, pre, first_entry);
         if (shares.entry >= 0) rows_segments<T, D, 1, true, kGroupStart>(a, shares, shares.entry, rings.rows, pre, plan, marks.rows);
     } else {
-        // the halves of the block go their own ways, so that one's first tiles come and its waves' sums are joined among the
-        // other's products
-        const int half = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 8), at = 2 * (block - for_groups);
-        if (threadIdx.x < 4) marks.few[threadIdx.x >> 1].tainted[threadIdx.x & 1] = 0;
-        if (threadIdx.x < 2) arrived[threadIdx.x] = 0;
-        Shares shares = share_of(a, of_groups, entries, at + half, 2 * (kCUs - for_groups), W, pre);
-        const int64_t next = shares.first + (half == 0 ? shares.share : -shares.share);  // the other half's first unit
-        for (int e = of_groups + static_cast<int>(threadIdx.x); e < entries; e += kThreads) {
-            if (holds_unit(a, pre, e, shares.first)) first_entry[half] = e;
-            if (holds_unit(a, pre, e, next)) first_entry[1 - half] = e;
-        }
+        // the teams of the block go their own ways, so that one's first tiles come and its waves' sums are joined among the
+        // others' products
+        const int team = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / (64 * W)), at = kTeams * (block - for_groups);
+        if (threadIdx.x < 2 * kTeams) marks.few[threadIdx.x >> 1].tainted[threadIdx.x & 1] = 0;
+        if (threadIdx.x < kTeams) arrived[threadIdx.x] = 0;
+        Shares shares = share_of(a, of_groups, entries, at + team, kTeams * (kCUs - for_groups), W, pre);
+        const int64_t first = shares.first - team * shares.share;  // the block's first unit
+        for (int e = of_groups + static_cast<int>(threadIdx.x); e < entries; e += kThreads)
+#pragma unroll
+            for (int i = 0; i < kTeams; ++i)
+                if (holds_unit(a, pre, e, first + i * shares.share)) first_entry[i] = e;
         __syncthreads();
         if (shares.first >= shares.end) return;
-        shares.entry = __builtin_amdgcn_readfirstlane(first_entry[half]);
-        few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few[half], pre, plan.spans, plan, marks.few[half],
-                                                   static_cast<int>(threadIdx.x) & 255, WavesSync<W>{&arrived[half]});
+        shares.entry = __builtin_amdgcn_readfirstlane(first_entry[team]);
+        few_segments<T, D, RT, true, W, kOwnStart>(a, shares, shares.entry, rings.few[team], pre, plan.spans, plan, marks.few[team],
+                                                   static_cast<int>(threadIdx.x) % (64 * W), WavesSync<W>{&arrived[team]});
     }
 }
 
@@ -191,11 +191,11 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
     if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
     if (batch * each * kv_heads > kMaxThreads / 64) return p;  // rows of group_join_kernel, a wave each
-    constexpr int64_t kHalves = 2 * kCUs;  // or blocks, two on a CU
+    constexpr int64_t kParts = (kTeams > 2 ? kTeams : 2) * kCUs;  // teams, or blocks, two on a CU
     p.own_first = kv_heads * of_groups * p.group_kept;
     p.own_later = p.own_first + kv_heads * own * p.rows_kept;
-    p.group_later = p.apart ? p.own_later + kHalves * p.own_tile : p.own_later;
-    const int64_t parts = p.group_later + (p.apart ? kCUs : kHalves) * p.group_tile;
+    p.group_later = p.apart ? p.own_later + kParts * p.own_tile : p.own_later;
+    const int64_t parts = p.group_later + (p.apart ? kCUs : kParts) * p.group_tile;
     p.tiles = tiles;
     p.part_o = static_cast<size_t>(parts * head_dim) * sizeof(float);
     p.part_ml = static_cast<size_t>(ceil_div(parts, 2) * 2) * sizeof(float2);
