@@ -541,35 +541,58 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             these.rows = min(Group, rows.rows - group0);
             slow_rows<T, D>(a, these, kvh, tiles, kKeys, first, n, done, parts, wave, static_cast<int>(blockDim.x) >> 6);
         }
-        // the halves' sums: the second group's through the key ring, its statistics through the value ring's first 2 KB
-        if (RW == 1 && !tainted) {
-            float* red = reinterpret_cast<float*>(&kring[0][0]);
-            float* stat = reinterpret_cast<float*>(&vring[0][0]);
-            static_assert(RW == 2 || sizeof(kring) >= DT * 16 * 256 * sizeof(float), "the key ring holds a group's sums");
-            if (grp == 1) {
+        // the halves' sums: either wave of two with the same rows joins half of the dimensions, and has those of the other's from
+        // the key ring, the statistics from the value ring's first 4 KB
+        constexpr int DH = RW == 1 ? DT / 2 : DT, Cols = 32 * DH;  // of a wave
+        const int col0 = RW == 1 ? grp * Cols : 0;
+        f32x16 sums[RW][DH];
+        int at_lane = lane;  // whose places are worked out here: kept through the loop, they would take its registers
+        asm volatile("" : "+v"(at_lane));
+        const int ec = at_lane & 31, ekg = at_lane >> 5;
+        float* stage = reinterpret_cast<float*>(&kring[0][0]) + wave * (32 * Cols);  // of 32 rows
+        static_assert(sizeof(kring) >= (RW == 1 ? 8 : 4) * 32 * Cols * sizeof(float), "the key ring holds all waves' sums of 32 rows");
+        if constexpr (RW == 1) {
+            if (!tainted) {
+                float* theirs = reinterpret_cast<float*>(&kring[0][0]) + (wave ^ 4) * (32 * Cols) + at_lane;
+                float* stat = reinterpret_cast<float*>(&vring[0][0]) + 64 * rwave + at_lane;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int dt = 0; dt < DH; ++dt) {
+                    if (grp == 0) {
+                        sums[0][dt] = o[0][dt];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) red[(16 * dt + i) * 256 + (t & 255)] = o[0][dt][i];
-                stat[t & 255] = m[0];
-                stat[256 + (t & 255)] = l[0];
-            }
-            __syncthreads();
-            if (grp == 0) {
-                const float m1 = stat[t], mn = fmaxf(m[0], m1);
+                        for (int i = 0; i < 16; ++i) theirs[(16 * dt + i) * 64] = o[0][DH + dt][i];
+                    } else {
+                        sums[0][dt] = o[0][DH + dt];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) theirs[(16 * dt + i) * 64] = o[0][dt][i];
+                    }
+                }
+                stat[512 * grp] = m[0];
+                stat[512 * grp + 256] = l[0];
+                __syncthreads();
+                const float m0 = stat[0], m1 = stat[512], mn = fmaxf(m0, m1);
                 const float mu = mn == -INFINITY ? 0.0f : mn;
-                const float f0 = __builtin_amdgcn_exp2f(m[0] - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+                const float f0 = __builtin_amdgcn_exp2f(m0 - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
                 m[0] = mn;
-                l[0] = l[0] * f0 + stat[256 + t] * f1;
+                l[0] = stat[256] * f0 + stat[768] * f1;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int dt = 0; dt < DH; ++dt)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[0][dt][i] = o[0][dt][i] * f0 + red[(16 * dt + i) * 256 + t] * f1;
+                    for (int i = 0; i < 16; ++i) {
+                        const float mine = sums[0][dt][i], other = stage[(16 * dt + i) * 64 + at_lane];
+                        sums[0][dt][i] = (grp == 0 ? mine : other) * f0 + (grp == 0 ? other : mine) * f1;
+                    }
             }
+        } else {
+#pragma unroll
+            for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+                for (int dt = 0; dt < DH; ++dt) sums[rw][dt] = o[rw][dt];
         }
         // a wave's rows through LDS, a row tile at a time, then whole rows to memory
-        uint16_t* ob = (RW == 1 ? &vring[0][0] + 1024 : &kring[0][0]) + rwave * (32 * D);
-        if (grp == 0 && !tainted) {
+        constexpr int OC = Cols / 8, FC = Cols / 4;  // 16-byte chunks of a row, in the type and in fp32
+        uint16_t* ob = (RW == 1 ? &vring[0][0] + 2048 : &kring[0][0]) + wave * (32 * Cols);
+        if (!tainted) {
 #pragma unroll
             for (int rw = 0; rw < RW; ++rw) {
                 float L = l[rw] + __shfl_xor(l[rw], 32, 64);
@@ -580,38 +603,42 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
                 }
                 const float inv = 1.0f / L;
                 if (kShared && !done) {
-                    const int at = rwave * (32 * RW) + 32 * rw + c;
-                    if (row0 + 32 * rw + c < rows.rows) {
-                        const int64_t part = parts + at;
-                        if (kg == 0) a.part_ml[part] = float2{M, L};
+                    const int64_t part = parts + rwave * (32 * RW) + 32 * rw;
+                    if (ekg == 0 && col0 == 0 && row0 + 32 * rw + ec < rows.rows) a.part_ml[part + ec] = float2{M, L};
 #pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
+                    for (int dt = 0; dt < DH; ++dt)
 #pragma unroll
-                            for (int g4 = 0; g4 < 4; ++g4) {
-                                f32x4 x;
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            f32x4 x;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e];
-                                *reinterpret_cast<f32x4*>(a.part_o + part * D + 32 * dt + 8 * g4 + 4 * kg) = x;
-                            }
+                            for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : sums[rw][dt][4 * g4 + e];
+                            *reinterpret_cast<f32x4*>(stage + ec * Cols + 4 * ((8 * dt + 2 * g4 + ekg) ^ (ec & (FC - 1)))) = x;
+                        }
+#pragma unroll
+                    for (int j = 0; j < FC / 2; ++j) {
+                        const int r = (64 * j + at_lane) / FC, ch = at_lane % FC;
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(stage + r * Cols + 4 * (ch ^ (r & (FC - 1))));
+                        if (row0 + 32 * rw + r < rows.rows) *reinterpret_cast<f32x4*>(a.part_o + (part + r) * D + col0 + 4 * ch) = x;
                     }
                     continue;
                 }
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int dt = 0; dt < DH; ++dt)
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
                         float x[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : o[rw][dt][4 * g4 + e] * inv;
-                        *reinterpret_cast<uint2*>(ob + c * D + 8 * ((4 * dt + g4) ^ (c & (C - 1))) + 4 * kg) =
+                        for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : sums[rw][dt][4 * g4 + e] * inv;
+                        *reinterpret_cast<uint2*>(ob + ec * Cols + 8 * ((4 * dt + g4) ^ (ec & (OC - 1))) + 4 * ekg) =
                             uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
                     }
 #pragma unroll
-                for (int j = 0; j < 32 / RowsPer; ++j) {
-                    const int r = RowsPer * j + lane / C, ch = lane % C;
-                    const u32x4 v = *vec(ob + r * D + 8 * (ch ^ (r & (C - 1))));
+                for (int j = 0; j < OC / 2; ++j) {
+                    const int r = (64 * j + at_lane) / OC, ch = at_lane % OC;
+                    const u32x4 v = *vec(ob + r * Cols + 8 * (ch ^ (r & (OC - 1))));
                     const int at_row = row0 + 32 * rw + r;
-                    if (at_row < rows.rows) *reinterpret_cast<u32x4*>(a.out + out_row(a, rows.b, kvh, at_row) * D + 8 * ch) = v;
+                    if (at_row < rows.rows)
+                        *reinterpret_cast<u32x4*>(a.out + out_row(a, rows.b, kvh, at_row) * D + col0 + 8 * ch) = v;
                 }
             }
         }
