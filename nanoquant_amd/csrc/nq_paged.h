@@ -19,6 +19,18 @@ struct Pages {
     const int32_t* table;
     int64_t table_stride;
     int table_pages, pages, page_size;
+    uint32_t inverse;  // 2^shift / page_size, rounded up: with 2^31 below that, exact for what is below 2^31
+    int shift;
+    Pages() = default;
+    Pages(const int32_t* table_, int64_t stride, int64_t table_pages_, int64_t pages_, int64_t page_size_)
+        : table(table_), table_stride(stride), table_pages(static_cast<int>(table_pages_)), pages(static_cast<int>(pages_)),
+          page_size(static_cast<int>(page_size_)), shift(31) {
+        while ((int64_t{1} << (shift - 31)) < page_size_) ++shift;
+        inverse = static_cast<uint32_t>((uint64_t{1} << shift) / static_cast<uint64_t>(page_size_) + 1);
+    }
+    __device__ int slot_of(int key) const {  // key / page_size, in three instructions instead of thirty
+        return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * inverse >> shift);
+    }
     __device__ int64_t capacity() const { return static_cast<int64_t>(table_pages) * page_size; }
     __device__ int page(int b, int slot) const {
         const int at = table[static_cast<int64_t>(b) * table_stride + slot];

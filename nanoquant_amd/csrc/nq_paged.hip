@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteArgs a) {
         src = a.q + row * a.q_stride + static_cast<int64_t>(head) * a.head_dim + d;
         dst = a.q_out + (row * a.heads + head) * a.head_dim + d;
     } else {
-        const int slot_page = static_cast<int>(p) / a.pages.page_size;
+        const int slot_page = a.pages.slot_of(static_cast<int>(p));
         const int page = a.pages.page(static_cast<int>(row / a.tokens), slot_page);
         if (page < 0) return;
         const bool key = head < a.heads + a.kv_heads;
@@ -406,7 +406,7 @@ int nq_paged_rope_write(int dtype, const void* q, int64_t q_stride, const void* 
     a.cos = rope_cos;
     a.sin = rope_sin;
     a.positions = positions;
-    a.pages = Pages{table, table_stride, static_cast<int>(table_pages), static_cast<int>(pages), static_cast<int>(page_size)};
+    a.pages = Pages(table, table_stride, table_pages, pages, page_size);
     a.k_pages = static_cast<uint16_t*>(k_pages);
     a.v_pages = static_cast<uint16_t*>(v_pages);
     a.q_out = static_cast<uint16_t*>(q_out);
@@ -466,7 +466,7 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
     a.q_stride = q_stride;
     a.k_pages = static_cast<const uint16_t*>(k_pages);
     a.v_pages = static_cast<const uint16_t*>(v_pages);
-    a.pages = Pages{table, table_stride, static_cast<int>(table_pages), static_cast<int>(pages), static_cast<int>(page_size)};
+    a.pages = Pages(table, table_stride, table_pages, pages, page_size);
     a.positions = positions;
     a.out = static_cast<uint16_t*>(out);
     a.batch = static_cast<int>(batch);

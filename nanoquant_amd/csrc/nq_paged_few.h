@@ -367,10 +367,10 @@ __device__ inline void slow_rows(const Args& a, const Rows<Args>& rows, int kvh,
         for (int i = 0; i < N; ++i) o[i] = 0.0f;
         for (int tile = first; tile < first + n; ++tile)
             for (int key = tiles.at(tile) * keys; key < (tiles.at(tile) + 1) * keys; ++key) {
-                const int slot = key / a.pages.page_size;
+                const int slot = a.pages.slot_of(key);
                 const int page = slot < a.pages.table_pages ? a.pages.page(rows.b, slot) : -1;
                 if (key > last || !rows.holds(key) || !(key >= start || key < a.sinks) || page < 0) continue;
-                const int64_t at = ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D + lane;
+                const int64_t at = ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.pages.page_size + key - slot * a.pages.page_size) * D + lane;
                 float s = 0.0f;
                 for (int i = 0; i < N; ++i) s = fmaf(T::to_float(q[64 * i]), T::to_float(a.k_pages[at + 64 * i]), s);
                 s = wave_sum(s) * a.scale;
@@ -512,11 +512,10 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
 
         const __attribute__((address_space(4))) int32_t* table =
             (const __attribute__((address_space(4))) int32_t*)(a.pages.table + static_cast<int64_t>(rows.b) * a.pages.table_stride);
-        // the pages of a tile's halves, -1 where there is none (past the table's end too)
-        auto page_of = [&](int key) {
-            const int at = key / a.pages.page_size;
-            if (at >= a.pages.table_pages) return -1;
-            const int page = table[at];
+        // the page of a table's slot, -1 where there is none (past the table's end too)
+        auto page_of = [&](int slot) {
+            if (slot >= a.pages.table_pages) return -1;
+            const int page = table[slot];
             return page >= 0 && page < a.pages.pages ? page : -1;
         };
         // a tile's keys and values go out on their own, the next ones as soon as these have been read
@@ -530,9 +529,10 @@ __device__ __forceinline__ void few_segments(const Args& a, const Shares& shares
             p.there = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * h, page = __builtin_amdgcn_readfirstlane(page_of(key));
+                const int key = key0 + 16 * h, slot = __builtin_amdgcn_readfirstlane(a.pages.slot_of(key));
+                const int page = __builtin_amdgcn_readfirstlane(page_of(slot));
                 p.there |= page >= 0 ? 1 << h : 0;
-                p.at[h] = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key % a.pages.page_size) * D;
+                p.at[h] = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * a.pages.page_size + key - slot * a.pages.page_size) * D;
             }
             return p;
         };

@@ -169,7 +169,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
             my_there = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = (key + 16 * i) / a.pages.page_size;
+                const int at = a.pages.slot_of(key + 16 * i);
                 const int page = at < a.pages.table_pages ? a.pages.page(rows.b, at) : -1;
                 my_there |= page >= 0 ? 1 << i : 0;
                 if (i == rwave) {

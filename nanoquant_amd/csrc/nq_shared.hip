@@ -285,7 +285,7 @@ int nq_paged_shared_attention(int dtype, const void* q, int64_t q_stride, const 
     a.q_stride = q_stride;
     a.k_pages = static_cast<const uint16_t*>(k_pages);
     a.v_pages = static_cast<const uint16_t*>(v_pages);
-    a.pages = Pages{table, table_stride, static_cast<int>(table_pages), static_cast<int>(pages), static_cast<int>(page_size)};
+    a.pages = Pages(table, table_stride, table_pages, pages, page_size);
     a.positions = positions;
     a.members = members;
     a.shared = shared;
