@@ -123,7 +123,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
         int row0;
         if constexpr (kGroups) {
             rows.b = __builtin_amdgcn_readfirstlane(plan.lead[entry]);
-            rows.group = entry / a.group_rows;
+            rows.group = __builtin_amdgcn_readfirstlane(small_quotient(entry, a.per_group_rows));
             rows.place = plan.place;
             rows.to = __builtin_amdgcn_readfirstlane(plan.ends[rows.group]);
             rows.rows = a.most * a.tokens * a.groups;

@@ -13,15 +13,15 @@ namespace {
 // D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 4.1 us for 128 rows, 9.3 for 8192 of
 // 128 dimensions, with several parts a row on their way at once (with half or twice as many 3 us more).
 template <typename T, int D>
-__global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int64_t count) {
+__global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint32_t count) {
     constexpr int L4 = D / 4, Groups = 64 / L4, kAhead = 4;
     const int lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);  // (sequence, token, head)
+    const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));  // (sequence, token, head)
     if (row >= count) return;
-    const int64_t token = row / a.heads;
-    const int head = static_cast<int>(row - token * a.heads), kvh = head / a.groups;
-    const int b = static_cast<int>(token / a.tokens);
-    const int r = static_cast<int>(token - static_cast<int64_t>(b) * a.tokens) * a.groups + head - kvh * a.groups;
+    const int token = static_cast<int>(row / static_cast<uint32_t>(a.heads));
+    const int head = static_cast<int>(row) - token * a.heads, kvh = __builtin_amdgcn_readfirstlane(small_quotient(head, a.per_groups));
+    const int b = __builtin_amdgcn_readfirstlane(small_quotient(token, a.per_tokens));
+    const int r = (token - b * a.tokens) * a.groups + head - kvh * a.groups;
     const int at = a.place[b];
     struct Parts {
         int64_t first, later;  // rows of the first part and, were it one of the later ones, of the first block's
@@ -34,10 +34,10 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
     };
     Parts common{0, 0, 0, 0};
     if (at >= 0) {
-        const int g = at / a.most, in_group = (at - g * a.most) * a.tokens * a.groups + r;
-        common = parts_of(g * a.group_rows + in_group / a.group_tile, in_group % a.group_tile);
+        const int g = small_quotient(at, a.per_most), in_group = (at - g * a.most) * a.tokens * a.groups + r;
+        common = parts_of(g * a.group_rows + (in_group >> a.group_shift), in_group & (a.group_tile - 1));
     }
-    const Parts own = parts_of(a.entries_of_groups() + b * a.row_groups + r / a.own_tile, r % a.own_tile);
+    const Parts own = parts_of(a.entries_of_groups() + b * a.row_groups + (r >> a.own_shift), r & (a.own_tile - 1));
     const int n = common.n + own.n, grp = lane / L4, d0 = 4 * (lane % L4);
     float M = -INFINITY, L = 0.0f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, int6
         M = top;
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (grp == 0) *reinterpret_cast<uint2*>(a.out + row * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+    if (grp == 0) *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(row) * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
 // Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as
@@ -213,6 +213,14 @@ void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
     a.group_tile = static_cast<int>(p.group_tile);
     a.group_kept = static_cast<int>(p.group_kept);
     a.own_tile = static_cast<int>(p.own_tile);
+    a.group_shift = __builtin_ctz(a.group_tile);
+    a.own_shift = __builtin_ctz(a.own_tile);
+    a.per_most = 1.0f / static_cast<float>(a.most);
+    a.per_each = 1.0f / static_cast<float>(a.tokens * a.groups);
+    a.per_groups = 1.0f / static_cast<float>(a.groups);
+    a.per_tokens = 1.0f / static_cast<float>(a.tokens);
+    a.per_group_rows = 1.0f / static_cast<float>(a.group_rows);
+    a.per_row_groups = 1.0f / static_cast<float>(a.row_groups);
     a.own_first = p.own_first;
     a.group_later = p.group_later;
     a.own_later = p.own_later;
@@ -228,7 +236,7 @@ void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
         else few_kernel<T, D, 2, true, GroupArgs><<<dim3(FewShape<D, 2>::kBlocks), 64 * kWaves, 0, st>>>(a);
     }
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
-    group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, rows);
+    group_join_kernel<T, D><<<dim3(static_cast<unsigned>(ceil_div(rows, 4))), 256, 0, st>>>(a, static_cast<uint32_t>(rows));
 }
 
 // A call's plan; tiles 0 where there is none.
