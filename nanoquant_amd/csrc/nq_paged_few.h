@@ -260,8 +260,12 @@ struct Shares {
     int entry;                  // of the first unit; -1: nothing to do
     __device__ int block_of(int64_t unit) const;
 };
-// a / b for 0 <= a < 2^53 and b > 0: the quotient in fp64 is off by less than its distance from the next integer.
-__device__ inline int64_t quotient(int64_t a, int64_t b) { return static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b)); }
+// a / b for 0 <= a < 2^53 and b > 0, the same for the wave: the quotient in fp64 is off by less than its distance from the next
+// integer. Of small a as small_quotient, with a reciprocal that is off by 2^-23.
+__device__ inline int64_t quotient(int64_t a, int64_t b) {
+    if (a < 1 << 20) return small_quotient(static_cast<int>(a), __builtin_amdgcn_rcpf(static_cast<float>(b)));
+    return static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b));
+}
 __device__ inline int Shares::block_of(int64_t unit) const { return static_cast<int>(quotient(unit - base, share)); }
 
 template <int kThreads, typename Count>
