@@ -421,7 +421,8 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  *   keys and values of batch tables (table_pages * page_size * kv_heads * head_dim * 4 bytes each) below 2^27 bytes, or 2^26 where
  *     most * rows is 32 at most (rows = tokens * heads / kv_heads), and rows beyond 64: where sharing saves less than it costs;
  *   more work than a launch lists: groups * ceil(most * rows / 128) + batch * ceil(rows / (rows > 16 ? 32 : 16)) entries beyond
- *     1024, or, where most * rows is 32 at most, groups + batch beyond 512; batch * tokens * heads beyond 2^25. */
+ *     1024, or, where most * rows is 32 at most, groups + batch beyond 512; entries times table_pages * page_size beyond about
+ *     2^36; batch * tokens * heads beyond 2^25. */
 size_t nq_paged_shared_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t table_pages, int64_t page_size, int64_t groups,
                                                  int64_t most);

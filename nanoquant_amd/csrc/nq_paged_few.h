@@ -10,7 +10,7 @@
 namespace nq {
 namespace {
 
-constexpr int kTile = 32;          // keys a wave of few_kernel takes at a time
+constexpr int kTileShift = 5, kTile = 1 << kTileShift;  // keys a wave of few_kernel takes at a time
 constexpr int kWaves = 4;          // of a block
 constexpr int kCUs = 256;
 // (sequence, row group) pairs of a launch, whose key counts every block adds up in LDS: 8 KB, with which two blocks still fit a
@@ -108,22 +108,21 @@ __device__ inline Tiles tiles_between(const PagedArgs& a, int lo, int hi) {
     return r;
 }
 
-// The same among the keys from `from` to before `to` (a group's shared ones, a member's others).
-template <int kKeys>
-__device__ inline Tiles tiles_within(const PagedArgs& a, int lo, int hi, int from, int to) {
-    Tiles r{0, from / kKeys, 1, from / kKeys};
+// The same among the keys from `from` to before `to` (a group's shared ones, a member's others), tiles of 2^shift.
+__device__ inline Tiles tiles_within(const PagedArgs& a, int shift, int lo, int hi, int from, int to) {
+    Tiles r{0, from >> shift, 1, from >> shift};
     const int last = min(hi, to - 1);
     if (last < from) return r;
     const int start = a.window > 0 ? max(from, lo - a.window + 1) : from;
-    const int sinks = min(a.sinks, min(start, to)), sink_tiles = sinks > from ? (sinks + kKeys - 1) / kKeys - r.front : 0;
+    const int sinks = min(a.sinks, min(start, to)), sink_tiles = sinks > from ? ((sinks - 1) >> shift) + 1 - r.front : 0;
     if (start > last) {  // the window begins behind them
         r.sink_tiles = sink_tiles;
         r.count = max(1, sink_tiles);
         return r;
     }
-    r.window_tile = start / kKeys;
+    r.window_tile = start >> shift;
     r.sink_tiles = min(r.window_tile - r.front, sink_tiles);
-    r.count = r.sink_tiles + last / kKeys - r.window_tile + 1;
+    r.count = r.sink_tiles + (last >> shift) - r.window_tile + 1;
     return r;
 }
 
@@ -208,17 +207,17 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
     if (blockIdx.x == 0)
         for (int b = t; b < a.batch; b += kThreads) a.place[b] = plan.place[b];
 }
-// The tiles of kKeys keys of an entry, whose span turns into their places. 0: nobody's
-template <int kKeys, int kEntries>
-__device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e) {
+// The tiles of 2^shift keys of an entry, whose span turns into their places. 0: nobody's
+template <int kEntries>
+__device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e, int shift) {
     if (plan.lead[e] == kNobody) return 0;
     plan.lead[e] &= ~kIdle;
     const int of_groups = a.entries_of_groups();
     const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.per_most), to = e < of_groups ? plan.ends[small_quotient(e, a.per_group_rows)] : INT32_MAX;
-    const Tiles r = tiles_within<kKeys>(a, plan.spans[e].x, plan.spans[e].y, from, to);
+    const Tiles r = tiles_within(a, shift, plan.spans[e].x, plan.spans[e].y, from, to);
     int slow = 0;
     if (e < of_groups && a.window > 0 && r.count > r.sink_tiles)
-        slow = min(max(0, plan.spans[e].y - a.window + 1), to - 1) / kKeys - r.window_tile + 1;
+        slow = (min(max(0, plan.spans[e].y - a.window + 1), to - 1) >> shift) - r.window_tile + 1;
     plan.slow[e] = static_cast<uint8_t>(min(max(slow, 0), 255));
     plan.spans[e] = int2{r.sink_tiles, r.window_tile};
     return r.count;
@@ -268,7 +267,8 @@ __device__ inline int64_t quotient(int64_t a, int64_t b) {
 }
 __device__ inline int Shares::block_of(int64_t unit) const { return static_cast<int>(quotient(unit - base, share)); }
 
-template <int kThreads, typename Count>
+// Sum: in what a wave's are added up, where they are exact
+template <int kThreads, typename Sum, typename Count>
 __device__ inline void prefix_sums(int entries, int64_t* pre, int64_t* wave_total, Count count) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int per = (entries + kThreads - 1) / kThreads;
@@ -280,7 +280,7 @@ __device__ inline void prefix_sums(int entries, int64_t* pre, int64_t* wave_tota
             sum += count(e);
         }
     }
-    const int64_t incl = static_cast<int64_t>(wave_scan(static_cast<double>(sum)));  // far below 2^53
+    const int64_t incl = static_cast<int64_t>(wave_scan(static_cast<Sum>(sum)));
     if (lane == 63) wave_total[wave] = incl;
     __syncthreads();
     int64_t before = incl - sum;
@@ -320,10 +320,10 @@ __device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int bloc
     r.entry = __builtin_amdgcn_readfirstlane(*s_entry);
     return r;
 }
-template <int kThreads, int kBlocks, typename Count>
+template <int kThreads, int kBlocks, typename Sum, typename Count>
 __device__ inline Shares make_shares(const PagedArgs& a, int entries, int least, int64_t* pre, int64_t* wave_total,
                                      int* s_entry, Count count) {
-    prefix_sums<kThreads>(entries, pre, wave_total, count);
+    prefix_sums<kThreads, Sum>(entries, pre, wave_total, count);
     return take_share<kThreads>(a, 0, entries, static_cast<int>(blockIdx.x), kBlocks, least, pre, s_entry);
 }
 
@@ -842,9 +842,9 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             plan_groups<64 * kWaves>(a, plan);
             entries += a.entries_of_groups();
         }
-        shares = make_shares<64 * kWaves, Shape::kBlocks>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
+        shares = make_shares<64 * kWaves, Shape::kBlocks, std::conditional_t<kGroups, int, double>>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
             if constexpr (kGroups) {
-                const int n = tiles_of_plan<kTile>(a, plan, e);
+                const int n = tiles_of_plan(a, plan, e, kTileShift);
                 return n == 0 ? 0 : n + kFewStart;
             } else {
                 const Tiles r = tiles_of_few(a, e, 16 * RT);

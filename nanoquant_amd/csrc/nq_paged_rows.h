@@ -8,7 +8,7 @@
 namespace nq {
 namespace {
 
-constexpr int kKeys = 64;   // keys of a tile
+constexpr int kKeysShift = 6, kKeys = 1 << kKeysShift;  // keys of a tile
 
 // An entry's tiles, for the blocks that share the work of all: a wave per entry, its tokens over the lanes. 4.7 us; in every
 // block of rows_kernel, whose entries have hundreds of tokens, it would cost more.
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(RW == 1 ? 512 : 256, RW == 1 ? 2 : 1) void rows_ker
     Shares shares{};
     int entry;
     if constexpr (kShared) {
-        shares = make_shares<64 * NW, kCUs>(a, a.batch * a.row_groups, kLeastTiles, pre, wave_total, &s_entry,
+        shares = make_shares<64 * NW, kCUs, double>(a, a.batch * a.row_groups, kLeastTiles, pre, wave_total, &s_entry,
                                             [&](int e) { return a.spans[e].z + kStart; });
         if (shares.entry < 0) return;
         entry = shares.entry;

@@ -129,10 +129,9 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
     __shared__ int first_entry[kTeams], arrived[kTeams];
     const int of_groups = a.entries_of_groups(), entries = of_groups + a.batch * a.row_groups;
     plan_groups<kThreads>(a, plan);
-    prefix_sums<kThreads>(entries, pre, wave_total, [&](int e) {
-        if (e >= of_groups) return tiles_of_plan<kTile>(a, plan, e) + kOwnStart;
-        const int n = tiles_of_plan<kKeys>(a, plan, e);
-        return n == 0 ? 0 : n + kGroupStart + plan.slow[e];  // a tile that is masked takes twice as long
+    prefix_sums<kThreads, int>(entries, pre, wave_total, [&](int e) {
+        const int n = tiles_of_plan(a, plan, e, e < of_groups ? kKeysShift : kTileShift);
+        return n == 0 ? 0 : e < of_groups ? n + kGroupStart + plan.slow[e] : n + kOwnStart;  // a tile that is masked takes twice as long
     });
     const int block = static_cast<int>(blockIdx.x);
     const int for_groups = blocks_for_groups<D>(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads);
@@ -191,6 +190,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
     if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
     if (batch * each * kv_heads > kMaxThreads / 64) return p;  // rows of group_join_kernel, a wave each
+    if ((of_groups + own) * (keys / kTile + 512) > INT32_MAX) return p;  // units, which are added up in 32 bits
     constexpr int64_t kParts = (kTeams > 2 ? kTeams : 2) * kCUs;  // teams, or blocks, two on a CU
     p.own_first = kv_heads * of_groups * p.group_kept;
     p.own_later = p.own_first + kv_heads * own * p.rows_kept;

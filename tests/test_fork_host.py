@@ -397,6 +397,7 @@ def test_c_abi_limits_of_shared_pages_need_no_gpu():
     assert nbytes(500, heads=65536, kv=65536, most=64) > 0 and nbytes(600, heads=65536, kv=65536, most=64) == 0
     assert nbytes(0) == nbytes(4, groups=0) == nbytes(4, most=0) == nbytes(4, heads=7) == nbytes(4, most=1 << 31) == 0
     assert nbytes(4, keys=1 << 31) == nbytes(4, page=0x7FFFFFFF) == nbytes(4, keys=0) == 0
+    assert nbytes(1000, keys=1 << 25) > 0 and nbytes(1000, keys=1 << 27) == 0  # 2^31 tiles of 32
     # 2^27 bytes of the tables' keys and values, 2^26 with few rows a group: 8 sequences of 2 kv heads of 128, 8 KB a position
     assert nbytes(8, keys=1 << 14) > 0 and nbytes(8, keys=(1 << 14) - 16) == 0
     assert nbytes(8, keys=1 << 13, most=8) > 0 and nbytes(8, keys=(1 << 13) - 16, most=8) == 0
