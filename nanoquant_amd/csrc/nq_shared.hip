@@ -10,7 +10,7 @@ namespace nq {
 namespace {
 
 // Adds up what few_kernel or shared_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave a row,
-// D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 4.1 us for 128 rows, 9.3 for 8192 of
+// D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 3.9 us for 128 rows, 7.0 for 8192 of
 // 128 dimensions, with several parts a row on their way at once (with half or twice as many 3 us more).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint32_t count) {
@@ -89,10 +89,10 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint
 // few_kernel does, a team of two waves each, in equal shares; all of them work out the same list. One launch, since the
 // sequences' part is bound by the read of keys and values and the groups' by products: in two launches, each on all CUs, 16
 // sequences with 8000 shared keys 47 us against 36, 60 conversations 179 against 152, 128 samples under a window 221 against
-// 161. Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 25 us, bound by latency
+// 161. Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 24 us, bound by latency
 // (the list, the first tiles' way, the waves' join); 60 in five groups with 100 to 4000 of their own 146, bound by the read
-// (5.0 TB/s, a large copy's rate); 128 under a window of 12011 keys 155, bound by rows_segments' products and exponentials, of
-// which the tiles in which windows begin take twice. 11 sequences of 5 tokens, heads of 64, 5000 shared keys: 23 us. How many
+// (5.0 TB/s, a large copy's rate); 128 under a window of 12011 keys 146, bound by rows_segments' products and exponentials, of
+// which the tiles in which windows begin take twice. 11 sequences of 5 tokens, heads of 64, 5000 shared keys: 21 us. How many
 // blocks either gets goes by what a unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how
 // much longer the groups' blocks take for their beginning and their end.
 constexpr float kGroupTime = 1200.0f, kGroupTime64 = 700.0f, kOwnTime = 400.0f, kOwnTime64 = 350.0f, kGroupMore = 4000.0f;
