@@ -411,8 +411,9 @@ int nq_paged_attention(int dtype, const void* q, int64_t q_stride, const void* k
  *   members   device int32 [groups, most], contiguous: the sequences of each group in any order; entries outside [0, batch) are
  *             nobody. A sequence in no group is on its own; of one that is named twice the last place counts.
  *   shared    device int32 [groups]: the first shared[g] entries of the table are the same in the rows of group g's members
- *             (none where it is not positive, all where it is more). Where they are not, the results of those sequences mean
- *             nothing; no memory outside the pool is read.
+ *             (none where it is not positive, all where it is more). Those of a member with a token serve for the members behind
+ *             it, whose rows may so lack pages (-1) that their windows are past, if the row before has them. Where rows differ
+ *             otherwise, the results of those sequences mean nothing; no memory outside the pool is read.
  * Everything else, the result but for rounding too, is as for nq_paged_attention.
  *   workspace nq_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no initial contents; calls that share one
  *             must not overlap.

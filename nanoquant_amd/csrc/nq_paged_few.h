@@ -149,12 +149,15 @@ __device__ inline Tiles tiles_of_few(const PagedArgs& a, int entry, int group) {
 }
 
 constexpr int kNobody = INT32_MAX, kIdle = 1 << 30;  // a sequence without tokens leads only where no other does
+constexpr int kSequenceBits = 10;  // of a batch's: each has an entry
 
 // What the blocks of a launch with groups work out before they take their shares, in LDS.
 template <int kEntries>
 struct GroupPlan {
     int place[kEntries];  // of a sequence: the last place that names it, -1
-    int lead[kEntries];   // of an entry: the sequence by whose row of the table its pages are found; kNobody
+    // of an entry: the sequence by whose row of the table its pages are found, with its place in the group above it until
+    // tiles_of_plan; kNobody. The first place that has a token: rows of later ones may lack pages that their windows are past
+    int lead[kEntries];
     int ends[kEntries];   // of a group: the shared keys
     int2 spans[kEntries];
     uint8_t slow[kEntries];  // of a group's entry: the tiles in which some member's window begins
@@ -163,6 +166,7 @@ struct GroupPlan {
 // All threads of the block.
 template <int kThreads, int kEntries>
 __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan) {
+    static_assert(kEntries <= 1 << kSequenceBits, "a sequence's number fits below its place, of 2^17, and kIdle");
     const int t = threadIdx.x, first = a.entries_of_groups(), each = a.tokens * a.groups, own = a.batch * a.row_groups;
     auto span_of = [&](int e) {
         const int b = small_quotient(e, a.per_row_groups), row = (e - b * a.row_groups) << a.own_shift;
@@ -196,11 +200,12 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
         plan.spans[first + e] = span;
         plan.lead[first + e] = b;
         if (at < 0) continue;
-        const int g = small_quotient(at, a.per_most), row0 = (at - g * a.most) * each + row;
+        const int g = small_quotient(at, a.per_most), in_group = at - g * a.most, row0 = in_group * each + row;
+        const int lead = in_group << kSequenceBits | b;
         for (int i = row0 >> a.group_shift; i <= (row0 + rows - 1) >> a.group_shift; ++i) {
             atomicMin(&plan.spans[g * a.group_rows + i].x, span.x);
             atomicMax(&plan.spans[g * a.group_rows + i].y, span.y);
-            atomicMin(&plan.lead[g * a.group_rows + i], span.y < 0 ? b | kIdle : b);
+            atomicMin(&plan.lead[g * a.group_rows + i], span.y < 0 ? lead | kIdle : lead);
         }
     }
     __syncthreads();
@@ -211,7 +216,7 @@ __device__ inline void plan_groups(const GroupArgs& a, GroupPlan<kEntries>& plan
 template <int kEntries>
 __device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& plan, int e, int shift) {
     if (plan.lead[e] == kNobody) return 0;
-    plan.lead[e] &= ~kIdle;
+    plan.lead[e] &= (1 << kSequenceBits) - 1;
     const int of_groups = a.entries_of_groups();
     const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.per_most), to = e < of_groups ? plan.ends[small_quotient(e, a.per_group_rows)] : INT32_MAX;
     const Tiles r = tiles_within(a, shift, plan.spans[e].x, plan.spans[e].y, from, to);

@@ -103,7 +103,14 @@ class PagedKVCache:
         self.members = self.shared = None
         self._outgrown = []  # those that graphs captured earlier read
         self.groups = self.saved = 0
-        self._common = [0] * batch  # entries that a sequence's row has in common with its group's
+        self._lists = []  # each group's sequences, and how many leading entries their rows have in common
+        self._common = [0] * batch  # the same number, of a sequence's group
+        self._missing = [0] * batch  # of those entries, the ones that the sequence has trimmed
+        # Where a sequence's slots come from, trimmed ones too: (stretch, its end) one after the other. Slots of the same stretch
+        # are the same page in every sequence that has one there. Stretches that sequences share end before ``_forked``
+        self._stretches = batch
+        self._lines = [[(b, self.max_pages)] for b in range(batch)]
+        self._forked = [0] * batch
 
     def _row(self, sequence: int):
         if not 0 <= sequence < self.batch:
@@ -127,26 +134,50 @@ class PagedKVCache:
         source, target = torch.tensor(moves, dtype=torch.int32).t().contiguous().to(self.table.device).unbind(0)
         copy_pages([*self.k, *self.v], source, target)
 
+    def _branch(self, sequence: int, line, slot: int) -> None:
+        """The sequence's slots are those of ``line`` before ``slot`` and its own from there on."""
+        kept, at = [], 0
+        for stretch, end in line:
+            if at < slot:
+                at = min(end, slot)
+                kept.append((stretch, at))
+        self._lines[sequence] = [*kept, (self._stretches, self.max_pages)]
+        self._stretches += 1
+        self._forked[sequence] = slot
+
+    def _reach(self, sequence: int, slots: int) -> int:
+        """The sequence's last slot before ``slots`` that has a page, and one more."""
+        row = self._host[sequence]
+        while slots and row[slots - 1] < 0:
+            slots -= 1
+        return slots
+
     def _regroup(self) -> None:
-        """``members`` and ``shared`` of the sequences whose first page is the same: what all of their rows begin with."""
-        alike = {}
-        for b, row in enumerate(self._host):
-            first = next(((i, page) for i, page in enumerate(row) if page >= 0), None)
-            if first is not None and self._owners[first[1]] > 1:
-                alike.setdefault(first, []).append(b)
-        lists, shared = [], []
+        """``members`` and ``shared`` of the sequences whose rows begin alike: all that do, with what all of them still have some
+        of. A slot that a sequence has trimmed is behind its window and so counts as alike."""
+        runs = []
+        before = []
+        for line, b in sorted((self._lines[b], b) for b in range(self.batch) if self._forked[b]):
+            common = _alike(before, line)
+            if common == 0:
+                runs.append(([b], self.max_pages))
+            else:
+                sequences, least = runs[-1]
+                runs[-1] = (sequences + [b], min(least, common))
+            before = line
+        self._lists = []
         self._common = [0] * self.batch
-        for sequences in alike.values():
-            rows = [self._host[b] for b in sequences]
-            low, high = min(rows), max(rows)  # what these two begin with all begin with
-            common = next((i for i, (x, y) in enumerate(zip(low, high)) if x != y), self.max_pages)
-            while common and low[common - 1] < 0:
-                common -= 1
-            if len(sequences) > 1 and common:
-                lists.append(sequences)
-                shared.append(common)
+        for sequences, least in runs:
+            reach = {b: self._reach(b, least) for b in sequences}
+            sequences = [b for b in sequences if reach[b]]
+            if len(sequences) > 1:
+                common = min(reach[b] for b in sequences)
                 for b in sequences:
                     self._common[b] = common
+                    self._missing[b] = self._host[b][:common].count(-1)
+                self._lists.append((sorted(sequences, key=self._lead), common))
+        self._lists.sort(key=lambda x: min(x[0]))
+        lists, shared = [sequences for sequences, _ in self._lists], [common for _, common in self._lists]
         self.groups = len(lists)
         position = 2 * self.k[0][0, :, 0].numel() * self.k[0].element_size() if self.k else 0
         most = self.window + self.sinks if self.window else self.max_len
@@ -165,6 +196,26 @@ class PagedKVCache:
         self.members.copy_(torch.tensor([x + [-1] * (most - len(x)) for x in lists], dtype=torch.int32).view(groups, most))
         self.shared.copy_(torch.tensor(shared + [0] * (groups - len(shared)), dtype=torch.int32))
 
+    def _lead(self, sequence: int):
+        """The order of a group: what a sequence has, those behind it have no more of, so its row serves for theirs. (Trimmed slots
+        begin where the sinks end in every row.)"""
+        return self._missing[sequence], sequence
+
+    def _reorder(self, sequence: int) -> None:
+        """The groups after the sequence has trimmed some of the slots in common. While it has the last of them, only its place
+        changes: 128 answers that trim one after the other would spend most of a step in ``_regroup``."""
+        common = self._common[sequence]
+        if self._host[sequence][common - 1] < 0:
+            self._regroup()
+            return
+        at = next(i for i, (sequences, _) in enumerate(self._lists) if sequence in sequences)
+        sequences = self._lists[at][0]
+        self._missing[sequence] = self._host[sequence][:common].count(-1)
+        order = sorted(sequences, key=self._lead)
+        if order != sequences:
+            sequences[:] = order
+            self.members[at, :len(order)].copy_(torch.tensor(order, dtype=torch.int32))
+
     def reserve(self, sequence: int, length: int, start: int = 0) -> None:
         """Pages for the sequence's positions ``start`` to ``length - 1`` (those it has stay). RuntimeError, and no change,
         where the pool has too few left."""
@@ -178,7 +229,8 @@ class PagedKVCache:
             row[i] = self._take()
         if need:
             self._store(sequence)
-            if need[0] < self._common[sequence]:
+            if need[0] < self._forked[sequence]:
+                self._branch(sequence, self._lines[sequence], need[0])
                 self._regroup()
 
     def _take_back(self, sequence: int, slots) -> int:
@@ -189,8 +241,6 @@ class PagedKVCache:
             row[i] = -1
         if gone:
             self._store(sequence)
-            if gone[0] < self._common[sequence]:
-                self._regroup()
         return len(gone)
 
     def trim(self, sequence: int, position: int) -> int:
@@ -199,12 +249,20 @@ class PagedKVCache:
         if self.window == 0:
             return 0
         first = min(max(0, position - self.window + 1) // self.page_size, self.max_pages)
-        return self._take_back(sequence, range(-(-self.sinks // self.page_size), first))
+        sinks = -(-self.sinks // self.page_size)
+        gone = self._take_back(sequence, range(sinks, first))
+        if gone and sinks < self._common[sequence]:
+            self._reorder(sequence)
+        return gone
 
     def release(self, sequence: int) -> int:
         """Take back all pages of a sequence (those that others share stay theirs); returns their number. Calls in flight on
         other streams must have ended."""
-        return self._take_back(sequence, range(self.max_pages))
+        gone = self._take_back(sequence, range(self.max_pages))
+        if self._forked[sequence]:
+            self._branch(sequence, [], 0)
+            self._regroup()
+        return gone
 
     def fork(self, source: int, targets, length: int) -> None:
         """The sequences ``targets``, which have no pages, get the first ``length`` positions of ``source``: its whole pages as
@@ -231,6 +289,9 @@ class PagedKVCache:
             if split:
                 self._host[b][whole] = self._take()
             self._store(b)
+            self._branch(b, self._lines[source], whole)
+        if targets:
+            self._forked[source] = max(self._forked[source], whole)
         self._regroup()
 
     def own(self, sequence: int, length: int, start: int) -> int:
@@ -251,8 +312,8 @@ class PagedKVCache:
                 self._drop(row[i])
                 row[i] = page
             self._store(sequence)
-            if shared[0] < self._common[sequence]:
-                self._regroup()
+            self._branch(sequence, self._lines[sequence], shared[0])
+            self._regroup()
         return len(shared)
 
     def compact(self) -> int:
@@ -270,6 +331,18 @@ class PagedKVCache:
             self._free = list(range(self.pages - 1, used - 1, -1))
             self.table.copy_(torch.tensor(self._host, dtype=torch.int32))
         return used
+
+
+def _alike(line, other) -> int:
+    """How many leading slots two of ``PagedKVCache._lines`` have in common."""
+    common = 0
+    for (stretch, end), (other_stretch, other_end) in zip(line, other):
+        if stretch != other_stretch:
+            break
+        common = min(end, other_end)
+        if end != other_end:
+            break
+    return common
 
 
 # ------------------------------------------------------------------------------------- arguments
@@ -461,7 +534,8 @@ def paged_shared_attention(q, k_pages, v_pages, table, positions, members, share
     ``members`` int32 [groups, most] are the sequences of each group (entries outside the batch, as -1, are nobody), whose rows
     of the table begin with the same ``shared`` (int32 [groups]) entries; see :meth:`PagedKVCache.fork`. Those pages are read
     once a group. A sequence in no group is on its own; of one that is named twice the last place counts. Where members' rows
-    do not begin alike, their results mean nothing.
+    do not begin alike, their results mean nothing; but a row may lack pages that its window is past (-1), and then stands
+    behind those of the group that have them.
 
     Other arguments and the result, but for rounding, are :func:`paged_attention`'s, which also takes the calls that the kernel
     does not: those that run torch ops, small ones, many tokens a sequence (prompts), and batches past about a thousand sequences

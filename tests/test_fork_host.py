@@ -163,6 +163,111 @@ def test_groups_under_a_window():
     assert cache.groups == 1 and int(cache.shared[0]) == 1
 
 
+def _groups_hold(cache):
+    """The groups are those that the rows make when asked anew, and what a member has, those before it in its group have too."""
+    state = [cache.members.tolist(), cache.shared.tolist(), cache.groups, cache.saved]
+    cache._regroup()
+    assert state == [cache.members.tolist(), cache.shared.tolist(), cache.groups, cache.saved]
+    for sequences, n in zip(cache.members.tolist(), cache.shared.tolist()):
+        rows = [cache._host[b][:n] for b in sequences if b >= 0]
+        for row, later in zip(rows, rows[1:]):
+            assert all(page == other or other == -1 for page, other in zip(row, later))
+
+
+@pytest.mark.parametrize("sinks", [0, 2])
+def test_members_that_trim_one_after_the_other_stay_a_group(sinks):
+    """At one position, partly into the prompt: the rows are alike again when the last has trimmed."""
+    cache = _cache(window=20, sinks=sinks, pages=60, max_len=80)
+    cache.reserve(0, 32)
+    cache.fork(0, [1, 2, 3], 32)
+    for b in range(4):
+        cache.reserve(b, 37, 32)
+    for b in (0, 2, 1, 3):
+        assert cache.trim(b, 36) == 4 - bool(sinks)
+        _groups_hold(cache)
+        assert cache.groups == 1 and int(cache.shared[0]) == 8 and set(cache.members[0].tolist()) == {0, 1, 2, 3}
+    _sound(cache)
+    assert cache.members.tolist()[0] == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("sinks", [0, 2])
+def test_members_that_trim_at_positions_of_their_own_stay_a_group(sinks):
+    """Answers at different lengths have the prompt's last pages in common, and differ in what is behind their windows."""
+    cache = _cache(window=30, sinks=sinks, pages=90, max_len=120)
+    cache.reserve(0, 64)
+    cache.fork(0, [1, 2, 3], 64)
+    at = [74, 66, 78, 70]
+    for b in range(4):
+        cache.reserve(b, at[b], 64)
+        cache.trim(b, at[b])
+        _groups_hold(cache)
+    assert cache.groups == 1 and int(cache.shared[0]) == 16
+    assert cache.members.tolist()[0] == [1, 3, 0, 2]  # the one that has the most comes first
+    cache.trim(1, 86)  # further than the others
+    _groups_hold(cache)
+    assert cache.members.tolist()[0] == [3, 0, 2, 1] and int(cache.shared[0]) == 16
+    cache.reserve(4, 9)
+    cache.release(3)
+    _groups_hold(cache)
+    assert cache.members.tolist()[0] == [0, 2, 1, -1]
+    cache.fork(2, [5], 78)  # the fork of one that has trimmed lacks the same pages
+    _groups_hold(cache)
+    assert cache.members.tolist()[0] == [0, 2, 5, 1]
+    cache.compact()
+    _groups_hold(cache)
+    cache.reserve(0, 78, 0)  # pages of its own where it had trimmed: its row begins otherwise now
+    _groups_hold(cache)
+    assert int(cache.shared[0]) == (1 if sinks else 16) and (0 in cache.members.tolist()[0]) == (sinks > 0)
+    for b in range(6):
+        cache.release(b)
+        _groups_hold(cache)
+    assert cache.groups == 0 and len(cache._free) == 90
+
+
+def test_forks_and_trims_at_random():
+    import random
+    rng = random.Random(9)
+    cache = _cache(batch=7, pages=70, max_len=64, window=18, sinks=3)
+    length = [0] * 7
+    grouped = 0
+    for step in range(400):
+        b = rng.randrange(7)
+        try:
+            what = rng.choice(["reserve", "reserve", "trim", "trim", "trim", "fork", "release", "own", "compact"])
+            if what == "reserve" and length[b] < 64:
+                n = rng.randint(length[b], min(64, length[b] + 20))
+                cache.reserve(b, n, rng.choice([length[b], length[b], 0]))
+                length[b] = n
+            elif what == "trim" and length[b]:
+                cache.trim(b, rng.randint(length[b] // 2, length[b]))
+            elif what == "fork":
+                targets = [c for c in range(7) if c != b and cache._host[c] == [-1] * cache.max_pages][:rng.randint(1, 3)]
+                n = rng.randint(length[b] // 2, length[b])
+                cache.fork(b, targets, n)
+                for c in targets:
+                    length[c] = n
+            elif what == "release" and rng.random() < 0.5:
+                cache.release(b)
+                length[b] = 0
+            elif what == "own":
+                cache.own(b, length[b], rng.randint(length[b] // 2, length[b]))
+            elif what == "compact":
+                cache.compact()
+        except RuntimeError:
+            assert len(cache._free) < 18
+        held = [0] * cache.pages
+        for row in cache._host:
+            for page in row:
+                if page >= 0:
+                    held[page] += 1
+        assert held == cache._owners and cache.table.tolist() == cache._host
+        if cache.members is not None:
+            grouped += cache.groups > 0
+            if rng.random() < 0.3:
+                _groups_hold(cache)
+    assert grouped > 200
+
+
 def test_many_forks_at_random():
     import random
     rng = random.Random(4)

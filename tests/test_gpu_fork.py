@@ -99,6 +99,60 @@ def test_attention_over_long_prompts(case):
     _check(y, ref, spread, torch.bfloat16, _keys(table, k))
 
 
+# (members, heads, kv_heads, head_dim, page_size, prompt, steps, tokens, window, sinks)
+TRIMMED = [
+    (40, 8, 2, 128, 16, 400, 30, 1, 150, 5),   # 160 rows a group
+    (70, 8, 2, 64, 32, 700, 40, 1, 333, 0),    # 280, no sinks
+    (9, 8, 2, 128, 16, 300, 6, 4, 100, 20),    # 144, drafted tokens
+    (7, 8, 2, 64, 16, 500, 20, 1, 200, 0),     # 28: one kernel for groups and sequences
+]
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=IDS)
+@pytest.mark.parametrize("case", TRIMMED, ids=ids)
+def test_forks_that_trim_behind_their_windows(case, dtype):
+    """Answers at lengths of their own, each trimmed at its position while they grow: what they see is in the row of the member
+    that has the most. Row groups' windows begin in many tiles. Against the table as it was without any trim."""
+    members, heads, kv, dim, page, prompt, steps, tokens, window, sinks = case
+    shape = LlamaShape(hidden=heads * dim, layers=1, heads=heads, kv_heads=kv, ffn=64, vocab=64)
+    g = torch.Generator(device="cuda").manual_seed(members)
+    room = prompt + 3 * members + steps * tokens
+    keys = -(-(1 << 27) // (members * kv * dim * 4))
+    cache = PagedKVCache(shape, members, prompt // page + members * (3 * members // page + steps * tokens // page + 4), page,
+                         max(room, keys), "cuda", dtype, window=window, sinks=sinks)
+    cache.k[0].normal_(generator=g), cache.v[0].normal_(generator=g)
+    first = members // 2  # not the one that trims least
+    cache.reserve(first, prompt)
+    others = [b for b in range(members) if b != first]
+    cache.fork(first, others, prompt)
+    shared = int(cache.shared[0])
+    assert shared == prompt // page
+    length = [prompt + 3 * ((11 * b + 5) % members) + tokens for b in range(members)]
+    whole = torch.full_like(cache.table, -1)
+    apart = False
+    for step in range(steps):
+        for b in range(members):
+            cache.reserve(b, length[b], length[b] - tokens if step else prompt)
+        whole = torch.where(cache.table >= 0, cache.table, whole)
+        for b in range(members):
+            cache.trim(b, length[b] - tokens)
+        if step % (steps // 2 - 1) == 1:
+            assert cache.groups == 1 and int(cache.shared[0]) == shared and cache.saved > 0
+            trimmed = (cache.table < 0)[:, :shared].sum(1)
+            apart |= bool(trimmed.max() > trimmed.min())
+            q = torch.randn(members, tokens, heads * dim, device="cuda", generator=g).to(dtype) * 1.5
+            pos = torch.tensor(length, device="cuda").unsqueeze(1) - tokens + torch.arange(tokens, device="cuda")
+            pos[3] = -1  # has no token in this step
+            y = attend(q, cache.k[0], cache.v[0], cache.table, pos, cache.members, cache.shared, window, sinks)
+            used = whole[:, :-(-room // page)]
+            ref, spread = oracle.attention(q, cache.k[0], cache.v[0], used, pos, window, sinks)
+            _check(y, ref, spread, dtype, window + sinks)
+            again = paged_attention(q, cache.k[0], cache.v[0], cache.table, pos, window, sinks)
+            _check(again, ref, spread, dtype, window + sinks)
+        length = [n + tokens for n in length]
+    assert apart
+
+
 def test_groups_as_a_caller_may_give_them():
     """Members named twice, in two groups, that are nobody; counts below zero and past the table; tables without padding."""
     q, k, v, table, pos, members, shared = shared_case(8, 2, 128, 16, [(6, [5, 40, 9])], [30, 7], 1, torch.float16, "cuda")
