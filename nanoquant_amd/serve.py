@@ -179,10 +179,7 @@ class PagedKVCache:
         self._lists.sort(key=lambda x: min(x[0]))
         lists, shared = [sequences for sequences, _ in self._lists], [common for _, common in self._lists]
         self.groups = len(lists)
-        position = 2 * self.k[0][0, :, 0].numel() * self.k[0].element_size() if self.k else 0
-        most = self.window + self.sinks if self.window else self.max_len
-        seen = [min(common * self.page_size, most) for common in shared]
-        self.saved = sum((len(sequences) - 1) * n * position for sequences, n in zip(lists, seen))
+        self._count_saved()
         most = max(map(len, lists), default=0)
         if self.members is None or self.members.shape[0] < len(lists) or self.members.shape[1] < most:
             old = (0, 0) if self.members is None else self.members.shape
@@ -195,6 +192,14 @@ class PagedKVCache:
         lists += [[]] * (groups - len(lists))
         self.members.copy_(torch.tensor([x + [-1] * (most - len(x)) for x in lists], dtype=torch.int32).view(groups, most))
         self.shared.copy_(torch.tensor(shared + [0] * (groups - len(shared)), dtype=torch.int32))
+
+    def _count_saved(self) -> None:
+        position = 2 * self.k[0][0, :, 0].numel() * self.k[0].element_size() if self.k else 0
+        most = self.window + self.sinks if self.window else self.max_len
+        self.saved = 0
+        for sequences, common in self._lists:
+            seen = [min((common - self._missing[b]) * self.page_size, most) for b in sequences]
+            self.saved += position * (sum(seen) - max(seen))
 
     def _lead(self, sequence: int):
         """The order of a group: what a sequence has, those behind it have no more of, so its row serves for theirs. (Trimmed slots
@@ -211,6 +216,7 @@ class PagedKVCache:
         at = next(i for i, (sequences, _) in enumerate(self._lists) if sequence in sequences)
         sequences = self._lists[at][0]
         self._missing[sequence] = self._host[sequence][:common].count(-1)
+        self._count_saved()
         order = sorted(sequences, key=self._lead)
         if order != sequences:
             sequences[:] = order

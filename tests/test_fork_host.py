@@ -188,6 +188,26 @@ def test_members_that_trim_one_after_the_other_stay_a_group(sinks):
         assert cache.groups == 1 and int(cache.shared[0]) == 8 and set(cache.members[0].tolist()) == {0, 1, 2, 3}
     _sound(cache)
     assert cache.members.tolist()[0] == [0, 1, 2, 3]
+    assert cache.saved == 3 * (4 + bool(sinks)) * 4 * (2 * 2 * 32 * 4)  # of eight pages, those that are left
+
+
+def test_pages_that_windows_are_past_save_nothing():
+    """Each member's own pages count, and those of the one that has the most are read anyway."""
+    position = 2 * 2 * 32 * 4
+    cache = _cache(window=40, sinks=4, pages=60, max_len=80)
+    cache.reserve(0, 32)
+    cache.fork(0, [1, 2], 32)
+    assert cache.saved == 2 * 32 * position
+    for b, at, left in ((0, 47, 28 + 32), (1, 51, 28 + 24), (2, 59, 24 + 16), (0, 70, 16 + 8)):
+        cache.reserve(b, at + 1, 32)
+        cache.trim(b, at)  # sees positions at - 39 on, and the first page's
+        assert cache.saved == left * position
+        _groups_hold(cache)
+    for b in (0, 1, 2):
+        cache.reserve(b, 80, 72)
+        cache.trim(b, 79)
+        _groups_hold(cache)
+    assert cache.groups == 1 and cache.saved == 2 * 4 * position  # the sinks' page
 
 
 @pytest.mark.parametrize("sinks", [0, 2])
