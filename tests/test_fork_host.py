@@ -244,6 +244,66 @@ def test_members_that_trim_at_positions_of_their_own_stay_a_group(sinks):
     assert cache.groups == 0 and len(cache._free) == 90
 
 
+WIDE = LlamaShape(hidden=1024, layers=1, heads=8, kv_heads=8, ffn=64, vocab=64)  # 8 KB a position
+
+
+def _groups(cache):
+    return [([b for b in x if b >= 0], n) for x, n in zip(cache.members.tolist(), cache.shared.tolist()) if n]
+
+
+def test_a_short_fork_leaves_the_others_their_pages():
+    """Seven answers to a prompt of a thousand tokens, and one that branches off after twenty."""
+    cache = PagedKVCache(WIDE, 12, 120, 16, 1040, "cpu", torch.float32)
+    cache.reserve(0, 1000)
+    cache.fork(0, range(1, 8), 1000)
+    saved = 7 * 62 * 16 * 8192
+    assert _groups(cache) == [([*range(8)], 62)] and cache.saved == saved
+    cache.fork(0, [8], 20)
+    assert _groups(cache) == [([*range(8)], 62)] and cache.saved == saved
+    cache.fork(3, [9, 10], 20)  # the short ones have a page in common with each other
+    assert _groups(cache) == [([*range(8)], 62), ([8, 9, 10], 1)] and cache.saved == saved + 2 * 16 * 8192
+    for b in range(1, 8):
+        cache.release(b)
+    assert _groups(cache) == [([0, 8, 9, 10], 1)]
+    _sound(cache)
+
+
+def test_groups_of_a_tree_of_forks():
+    """Second prompts behind a first one: groups of their own where they are long, one group where they are short."""
+    for second, want in ((30, [([0, 2, 4, 6], 70), ([1, 3, 5, 7], 70)]), (2, [([*range(8)], 40)])):
+        cache = PagedKVCache(WIDE, 8, 160, 16, 1280, "cpu", torch.float32)
+        cache.reserve(0, 40 * 16)
+        cache.fork(0, [1], 40 * 16)
+        for b in (0, 1):
+            cache.reserve(b, (40 + second) * 16)
+            cache.fork(b, [b + 2, b + 4, b + 6], (40 + second) * 16)
+        assert _groups(cache) == want
+        _sound(cache)
+    # each fork a little earlier than the one before: together while that saves more
+    cache = PagedKVCache(WIDE, 11, 100, 16, 1280, "cpu", torch.float32)
+    cache.reserve(0, 64 * 16)
+    for b, n in enumerate((60, 58, 56, 54, 52, 50, 9, 8, 1), 1):
+        cache.fork(0, [b], n * 16)
+    assert _groups(cache) == [([*range(7)], 50), ([7, 8], 8)]
+    _sound(cache)
+
+
+def test_a_member_past_the_prompt_leaves_the_others_their_pages():
+    for sinks in (0, 16):
+        cache = PagedKVCache(WIDE, 5, 240, 16, 1600, "cpu", torch.float32, window=600, sinks=sinks)
+        cache.reserve(0, 800)
+        cache.fork(0, [1, 2, 3], 800)
+        cache.reserve(2, 1500, 800)
+        cache.trim(2, 1499)
+        assert _groups(cache) == [([0, 1, 3], 50)] and cache.saved == 2 * (600 + sinks) * 8192
+        _groups_hold(cache)
+        for b in (0, 3, 1):
+            cache.reserve(b, 1500, 800)
+            cache.trim(b, 1499)
+            _groups_hold(cache)
+        assert _groups(cache) == ([([0, 1, 2, 3], 1)] if sinks else [])
+
+
 def test_forks_and_trims_at_random():
     import random
     rng = random.Random(9)
