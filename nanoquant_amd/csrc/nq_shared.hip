@@ -176,8 +176,9 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     // in 4000 shared keys 64.0 us against 55.8 of the plain attention, of 8 tokens 40.8 against 43.2.
     if (each > 64) return p;
     // Tables whose keys and values are read in the time that the shared kernel needs to begin and to join: two sequences in 4000
-    // shared keys, 8 kv heads, 18.7 us against 14.3 (39 MB), 30 in 100 21.7 against 9.5 (55), eight of heads of 64 in 4000 21.1
-    // against 19.2 (78), four of 32 kv heads in 1000 18.4 against 18.8 (75), eight in 4000 25.5 against 26.9 (155).
+    // shared keys, 8 kv heads, 19.2 us against 16.2 of the plain attention (33 MB), 40 in 250 22.9 against 12.1 (57), eight of heads
+    // of 64 in 4000 17.1 against 19.9 (67), four of 32 kv heads in 1000 16.4 against 20.5 (70), eight of 8 in 4000 24.8 against 29.2
+    // (134). Wider tables say nothing of the keys in them: who calls this knows what it saves.
     const int64_t bytes = batch * keys * kv_heads * head_dim * 4;
     if (bytes < (p.apart ? int64_t{1} << 27 : int64_t{1} << 26)) return p;
     const int tiles = (p.apart ? each : together) > 16 ? 2 : 1;

@@ -87,7 +87,7 @@ class PagedKVCache:
     :func:`paged_shared_attention` takes it, and ``groups`` how many such groups there are; ``saved`` is what reading each
     group's pages once saves in a layer, in bytes. Their memory stays as long as no more groups and no larger ones come up than
     ever before, so a graph captured with the largest follows their changes; one captured before reads groups of nobody from
-    then on, which is right, but reads each sequence's pages for itself. The model's layers use them from 64 MB saved on.
+    then on, which is right, but reads each sequence's pages for itself. The model's layers use them from 100 MB saved on.
     """
 
     def __init__(self, shape, batch: int, pages: int, page_size: int, max_len: int, device, dtype, window: int = 0,
@@ -577,7 +577,7 @@ def paged_shared_attention(q, k_pages, v_pages, table, positions, members, share
 
     Other arguments and the result, but for rounding, are :func:`paged_attention`'s, which also takes the calls that the kernel
     does not: those that run torch ops, small ones, many tokens a sequence (prompts), and batches past about a thousand sequences
-    (``nq_paged_shared_attention`` says where). It pays from about 64 MB of keys and values that are not read again."""
+    (``nq_paged_shared_attention`` says where). It pays from about 100 MB of keys and values that are not read again."""
     what = "paged_shared_attention"
     given = (q, k_pages, v_pages, table, positions, members, shared)
     if _native_shared is not None and q.is_cuda and _only_eager(*given):
@@ -650,7 +650,13 @@ def copy_pages(pools, source, target) -> None:
         pool[target] = pool[source]
 
 
-_WORTH_SHARING = 1 << 26  # bytes: what the longer beginning and the join of the attention over shared pages take, 10 us
+# Bytes that groups save in a layer, from which the attention over shared pages is the faster one. Its beginning and its join take
+# up to 10 us more, and what the plain one reads again comes in part from caches. Captured steps over many layers, us with and
+# without groups, 64 heads of 8 kv heads of 128: 2 sequences in 16000 shared keys (66 MB) 28.9 and 23.5, 100 in 250 (97) 29.4 and
+# 22.8, 8 in 4000 (115) 24.8 and 29.2, 16 in 4000 (246) 26.5 and 43.4; heads of 64, 40 in 1000 (79) 19.1 and 16.6, 16 in 4000 (123)
+# 19.4 and 26.1; 32 kv heads, 2 in 4000 (66) 24.8 and 29.7, 8 in 1000 (114) 18.2 and 19.7. Past it still slower: 40 in 1000 (158)
+# 25.1 and 21.4, 4 in 16000 (197) 32.4 and 28.4.
+_WORTH_SHARING = 100 << 20
 
 
 def paged_rotary_attention(shape, layer: int, q, k, v, cos, sin, positions, cache: PagedKVCache):

@@ -6,7 +6,7 @@ import torch
 
 import fork_oracle
 import serve_oracle as oracle
-from nanoquant_amd import (PagedKVCache, _lib, copy_pages, paged_attention, paged_shared_attention, token_logprobs)
+from nanoquant_amd import (PagedKVCache, _lib, copy_pages, paged_attention, paged_shared_attention, serve, token_logprobs)
 from nanoquant_amd.decode import LlamaShape, random_llama
 
 TINY = LlamaShape(hidden=128, layers=2, heads=4, kv_heads=2, ffn=320, vocab=500)
@@ -302,6 +302,25 @@ def test_a_member_past_the_prompt_leaves_the_others_their_pages():
             cache.trim(b, 1499)
             _groups_hold(cache)
         assert _groups(cache) == ([([0, 1, 2, 3], 1)] if sinks else [])
+
+
+@pytest.mark.parametrize("answers,prompt,heads,dim,faster", [
+    (100, 250, 8, 128, False), (2, 16000, 8, 128, False), (40, 1000, 8, 64, False), (16, 4000, 8, 128, True), (16, 4000, 8, 64, True),
+    (8, 1000, 32, 128, True)])
+def test_a_layer_reads_groups_where_that_was_measured_to_be_faster(answers, prompt, heads, dim, faster, monkeypatch):
+    shape = LlamaShape(hidden=heads * dim, layers=1, heads=heads, kv_heads=heads, ffn=64, vocab=64)
+    cache = PagedKVCache(shape, answers, prompt // 16 + answers + 1, 16, prompt + 32, "cpu", torch.bfloat16)
+    cache.reserve(0, prompt // 16 * 16)
+    cache.fork(0, range(1, answers), prompt // 16 * 16)
+    for b in range(answers):
+        cache.reserve(b, prompt // 16 * 16 + 1)
+    took = []
+    monkeypatch.setattr(serve, "paged_shared_attention", lambda *x: took.append(True))
+    monkeypatch.setattr(serve, "paged_attention", lambda *x: took.append(False))
+    x = torch.zeros(answers, 1, heads * dim, dtype=torch.bfloat16)
+    angles = torch.zeros(answers, 1, dim)
+    serve.paged_rotary_attention(shape, 0, x, x, x, angles, angles, torch.full((answers, 1), prompt // 16 * 16), cache)
+    assert took == [faster]
 
 
 def test_forks_and_trims_at_random():
