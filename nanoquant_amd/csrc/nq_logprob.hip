@@ -332,10 +332,12 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
                 // a lane's logits go through LDS to as many lanes
                 for (; some != 0; some &= some - 1) {
                     const int from = __builtin_ctzll(some);
+                    wave_handover();
                     if (lane == from) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) lane_words[wave][i] = v[i / 4][i % 4];
                     }
+                    wave_handover();
                     const int i = lane % kBatch;
                     hold(logit_of(lane_words[wave][i / kEach], i % kEach), row.element_of(c, 64 * wave + from, i), lane < kBatch);
                 }

@@ -6,6 +6,15 @@
 
 namespace nq {
 
+// Between what some lanes of a wave write to LDS and others of it read there, and before what is read may be written again. LDS
+// takes a wave's accesses in order, so this is no instruction; it keeps the compiler from using what a lane that wrote nothing
+// read before, or from moving the accesses past each other.
+__device__ inline void wave_handover() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Largest over lanes l, l ^ 16, l ^ 32 and l ^ 48; over l and l ^ 32.
 __device__ inline float max_xor32(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
