@@ -602,6 +602,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
                     M = -INFINITY;
                 }
                 const float inv = 1.0f / L;
+                wave_handover();
                 if (kShared && !done) {
                     const int64_t part = parts + rwave * (32 * RW) + 32 * rw;
                     if (ekg == 0 && col0 == 0 && row0 + 32 * rw + ec < rows.rows) a.part_ml[part + ec] = float2{M, L};
@@ -614,6 +615,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
                             for (int e = 0; e < 4; ++e) x[e] = L == 0.0f ? 0.0f : sums[rw][dt][4 * g4 + e];
                             *reinterpret_cast<f32x4*>(stage + ec * Cols + 4 * ((8 * dt + 2 * g4 + ekg) ^ (ec & (FC - 1)))) = x;
                         }
+                    wave_handover();
 #pragma unroll
                     for (int j = 0; j < FC / 2; ++j) {
                         const int r = (64 * j + at_lane) / FC, ch = at_lane % FC;
@@ -632,6 +634,7 @@ __device__ __forceinline__ void rows_segments(const Args& a, const Shares& share
                         *reinterpret_cast<uint2*>(ob + ec * Cols + 8 * ((4 * dt + g4) ^ (ec & (OC - 1))) + 4 * ekg) =
                             uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
                     }
+                wave_handover();
 #pragma unroll
                 for (int j = 0; j < OC / 2; ++j) {
                     const int r = (64 * j + at_lane) / OC, ch = at_lane % OC;
