@@ -468,7 +468,10 @@ Plan make_plan(int64_t rows, int64_t vocab, int64_t top, int piece) {
     p.wide = rows <= kCUs && vocab >= 8192;
     const int64_t chunk = (p.wide ? 1024 : 256) * 4 * piece;
     p.full = ceil_div(vocab + piece - 1, chunk);
-    // Whole rows need no second launch to join their parts, 5 us: 777 rows of 32000 14.4 us, 19.5 cut; 100 of 16000 11.2 and 15.0
+    // Whole rows need no second launch to join their parts, 5 us: 100 rows of 16000 11.2 us, 15.0 cut. In bf16, 777 of 32000 15.4 and
+    // 19.6, 400 of 16000 7.1 and 10.0. Few long rows leave a CU one block or two, which takes what the join would: of 128000, 257 rows
+    // 20.2 and 20.2, with five alternatives 28.8 and 26.0, 513 34.5 and 34.8, 777 50.4 and 47.5, 1280 68.2 and 68.7; in fp32 28.1 and
+    // 27.0, 36.1 and 35.5, 54.9 and 54.4, 81.4 and 79.0, 122.8 and 123.1.
     if (p.wide) p.share = p.full <= 2 ? p.full : ceil_div(p.full, kCUs / rows);
     else if (rows <= kPerCU * kCUs) p.share = p.full;
     else p.share = ceil_div(rows * p.full, kPerCU * kCUs);

@@ -635,3 +635,60 @@ def test_a_model_answers_a_prompt_several_times(monkeypatch):
             assert (logits[live] - want[live]).abs().max() < 0.05 * want.abs().max()
             fork_oracle.check_score([s[live] for s in scores], fork_oracle.score(logits[live], ids[live], 4, 1.0))
     assert len(calls) >= 2 * shape.layers and forked.saved == 3 * 4 * page * 2 * 2 * 128 * 2  # of four members, four pages
+
+
+def test_a_model_answers_under_a_window(monkeypatch):
+    """Answers of lengths of their own whose pages are taken back behind their windows between the replays of a captured step."""
+    shape = LlamaShape(hidden=1024, layers=2, heads=8, kv_heads=2, ffn=1408, vocab=1003)
+    model = random_llama(shape, bpw=1.0, device="cuda", dtype=torch.float16).eval()
+    model.prepare_kernels("gemv", torch.float16)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    answers, P, page, more, window, sinks = 6, 100, 16, 40, 70, 5
+    prompt = torch.randint(0, shape.vocab, (P,), device="cuda", generator=g)
+    begin = [17, 0, 5, 30, 11, 24]  # tokens of each answer before the others' first
+    texts = torch.randint(0, shape.vocab, (answers, more + max(begin)), device="cuda", generator=g)
+    calls = []
+    monkeypatch.setattr(serve, "_WORTH_SHARING", 1)
+    monkeypatch.setattr(serve, "paged_shared_attention", lambda *x: calls.append(1) or attend(*x))
+    with torch.no_grad():
+        alone, forked = caches = [PagedKVCache(shape, answers, 120, page, 40000, "cuda", torch.float16, window=window, sinks=sinks)
+                                  for _ in range(2)]
+        every = torch.arange(P, device="cuda").expand(answers, -1)
+        for b in range(answers):
+            alone.reserve(b, P + begin[b] + more)
+        model(prompt.expand(answers, -1), every, alone)
+        forked.reserve(3, P)
+        model(prompt.expand(answers, -1), torch.where(torch.arange(answers, device="cuda").unsqueeze(1) == 3, every, -1), forked)
+        forked.fork(3, [b for b in range(answers) if b != 3], P)
+        for b in range(answers):
+            forked.reserve(b, P + begin[b] + 1, P)
+        head = max(begin)
+        at = torch.arange(P, P + head, device="cuda").expand(answers, -1)
+        at = torch.where(at < P + torch.tensor(begin, device="cuda").unsqueeze(1), at, -1)
+        for cache in caches:
+            model(texts[:, :head], at, cache)
+        place = P + torch.tensor(begin, device="cuda").unsqueeze(1)
+        ids, pos = texts.gather(1, place - P), place.clone()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            model(ids, pos, forked)  # the same keys again at the first replay
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = model(ids, pos, forked)
+        lead = set()
+        for t in range(more):
+            for b in range(answers):
+                forked.reserve(b, P + begin[b] + t + 1, P + begin[b] + t)
+                forked.trim(b, P + begin[b] + t)
+            lead.add(int(forked.members[0, 0]))
+            pos.copy_(place + t)
+            ids.copy_(texts.gather(1, pos - P))
+            graph.replay()
+            want = model(ids, pos, alone)
+            torch.cuda.synchronize()
+            # as above: the two ways round the probabilities' sums apart
+            assert (logits - want).abs().max() < 0.05 * want.abs().max()
+        assert forked.trim(0, 0) == 0 and (forked.table[:, 1:] >= 0).sum() < answers * 7 and lead == {0, 1}
+    assert len(calls) >= 2 * shape.layers
