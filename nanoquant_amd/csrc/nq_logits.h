@@ -84,7 +84,8 @@ struct LogitRow {
         for (int i = 0; i < kPieces; ++i) Elem<T>::unpack(v[i], x + N * i);
         if (at_edge(k)) {
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) x[i] = static_cast<unsigned>(element(k, i)) < static_cast<unsigned>(vocab) ? x[i] : -INFINITY;
+            for (int i = 0; i < kBatch; ++i)
+                x[i] = static_cast<unsigned>(element(k, i)) < static_cast<unsigned>(vocab) ? x[i] : -INFINITY;
         }
     }
 };

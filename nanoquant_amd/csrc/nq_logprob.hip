@@ -32,13 +32,17 @@ __device__ inline uint32_t order_bits(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);  // -0 becomes 0
     return x != x ? 0xFFFFFFFFu : u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
 }
-__device__ inline float from_order_bits(uint32_t k) { return __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ inline float from_order_bits(uint32_t k) {
+    return __builtin_bit_cast(float, k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
+}
 __device__ inline uint64_t order_key(float x, int at) {
     return static_cast<uint64_t>(order_bits(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(at));
 }
 __device__ inline bool is_key(uint64_t key) { return key >> 32 != 0; }
 __device__ inline int key_index(uint64_t key) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)); }
-__device__ inline float key_logit(uint64_t key) { return is_key(key) ? from_order_bits(static_cast<uint32_t>(key >> 32)) : -INFINITY; }
+__device__ inline float key_logit(uint64_t key) {
+    return is_key(key) ? from_order_bits(static_cast<uint32_t>(key >> 32)) : -INFINITY;
+}
 
 // Of e = 2^d and e d, d = x scale - ref: what ref has of a rounding, all d have in common, and log p = x scale - ref - log2 s.
 struct Sums {
@@ -297,7 +301,8 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? kPerCU : 4) void score_
             sums.d += d;
             if (a.top == 0) continue;
             most_yet = fmaxf(most_yet, most);
-            if (((c - c0) & (c - c0 - 1)) == 0) {  // a bound from all waves, the block's lanes in 64 groups: chunks 0, 1, 2, 4, 8 ...
+            // a bound from all waves, the block's lanes in 64 groups: chunks 0, 1, 2, 4, 8 ...
+            if (((c - c0) & (c - c0 - 1)) == 0) {
                 lane_most[turn][wave][lane] = most_yet;
                 __syncthreads();
                 float x = lane_most[turn][0][lane];

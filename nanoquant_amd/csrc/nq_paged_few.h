@@ -161,7 +161,9 @@ struct GroupPlan {
     int ends[kEntries];   // of a group: the shared keys
     int2 spans[kEntries];
     uint8_t slow[kEntries];  // of a group's entry: the tiles in which some member's window begins
-    __device__ int from(int b, float per_most) const { return place[b] < 0 ? 0 : ends[small_quotient(place[b], per_most)]; }  // of a sequence's own keys
+    __device__ int from(int b, float per_most) const {  // of a sequence's own keys
+        return place[b] < 0 ? 0 : ends[small_quotient(place[b], per_most)];
+    }
 };
 // All threads of the block.
 template <int kThreads, int kEntries>
@@ -218,7 +220,8 @@ __device__ inline int tiles_of_plan(const GroupArgs& a, GroupPlan<kEntries>& pla
     if (plan.lead[e] == kNobody) return 0;
     plan.lead[e] &= (1 << kSequenceBits) - 1;
     const int of_groups = a.entries_of_groups();
-    const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.per_most), to = e < of_groups ? plan.ends[small_quotient(e, a.per_group_rows)] : INT32_MAX;
+    const int from = e < of_groups ? 0 : plan.from(plan.lead[e], a.per_most);
+    const int to = e < of_groups ? plan.ends[small_quotient(e, a.per_group_rows)] : INT32_MAX;
     const Tiles r = tiles_within(a, shift, plan.spans[e].x, plan.spans[e].y, from, to);
     int slow = 0;
     if (e < of_groups && a.window > 0 && r.count > r.sink_tiles)
@@ -234,7 +237,9 @@ __device__ inline uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFF
 __device__ inline uint32_t seen_bits(int key0, int last, int start, int sinks) {  // of keys key0 .. key0 + 31
     return low_bits(last - key0 + 1) & (~low_bits(start - key0) | low_bits(sinks - key0));
 }
-__device__ inline uint32_t bit_mask(uint32_t bits, int i) { return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), i, 1)); }
+__device__ inline uint32_t bit_mask(uint32_t bits, int i) {
+    return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), i, 1));
+}
 __device__ inline float or_minus_inf(float x, uint32_t bits, int i) {  // x where bit i is set
     return __builtin_bit_cast(float, bit_select(bit_mask(bits, i), __builtin_bit_cast(uint32_t, x), 0xFF800000u));
 }
@@ -316,7 +321,8 @@ __device__ inline bool holds_unit(const PagedArgs& a, const int64_t* pre, int e,
     return pre[e] * a.kv_heads <= unit && unit < pre[e + 1] * a.kv_heads;
 }
 template <int kThreads>
-__device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre, int* s_entry) {
+__device__ inline Shares take_share(const PagedArgs& a, int e0, int e1, int block, int blocks, int least, const int64_t* pre,
+                                    int* s_entry) {
     Shares r = share_of(a, e0, e1, block, blocks, least, pre);
     if (r.first >= r.end) return r;
     for (int e = e0 + static_cast<int>(threadIdx.x); e < e1; e += kThreads)
@@ -847,7 +853,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
             plan_groups<64 * kWaves>(a, plan);
             entries += a.entries_of_groups();
         }
-        shares = make_shares<64 * kWaves, Shape::kBlocks, std::conditional_t<kGroups, int, double>>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
+        using Sum = std::conditional_t<kGroups, int, double>;
+        shares = make_shares<64 * kWaves, Shape::kBlocks, Sum>(a, entries, kLeastShare, pre, wave_total, &s_entry, [&](int e) {
             if constexpr (kGroups) {
                 const int n = tiles_of_plan(a, plan, e, kTileShift);
                 return n == 0 ? 0 : n + kFewStart;
@@ -865,7 +872,8 @@ __global__ __launch_bounds__(64 * kWaves, (FewShape<D, RT>::kPerCU)) void few_ke
     }
     const int2* spans = own_spans;
     if constexpr (kGroups) spans = plan.spans;
-    few_segments<T, D, RT, kShared, kWaves, kFewStart>(a, shares, entry, ring, pre, spans, plan, marks, static_cast<int>(threadIdx.x), BlockSync{});
+    few_segments<T, D, RT, kShared, kWaves, kFewStart>(a, shares, entry, ring, pre, spans, plan, marks,
+                                                       static_cast<int>(threadIdx.x), BlockSync{});
 }
 
 }  // namespace

@@ -9,9 +9,9 @@
 namespace nq {
 namespace {
 
-// Adds up what few_kernel or shared_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave a row,
-// D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 3.9 us for 128 rows, 7.0 for 8192 of
-// 128 dimensions, with several parts a row on their way at once (with half or twice as many 3 us more).
+// Adds up what few_kernel or shared_kernel left of a row: the parts of its group's shared keys and of its sequence's own. A wave
+// a row, D / 4 lanes a part. Bound by its chain of loads (the sequence's place, its entries' blocks, their parts): 3.9 us for 128
+// rows, 7.0 for 8192 of 128 dimensions, with several parts a row on their way at once (with half or twice as many 3 us more).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint32_t count) {
     constexpr int L4 = D / 4, Groups = 64 / L4, kAhead = 4;
@@ -19,7 +19,8 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint
     const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));  // (sequence, token, head)
     if (row >= count) return;
     const int token = static_cast<int>(row / static_cast<uint32_t>(a.heads));
-    const int head = static_cast<int>(row) - token * a.heads, kvh = __builtin_amdgcn_readfirstlane(small_quotient(head, a.per_groups));
+    const int head = static_cast<int>(row) - token * a.heads;
+    const int kvh = __builtin_amdgcn_readfirstlane(small_quotient(head, a.per_groups));
     const int b = __builtin_amdgcn_readfirstlane(small_quotient(token, a.per_tokens));
     const int r = (token - b * a.tokens) * a.groups + head - kvh * a.groups;
     const int at = a.place[b];
@@ -49,8 +50,8 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint
             const int part = min(i0 + i * Groups, n - 1);
             const bool of_common = part < common.n;
             const int k = of_common ? part : part - common.n;
-            const int64_t from = k == 0 ? (of_common ? common.first : own.first)
-                                        : (of_common ? common.later : own.later) + static_cast<int64_t>(k) * (of_common ? common.step : own.step);
+            const int64_t later = (of_common ? common.later : own.later) + static_cast<int64_t>(k) * (of_common ? common.step : own.step);
+            const int64_t from = k == 0 ? (of_common ? common.first : own.first) : later;
             ml[i] = a.part_ml[from];
             x[i] = *reinterpret_cast<const f32x4*>(a.part_o + from * D + d0);
         }
@@ -82,16 +83,18 @@ __global__ __launch_bounds__(256) void group_join_kernel(const GroupArgs a, uint
         M = top;
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (grp == 0) *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(row) * D + d0) = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+    if (grp == 0)
+        *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(row) * D + d0) =
+            uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
 // Groups of more than 32 rows: some of the blocks take their entries as rows_kernel does, the others the sequences' as
 // few_kernel does, a team of two waves each, in equal shares; all of them work out the same list. One launch, since the
 // sequences' part is bound by the read of keys and values and the groups' by products: in two launches, each on all CUs, 16
 // sequences with 8000 shared keys 47 us against 36, 60 conversations 179 against 152, 128 samples under a window 221 against
-// 161. Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 24 us, bound by latency
+// 161. Now, of 64 heads of 8 kv heads: 16 sequences with 8000 shared keys and 20 to 700 of their own 23 us, bound by latency
 // (the list, the first tiles' way, the waves' join); 60 in five groups with 100 to 4000 of their own 146, bound by the read
-// (5.0 TB/s, a large copy's rate); 128 under a window of 12011 keys 146, bound by rows_segments' products and exponentials, of
+// (5.0 TB/s, a large copy's rate); 128 under a window of 12011 keys 137 to 145, bound by rows_segments' products and exponentials, of
 // which the tiles in which windows begin take twice. 11 sequences of 5 tokens, heads of 64, 5000 shared keys: 21 us. How many
 // blocks either gets goes by what a unit takes of a CU, in ns: a tile of 64 keys and 128 rows, or one of 32 keys; and by how
 // much longer the groups' blocks take for their beginning and their end.
@@ -106,8 +109,9 @@ template <int D>
 __device__ inline int blocks_for_groups(int64_t group_units, int64_t own_units) {
     if (group_units == 0) return 0;
     const int n = 4 * (static_cast<int>(threadIdx.x) & 63) + 2;
-    const float g = static_cast<float>(group_units) * (D == 128 ? kGroupTime : kGroupTime64) * __builtin_amdgcn_rcpf(static_cast<float>(n));
-    const float s = static_cast<float>(own_units) * (D == 128 ? kOwnTime : kOwnTime64) * __builtin_amdgcn_rcpf(static_cast<float>(kCUs - n));
+    const float group_time = D == 128 ? kGroupTime : kGroupTime64, own_time = D == 128 ? kOwnTime : kOwnTime64;
+    const float g = static_cast<float>(group_units) * group_time * __builtin_amdgcn_rcpf(static_cast<float>(n));
+    const float s = static_cast<float>(own_units) * own_time * __builtin_amdgcn_rcpf(static_cast<float>(kCUs - n));
     const int late = __popcll(__ballot(g + kGroupMore > s));  // the lanes at which the groups' part ends last: the first ones
     return min(4 * late + 2, kCUs - 2);
 }
@@ -131,7 +135,8 @@ __global__ __launch_bounds__(512, 2) void shared_kernel(const GroupArgs a) {
     plan_groups<kThreads>(a, plan);
     prefix_sums<kThreads, int>(entries, pre, wave_total, [&](int e) {
         const int n = tiles_of_plan(a, plan, e, e < of_groups ? kKeysShift : kTileShift);
-        return n == 0 ? 0 : e < of_groups ? n + kGroupStart + plan.slow[e] : n + kOwnStart;  // a tile that is masked takes twice as long
+        // a tile that is masked takes twice as long
+        return n == 0 ? 0 : e < of_groups ? n + kGroupStart + plan.slow[e] : n + kOwnStart;
     });
     const int block = static_cast<int>(blockIdx.x);
     const int for_groups = blocks_for_groups<D>(pre[of_groups] * a.kv_heads, (pre[entries] - pre[of_groups]) * a.kv_heads);
@@ -168,7 +173,8 @@ struct Plan {
     size_t part_o, part_ml, desc, place, bytes;
 };
 
-Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t keys, int64_t sharing, int64_t most) {
+Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, int64_t head_dim, int64_t keys, int64_t sharing,
+               int64_t most) {
     Plan p{};
     const int64_t each = tokens * groups, together = most * each;
     p.apart = together > 32;
@@ -189,6 +195,8 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t groups, int64_t kv_heads, 
     p.group_kept = std::min(together, p.group_tile);
     p.rows_kept = std::min(each, p.own_tile);
     const int64_t of_groups = sharing * p.group_rows, own = batch * p.row_groups;
+    // Past the list of either kernel the plain attention reads every sequence's pages, of small groups also where the other's list
+    // would hold them.
     if (of_groups + own > (p.apart ? kEntries : kFewEntries)) return p;
     if (batch * each * kv_heads > kMaxThreads / 64) return p;  // rows of group_join_kernel, a wave each
     if ((of_groups + own) * (keys / kTile + 512) > INT32_MAX) return p;  // units, which are added up in 32 bits
@@ -241,8 +249,8 @@ void launch_shared(GroupArgs a, const Plan& p, char* ws, hipStream_t st) {
 }
 
 // A call's plan; tiles 0 where there is none.
-Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t table_pages, int64_t page_size,
-             int64_t sharing, int64_t most) {
+Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t table_pages,
+             int64_t page_size, int64_t sharing, int64_t most) {
     if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65536 || batch > INT32_MAX ||
         tokens > INT32_MAX || batch * tokens > INT32_MAX / heads || sharing <= 0 || most <= 0 || sharing > INT32_MAX ||
         most > INT32_MAX / sharing || most > INT32_MAX / (tokens * heads) || (head_dim != 64 && head_dim != 128) ||

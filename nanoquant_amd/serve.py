@@ -255,8 +255,8 @@ class PagedKVCache:
             self.members[at, :len(order)].copy_(torch.tensor(order, dtype=torch.int32))
 
     def reserve(self, sequence: int, length: int, start: int = 0) -> None:
-        """Pages for the sequence's positions ``start`` to ``length - 1`` (those it has stay). RuntimeError, and no change,
-        where the pool has too few left."""
+        """Pages for the sequence's positions ``start`` to ``length - 1`` (those it has stay, shared ones too: a sequence that
+        was set back needs ``own`` before it writes there). RuntimeError, and no change, where the pool has too few left."""
         row = self._row(sequence)
         if not 0 <= start <= length <= self.max_len:
             raise ValueError(f"positions {start} to {length} do not fit max_len {self.max_len}")
@@ -282,8 +282,8 @@ class PagedKVCache:
         return len(gone)
 
     def trim(self, sequence: int, position: int) -> int:
-        """Take back the pages that no token from ``position`` on sees under the window; returns their number. Calls in
-        flight on other streams must have ended."""
+        """Take back the pages that no token from ``position`` on sees under the window; returns their number. Groups last as
+        long as their members still have some of the pages in common. Calls in flight on other streams must have ended."""
         if self.window == 0:
             return 0
         first = min(max(0, position - self.window + 1) // self.page_size, self.max_pages)
