@@ -223,8 +223,9 @@ class PagedKVCache:
             shape = (max(old[0], len(lists)), max(old[1], most))
             if self.members is not None:
                 self._outgrown.append((self.members.fill_(-1), self.shared.zero_()))
-            self.members = torch.empty(shape, dtype=torch.int32, device=self.table.device)
-            self.shared = torch.empty(shape[0], dtype=torch.int32, device=self.table.device)
+            with torch.inference_mode(False):  # as the table's, whose changes may come outside it
+                self.members = torch.empty(shape, dtype=torch.int32, device=self.table.device)
+                self.shared = torch.empty(shape[0], dtype=torch.int32, device=self.table.device)
         groups, most = self.members.shape
         lists += [[]] * (groups - len(lists))
         self.members.copy_(torch.tensor([x + [-1] * (most - len(x)) for x in lists], dtype=torch.int32).view(groups, most))

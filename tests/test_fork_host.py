@@ -585,6 +585,20 @@ def test_groups_that_outgrow_their_tensors_leave_nobody_in_the_old_ones():
     assert any(a is members and b is shared for a, b in cache._outgrown)  # their memory is nobody else's
 
 
+def test_groups_made_in_inference_mode_change_outside_it():
+    cache = _cache()
+    with torch.inference_mode():
+        cache.reserve(0, 9)
+        cache.fork(0, [1], 9)
+    cache.fork(0, [2, 3], 9)
+    assert cache.members.tolist() == [[0, 1, 2, 3]]
+    cache.release(1)
+    with torch.inference_mode():
+        cache.release(2)
+    assert cache.members.tolist() == [[0, 3, -1, -1]]
+    _sound(cache)
+
+
 def test_c_abi_limits_of_shared_pages_need_no_gpu():
     """What a launch lists: row groups of groups and of sequences, and a wave for each row of the output in 32-bit threads; and
     what is left to the plain attention."""
